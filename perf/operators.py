@@ -8,8 +8,8 @@ and attend over them.  ``own = False`` computes the operators in elementary torc
 A page tensor is uint8 [pages, heads, positions / 16, 18 * dim]: for 16 positions of one head, 8 dim bytes of key codes, dim bytes of
 key scales, 8 dim bytes of value codes, dim bytes of value scales.  A code stands for (code - 8) * scale, a scale (bf16) belongs to 32
 neighbouring components.  Keys of a position: the eight codes 32 g + 8 c .. + 7 are 32-bit word c * dim / 32 + g.  Values: unit
-(i, g, c) of 16 bytes holds components 64 i + 8 g .. + 7 of positions 2 c, 2 c + 1, 2 c + 8, 2 c + 9, as 16-bit halves in the order
-pair of positions, half of the components, position.
+(i, g, c) of 16 bytes holds components 64 i + 4 g .. + 3 and the four 32 further, of positions 2 c, 2 c + 1, 2 c + 8 and 2 c + 9, as
+16-bit fours of codes in the order pair of positions, four, position.
 """
 from __future__ import annotations
 
@@ -193,7 +193,7 @@ def _pack(k, v):
     p, h, t, d = k.shape
     (kc, ks), (vc, vs) = _quantise(k), _quantise(v)
     kc = kc.view(p, h, t // 16, 16, d // 32, 4, 8).transpose(4, 5).reshape(p, h, t // 16, 16 * d)
-    vc = vc.view(p, h, t // 16, 2, 4, 2, d // 64, 8, 2, 4).permute(0, 1, 2, 6, 7, 4, 3, 8, 5, 9).reshape(p, h, t // 16, 16 * d)
+    vc = vc.view(p, h, t // 16, 2, 4, 2, d // 64, 2, 8, 4).permute(0, 1, 2, 6, 8, 4, 3, 7, 5, 9).reshape(p, h, t // 16, 16 * d)
     raw = [x.reshape(p, h, t // 16, d // 2).contiguous().view(torch.uint8) for x in (ks, vs)]
     return torch.cat([_bytes(kc), raw[0], _bytes(vc), raw[1]], dim=-1)
 
@@ -208,7 +208,7 @@ def _unpack(pages):
     d = b // 18
     kc, ks, vc, vs = pages.split([8 * d, d, 8 * d, d], dim=-1)
     kc = _nibbles(kc).view(p, h, n, 16, 4, d // 32, 8).transpose(4, 5).reshape(p, h, n * 16, d)
-    vc = _nibbles(vc).view(p, h, n, d // 64, 8, 4, 2, 2, 2, 4).permute(0, 1, 2, 6, 5, 8, 3, 4, 7, 9).reshape(p, h, n * 16, d)
+    vc = _nibbles(vc).view(p, h, n, d // 64, 8, 4, 2, 2, 2, 4).permute(0, 1, 2, 6, 5, 8, 3, 7, 4, 9).reshape(p, h, n * 16, d)
     ks, vs = (x.contiguous().view(torch.bfloat16).view(p, h, n * 16, d // 32) for x in (ks, vs))
     return _values(kc, ks), _values(vc, vs)
 
@@ -374,8 +374,8 @@ def _exact_memory(pages):
     d = b // 18
     t, c = torch.arange(16, device="cuda")[:, None], torch.arange(d, device="cuda")[None, :]
     key = t * (d // 2) + 4 * ((c % 32 // 8) * (d // 32) + c // 32) + c % 8 // 2
-    unit = (c // 64 * 8 + c % 64 // 8) * 4 + t % 8 // 2
-    value = 9 * d + 16 * unit + 8 * (t // 8) + 4 * (c % 8 // 4) + 2 * (t % 2) + c % 4 // 2
+    unit = (c // 64 * 8 + c % 32 // 4) * 4 + t % 8 // 2
+    value = 9 * d + 16 * unit + 8 * (t // 8) + 4 * (c % 64 // 32) + 2 * (t % 2) + c % 4 // 2
     made = []
     for at, scales in ((key, 8 * d), (value, 17 * d)):
         code = (pages[..., at] >> (4 * (c % 2)).to(torch.uint8).expand(16, d)) & 15
