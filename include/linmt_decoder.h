@@ -302,6 +302,158 @@ int linmt_k_softmax_topk(const float* logits, int32_t R, int32_t V, int32_t kk, 
 int linmt_gemm_f32_noalloc(const float* d_x, const float* d_wt, float* d_y, int32_t R, int32_t K, int32_t N,
                            int32_t device);
 
+/* ------------------------------------------------------------------------------------
+ * 4. Operators on device tensors, for programs that run their own model and want a decoding step's
+ *    parts: beam selection and reordering, pages for a growing memory, keys and values in them in
+ *    4 bits, attention over them.  They have no counterpart in the reference, whose beam search runs on the
+ *    host (src/decoder.h:340-525) and whose attention reads dense states.
+ *
+ *    Every pointer inside the argument structs is a DEVICE pointer on `device`, every stride is in elements unless
+ *    it says bytes.  A call checks its arguments, issues its kernels on `stream` (a cudaStream_t, NULL = the default
+ *    stream) and returns without waiting; nothing is allocated and nothing is kept between calls, so calls may run at once
+ *    and may be captured into a graph, as long as their outputs and workspaces are not shared.  The current device is left as it
+ *    was.  LINMT_EINVAL: an argument is not allowed; LINMT_ELIMIT: a size is beyond what the kernel is made for;
+ *    LINMT_ECUDA: the launch was refused; linmt_op_error() has the text, per host thread.  `size` is sizeof the struct.
+ * ------------------------------------------------------------------------------------ */
+enum { LINMT_F32 = 0, LINMT_BF16 = 1, LINMT_F16 = 2 };
+
+const char* linmt_op_error(void);
+
+/* Beam selection: of the k * vocab continuations of each sentence's beams the k best, best first.
+ *   a live beam b      offers every word v with score_b + x_v - log sum_u exp(x_u) over its allowed logits x
+ *   a finished beam    offers `eos` alone, with its score as it is; its logits are not read
+ *   a beam whose score is not finite, and one with a NaN or +inf at an allowed place, offers nothing
+ * Equal sums go to the lowest b * vocab + v.  The order is that of 64-bit arithmetic: sums of two beams that lie closer than
+ * 32 bits can tell apart are compared again with 64-bit normalisers.  Words that are not allowed may hold anything;
+ * one whose logit is -inf is never chosen.  Slots that nothing is left for get token eos, parent = the slot itself, score -inf, done 1.
+ * out_* may be the arrays `scores` and `done`. */
+typedef struct linmt_beam_select_args {
+  uint32_t size;
+  int32_t device;
+  void* stream;
+  const void* logits;        /* [n][k][vocab], LINMT_F32 / BF16 / F16, words contiguous, aligned to their type */
+  int64_t stride_n, stride_k;
+  const float* scores;       /* [n][k] */
+  const uint8_t* done;       /* [n][k], not 0 = finished; may be NULL */
+  const uint32_t* allowed;   /* bit v % 32 of word v / 32 set = word v allowed, ceil(vocab / 32) words; may be NULL */
+  int64_t allowed_stride;    /* words from one sentence's list to the next, 0 = one list for all */
+  int32_t* out_tokens;       /* [n][k] */
+  int32_t* out_parents;      /* [n][k], 0 .. k-1 */
+  float* out_scores;         /* [n][k] */
+  uint8_t* out_done;         /* [n][k]: parent was finished, or the token is eos */
+  int32_t n, k, vocab, eos, dtype;   /* k <= 32, k * vocab < 2^31 */
+} linmt_beam_select_args;
+int linmt_beam_select(const linmt_beam_select_args* args);
+
+/* Rows of states follow their beams: dst[l][i][j] = src[l][i][parents[i][j]] for every state, one launch for up to 16 of them.
+ * dst may be src (the same pointer and strides); otherwise the two must not overlap.  A parent outside 0 .. k-1 takes the row's own. */
+typedef struct linmt_beam_state {
+  const void* src;
+  void* dst;
+  int64_t src_stride_l, src_stride_n, src_stride_k;   /* bytes */
+  int64_t dst_stride_l, dst_stride_n, dst_stride_k;
+  int64_t row_bytes;
+  int64_t layers;
+} linmt_beam_state;
+typedef struct linmt_beam_reorder_args {
+  uint32_t size;
+  int32_t device;
+  void* stream;
+  const int32_t* parents;    /* [n][k] */
+  int32_t n, k;              /* k <= 32 */
+  int32_t n_states, reserved;
+  linmt_beam_state state[16];
+} linmt_beam_reorder_args;
+int linmt_beam_reorder(const linmt_beam_reorder_args* args);
+
+/* Pages for sentences that grow from old_len to new_len positions: every page column p of sentence i with
+ * ceil(old / page) <= p < ceil(new / page) gets the next entry of `free_pages`, sentence by sentence, and every new position its
+ * slot = table[i][pos / page] * page + pos % page, sentence by sentence.  Lengths are taken as 0 .. width * page, a shorter new length as the
+ * old one.  Where the free list has run out a column gets -1; a position in a column that holds none of the pool's pages gets slot -1;
+ * so do slots behind the last new position.  out_used = used + the pages that were wanted (more than n_free: the list ran out). */
+typedef struct linmt_plan_pages_args {
+  uint32_t size;
+  int32_t device;
+  void* stream;
+  const int32_t* old_len;    /* [n]; NULL = all 0 */
+  const int32_t* new_len;    /* [n] */
+  int32_t* table;            /* [n][width], rows `table_stride` apart */
+  int64_t table_stride;
+  const int32_t* free_pages; /* [n_free] */
+  const int32_t* used;       /* [1]: entries of free_pages that are taken already */
+  int32_t* out_used;         /* [1], not the array `used` */
+  int64_t* out_slots;        /* [total] */
+  int32_t* out_starts;       /* [n + 1]: first new position of each sentence in out_slots */
+  int32_t n, width, page, n_free;    /* n <= 16384 */
+  int64_t total;
+} linmt_plan_pages_args;
+int linmt_plan_pages(const linmt_plan_pages_args* args);
+
+/* A pool of pages in 4 bits: [n_pages][heads][page / 16] tiles of 18 * dim bytes (dim 64 or 128, page a multiple of 16), 16-byte
+ * aligned.  A tile holds 16 positions of one head:
+ *   8 dim bytes of key codes (4 bits, low half of a byte first): the codes of components 32 g + 8 c .. + 7 of position t are the
+ *     32-bit word t * dim / 8 + c * dim / 32 + g
+ *   dim bytes of key scales: bf16 [16][dim / 32]
+ *   8 dim bytes of value codes: 16-byte unit (i * 8 + g) * 4 + c has, as 16-bit fours of codes [2][2][2], for position
+ *     8 a + 2 c + b and components 64 i + 32 h + 4 g .. + 3 the four [a][h][b]
+ *   dim bytes of value scales: bf16 [16][dim / 32]
+ * A code stands for (code - 8) * scale.  scale = bf16(m / -8), m the component of largest size of the 32 (the positive one of two);
+ * code = 8 + x / scale rounded to the nearest even integer and held to -8 .. 7, computed in 32 bits; scale 0: code 8.  NaN is
+ * taken as 0, larger sizes as the largest finite bf16. */
+typedef struct linmt_pages4 {
+  void* data;
+  int64_t stride_page, stride_head;   /* bytes, multiples of 16; the tiles of a page's head are contiguous */
+  int32_t n_pages, heads, page, dim;
+} linmt_pages4;
+
+/* Keys and values of `t` positions into (write) or out of (read) the slots of a pool.  A slot outside 0 .. n_pages * page - 1 is not written, and reads
+ * as zeros.  Slots of a write must differ: what two writes of one slot leave there is not defined. */
+typedef struct linmt_pages4_rows_args {
+  uint32_t size;
+  int32_t device;
+  void* stream;
+  linmt_pages4 pages;
+  const int64_t* slots;      /* [t] */
+  void* k;                   /* [t][heads][dim], components contiguous; 16-byte aligned rows */
+  void* v;
+  int64_t k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  int32_t t, dtype;
+} linmt_pages4_rows_args;
+int linmt_write_pages4(const linmt_pages4_rows_args* args);
+int linmt_read_pages4(const linmt_pages4_rows_args* args);
+
+/* Attention of g query rows per sentence (its beams) over the sentence's positions in a pool.  Query head h reads head
+ * h / (heads / pages.heads) of the pool; position t of sentence i is row t % page of page table[i][t / page].
+ *   s = scale * q . k_t;  cap > 0: s = cap * tanh(s / cap);  slope: s -= slope[h] * |t - centre[i][row]|
+ *   seen: first[i][row] <= t < last[i][row] (NULL: all), 0 <= t < len[i], and the table names a page of the pool
+ *   out = sum over seen of softmax(s) * v_t; lse = log sum over seen of exp(s).  Nothing seen: 0 and -inf.
+ * `len` beyond width * page is taken as that.  Sums are held in 32 bits; 32-bit queries are multiplied as three bf16 terms.
+ * `workspace`: linmt_attend_pages4_workspace bytes, 16-byte aligned, the call's own until it has run; NULL where that is 0. */
+typedef struct linmt_attend_pages4_args {
+  uint32_t size;
+  int32_t device;
+  void* stream;
+  linmt_pages4 pages;
+  const void* q;             /* [n][g][heads][dim], components contiguous, rows 4-byte aligned */
+  int64_t q_stride_n, q_stride_g, q_stride_h;
+  void* out;                 /* as q, strides of its own */
+  int64_t out_stride_n, out_stride_g, out_stride_h;
+  float* lse;                /* [n][g][heads]; may be NULL */
+  const int32_t* table;      /* [n][width], rows `table_stride` apart */
+  int64_t table_stride;
+  const int32_t* len;        /* [n] */
+  const float* slope;        /* [heads]; may be NULL */
+  const float* centre;       /* [n][g]; with slope */
+  const int32_t* first;      /* [n][g]; may be NULL */
+  const int32_t* last;       /* [n][g]; with first */
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t n, g, heads, width, dtype;
+  float scale, cap;
+} linmt_attend_pages4_args;
+int64_t linmt_attend_pages4_workspace(const linmt_attend_pages4_args* args);   /* bytes, or -1: see linmt_op_error */
+int linmt_attend_pages4(const linmt_attend_pages4_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -38,7 +38,9 @@ EXPORTS = ["python_decoder_init", "python_decoder_do_job", "linmt_default_option
            "linmt_create_from_weights", "linmt_create_from_weights_on", "linmt_device_count", "linmt_front_error", "linmt_create", "linmt_destroy", "linmt_last_error", "linmt_beam",
            "linmt_decode_batch", "linmt_decode_batch_device", "linmt_get_stats", "linmt_set_kernel_timing", "linmt_kernel_times",
            "linmt_translate", "linmt_k_gemm", "linmt_k_logits", "linmt_k_softmax_topk", "linmt_gemm_f32_noalloc", "linmt_decode_file", "linmt_score_batch",
-           "linmt_read_model_file", "python_unk_init", "python_unk_do_job", "linmt_unk_create", "linmt_unk_process", "linmt_unk_destroy"]
+           "linmt_read_model_file", "python_unk_init", "python_unk_do_job", "linmt_unk_create", "linmt_unk_process", "linmt_unk_destroy",
+           "linmt_op_error", "linmt_beam_select", "linmt_beam_reorder", "linmt_plan_pages", "linmt_write_pages4", "linmt_read_pages4",
+           "linmt_attend_pages4", "linmt_attend_pages4_workspace"]
 
 _lib = None
 
@@ -96,5 +98,10 @@ def load():
     lib.linmt_unk_process.argtypes = [C.c_void_p, C.c_char_p, C.c_char_p, C.c_char_p, C.c_int32]
     lib.linmt_unk_destroy.argtypes = [C.c_void_p]
     lib.linmt_score_batch.argtypes = [C.c_void_p] * 5 + [C.c_int32, C.c_void_p, C.c_void_p, C.c_int32]
+    lib.linmt_op_error.restype = C.c_char_p
+    for name in ("linmt_beam_select", "linmt_beam_reorder", "linmt_plan_pages", "linmt_write_pages4", "linmt_read_pages4", "linmt_attend_pages4"):
+        getattr(lib, name).argtypes = [C.c_char_p]     # the argument struct as packed bytes (device_ops)
+    lib.linmt_attend_pages4_workspace.argtypes = [C.c_char_p]
+    lib.linmt_attend_pages4_workspace.restype = C.c_int64
     _lib = lib
     return lib
