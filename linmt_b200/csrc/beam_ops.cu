@@ -19,57 +19,69 @@ namespace {
 
 // ---- selection ---------------------------------------------------------------------------------
 //
-// One cluster of 8 CTAs per sentence.  The work of a sentence is its live rows, each cut into as many stretches as there are warps for
-// it; the clusters' CTAs exchange what they find through distributed shared memory, so a step is one launch without a workspace.
+// One cluster of C CTAs per sentence.  The work of a sentence is its live rows, each cut into as many stretches as there are warps for
+// it; the cluster's CTAs exchange what they find through distributed shared memory, so a step is one launch without a workspace.
 //   1  A warp reads its stretch once: per lane the running maximum and the sum of exponentials relative to it, and where
-//      the lane's maximum lies.
-//   2  Every CTA has the normalisers of all rows.  The best of each four lanes is a bid, a candidate's sum with an upper bound of
-//      its index; the kNeed-th best bid of the cluster is a bar that at least kNeed = k + kBeyond candidates reach.
-//   3  Only the stretches of lanes whose bid reaches the bar are read again (some kNeed of 1000, from L2).
+//      the lane's maximum lies; per chunk of 128 vectors the maximum.
+//   2  Every CTA has the normalisers of all rows.  A lane's best is a bid, a candidate's sum with an upper bound of its index; the
+//      `need`-th best bid of the cluster is a bar that at least need = k + kBeyond candidates reach.
+//   3  Only the chunks whose maximum can reach the bar are read again (some `need` of hundreds, from L2).
 //   4  The candidates found, some dozens, are ranked by counting.
-// Sums are compared in 64 bits, but exponentials cost four to five instructions in 32 bits and twenty in 64, and the logits arrive at a rate that
-// allows for the former.  So the normaliser is summed in 32 bits with a bound on its error (row_error); where two
-// neighbours of the final order come from different rows and lie closer than twice that, their rows' normalisers are summed once more in 64 bits
-// and the steps from 2 on repeat.  Some 1 sentence in 500 needs it, for 2 us.
-constexpr int kClusterCtas = 8;
+// Sums are compared in 64 bits (as integers of the same order: a comparison of two doubles costs several times one of two integers), but
+// exponentials cost five instructions in 32 bits and twenty in 64, and the logits arrive at a rate that allows for the former.  So the
+// normaliser is summed in 32 bits with a bound on its error (row_error); where two neighbours of the final order come from different rows and
+// lie closer than twice that, their rows' normalisers are summed once more in 64 bits and the steps from 2 on repeat.
+constexpr int kMaxC = 8;
 constexpr int kMaxK = 32;
-constexpr int kMaxWarps = 16;
-constexpr int kUnits = kClusterCtas * kMaxWarps;
+constexpr int kWarps = 12;                       // 96 of a cluster of 8: 12 beams leave none without a stretch, 5, 7, 16, 31 few
 constexpr int kBeyond = 8;                       // candidates past the k-th that the order is checked on
 constexpr int kChunkVecs = 128;                  // a warp's step: four 16-byte vectors a lane
-// Lanes that reach the bar: kNeed fours, and at most 7 more of the bar's own chunk whose index bounds overlap its.  Each gives up to
-// max(32, kNeed) candidates; finished rows add one each.
-constexpr int kMaxList = (kMaxK + kBeyond + 7) * (kMaxK + kBeyond) + kMaxK;
-constexpr int kSorted = 64;                      // of them that are put in order (>= kNeed)
+constexpr int kMaxima = 64;                      // maxima that a warp keeps: of one chunk each, of more where its stretch has more
+constexpr int kMany = 200;                       // candidates of a CTA that are listed as they are found; of more the best `need`
+constexpr int kMaxList = kMaxC * kMany + kMaxK;  // finished rows add one each
+constexpr int kSorted = 64;                      // of them that are put in order (>= need)
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr double kNone = -1.7976931348623157e308;   // below every candidate (sums of finite numbers below 1e39 in size)
+typedef long long Key;                           // a sum, as an integer that is ordered alike
+constexpr Key kNone = -0x7fffffffffffffffll - 1; // below every sum
 
-// A candidate is its sum and `at` = row * vocab + word.
-__device__ __forceinline__ bool before(double s, int32_t at, double s2, int32_t at2) { return s > s2 || (s == s2 && at < at2); }
+__device__ __forceinline__ Key key_of(double sum) {
+  const long long b = __double_as_longlong(sum + 0.0);      // (-0 counts as 0)
+  return b ^ ((b >> 63) & 0x7fffffffffffffffll);
+}
+__device__ __forceinline__ double sum_of_key(Key k) { return __longlong_as_double(k ^ ((k >> 63) & 0x7fffffffffffffffll)); }
+// A candidate is its key and `at` = row * vocab + word.
+__device__ __forceinline__ bool before(Key s, int32_t at, Key s2, int32_t at2) { return (s > s2) | ((s == s2) & (at < at2)); }
 // The same among bids, whose index is a bound that two may share: those go by their place in the list, so that ranks are distinct.
-__device__ __forceinline__ bool bid_before(double s, int32_t at, int i, double s2, int32_t at2, int i2) {
-  return s > s2 || (s == s2 && (at < at2 || (at == at2 && i < i2)));
+__device__ __forceinline__ bool bid_before(Key s, int32_t at, int i, Key s2, int32_t at2, int i2) {
+  return (s > s2) | ((s == s2) & ((at < at2) | ((at == at2) & (i < i2))));
 }
 
 struct SelectSmem {
-  float unit_max[kUnits];
-  double unit_sum[kUnits];
+  float unit_max[kMaxC * kWarps];
+  double unit_sum[kMaxC * kWarps];
   double row_lse[kMaxK];         // log of the row's sum, relative to row_max
   float row_max[kMaxK];
   float score[kMaxK];
   int32_t live[kMaxK];           // rows that are read, in order
   uint32_t done_bits, finite_bits, exact_bits, ask_bits;   // per row: finished; score is finite; summed in 64 bits; to be summed so
   int32_t n_live;
-  double bid_sum[kMaxWarps * 8];
-  int32_t bid_at[kMaxWarps * 8];
-  double top_sum[kClusterCtas * (kMaxK + kBeyond)];
-  int32_t top_at[kClusterCtas * (kMaxK + kBeyond)];
-  double bar_sum;
+  Key bid[kWarps * 32];                      // each warp's, in order
+  int32_t bid_at[kWarps * 32];
+  float chunk_max[kWarps][kMaxima];
+  Key top[kMaxC * 32];                       // each CTA's best bids, in order
+  int32_t top_at[kMaxC * 32];
+  Key bar;
   int32_t bar_at;
   int32_t n_list;
-  double list_sum[kMaxList];
+  int32_t n_todo, n_found;
+  uint16_t todo[kWarps * kMaxima];           // chunks to be read again: warp * kMaxima + kept maximum
+  Key found[kMany];
+  int32_t found_at[kMany];
+  Key most[kWarps];
+  int32_t most_at[kWarps];
+  Key list[kMaxList];
   int32_t list_at[kMaxList];
-  double sorted_sum[kSorted];
+  Key sorted[kSorted];
   int32_t sorted_at[kSorted];
 };
 
@@ -88,45 +100,114 @@ struct SelectParams {
   int k, vocab, eos;
 };
 
+// Bytes of x picked by the four digits of `which`; a digit with its 8 set gives eight copies of the byte's top bit.
+__device__ __forceinline__ uint32_t top_bits(uint32_t x, uint32_t which) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, 0, %2;" : "=r"(r) : "r"(x), "r"(which));
+  return r;
+}
+
+template <class T> struct Packed;      // elements in the 32-bit words of a 16-byte vector
+template <> struct Packed<float> {
+  static constexpr uint32_t kNegInf = 0xff800000u;
+  static constexpr int kPer = 1;
+  static __device__ __forceinline__ void get(uint32_t w, float (&x)[1]) { x[0] = __uint_as_float(w); }
+  static __device__ __forceinline__ float max4(uint4 r) { return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w))); }
+  static __device__ __forceinline__ uint32_t bits(float x) { return __float_as_uint(x); }
+};
+template <> struct Packed<__nv_bfloat16> {
+  static constexpr uint32_t kNegInf = 0xff80ff80u;
+  static constexpr int kPer = 2;
+  static __device__ __forceinline__ void get(uint32_t w, float (&x)[2]) { x[0] = __uint_as_float(w << 16); x[1] = __uint_as_float(w & 0xffff0000u); }
+  static __device__ __forceinline__ float max4(uint4 r) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ uint32_t bits(__nv_bfloat16 x) { return __bfloat16_as_ushort(x); }
+};
+template <> struct Packed<__half> {
+  static constexpr uint32_t kNegInf = 0xfc00fc00u;
+  static constexpr int kPer = 2;
+  static __device__ __forceinline__ void get(uint32_t w, float (&x)[2]) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    x[0] = f.x;
+    x[1] = f.y;
+  }
+  static __device__ __forceinline__ float max4(uint4 r) {
+    const __half2* h = reinterpret_cast<const __half2*>(&r);
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ uint32_t bits(__half x) { return __half_as_ushort(x); }
+};
+
 // A row as 16-byte vectors counted from the boundary at or before its first element.
 template <class T>
 struct Row {
-  static constexpr int E = 16 / sizeof(T);
+  static constexpr int E = 16 / sizeof(T), P = Packed<T>::kPer;
   const T* p;
   const uint32_t* allowed;
-  int vocab, shift, n_vecs, n_words;
+  int vocab, shift, n_vecs, whole0, whole1;      // vectors whole0 .. whole1 - 1 lie in the row from end to end
 
   __device__ Row(const T* p_, int vocab_, const uint32_t* allowed_) : p(p_), allowed(allowed_), vocab(vocab_) {
     shift = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
     n_vecs = (int)(((int64_t)vocab + shift + E - 1) / E);
-    n_words = (vocab + 31) / 32;
+    whole0 = shift != 0;
+    whole1 = (int)(((int64_t)vocab + shift) / E);
   }
-  __device__ bool whole(int v) const { return v * (int64_t)E >= shift && (v + 1) * (int64_t)E <= (int64_t)vocab + shift; }
+  __device__ bool whole(int v) const { return v >= whole0 && v < whole1; }
   __device__ bool may(int at) const { return !allowed || ((__ldg(allowed + (at >> 5)) >> (at & 31)) & 1); }
+  __device__ static uint4 nothing() { return make_uint4(Packed<T>::kNegInf, Packed<T>::kNegInf, Packed<T>::kNegInf, Packed<T>::kNegInf); }
+  // Vector v as it lies there, if all of it belongs to the row.
   __device__ uint4 raw(int v) const { return __ldg(reinterpret_cast<const uint4*>(p + ((int64_t)v * E - shift))); }
-  // Elements of vector v, -inf for what lies outside the row or is not allowed.
-  __device__ void elements(int v, bool is_whole, uint4 r, float (&x)[E]) const {
+  // The same with -inf for what lies outside the row or is not allowed.
+  __device__ uint4 clean(int v, bool is_whole, uint4 r) const {
+    uint32_t w[4] = {r.x, r.y, r.z, r.w};
     const int first = v * E - shift;
     if (is_whole) {
-      const T* e = reinterpret_cast<const T*>(&r);
+      if (!allowed) return r;
+      uint32_t bits;
+      if (shift == 0) {
+        bits = __ldg(reinterpret_cast<const uint8_t*>(allowed) + (first >> 3)) >> (first & 7);
+      } else {
+        const int at = first >> 5;
+        bits = __funnelshift_r(__ldg(allowed + at), (first & 31) + E > 32 ? __ldg(allowed + at + 1) : 0u, first & 31);
+      }
 #pragma unroll
-      for (int i = 0; i < E; ++i) x[i] = to_float(e[i]);
-      if (allowed) {
-        const int w = first >> 5;
-        const uint32_t lo = __ldg(allowed + w), hi = (first & 31) + E > 32 ? __ldg(allowed + w + 1) : 0u;
-        const uint32_t bits = __funnelshift_r(lo, hi, first & 31);
+      for (int h = 0; h < E / 4; ++h) {
+        // four bits to the tops of four bytes, and those over the elements' width
+        const uint32_t tops = ((bits >> (4 * h)) & 15) * 0x10204080u;
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = (bits >> i) & 1 ? x[i] : -INFINITY;
+        for (int i = 0; i < 4 / P; ++i) {
+          const uint32_t keep = top_bits(tops, P == 1 ? 0x8888 + 0x1111 * i : 0x9988 + 0x2222 * i);
+          uint32_t& x = w[h * (4 / P) + i];
+          x = (x & keep) | (Packed<T>::kNegInf & ~keep);
+        }
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int at = first + i;
-        x[i] = at >= 0 && at < vocab && may(at) ? to_float(p[at]) : -INFINITY;
+      for (int i = 0; i < 4; ++i) {
+        w[i] = Packed<T>::kNegInf;
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+          const int at = first + i * P + e;
+          if (at >= 0 && at < vocab && may(at)) {
+            const uint32_t b = Packed<T>::bits(p[at]);
+            w[i] = P == 1 ? b : e == 0 ? (w[i] & 0xffff0000u) | b : (w[i] & 0xffffu) | b << 16;
+          }
+        }
       }
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
+
+// A float as an integer that is ordered alike.
+__device__ __forceinline__ int ordered(float x) {
+  const int b = __float_as_int(x + 0.f);
+  return b ^ ((b >> 31) & 0x7fffffff);
+}
 
 __device__ __forceinline__ float exp2_of(float x) {
   float y;
@@ -139,13 +220,13 @@ __device__ __forceinline__ float exp2_of(float x) {
 // addition and one change of the maximum.
 __device__ __forceinline__ double row_error(int chunks) { return 4.2e-6 + 4.5e-7 * chunks; }
 
-template <class T>
-__global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kMaxWarps * 32, 1) select_kernel(const SelectParams<T> a) {
-  constexpr int E = Row<T>::E;
+template <class T, int C>
+__global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectParams<T> a) {
+  constexpr int E = Row<T>::E, kUnits = C * kWarps;
   __shared__ SelectSmem s;
   cg::cluster_group cluster = cg::this_cluster();
-  const int cta = (int)cluster.block_rank(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
-  const int sent = blockIdx.x / kClusterCtas, k = a.k, need = k + kBeyond;
+  const int cta = (int)cluster.block_rank(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int sent = blockIdx.x / C, k = a.k, need = k + kBeyond;
 
   cluster.barrier_arrive();        // (waited for before the first write into another CTA's memory: all of them run by then)
   if (warp == 0) {
@@ -162,8 +243,8 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kMaxWarps
   __syncthreads();
 
   // Units: (live row, stretch), dealt to the cluster's CTAs in turn so that every CTA has a part of every row.
-  const int n_live = s.n_live, per_row = n_live ? kClusterCtas * warps / n_live : 1;
-  const int unit = warp * kClusterCtas + cta;
+  const int n_live = s.n_live, per_row = n_live ? kUnits / n_live : 1;
+  const int unit = warp * C + cta;
   const bool busy = unit < per_row * n_live;
   const int row = busy ? s.live[unit / per_row] : 0, part = busy ? unit % per_row : 0;
   const Row<T> r(a.logits + sent * a.stride_n + row * a.stride_k, a.vocab, a.allowed ? a.allowed + sent * a.allowed_stride : nullptr);
@@ -172,27 +253,34 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kMaxWarps
   // 1. the stretch, once
   float top = -INFINITY, sum = 0.f;
   int top_vec = 0;                       // first vector of the warp's chunk that the lane's maximum is in
-  for (int vb = v0; vb < v1; vb += kChunkVecs) {
+  const int n_chunks = (v1 - v0 + kChunkVecs - 1) / kChunkVecs;
+  const int most_chunks = ((a.vocab / E + 2) / per_row + kChunkVecs) / kChunkVecs;      // of any stretch of the sentence
+  int group = 0;                         // chunks of a kept maximum, as a power of 2
+  while ((most_chunks - 1) >> group >= kMaxima) ++group;
+  for (int c = 0; c < n_chunks; ++c) {
+    const int vb = v0 + c * kChunkVecs;
     uint4 raw[4];
-    bool whole[4];
+    float m;
+    if (vb >= r.whole0 && vb + kChunkVecs <= min(v1, r.whole1)) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int v = vb + lane + 32 * j;
-      whole[j] = v < v1 && r.whole(v);
-      raw[j] = whole[j] ? r.raw(v) : make_uint4(0, 0, 0, 0);
-    }
-    float x[4][E], m = -INFINITY;
+      for (int j = 0; j < 4; ++j) raw[j] = r.raw(vb + lane + 32 * j);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int v = vb + lane + 32 * j;
-      if (v < v1) {
-        r.elements(v, whole[j], raw[j], x[j]);
-      } else {
+      for (int j = 0; j < 4; ++j) raw[j] = r.clean(vb + lane + 32 * j, true, raw[j]);
+    } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[j][i] = -INFINITY;
+      for (int j = 0; j < 4; ++j) {
+        const int v = vb + lane + 32 * j;
+        const bool whole = v < v1 && r.whole(v);
+        raw[j] = whole ? r.raw(v) : r.nothing();
+        if (v < v1) raw[j] = r.clean(v, whole, raw[j]);
       }
-#pragma unroll
-      for (int i = 0; i < E; ++i) m = fmaxf(m, x[j][i]);
+    }
+    m = fmaxf(fmaxf(Packed<T>::max4(raw[0]), Packed<T>::max4(raw[1])), fmaxf(Packed<T>::max4(raw[2]), Packed<T>::max4(raw[3])));
+    const int chunk_max = __reduce_max_sync(~0u, ordered(m));
+    if (lane == 0) {
+      float* const slot = &s.chunk_max[warp][c >> group];
+      const float cm = __int_as_float(chunk_max ^ ((chunk_max >> 31) & 0x7fffffff));
+      *slot = c & ((1 << group) - 1) ? fmaxf(*slot, cm) : cm;
     }
     if (m > top) {
       sum *= exp2_of((top - m) * kLog2e);
@@ -203,9 +291,15 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kMaxWarps
     float part_sum[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+      const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
       part_sum[j] = 0.f;
 #pragma unroll
-      for (int i = 0; i < E; ++i) part_sum[j] += exp2_of((x[j][i] - base) * kLog2e);
+      for (int i = 0; i < 4; ++i) {
+        float x[Packed<T>::kPer];
+        Packed<T>::get(w[i], x);
+#pragma unroll
+        for (int e = 0; e < Packed<T>::kPer; ++e) part_sum[j] += exp2_of((x[e] - base) * kLog2e);
+      }
     }
     sum += (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
   }
@@ -217,40 +311,45 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kMaxWarps
 #pragma unroll
   for (int o = 16; o; o >>= 1) wsum += __shfl_xor_sync(~0u, wsum, o);
   cluster.barrier_wait();
-  if (busy && lane < kClusterCtas) {
+  if (busy && lane < C) {
     SelectSmem* to = cluster.map_shared_rank(&s, lane);
     to->unit_max[unit] = wtop;
     to->unit_sum[unit] = (double)wsum;
   }
   cluster.sync();
 
-  // The four lanes' bid: the largest maximum, and of equal ones the first chunk.
-  float bid = top;
-  int bid_vec = top_vec;
-#pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    const float b2 = __shfl_xor_sync(~0u, bid, o);
-    const int v2 = __shfl_xor_sync(~0u, bid_vec, o);
-    if (b2 > bid || (b2 == bid && v2 < bid_vec)) { bid = b2; bid_vec = v2; }
-  }
-  const int four = lane >> 2, four_lane = lane & 3;
+  // The lanes' bids, best first: by the largest logit, of equal ones by the bound of its index.  All of a warp's are of one row, so that
+  // their order holds whatever the normaliser.
   const int row_base = row * a.vocab;
-  const int bid_first = row_base + max(0, (bid_vec + 4 * four) * E - r.shift);
-  const int bid_last = row_base + min(a.vocab - 1, (bid_vec + 4 * four + 3 + 96) * E + E - 1 - r.shift);
+  uint64_t lane_bid = (uint64_t)((uint32_t)ordered(top) ^ 0x80000000u) << 32 | (uint32_t)~(row_base + min(a.vocab - 1, (top_vec + lane + 96) * E + E - 1 - r.shift));
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int o = size >> 1; o; o >>= 1) {
+      const uint64_t other = __shfl_xor_sync(~0u, lane_bid, o);
+      const bool larger_first = ((lane & size) == 0) == ((lane & o) == 0);
+      lane_bid = (lane_bid > other) == larger_first ? lane_bid : other;
+    }
+  const int best_bits = (int)((uint32_t)(lane_bid >> 32) ^ 0x80000000u), best_at = (int)~(uint32_t)lane_bid;
+  const float best = __int_as_float(best_bits ^ ((best_bits >> 31) & 0x7fffffff));
   const double near = 2 * row_error((a.vocab / E + 2) / (per_row * kChunkVecs) + 2);
   SelectSmem* const lead = cluster.map_shared_rank(&s, 0);
 
-  // Normalisers of the rows that this CTA's thread `tid` looks after, from the units' sums.
-  if (tid < n_live) {
+  // The rows' normalisers from the units' sums, a warp for each.
+  for (int i = warp; i < n_live; i += kWarps) {
     float m = -INFINITY;
-    for (int i = 0; i < per_row; ++i) m = fmaxf(m, s.unit_max[tid * per_row + i]);
+    for (int u = lane; u < per_row; u += 32) m = fmaxf(m, s.unit_max[i * per_row + u]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
     double t = 0.0;
-    for (int i = 0; i < per_row; ++i) {
-      const int u = tid * per_row + i;
+    for (int u = i * per_row + lane; u < (i + 1) * per_row; u += 32)
       t += s.unit_max[u] == -INFINITY ? s.unit_sum[u] : s.unit_sum[u] * exp((double)s.unit_max[u] - (double)m);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
+    if (lane == 0) {
+      s.row_max[s.live[i]] = m;
+      s.row_lse[s.live[i]] = m == -INFINITY ? (double)NAN : log(t);
     }
-    s.row_max[s.live[tid]] = m;
-    s.row_lse[s.live[tid]] = m == -INFINITY ? (double)NAN : log(t);
   }
   __syncthreads();
 
@@ -258,91 +357,165 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kMaxWarps
     // 2. bids and the bar
     const double score = busy ? s.score[row] : 0.0, base = busy ? s.row_max[row] : 0.0, lse = busy ? s.row_lse[row] : 0.0;
     auto sum_of = [&](float x) { return score + (((double)x - base) - lse); };
-    double bid_sum = busy && bid != -INFINITY ? sum_of(bid) : kNone;
-    if (!(bid_sum > kNone)) bid_sum = kNone;              // a row without a normaliser (NaN, +inf, nothing allowed) bids nothing
-    const int bid_at = bid_sum == kNone ? 0x7fffffff : bid_last;
-    if (four_lane == 0) { s.bid_sum[warp * 8 + four] = bid_sum; s.bid_at[warp * 8 + four] = bid_at; }
-    if (tid == 0) s.n_list = 0;
-    __syncthreads();
+    const double best_sum = busy && best != -INFINITY ? sum_of(best) : (double)NAN;
+    const Key bid = best_sum == best_sum ? key_of(best_sum) : kNone;       // a row without a normaliser (NaN, +inf, nothing allowed) bids nothing
+    int bid_at = bid == kNone ? 0x7fffffff : best_at;
     {
-      int rank = 0;
-      for (int i = four_lane; i < warps * 8; i += 4) rank += bid_before(s.bid_sum[i], s.bid_at[i], i, bid_sum, bid_at, warp * 8 + four);
-      rank += __shfl_xor_sync(~0u, rank, 1);
-      rank += __shfl_xor_sync(~0u, rank, 2);
-      if (rank < need) {
-        for (int c = four_lane; c < kClusterCtas; c += 4) {
-          SelectSmem* to = cluster.map_shared_rank(&s, c);
-          to->top_sum[cta * need + rank] = bid_sum;
-          to->top_at[cta * need + rank] = bid_at;
+      // Logits that differ may give equal sums (1e-20 and 2e-20): among those the bounds have to rise too, and a larger bound is one as well.
+      const Key prev = __shfl_up_sync(~0u, bid, 1);
+      const int prev_at = __shfl_up_sync(~0u, bid_at, 1);
+      if (__any_sync(~0u, lane && prev == bid && prev_at > bid_at)) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const Key k2 = __shfl_up_sync(~0u, bid, o);
+          const int a2 = __shfl_up_sync(~0u, bid_at, o);
+          if (lane >= o && k2 == bid) bid_at = max(bid_at, a2);
         }
+      }
+    }
+    // The CTA's 32 best: two sorted lists' are the larger of each pair from opposite ends, put in order by five exchanges.
+    Key mine = bid;
+    int mine_at = bid_at;
+    for (int left = kWarps; left > 1; left = (left + 1) / 2) {
+      const int half = (left + 1) / 2;
+      if (warp >= half && warp < left) { s.bid[tid] = mine; s.bid_at[tid] = mine_at; }
+      __syncthreads();
+      if (warp + half < left) {
+        const int j = (warp + half) * 32 + 31 - lane;
+        const Key k2 = s.bid[j];
+        const int a2 = s.bid_at[j];
+        if (before(k2, a2, mine, mine_at)) { mine = k2; mine_at = a2; }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+          const Key k3 = __shfl_xor_sync(~0u, mine, o);
+          const int a3 = __shfl_xor_sync(~0u, mine_at, o);
+          if (before(k3, a3, mine, mine_at) == ((lane & o) == 0)) { mine = k3; mine_at = a3; }
+        }
+      }
+    }
+    if (tid == 0) s.n_list = s.n_todo = s.n_found = 0;
+    if (warp == 0) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        SelectSmem* to = cluster.map_shared_rank(&s, c);
+        to->top[cta * 32 + lane] = mine;
+        to->top_at[cta * 32 + lane] = mine_at;
       }
     }
     cluster.sync();
-    const int n_top = kClusterCtas * need;
-    for (int b0 = 0; b0 < n_top; b0 += blockDim.x / 2) {        // two threads a bid
-      const int b = min(b0 + (tid >> 1), n_top - 1);
-      const double bs = s.top_sum[b];
+    // A thread counts, by bisection, what one CTA's list has before one bid of all.
+    const int len = min(need, 32);
+    for (int t0 = 0; t0 < C * C * len; t0 += kWarps * 32) {
+      const int n = min(t0 + tid, C * C * len - 1) / C, b = n / len * 32 + n % len, in = tid % C;
+      const Key bk = s.top[b];
       const int ba = s.top_at[b];
-      int rank = 0;
-      for (int j = tid & 1; j < n_top; j += 2) rank += bid_before(s.top_sum[j], s.top_at[j], j, bs, ba, b);
-      rank += __shfl_xor_sync(~0u, rank, 1);
-      if (rank == need - 1) { s.bar_sum = bs; s.bar_at = ba; }
+      int lo = 0, hi = len;                  // entries before lo are before the bid, those from hi on are not
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1, j = in * 32 + mid;
+        if (bid_before(s.top[j], s.top_at[j], j, bk, ba, b)) lo = mid + 1; else hi = mid;
+      }
+#pragma unroll
+      for (int o = 1; o < C; o <<= 1) lo += __shfl_xor_sync(~0u, lo, o);
+      if (lo == need - 1) { s.bar = bk; s.bar_at = ba; }
     }
     __syncthreads();
 
-    // 3. the stretches whose bid reaches the bar
-    const double bar_sum = s.bar_sum;
+    // 3. the chunks whose maximum can reach the bar, shared out among the CTA's warps: most are of one or two rows
+    const Key bar = s.bar;
     const int bar_at = s.bar_at;
-    // Calls found(sum, at) for what the lane holds of four f's candidates that reach the bar: of two chunks a turn, a vector a lane.
-    auto sweep = [&](int f, auto&& found) {
-      for (int vb = v0; vb < v1; vb += 2 * kChunkVecs) {
-        const int c = lane & 15, v = vb + (lane >> 4) * kChunkVecs + 4 * f + (c & 3) + 32 * (c >> 2);
-        if (v >= v1) continue;
-        float x[E];
-        const bool whole = r.whole(v);
-        r.elements(v, whole, whole ? r.raw(v) : make_uint4(0, 0, 0, 0), x);
+    // What an element of a row has to be to come near the bar, with room for the roundings on the way: spares the others the 64-bit sum.
+    auto floor_of = [&](double sc, double ls, double bs) {
+      if (bar == kNone) return -INFINITY;
+      const double lowest = sum_of_key(bar) - sc + ls + bs;
+      return (float)(lowest - 1e-6 * (1.0 + fabs(lowest) + fabs(sc) + fabs(ls) + fabs(bs)));
+    };
+    if (__shfl_sync(~0u, bid, 0) != kNone) {           // (a warp's best bid is its best candidate's sum)
+      const float floor_x = floor_of(score, lse, base);
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-          if (x[i] == -INFINITY) continue;
-          const int at = row_base + v * E - r.shift + i;
-          const double c_sum = sum_of(x[i]);
-          if (!before(bar_sum, bar_at, c_sum, at)) found(c_sum, at);
+      for (int h = 0; h < kMaxima / 32; ++h) {
+        const int g = lane + 32 * h;
+        const float cm = g << group < n_chunks ? s.chunk_max[warp][g] : -INFINITY;
+        if (cm >= floor_x && cm != -INFINITY) s.todo[atomicAdd(&s.n_todo, 1)] = (uint16_t)(warp * kMaxima + g);
+      }
+    }
+    __syncthreads();
+    const int n_todo = s.n_todo;
+    // Calls found(hit, key, at) for the elements of the warp's share that come near, every lane together.
+    auto sweep = [&](auto&& found) {
+      for (int i = warp; i < n_todo; i += kWarps) {
+        const int w = s.todo[i] / kMaxima, g = s.todo[i] % kMaxima, u = w * C + cta, rw = s.live[u / per_row], pt = u % per_row;
+        const Row<T> q(a.logits + sent * a.stride_n + rw * a.stride_k, a.vocab, r.allowed);
+        const int q0 = (int)((int64_t)q.n_vecs * pt / per_row), q1 = (int)((int64_t)q.n_vecs * (pt + 1) / per_row);
+        const double sc = s.score[rw], bs = s.row_max[rw], ls = s.row_lse[rw];
+        const float floor_x = floor_of(sc, ls, bs);
+        const int c1 = min((g + 1) << group, (q1 - q0 + kChunkVecs - 1) / kChunkVecs);
+        for (int c = g << group; c < c1; ++c) {
+          const int vb = q0 + c * kChunkVecs + lane;
+          uint4 raw[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) raw[j] = vb + 32 * j < q1 && q.whole(vb + 32 * j) ? q.raw(vb + 32 * j) : q.nothing();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int v = vb + 32 * j;
+            if (v < q1) raw[j] = q.clean(v, q.whole(v), raw[j]);
+            if (!__any_sync(~0u, Packed<T>::max4(raw[j]) >= floor_x)) continue;
+            const uint32_t word[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) {
+              float x[Packed<T>::kPer];
+              Packed<T>::get(word[i4], x);
+#pragma unroll
+              for (int e = 0; e < Packed<T>::kPer; ++e) {
+                const bool close = x[e] >= floor_x && x[e] != -INFINITY;
+                const int at = rw * a.vocab + v * E - q.shift + i4 * Packed<T>::kPer + e;
+                const Key key = close ? key_of(sc + (((double)x[e] - bs) - ls)) : kNone;
+                if (close && !before(bar, bar_at, key, at)) found(key, at);
+              }
+            }
+          }
         }
       }
     };
-    auto put = [&](double c_sum, int at) {
-      const int slot = atomicAdd(&lead->n_list, 1);
-      if (slot < kMaxList - kMaxK) { lead->list_sum[slot] = c_sum; lead->list_at[slot] = at; }
-    };
-    uint32_t todo = __ballot_sync(~0u, four_lane == 0 && bid_sum > kNone && !before(bar_sum, bar_at, bid_sum, bid_first));
-    while (todo) {
-      const int f = (__ffs(todo) - 1) >> 2;
-      todo &= todo - 1;
-      int n = 0;
-      sweep(f, [&](double, int) { ++n; });
-      n = __reduce_add_sync(~0u, n);
-      if (n <= 32) {
-        sweep(f, put);
-        continue;
+    sweep([&](Key key, int at) {
+      const int slot = atomicAdd(&s.n_found, 1);
+      if (slot < kMany) { s.found[slot] = key; s.found_at[slot] = at; }
+    });
+    __syncthreads();
+    const int n_found = s.n_found;
+    if (n_found <= kMany) {
+      if (warp == 0) {
+        int first = 0;
+        if (lane == 0 && n_found) first = atomicAdd(&lead->n_list, n_found);
+        first = __shfl_sync(~0u, first, 0);
+        for (int i = lane; i < n_found; i += 32) { lead->list[first + i] = s.found[i]; lead->list_at[first + i] = s.found_at[i]; }
       }
-      double prev_sum = 0.0;                 // many (equal or sorted logits): the best `need` of them, one by one
+    } else {
+      Key prev = kNone;                      // many (equal or sorted logits): the best `need` of them, one by one
       int prev_at = 0;
       for (int turn = 0; turn < need; ++turn) {
-        double best_sum = kNone;
-        int best_at = 0x7fffffff;
-        sweep(f, [&](double c_sum, int at) {
-          if ((turn == 0 || before(prev_sum, prev_at, c_sum, at)) && before(c_sum, at, best_sum, best_at)) { best_sum = c_sum; best_at = at; }
+        Key most = kNone;
+        int most_at = 0x7fffffff;
+        sweep([&](Key key, int at) {
+          if ((turn == 0 || before(prev, prev_at, key, at)) && before(key, at, most, most_at)) { most = key; most_at = at; }
         });
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
-          const double s2 = __shfl_xor_sync(~0u, best_sum, o);
-          const int a2 = __shfl_xor_sync(~0u, best_at, o);
-          if (before(s2, a2, best_sum, best_at)) { best_sum = s2; best_at = a2; }
+          const Key k2 = __shfl_xor_sync(~0u, most, o);
+          const int a2 = __shfl_xor_sync(~0u, most_at, o);
+          if (before(k2, a2, most, most_at)) { most = k2; most_at = a2; }
         }
-        if (best_sum == kNone) break;
-        if (lane == 0) put(best_sum, best_at);
-        prev_sum = best_sum;
-        prev_at = best_at;
+        if (lane == 0) { s.most[warp] = most; s.most_at[warp] = most_at; }
+        __syncthreads();
+        for (int w = 0; w < kWarps; ++w)
+          if (before(s.most[w], s.most_at[w], most, most_at)) { most = s.most[w]; most_at = s.most_at[w]; }
+        if (tid == 0) {
+          const int slot = atomicAdd(&lead->n_list, 1);
+          lead->list[slot] = most;
+          lead->list_at[slot] = most_at;
+        }
+        prev = most;
+        prev_at = most_at;
+        __syncthreads();
       }
     }
     cluster.sync();
@@ -350,40 +523,36 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kMaxWarps
     // 4. the order
     int n_sorted = 0;
     if (cta == 0) {
-      if (warp == 0) {
-        const int n = min(s.n_list, kMaxList - kMaxK);
-        const uint32_t ended = s.done_bits & s.finite_bits;
-        __syncwarp();
-        if ((ended >> lane) & 1) {
-          const int slot = n + __popc(ended & ((1u << lane) - 1));
-          s.list_sum[slot] = s.score[lane];
-          s.list_at[slot] = lane * a.vocab + a.eos;
-        }
-        if (lane == 0) s.n_list = n + __popc(ended);
+      const int n_listed = s.n_list;
+      const uint32_t ended = s.done_bits & s.finite_bits;
+      const int n = n_listed + __popc(ended);
+      if (warp == 0 && ((ended >> lane) & 1)) {
+        const int slot = n_listed + __popc(ended & ((1u << lane) - 1));
+        s.list[slot] = key_of((double)s.score[lane]);
+        s.list_at[slot] = lane * a.vocab + a.eos;
       }
       __syncthreads();
-      const int n = s.n_list;
       n_sorted = min(n, kSorted);
-      for (int i = tid; i < n; i += blockDim.x) {
-        const double cs = s.list_sum[i];
+      for (int i = tid; i < n; i += kWarps * 32) {
+        const Key ck = s.list[i];
         const int ca = s.list_at[i];
         int rank = 0;
-        for (int j = 0; j < n; ++j) rank += before(s.list_sum[j], s.list_at[j], cs, ca);
-        if (rank < kSorted) { s.sorted_sum[rank] = cs; s.sorted_at[rank] = ca; }
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) rank += before(s.list[j], s.list_at[j], ck, ca);
+        if (rank < kSorted) { s.sorted[rank] = ck; s.sorted_at[rank] = ca; }
       }
       __syncthreads();
       if (warp == 0) {
         // Pair i = sorted i and i + 1.  The first pair from the k-th on that is not near closes the order: what comes behind it cannot be
         // among the k best.  A near pair of two rows before that, one of them summed in 32 bits, has to be settled.
-        uint32_t near_bits[2], ask = 0;
-        uint32_t unsure_bits[2];
+        uint32_t near_bits[2], unsure_bits[2], ask = 0;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int i = lane + 32 * h;
           bool is_near = false, unsure = false;
           if (i + 1 < n_sorted) {
             const uint32_t r1 = s.sorted_at[i] / a.vocab, r2 = s.sorted_at[i + 1] / a.vocab;
-            is_near = s.sorted_sum[i] - s.sorted_sum[i + 1] < near;
+            is_near = sum_of_key(s.sorted[i]) - sum_of_key(s.sorted[i + 1]) < near;
             unsure = is_near && r1 != r2 && !((s.exact_bits >> r1) & (s.exact_bits >> r2) & 1);
           }
           near_bits[h] = __ballot_sync(~0u, is_near);
@@ -399,9 +568,9 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kMaxWarps
           if ((matter >> i) & 1) ask |= (1u << (s.sorted_at[i] / a.vocab)) | (1u << (s.sorted_at[i + 1] / a.vocab));
         }
         ask = __reduce_or_sync(~0u, ask);
-        if (close >= n_sorted - 1 && n_sorted >= k && bar_sum > kNone) ask = ~0u;      // the list ends before the order is closed
+        if (close >= n_sorted - 1 && n_sorted >= k && bar != kNone) ask = ~0u;      // the list ends before the order is closed
         ask &= s.finite_bits & ~s.exact_bits;
-        if (lane < kClusterCtas) cluster.map_shared_rank(&s, lane)->ask_bits = ask;
+        if (lane < C) cluster.map_shared_rank(&s, lane)->ask_bits = ask;
       }
     }
     cluster.sync();
@@ -413,7 +582,7 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kMaxWarps
         const int at = some ? s.sorted_at[tid] : 0, parent = some ? at / a.vocab : tid, token = some ? at - parent * a.vocab : a.eos;
         a.out_tokens[o] = token;
         a.out_parents[o] = parent;
-        a.out_scores[o] = some ? (float)s.sorted_sum[tid] : -INFINITY;
+        a.out_scores[o] = some ? (float)sum_of_key(s.sorted[tid]) : -INFINITY;
         if (a.out_done) a.out_done[o] = !some || ((s.done_bits >> parent) & 1) || token == a.eos;
       }
       return;
@@ -427,13 +596,16 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kMaxWarps
         if (r.may(at)) t += exp((double)to_float(r.p[at]) - base);
 #pragma unroll
       for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
-      if (lane < kClusterCtas) cluster.map_shared_rank(&s, lane)->unit_sum[unit] = t;
+      if (lane < C) cluster.map_shared_rank(&s, lane)->unit_sum[unit] = t;
     }
     cluster.sync();
-    if (tid < n_live && ((ask >> s.live[tid]) & 1)) {
+    for (int i = warp; i < n_live; i += kWarps) {
+      if (!((ask >> s.live[i]) & 1)) continue;
       double t = 0.0;
-      for (int i = 0; i < per_row; ++i) t += s.unit_sum[tid * per_row + i];
-      s.row_lse[s.live[tid]] = log(t);
+      for (int u = lane; u < per_row; u += 32) t += s.unit_sum[i * per_row + u];
+#pragma unroll
+      for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
+      if (lane == 0) s.row_lse[s.live[i]] = log(t);
     }
     if (tid == 0) s.exact_bits |= ask;
     __syncthreads();
@@ -441,11 +613,24 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kMaxWarps
 }
 
 template <class T>
-cudaError_t launch_select(const linmt_beam_select_args& g, int warps) {
+cudaError_t launch_select(const linmt_beam_select_args& g) {
   SelectParams<T> p{static_cast<const T*>(g.logits), g.stride_n, g.stride_k, g.scores, g.done, g.allowed, g.allowed_stride,
                     g.out_tokens, g.out_parents, g.out_scores, g.out_done, g.k, g.vocab, g.eos};
-  select_kernel<T><<<dim3((unsigned)g.n * kClusterCtas), dim3(warps * 32), 0, static_cast<cudaStream_t>(g.stream)>>>(p);
-  return cudaGetLastError();
+  // As many CTAs for a sentence as leave every sentence on the GPU at once (two CTAs on an SM, clusters of 8 only reach 33): a second
+  // round of clusters costs its latencies, some 6 us, again.  24 warps of 2 CTAs have a row each for 24 beams at most.
+  const int c = g.n <= 33 ? 8 : g.n <= 74 || g.k > 2 * kWarps ? 4 : 2;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = c;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)g.n * c);
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.stream = static_cast<cudaStream_t>(g.stream);
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, c == 8 ? select_kernel<T, 8> : c == 4 ? select_kernel<T, 4> : select_kernel<T, 2>, p);
+  return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
 // ---- reordering --------------------------------------------------------------------------------
@@ -522,13 +707,7 @@ int linmt_beam_select(const linmt_beam_select_args* g) {
   if (g->n == 0) return LINMT_OK;
   OnDevice on(g->device);
   if (on.err != cudaSuccess) return op_cuda(on.err, "beam_select");
-  // Warps of a CTA: as many as leave the fewest without a stretch when every beam is live (12 beams: 96 of 8 x 12).
-  int warps = kMaxWarps, most = 0;
-  for (int w = kMaxWarps; w >= kMaxWarps / 2; --w) {
-    const int used = kClusterCtas * w / g->k * g->k * 1000 / (kClusterCtas * w);
-    if (used > most) { most = used; warps = w; }
-  }
-  const cudaError_t e = g->dtype == LINMT_F32 ? launch_select<float>(*g, warps) : g->dtype == LINMT_BF16 ? launch_select<__nv_bfloat16>(*g, warps) : launch_select<__half>(*g, warps);
+  const cudaError_t e = g->dtype == LINMT_F32 ? launch_select<float>(*g) : g->dtype == LINMT_BF16 ? launch_select<__nv_bfloat16>(*g) : launch_select<__half>(*g);
   return e == cudaSuccess ? LINMT_OK : op_cuda(e, "beam_select");
 }
 

@@ -130,6 +130,23 @@ def test_select_ties_go_to_the_lowest_index(ops, k, v, dtype):
             select_check(ops, x, scores)
 
 
+@pytest.mark.parametrize("n,k,v", [(1, 12, 30000), (80, 5, 9001), (50, 9, 4003), (80, 31, 1500)])
+def test_select_one_beam_ahead(ops, n, k, v):
+    """All that is chosen lies in one row, in few of its places, or in logits too small to tell apart; for one sentence and for so many that each has few CTAs."""
+    rng = _rng(n, k, v, 3)
+    x = _logits(rng, n, k, v, F16)
+    scores = torch.full((n, k), -50.0, device="cuda")
+    ahead = _cuda(rng.integers(0, k, (n, 1)))
+    scores.scatter_(1, ahead, -1.0)
+    select_check(ops, x, scores)
+    order = x.sort(dim=2, descending=True).values          # the best words next to each other
+    select_check(ops, order, scores)
+    select_check(ops, order, torch.zeros_like(scores))
+    tiny = _cuda((rng.normal(0, 1, (n, k, v)) * 1e-20).astype(np.float32))
+    select_check(ops, tiny, scores)
+    select_check(ops, tiny, torch.zeros_like(scores))
+
+
 @pytest.mark.parametrize("v", [1000, 30000])
 def test_select_between_beams_closer_than_32_bits(ops, v):
     """Rows that are permutations of each other under scores one step of 32 bits apart: candidates 1e-6 apart, and 2.4e-7 at smaller scores, which a 32-bit
