@@ -1,0 +1,433 @@
+// device_ops_torch.cpp -- the operators on device tensors for torch: checks a call's tensors, fills the argument struct of the C ABI, allocates
+// what was not given, and calls.  In C++ because a step's calls are shorter than the same checks in Python take (20 to 40 us a call there, 3 to 7
+// here).  What each function takes and returns is described in linmt_b200/device_ops.py, which passes its arguments on in order.
+#include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cmath>
+#include <string>
+#include <vector>
+
+#include "../../include/linmt_decoder.h"
+
+namespace {
+
+using at::Tensor;
+PyObject* g_error = nullptr;       // linmt_b200.decoder.LinmtError
+
+#define NEED(ok, ...) TORCH_CHECK_VALUE(ok, __VA_ARGS__)
+
+const Tensor& tensor(PyObject* o, const char* name) {
+  NEED(THPVariable_Check(o), name, " has to be a CUDA tensor");
+  return THPVariable_Unpack(o);
+}
+const Tensor& on_cuda(PyObject* o, const char* name) {
+  const Tensor& t = tensor(o, name);
+  NEED(t.is_cuda() && t.layout() == at::kStrided, name, " has to be a CUDA tensor");
+  return t;
+}
+const Tensor& on_device(PyObject* o, const char* name, int dev) {
+  const Tensor& t = on_cuda(o, name);
+  NEED(t.get_device() == dev, name, " has to be a tensor on CUDA device ", dev);
+  return t;
+}
+// A contiguous tensor of the given type and shape on the call's device.
+const Tensor& dense(PyObject* o, const char* name, int dev, at::ScalarType type, at::IntArrayRef shape) {
+  const Tensor& t = on_device(o, name, dev);
+  NEED(t.scalar_type() == type, name, " has to be ", type, ", not ", t.scalar_type());
+  NEED(t.sizes() == shape, name, " has to have the shape ", shape, ", not ", t.sizes());
+  NEED(t.is_contiguous(), name, " has to be contiguous");
+  return t;
+}
+uint8_t* flags(PyObject* o, const char* name, int dev, at::IntArrayRef shape) {
+  const Tensor& t = on_device(o, name, dev);
+  NEED(t.scalar_type() == at::kBool || t.scalar_type() == at::kByte, name, " has to be a bool or uint8 tensor");
+  return static_cast<uint8_t*>(dense(o, name, dev, t.scalar_type(), shape).data_ptr());
+}
+int dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? LINMT_F32 : t.scalar_type() == at::kBFloat16 ? LINMT_BF16 : t.scalar_type() == at::kHalf ? LINMT_F16 : -1; }
+int int32_of(int64_t v, const char* name) {
+  NEED(v >= INT32_MIN && v <= INT32_MAX, name, " = ", v, " is too large");
+  return (int)v;
+}
+int64_t integer(PyObject* o, const char* name) {
+  PyObject* i = PyNumber_Index(o);
+  if (!i) throw python_error();
+  const long long v = PyLong_AsLongLong(i);
+  Py_DECREF(i);
+  if (v == -1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    NEED(false, name, " is too large");
+  }
+  return v;
+}
+double real(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+Tensor make(at::IntArrayRef shape, at::ScalarType type, int dev) { return Tensor(at::detail::empty_cuda(shape, type, c10::Device(at::kCUDA, (c10::DeviceIndex)dev), std::nullopt)); }
+void* stream_of(int dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
+void done_or_raise(int rc) {
+  if (rc == LINMT_OK) return;
+  NEED(rc != LINMT_EINVAL && rc != LINMT_ELIMIT, linmt_op_error());
+  PyErr_Format(g_error, "%s (%d)", linmt_op_error(), rc);
+  throw python_error();
+}
+void arguments(Py_ssize_t got, Py_ssize_t want) { TORCH_CHECK_TYPE(got == want, "takes ", want, " arguments, got ", got); }
+// Two places of a tensor that is written share no memory, as far as strides of 0 say.
+bool apart(const Tensor& t) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) == 0) return false;
+  return true;
+}
+
+PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  arguments(n_args, 6);
+  const Tensor& logits = on_cuda(a[0], "logits");
+  const int dev = logits.get_device();
+  NEED(logits.dim() == 3 && dtype_of(logits) >= 0, "logits have to be [n, k, vocab] in float32, bfloat16 or float16");
+  const int64_t n = logits.size(0), k = logits.size(1), v = logits.size(2);
+  NEED(v >= 1 && (logits.stride(2) == 1 || v == 1), "the words of a row of logits have to be contiguous");
+  const int64_t shape[2] = {n, k};
+  linmt_beam_select_args g{};
+  g.size = sizeof(g);
+  g.device = dev;
+  g.logits = logits.data_ptr();
+  g.stride_n = logits.stride(0);
+  g.stride_k = logits.stride(1);
+  g.scores = static_cast<const float*>(dense(a[1], "scores", dev, at::kFloat, shape).data_ptr());
+  if (a[2] != Py_None) g.done = flags(a[2], "done", dev, shape);
+  if (a[3] != Py_None) {
+    const Tensor& allowed = on_device(a[3], "allowed", dev);
+    const int64_t words = (v + 31) / 32;
+    NEED(allowed.dim() == 2 && (allowed.size(0) == 1 || allowed.size(0) == n), "allowed has to be [1 or n, ceil(vocab / 32)]");
+    const int64_t want[2] = {allowed.size(0), words};
+    g.allowed = static_cast<const uint32_t*>(dense(a[3], "allowed", dev, at::kInt, want).data_ptr());
+    g.allowed_stride = allowed.size(0) == 1 ? 0 : words;
+  }
+  g.n = int32_of(n, "n");
+  g.k = int32_of(k, "k");
+  g.vocab = int32_of(v, "vocab");
+  g.eos = int32_of(integer(a[4], "eos"), "eos");
+  g.dtype = dtype_of(logits);
+  Tensor t[4];
+  if (a[5] == Py_None) {
+    t[0] = make(shape, at::kInt, dev);
+    t[1] = make(shape, at::kInt, dev);
+    t[2] = make(shape, at::kFloat, dev);
+    t[3] = make(shape, at::kBool, dev);
+  } else {
+    NEED(PyTuple_Check(a[5]) && PyTuple_GET_SIZE(a[5]) == 4, "out has to be (tokens, parents, scores, done)");
+    t[0] = dense(PyTuple_GET_ITEM(a[5], 0), "out[0]", dev, at::kInt, shape);
+    t[1] = dense(PyTuple_GET_ITEM(a[5], 1), "out[1]", dev, at::kInt, shape);
+    t[2] = dense(PyTuple_GET_ITEM(a[5], 2), "out[2]", dev, at::kFloat, shape);
+    flags(PyTuple_GET_ITEM(a[5], 3), "out[3]", dev, shape);
+    t[3] = THPVariable_Unpack(PyTuple_GET_ITEM(a[5], 3));
+    NEED(n * k == 0 || t[0].data_ptr() != t[1].data_ptr(), "out[0] and out[1] are one tensor");
+  }
+  g.out_tokens = static_cast<int32_t*>(t[0].data_ptr());
+  g.out_parents = static_cast<int32_t*>(t[1].data_ptr());
+  g.out_scores = static_cast<float*>(t[2].data_ptr());
+  g.out_done = static_cast<uint8_t*>(t[3].data_ptr());
+  if (n) {
+    g.stream = stream_of(dev);
+    done_or_raise(linmt_beam_select(&g));
+  }
+  if (a[5] != Py_None) {
+    Py_INCREF(a[5]);
+    return a[5];
+  }
+  PyObject* r = PyTuple_New(4);
+  if (!r) throw python_error();
+  for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(r, i, THPVariable_Wrap(std::move(t[i])));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+struct Strides { int64_t layers, l, n, k, row; };      // in bytes; row: bytes of one
+
+Strides strides_of(const Tensor& x, int64_t n, int64_t k, const char* what, Py_ssize_t i) {
+  const int64_t d = x.dim(), size = x.element_size();
+  NEED(d >= 2 && d <= 4, what, "[", i, "] has to be [n, k], [n, k, width] or [layers, n, k, width]");
+  const int f = d == 4;
+  NEED(x.size(f) == n && x.size(f + 1) == k, what, "[", i, "] has to have the sentences and beams of parents, not ", x.sizes());
+  const int64_t width = d == 2 ? 1 : x.size(d - 1);
+  NEED(d == 2 || width <= 1 || x.stride(d - 1) == 1, "the rows of ", what, "[", i, "] have to be contiguous");
+  return {f ? x.size(0) : 1, f ? x.stride(0) * size : 0, x.stride(f) * size, x.stride(f + 1) * size, width * size};
+}
+// First byte, and the one behind the last.
+std::pair<const char*, const char*> span(const Tensor& x) {
+  int64_t last = 0;
+  for (int64_t i = 0; i < x.dim(); ++i) last += (x.size(i) - 1) * x.stride(i);
+  const char* p = static_cast<const char*>(x.data_ptr());
+  return {p, p + (last + 1) * x.element_size()};
+}
+
+PyObject* beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  arguments(n_args, 3);
+  const Tensor& parents = on_cuda(a[1], "parents");
+  const int dev = parents.get_device();
+  NEED(parents.dim() == 2, "parents have to be [n, k]");
+  const int64_t n = parents.size(0), k = parents.size(1);
+  dense(a[1], "parents", dev, at::kInt, parents.sizes());
+  NEED(PyList_Check(a[0]) && PyList_Check(a[2]) && PyList_GET_SIZE(a[0]) == PyList_GET_SIZE(a[2]), "out has to have a tensor for every state");
+  linmt_beam_reorder_args g;
+  g.size = sizeof(g);
+  g.device = dev;
+  g.stream = stream_of(dev);
+  g.parents = static_cast<const int32_t*>(parents.data_ptr());
+  g.n = int32_of(n, "n");
+  g.k = int32_of(k, "k");
+  g.reserved = 0;
+  const Py_ssize_t all = PyList_GET_SIZE(a[0]);
+  std::vector<linmt_beam_state> states;
+  states.reserve((size_t)all);
+  for (Py_ssize_t i = 0; i < all; ++i) {
+    PyObject *ox = PyList_GET_ITEM(a[0], i), *oy = PyList_GET_ITEM(a[2], i);
+    const Tensor &x = on_device(ox, "states", dev), &y = on_device(oy, "out", dev);
+    const Strides s = strides_of(x, n, k, "states", i);
+    Strides d = s;
+    if (oy != ox) {
+      NEED(y.scalar_type() == x.scalar_type() && y.sizes() == x.sizes(), "out[", i, "] has to be like states[", i, "]");
+      d = strides_of(y, n, k, "out", i);
+    }
+    if (x.numel() == 0) continue;
+    NEED(apart(y), "out[", i, "] has rows that share memory");
+    if (oy != ox) {
+      const auto from = span(x), to = span(y);
+      NEED(to.first >= from.second || from.first >= to.second || (from == to && s.l == d.l && s.n == d.n && s.k == d.k), "out[", i, "] overlaps states[", i, "]");
+    }
+    const auto to = span(y), by = span(parents);
+    NEED(to.first >= by.second || by.first >= to.second, "out[", i, "] overlaps parents");
+    for (const linmt_beam_state& before : states) NEED(before.dst != y.data_ptr(), "out[", i, "] is written twice");
+    states.push_back({x.data_ptr(), y.data_ptr(), s.l, s.n, s.k, d.l, d.n, d.k, s.row, s.layers});
+  }
+  for (size_t i = 0; i < states.size(); i += 16) {
+    g.n_states = (int)std::min<size_t>(16, states.size() - i);
+    std::copy(states.begin() + i, states.begin() + i + g.n_states, g.state);
+    done_or_raise(linmt_beam_reorder(&g));
+  }
+  Py_INCREF(a[2]);
+  return a[2];
+  END_HANDLE_TH_ERRORS
+}
+
+// A table [n][width] of int32 with contiguous rows.
+const Tensor& table_of(PyObject* o, int dev, int64_t n) {
+  const Tensor& t = on_device(o, "table", dev);
+  NEED(t.scalar_type() == at::kInt && t.dim() == 2 && t.size(0) == n, "table has to be [n, width] int32");
+  NEED(t.size(1) <= 1 || t.stride(1) == 1, "the rows of table have to be contiguous");
+  return t;
+}
+
+PyObject* plan_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  arguments(n_args, 7);
+  const Tensor& now = on_cuda(a[1], "new");
+  const int dev = now.get_device();
+  NEED(now.dim() == 1, "new has to be [n]");
+  const int64_t n = now.size(0), shape[1] = {n}, one[1] = {1}, total = integer(a[6], "total");
+  linmt_plan_pages_args g{};
+  g.size = sizeof(g);
+  g.device = dev;
+  g.stream = stream_of(dev);
+  g.new_len = static_cast<const int32_t*>(dense(a[1], "new", dev, at::kInt, shape).data_ptr());
+  if (a[0] != Py_None) g.old_len = static_cast<const int32_t*>(dense(a[0], "old", dev, at::kInt, shape).data_ptr());
+  const Tensor& table = table_of(a[2], dev, n);
+  NEED(table.stride(0) >= table.size(1) || n <= 1, "the rows of table share memory");
+  g.table = static_cast<int32_t*>(table.data_ptr());
+  g.table_stride = table.stride(0);
+  const Tensor& free = on_device(a[3], "free", dev);
+  NEED(free.dim() == 1, "free has to be [n_free]");
+  g.free_pages = static_cast<const int32_t*>(dense(a[3], "free", dev, at::kInt, free.sizes()).data_ptr());
+  g.used = static_cast<const int32_t*>(dense(a[4], "used", dev, at::kInt, one).data_ptr());
+  NEED(total >= 0, "total is negative");
+  g.n = int32_of(n, "n");
+  g.width = int32_of(table.size(1), "width");
+  g.page = int32_of(integer(a[5], "page"), "page");
+  g.n_free = int32_of(free.size(0), "n_free");
+  g.total = total;
+  Tensor slots = make({total}, at::kLong, dev), starts = make({n + 1}, at::kInt, dev), used = make(one, at::kInt, dev);
+  g.out_slots = static_cast<int64_t*>(slots.data_ptr());
+  g.out_starts = static_cast<int32_t*>(starts.data_ptr());
+  g.out_used = static_cast<int32_t*>(used.data_ptr());
+  done_or_raise(linmt_plan_pages(&g));
+  PyObject* r = PyTuple_New(3);
+  if (!r) throw python_error();
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(slots)));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(starts)));
+  PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(std::move(used)));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+linmt_pages4 pool_of(PyObject* o, int dev) {
+  const Tensor& p = on_device(o, "pages", dev);
+  NEED(p.scalar_type() == at::kByte && p.dim() == 4 && p.size(3) % 18 == 0, "pages have to be uint8 [n_pages, heads, page / 16, 18 * dim]");
+  NEED(p.stride(3) == 1 && (p.stride(2) == p.size(3) || p.size(2) == 1), "the tiles of a page's head have to be contiguous");
+  return {p.data_ptr(), p.stride(0), p.stride(1), int32_of(p.size(0), "n_pages"), int32_of(p.size(1), "heads"), int32_of(p.size(2) * 16, "page"), int32_of(p.size(3) / 18, "dim")};
+}
+
+int64_t slots_of(PyObject* o, int dev, linmt_pages4_rows_args& g) {
+  const Tensor& slots = on_cuda(o, "slots");
+  NEED(slots.dim() == 1, "slots have to be [t]");
+  g.slots = static_cast<const int64_t*>(dense(o, "slots", dev, at::kLong, slots.sizes()).data_ptr());
+  g.t = int32_of(slots.size(0), "t");
+  return slots.size(0);
+}
+void rows_of(const Tensor& x, const char* name, const linmt_pages4_rows_args& g, void*& p, int64_t& t, int64_t& h) {
+  const int64_t want[3] = {g.t, g.pages.heads, g.pages.dim};
+  NEED(dtype_of(x) == g.dtype && g.dtype >= 0, name, " has to be float32, bfloat16 or float16, k and v alike");
+  NEED(x.sizes() == at::IntArrayRef(want), name, " has to have the shape ", at::IntArrayRef(want), ", not ", x.sizes());
+  NEED(x.stride(2) == 1, "the components of ", name, " have to be contiguous");
+  p = x.data_ptr();
+  t = x.stride(0);
+  h = x.stride(1);
+}
+
+PyObject* write_pages4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  arguments(n_args, 4);
+  const int dev = on_cuda(a[1], "slots").get_device();
+  linmt_pages4_rows_args g{};
+  g.size = sizeof(g);
+  g.device = dev;
+  g.stream = stream_of(dev);
+  g.pages = pool_of(a[0], dev);
+  slots_of(a[1], dev, g);
+  const Tensor &k = on_device(a[2], "k", dev), &v = on_device(a[3], "v", dev);
+  g.dtype = dtype_of(k);
+  rows_of(k, "k", g, g.k, g.k_stride_t, g.k_stride_h);
+  rows_of(v, "v", g, g.v, g.v_stride_t, g.v_stride_h);
+  done_or_raise(linmt_write_pages4(&g));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* read_pages4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  arguments(n_args, 3);
+  const int dev = on_cuda(a[1], "slots").get_device();
+  linmt_pages4_rows_args g{};
+  g.size = sizeof(g);
+  g.device = dev;
+  g.stream = stream_of(dev);
+  g.pages = pool_of(a[0], dev);
+  const int64_t shape[3] = {slots_of(a[1], dev, g), g.pages.heads, g.pages.dim};
+  const int64_t type = integer(a[2], "dtype");
+  NEED(type >= 0 && type <= 2, "dtype has to be float32, bfloat16 or float16");
+  const at::ScalarType st = type == LINMT_F32 ? at::kFloat : type == LINMT_BF16 ? at::kBFloat16 : at::kHalf;
+  Tensor k = make(shape, st, dev), v = make(shape, st, dev);
+  g.dtype = (int)type;
+  rows_of(k, "k", g, g.k, g.k_stride_t, g.k_stride_h);
+  rows_of(v, "v", g, g.v, g.v_stride_t, g.v_stride_h);
+  done_or_raise(linmt_read_pages4(&g));
+  PyObject* r = PyTuple_New(2);
+  if (!r) throw python_error();
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(k)));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(v)));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* attend_pages4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  arguments(n_args, 12);
+  const Tensor& q = on_cuda(a[0], "q");
+  const int dev = q.get_device();
+  linmt_attend_pages4_args g{};
+  g.size = sizeof(g);
+  g.device = dev;
+  g.stream = stream_of(dev);
+  g.pages = pool_of(a[1], dev);
+  g.dtype = dtype_of(q);
+  NEED(q.dim() == 4 && g.dtype >= 0 && q.size(3) == g.pages.dim, "q has to be [n, g, heads, ", g.pages.dim, "] in float32, bfloat16 or float16");
+  NEED(q.stride(3) == 1, "the components of q have to be contiguous");
+  const int64_t n = q.size(0), rows = q.size(1), heads = q.size(2), by_n[1] = {n}, by_head[1] = {heads}, by_row[2] = {n, rows}, by_all[3] = {n, rows, heads};
+  g.n = int32_of(n, "n");
+  g.g = int32_of(rows, "g");
+  g.heads = int32_of(heads, "heads");
+  g.q = q.data_ptr();
+  g.q_stride_n = q.stride(0);
+  g.q_stride_g = q.stride(1);
+  g.q_stride_h = q.stride(2);
+  const Tensor& table = table_of(a[2], dev, n);
+  g.table = static_cast<const int32_t*>(table.data_ptr());
+  g.table_stride = table.stride(0);
+  g.width = int32_of(table.size(1), "width");
+  g.len = static_cast<const int32_t*>(dense(a[3], "lens", dev, at::kInt, by_n).data_ptr());
+  g.scale = a[4] == Py_None ? 1.f / std::sqrt((float)g.pages.dim) : (float)real(a[4]);
+  g.cap = (float)real(a[5]);
+  NEED((a[6] == Py_None) == (a[7] == Py_None), "slope goes with centre");
+  NEED((a[8] == Py_None) == (a[9] == Py_None), "first goes with last");
+  if (a[6] != Py_None) {
+    g.slope = static_cast<const float*>(dense(a[6], "slope", dev, at::kFloat, by_head).data_ptr());
+    g.centre = static_cast<const float*>(dense(a[7], "centre", dev, at::kFloat, by_row).data_ptr());
+  }
+  if (a[8] != Py_None) {
+    g.first = static_cast<const int32_t*>(dense(a[8], "first", dev, at::kInt, by_row).data_ptr());
+    g.last = static_cast<const int32_t*>(dense(a[9], "last", dev, at::kInt, by_row).data_ptr());
+  }
+  Tensor out, lse;
+  if (a[10] == Py_None) {
+    out = make(q.sizes(), q.scalar_type(), dev);
+  } else {
+    out = on_device(a[10], "out", dev);
+    NEED(out.scalar_type() == q.scalar_type() && out.sizes() == q.sizes() && out.stride(3) == 1, "out has to be like q, its components contiguous");
+    NEED(apart(out), "out has rows that share memory");
+  }
+  g.out = out.data_ptr();
+  g.out_stride_n = out.stride(0);
+  g.out_stride_g = out.stride(1);
+  g.out_stride_h = out.stride(2);
+  const int want_lse = PyObject_IsTrue(a[11]);
+  if (want_lse < 0) throw python_error();
+  if (want_lse) {
+    lse = make(by_all, at::kFloat, dev);
+    g.lse = static_cast<float*>(lse.data_ptr());
+  }
+  Tensor ws;
+  if (q.numel()) {
+    const int64_t need = linmt_attend_pages4_workspace(&g);
+    NEED(need >= 0, linmt_op_error());
+    if (need) {
+      ws = make({need}, at::kByte, dev);     // goes back to torch's pool of this stream behind the call's kernels
+      g.workspace = ws.data_ptr();
+      g.workspace_bytes = need;
+    }
+    done_or_raise(linmt_attend_pages4(&g));
+  }
+  PyObject* o = a[10];
+  if (o == Py_None) o = THPVariable_Wrap(std::move(out));
+  else Py_INCREF(o);
+  if (!want_lse) return o;
+  PyObject* r = PyTuple_New(2);
+  if (!r) { Py_DECREF(o); throw python_error(); }
+  PyTuple_SET_ITEM(r, 0, o);
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(lse)));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
+PyCFunction fast() { return reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(F)); }
+
+}  // namespace
+
+extern "C" __attribute__((visibility("default"))) PyObject* PyInit__device_ops() {
+  static PyMethodDef methods[] = {{"beam_select", fast<beam_select>(), METH_FASTCALL, nullptr}, {"beam_reorder", fast<beam_reorder>(), METH_FASTCALL, nullptr},
+                                  {"plan_pages", fast<plan_pages>(), METH_FASTCALL, nullptr},   {"write_pages4", fast<write_pages4>(), METH_FASTCALL, nullptr},
+                                  {"read_pages4", fast<read_pages4>(), METH_FASTCALL, nullptr}, {"attend_pages4", fast<attend_pages4>(), METH_FASTCALL, nullptr},
+                                  {nullptr, nullptr, 0, nullptr}};
+  static PyModuleDef module = {PyModuleDef_HEAD_INIT, "_device_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+  PyObject* decoder = PyImport_ImportModule("linmt_b200.decoder");
+  if (!decoder) return nullptr;
+  g_error = PyObject_GetAttrString(decoder, "LinmtError");
+  Py_DECREF(decoder);
+  return g_error ? PyModule_Create(&module) : nullptr;
+}

@@ -274,7 +274,7 @@ def test_reorder_refuses(ops):
     a = x[:, :4]
     for bad in (lambda: ops.beam_reorder([a], parents.long()), lambda: ops.beam_reorder([a], parents, out=[x[:, 2:6]]), lambda: ops.beam_reorder([a, a], parents),
                 lambda: ops.beam_reorder([x], parents), lambda: ops.beam_reorder([a.transpose(1, 2)[:, :2].transpose(1, 2)[:, :4, :2].transpose(0, 1)], parents),
-                lambda: ops.beam_reorder([x[:, :1].expand(2, 4, 64)], parents), lambda: ops.beam_reorder([a], parents, out=[a.to(F16)]), lambda: ops.beam_reorder([a], parents, out=[]),
+                lambda: ops.beam_reorder([x[:, :1].expand(2, 4, 64)], parents), lambda: ops.beam_reorder([a], parents, out=[a.to(F16)]), lambda: ops.beam_reorder([a], parents, out=[]), lambda: ops.beam_reorder([parents], parents),
                 lambda: ops.beam_reorder([torch.zeros(2, 40, 4, device="cuda")], torch.zeros(2, 40, dtype=torch.int32, device="cuda"))):
         with pytest.raises((ValueError, RuntimeError)):
             bad()
