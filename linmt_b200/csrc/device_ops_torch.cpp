@@ -284,7 +284,7 @@ void rows_of(const Tensor& x, const char* name, const linmt_pages4_rows_args& g,
   const int64_t want[3] = {g.t, g.pages.heads, g.pages.dim};
   NEED(dtype_of(x) == g.dtype && g.dtype >= 0, name, " has to be float32, bfloat16 or float16, k and v alike");
   NEED(x.sizes() == at::IntArrayRef(want), name, " has to have the shape ", at::IntArrayRef(want), ", not ", x.sizes());
-  NEED(x.stride(2) == 1, "the components of ", name, " have to be contiguous");
+  NEED(x.stride(2) == 1 || x.numel() == 0, "the components of ", name, " have to be contiguous");
   p = x.data_ptr();
   t = x.stride(0);
   h = x.stride(1);
@@ -347,7 +347,7 @@ PyObject* attend_pages4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   g.pages = pool_of(a[1], dev);
   g.dtype = dtype_of(q);
   NEED(q.dim() == 4 && g.dtype >= 0 && q.size(3) == g.pages.dim, "q has to be [n, g, heads, ", g.pages.dim, "] in float32, bfloat16 or float16");
-  NEED(q.stride(3) == 1, "the components of q have to be contiguous");
+  NEED(q.stride(3) == 1 || q.numel() == 0, "the components of q have to be contiguous");
   const int64_t n = q.size(0), rows = q.size(1), heads = q.size(2), by_n[1] = {n}, by_head[1] = {heads}, by_row[2] = {n, rows}, by_all[3] = {n, rows, heads};
   g.n = int32_of(n, "n");
   g.g = int32_of(rows, "g");

@@ -5,12 +5,18 @@
 // A sentence's beams, and the query heads that share a head of the pool, read the same positions: up to 16 rows are the left
 // operand of mma.m16n8k16, so every code is loaded and unpacked once for all of them.  (tcgen05.mma wants both operands of at least 64
 // rows, and codes unpacked into shared memory first; with 16 rows the unpacking, not the product, is what takes the time.)
-//   Scales stay out of the products: a key's is multiplied onto its group's sum, a value's into the weight on the left, and
-//   the codes minus 8 are exact in bf16 and fp16.  So 16-bit queries lose nothing against the 4-bit values as they stand.
-//   Weights are rounded to bf16 once for bf16 queries (2^-8 each at most, on average over the positions far less, and the output's own
-//   rounding is as large); for fp16 they are taken as two bf16 terms (2^-16), for fp32 weights and queries as three (2^-24).
+//   Scales stay out of the products: a key's is multiplied onto its group's sum, a value's into the weight on the left.
+//   16-bit queries (attend16_kernel).  A word's codes become matrix operands with one AND each: an integer in the low bits of a
+//   bf16 or fp16 number is a subnormal one, that integer times 2^-133 or 2^-24, and stays so up to 255 and 2047, so every second
+//   code may be left four bits up and its 16 taken out elsewhere (of the queries before, of the output's columns after).  What is then too much, 8 for each
+//   code, goes off by a product of its own: the queries' sums with the keys' scales, and the weights' sums.  That is 5
+//   instructions for 8 codes where a code minus 8 in normal form takes 11, in a kernel bound by what it can issue.  Queries are scaled to
+//   fp16's upper range by a power of 2 for each row, weights by one for each warp (after the first values' scale), so that nothing that matters
+//   falls out of range.  Weights are rounded to bf16 once for bf16 queries (2^-8 each at most, on average over the positions far less, and the output's
+//   own rounding is as large); for fp16 they are taken as two bf16 terms (2^-16).
+//   32-bit queries (attend32_kernel) are three bf16 terms, the weights too (2^-24), the codes minus 8 in normal form.
 // Every warp has a ring of tiles of its own (cp.async, no barrier among warps) and its own maximum and sums; the CTA's four are
-// joined through shared memory at the end, and where a sentence's positions are split over CTAs a second kernel joins those.
+// joined through shared memory at the end of a piece of work, and where a sentence's positions are shared by CTAs a second kernel joins those.
 #include <atomic>
 
 #include "device_ops.h"
@@ -21,10 +27,15 @@ namespace ops {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kStages = 4;
+constexpr int kStages = 4;         // of attend32_kernel: tiles
+constexpr int kPairStages = 3;     // of attend16_kernel: pairs of tiles
 constexpr int kRows = 16;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kTerms = 3;          // bf16 terms of a 32-bit query and weight
 constexpr float kSlack = 8.f;      // the reference maximum follows the true one only when it lags by 2^8: few tiles rescale the sums
+
+template <class T> struct Fp16 { static constexpr bool value = false; };
+template <> struct Fp16<__half> { static constexpr bool value = true; };
 
 struct AttendParams {
   const unsigned char* data;
@@ -43,14 +54,10 @@ struct AttendParams {
   const int32_t* first;
   const int32_t* last;
   float* ws;
-  int32_t n, g, heads, rep, width, row_tiles, splits;
+  int32_t n, g, heads, rep, width, row_tiles;
   float scale, cap;
+  int32_t q_wide, o_wide;    // the rows of q are 16-byte aligned; fours of components of out are aligned to their size
 };
-
-template <class T> struct Terms;
-template <> struct Terms<__nv_bfloat16> { static constexpr int q = 1, p = 1; };
-template <> struct Terms<__half> { static constexpr int q = 1, p = 2; };
-template <> struct Terms<float> { static constexpr int q = 3, p = 3; };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -59,6 +66,15 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint4& a, uint32_t
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+// The same onto nothing.
+__device__ __forceinline__ void mma_bf16_first(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -69,18 +85,11 @@ __device__ __forceinline__ uint32_t lop_and_or(uint32_t x, uint32_t m, uint32_t 
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(m), "r"(o));
   return r;
 }
-// Codes i (low half) and i + 4 (high half) of a word, minus 8.  An integer below 128 laid into the low bits of 128.0 (bf16) or 1024.0 (fp16) adds
-// itself to it.
+// Codes i (low half) and i + 4 (high half) of a word, minus 8.  An integer below 128 laid into the low bits of 128.0 adds itself to it.
 template <int I>
 __device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {
   const uint32_t b = lop_and_or(w >> (4 * I), 0x000f000fu, 0x43004300u), off = 0x43084308u;      // 128 + code, 136
   __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&off));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
-template <int I>
-__device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
-  const uint32_t b = lop_and_or(w >> (4 * I), 0x000f000fu, 0x64006400u), off = 0x64086408u;      // 1024 + code, 1032
-  __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&off));
   return *reinterpret_cast<uint32_t*>(&r);
 }
 __device__ __forceinline__ float bf16_low(uint32_t x) { return __uint_as_float(x << 16); }
@@ -90,307 +99,202 @@ __device__ __forceinline__ float exp2_of(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-template <class T> __device__ __forceinline__ float tanh_of(float x) {
-  // 1 - 2 / (e^2x + 1), good to 2e-7 of 1: what a 16-bit result can see of it.
-  const float e = exp2_of(x * (2 * kLog2e));
-  return 1.f - __fdividef(2.f, e + 1.f);
-}
-template <> __device__ __forceinline__ float tanh_of<float>(float x) { return tanhf(x); }
+// tanh as 1 - 2 / (e^2x + 1), good to 2e-7 of 1: what a 16-bit result can see of it.
+__device__ __forceinline__ float tanh_of(float x) { return 1.f - __fdividef(2.f, exp2_of(x * (2 * kLog2e)) + 1.f); }
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// The kernel behind this one may be launched now; it waits for this one's end before it reads (join's wait_for_last).
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Four components of row `at` of a sentence's head of the pool, and with the first the log of its weight.
+template <class T>
+__device__ __forceinline__ void write_row(const AttendParams& a, int sent, int kvh, int at, int d, const float4& sum, float top, float weight) {
+  const int g = at / a.rep, h = kvh * a.rep + at - g * a.rep;
+  const float f = weight > 0.f ? 1.f / weight : 0.f;
+  T* const to = static_cast<T*>(a.out) + sent * a.o_n + g * a.o_g + h * a.o_h + d;
+  struct alignas(4 * sizeof(T)) Four { T v[4]; };
+  const Four v{{from_float<T>(sum.x * f), from_float<T>(sum.y * f), from_float<T>(sum.z * f), from_float<T>(sum.w * f)}};
+  if (a.o_wide) {
+    *reinterpret_cast<Four*>(to) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i] = v.v[i];
+  }
+  if (d == 0 && a.lse) a.lse[((int64_t)sent * a.g + g) * a.heads + h] = weight > 0.f ? (top + log2f(weight)) * 0.69314718055994531f : -INFINITY;
+}
+
+// ---- who does what
+//
+// The work is a list of pairs of tiles (32 positions): sentence by sentence, in each by head of the pool and row tile (a segment), a segment's
+// pairs in order.  It is cut into as many equal parts as CTAs fit on the GPU at once, each of at least kLeast pairs: a segment
+// longer than a part is then shared by several CTAs, whose parts the join kernel adds up, and a CTA may have several short ones.  Lengths
+// are known on the device only, so every CTA adds them up itself.  A short segment counts as kLeast pairs, its fixed costs being as large, and
+// segments of up to kLeast pairs or an eighth of a part are not cut: the CTA that has their first pair takes them whole.
+constexpr int kLeast = 8;
+struct Share {
+  int64_t begin, end;      // the CTA's pairs
+  int64_t first;           // number of the first pair of sentence `sent`
+  int64_t per;             // pairs of a part
+  int sent, whole;         // sentence of `begin`; segments of up to `whole` pairs are not cut
+};
+__device__ __forceinline__ int length_of(const AttendParams& a, int sent) {
+  return min(max(__ldg(a.len + sent), 0), (int)min((int64_t)a.width * a.page, (int64_t)0x7fffffff));
+}
+__device__ __forceinline__ int pairs_of(const AttendParams& a, int sent) { return max(kLeast, (int)(((int64_t)length_of(a, sent) + 31) / 32)); }
+
+// Share of block `blockIdx.x` of `blocks`; all threads of the CTA (a multiple of 32, at most 128) call it.
+__device__ __forceinline__ Share share_of(const AttendParams& a, int blocks) {
+  __shared__ int64_t sums[4];
+  __shared__ int64_t found_first;
+  __shared__ int found_sent;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, segments = a.pool_heads * a.row_tiles;
+  const int each = (a.n + threads - 1) / threads, i0 = min(a.n, tid * each), i1 = min(a.n, i0 + each);
+  int64_t mine = 0;
+  for (int i = i0; i < i1; ++i) mine += pairs_of(a, i);
+  int64_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(~0u, upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < threads / 32; ++w) {
+    if (w == warp) upto += total;
+    total += sums[w];
+  }
+  Share s;
+  s.per = max((int64_t)kLeast, (total * segments + blocks - 1) / blocks);
+  s.begin = min(total * segments, blockIdx.x * s.per);
+  s.end = min(total * segments, s.begin + s.per);
+  s.whole = (int)min((int64_t)0x7fffffff, max((int64_t)kLeast, s.per / 8));
+  if (i0 < i1 && s.begin >= (upto - mine) * segments && s.begin < upto * segments) {
+    int64_t before = (upto - mine) * segments;
+    int i = i0;
+    for (;; ++i) {
+      const int64_t next = before + (int64_t)pairs_of(a, i) * segments;
+      if (s.begin < next) break;
+      before = next;
+    }
+    found_first = before;
+    found_sent = i;
+  }
+  __syncthreads();
+  s.first = found_first;
+  s.sent = found_sent;
+  return s;
+}
+
+// One CTA's piece of a segment.
+struct Piece {
+  int sent, kvh, rt;
+  int p0, p1, pairs;       // pairs p0 .. p1 - 1 of the segment's
+  int64_t start;           // number of the segment's first pair
+};
+// The piece that begins at s.begin; false where the CTA has none left.  Moves s on behind it.
+__device__ __forceinline__ bool next_piece(const AttendParams& a, Share& s, Piece& p) {
+  const int segments = a.pool_heads * a.row_tiles;
+  while (s.begin < s.end) {
+    p.pairs = pairs_of(a, s.sent);
+    const int64_t in = s.begin - s.first, seg = in / p.pairs;
+    if (seg >= segments) {
+      s.first += (int64_t)p.pairs * segments;
+      ++s.sent;
+      continue;
+    }
+    p.sent = s.sent;
+    p.kvh = (int)seg / a.row_tiles;
+    p.rt = (int)seg - p.kvh * a.row_tiles;
+    p.start = s.first + seg * p.pairs;
+    p.p0 = (int)(s.begin - p.start);
+    p.p1 = (int)min((int64_t)p.pairs, s.end - p.start);
+    s.begin = p.start + p.p1;
+    if (p.pairs <= s.whole) {
+      if (p.p0 > 0) {           // the CTA before has all of it
+        s.begin = p.start + p.pairs;
+        continue;
+      }
+      p.p1 = p.pairs;
+      s.begin = p.start + p.pairs;
+    }
+    return true;
+  }
+  return false;
+}
+
 template <class T, int D>
 constexpr int attend_smem() {
-  return kWarps * kStages * 18 * D + (Terms<T>::q > 1 ? Terms<T>::q * (D / 16) * 512 : 0);
+  if constexpr (sizeof(T) == 2) return kWarps * kPairStages * 2 * 18 * D;
+  else return kWarps * kStages * 18 * D + kTerms * (D / 16) * 512;
 }
 
 // The pair of query components that a lane's 32 bits of the left operand hold, as term `term` of their bf16 expansion.
-template <class T>
-__device__ __forceinline__ uint32_t query_pair(const T* row, int d, int term) {
+__device__ __forceinline__ uint32_t query_pair(const float* row, int d, int term) {
   if (!row) return 0u;
-  if constexpr (sizeof(T) == 2) {
-    const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
-    return (uint32_t)__ldg(r + d) | (uint32_t)__ldg(r + d + 4) << 16;
-  } else {
-    float lo = __ldg(row + d), hi = __ldg(row + d + 4);
-    for (int i = 0; i < term; ++i) {
-      lo -= __bfloat162float(__float2bfloat16_rn(lo));
-      hi -= __bfloat162float(__float2bfloat16_rn(hi));
-    }
-    return pack_bf16(lo, hi);
+  float lo = __ldg(row + d), hi = __ldg(row + d + 4);
+  for (int i = 0; i < term; ++i) {
+    lo -= __bfloat162float(__float2bfloat16_rn(lo));
+    hi -= __bfloat162float(__float2bfloat16_rn(hi));
   }
+  return pack_bf16(lo, hi);
 }
 
-template <class T, int D>
-__global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_constant__ AttendParams a) {
-  constexpr int NG = D / 32, kTileBytes = pages4::tile_bytes(D), QT = Terms<T>::q, PT = Terms<T>::p;
-  extern __shared__ __align__(16) unsigned char smem[];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, c = lane & 3;
-  int64_t job = blockIdx.x;
-  const int split = (int)(job % a.splits);
-  job /= a.splits;
-  const int64_t out_tile = job;            // (sentence, head of the pool, row tile)
-  const int rt = (int)(job % a.row_tiles);
-  job /= a.row_tiles;
-  const int kvh = (int)(job % a.pool_heads), sent = (int)(job / a.pool_heads);
-  const int n_rows = min(kRows, a.g * a.rep - rt * kRows);
+// What a piece's rows see.
+struct Job {
+  int n_rows;
+  int lo[2], hi[2];            // the lane's rows gid and gid + 8
+  float slope[2], centre[2];   // their bias, in powers of 2
+  int all_lo, all_hi;          // what all of them see
+  int t0, t1;                  // the piece's tiles
+};
 
-  // The lane's rows gid and gid + 8: query row and head, what they see, their bias.
-  const int cap_len = (int)min((int64_t)a.width * a.page, (int64_t)0x7fffffff), len = min(max(__ldg(a.len + sent), 0), cap_len);
-  const T* q_row[2];
-  int lo[2], hi[2];
-  float slope[2], centre[2];
+template <class T>
+__device__ __forceinline__ Job job_of(const AttendParams& a, const Piece& p, const T* (&q_row)[2]) {
+  Job j;
+  const int gid = (threadIdx.x & 31) >> 2, len = length_of(a, p.sent);
+  j.n_rows = min(kRows, a.g * a.rep - p.rt * kRows);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int r = gid + 8 * i, at = rt * kRows + r, g = at / a.rep, h = kvh * a.rep + at % a.rep;
-    const bool have = r < n_rows;
-    q_row[i] = have ? static_cast<const T*>(a.q) + sent * a.q_n + g * a.q_g + h * a.q_h : nullptr;
-    lo[i] = have ? (a.first ? max(__ldg(a.first + (int64_t)sent * a.g + g), 0) : 0) : 0x7fffffff;
-    hi[i] = have ? (a.last ? min(__ldg(a.last + (int64_t)sent * a.g + g), len) : len) : 0;
-    slope[i] = have && a.slope ? __ldg(a.slope + h) * kLog2e : 0.f;
-    centre[i] = have && a.slope ? __ldg(a.centre + (int64_t)sent * a.g + g) : 0.f;
+    const int r = gid + 8 * i, at = p.rt * kRows + r, g = at / a.rep, h = p.kvh * a.rep + at - g * a.rep;
+    const bool have = r < j.n_rows;
+    q_row[i] = have ? static_cast<const T*>(a.q) + p.sent * a.q_n + g * a.q_g + h * a.q_h : nullptr;
+    j.lo[i] = have ? (a.first ? max(__ldg(a.first + (int64_t)p.sent * a.g + g), 0) : 0) : 0x7fffffff;
+    j.hi[i] = have ? (a.last ? min(__ldg(a.last + (int64_t)p.sent * a.g + g), len) : len) : 0;
+    j.slope[i] = have && a.slope ? __ldg(a.slope + h) * kLog2e : 0.f;
+    j.centre[i] = have && a.slope ? __ldg(a.centre + (int64_t)p.sent * a.g + g) : 0.f;
   }
-  // What any row sees, and what all of them see.
-  int any_lo = lo[0] < hi[0] ? lo[0] : 0x7fffffff, any_hi = lo[0] < hi[0] ? hi[0] : 0;
-  if (lo[1] < hi[1]) { any_lo = min(any_lo, lo[1]); any_hi = max(any_hi, hi[1]); }
-  int all_lo = gid < n_rows ? lo[0] : 0, all_hi = gid < n_rows ? hi[0] : 0x7fffffff;
-  if (gid + 8 < n_rows) { all_lo = max(all_lo, lo[1]); all_hi = min(all_hi, hi[1]); }
-#pragma unroll
-  for (int o = 4; o < 32; o <<= 1) {
-    any_lo = min(any_lo, __shfl_xor_sync(~0u, any_lo, o));
-    any_hi = max(any_hi, __shfl_xor_sync(~0u, any_hi, o));
-    all_lo = max(all_lo, __shfl_xor_sync(~0u, all_lo, o));
-    all_hi = min(all_hi, __shfl_xor_sync(~0u, all_hi, o));
-  }
-  const int tile0 = any_lo < any_hi ? any_lo / pages4::kTile : 0, tile1 = any_lo < any_hi ? (any_hi - 1) / pages4::kTile + 1 : 0;
-  const int per_split = (tile1 - tile0 + a.splits - 1) / a.splits;
-  const int t0 = min(tile1, tile0 + split * per_split), t1 = min(tile1, t0 + per_split);
+  int any_lo = j.lo[0] < j.hi[0] ? j.lo[0] : 0x7fffffff, any_hi = j.lo[0] < j.hi[0] ? j.hi[0] : 0;
+  if (j.lo[1] < j.hi[1]) { any_lo = min(any_lo, j.lo[1]); any_hi = max(any_hi, j.hi[1]); }
+  j.all_lo = gid < j.n_rows ? j.lo[0] : 0;
+  j.all_hi = gid < j.n_rows ? j.hi[0] : 0x7fffffff;
+  if (gid + 8 < j.n_rows) { j.all_lo = max(j.all_lo, j.lo[1]); j.all_hi = min(j.all_hi, j.hi[1]); }
+  any_lo = __reduce_min_sync(~0u, any_lo);
+  any_hi = __reduce_max_sync(~0u, any_hi);
+  j.all_lo = __reduce_max_sync(~0u, j.all_lo);
+  j.all_hi = __reduce_min_sync(~0u, j.all_hi);
+  const bool any = any_lo < any_hi;
+  j.t0 = max(2 * p.p0, any ? any_lo / pages4::kTile & ~1 : 0);
+  j.t1 = max(j.t0, min(2 * p.p1, any ? (any_hi - 1) / pages4::kTile + 1 : 0));
+  return j;
+}
 
-  // Queries as left operands: step (group, half) takes components 32 group + 8 c + 2 half + {0, 4 | 1, 5}.
-  uint4 qa[QT == 1 ? NG * 2 : 1];
-  uint4* const q_smem = reinterpret_cast<uint4*>(smem + kWarps * kStages * kTileBytes);
-  if constexpr (QT == 1) {
-#pragma unroll
-    for (int s = 0; s < NG * 2; ++s) {
-      const int d = 32 * (s >> 1) + 8 * c + 2 * (s & 1);
-      qa[s] = make_uint4(query_pair(q_row[0], d, 0), query_pair(q_row[1], d, 0), query_pair(q_row[0], d + 1, 0), query_pair(q_row[1], d + 1, 0));
-    }
-  } else {
-    for (int s = warp; s < QT * NG * 2; s += kWarps) {
-      const int term = s / (NG * 2), d = 32 * ((s % (NG * 2)) >> 1) + 8 * c + 2 * (s & 1);
-      q_smem[s * 32 + lane] = make_uint4(query_pair(q_row[0], d, term), query_pair(q_row[1], d, term), query_pair(q_row[0], d + 1, term), query_pair(q_row[1], d + 1, term));
-    }
-    __syncthreads();
-  }
-
-  float o[NG][4][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  const float to_log2 = a.cap > 0.f ? a.scale / a.cap : a.scale * kLog2e, cap_log2 = a.cap * kLog2e;
-  unsigned char* const ring = smem + warp * kStages * kTileBytes;
-  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-  const int32_t* const table = a.table + sent * a.table_stride;
-  const unsigned char* const head = a.data + kvh * a.stride_head;
-  const int tiles_per_page = a.page / pages4::kTile;
-  const int mine = t1 - t0 > warp ? (t1 - t0 - warp + kWarps - 1) / kWarps : 0;        // this warp's tiles: t0 + warp + kWarps i
-
-  // Where this warp's tiles are: looked up 32 at a time, one by each lane, a batch ahead of their use.
-  int64_t where = -1;
-  uint32_t bad = 0;                // bit of a stage: it holds no tile of the pool
-  auto fetch = [&](int i) {
-    if ((i & 31) == 0) {
-      where = -1;
-      if (i + lane < mine) where = pages4::tile_offset(table, t0 + warp + kWarps * (i + lane), tiles_per_page, a.n_pages, a.stride_page, D);
-    }
-    const int64_t at = __shfl_sync(~0u, where, i & 31);
-    const int stage = i % kStages;
-    if (i < mine && at >= 0) {
-      bad &= ~(1u << stage);
-#pragma unroll
-      for (int b = 0; b < (kTileBytes + 511) / 512; ++b) {
-        const int byte = b * 512 + lane * 16;
-        if (byte < kTileBytes) copy16(ring_at + stage * kTileBytes + byte, head + at + byte);
-      }
-    } else {
-      bad |= 1u << stage;
-    }
-    copy_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) fetch(i);
-
-  for (int i = 0; i < mine; ++i) {
-    copy_wait<kStages - 2>();
-    __syncwarp();                       // every lane's part of tile i is there, and tile i - 1 has been read by all
-    fetch(i + kStages - 1);
-    if ((bad >> (i % kStages)) & 1) continue;
-    const unsigned char* const tile = ring + (i % kStages) * kTileBytes;
-    const int pos = (t0 + warp + kWarps * i) * pages4::kTile;
-
-    // scores: x[j][0..3] = rows gid, gid, gid + 8, gid + 8 at positions pos + 8 j + 2 c + {0, 1, 0, 1}
-    float x[2][4];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      uint32_t w[NG], sc[NG];
-      const unsigned char* const kw = tile + (8 * j + gid) * (D / 2) + c * (4 * NG);
-      const unsigned char* const ks = tile + pages4::key_scales(D) + (8 * j + 2 * c) * (2 * NG);
-      if constexpr (NG == 4) {
-        *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(kw);
-        *reinterpret_cast<uint4*>(sc) = *reinterpret_cast<const uint4*>(ks);
-      } else {
-        *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(kw);
-        *reinterpret_cast<uint2*>(sc) = *reinterpret_cast<const uint2*>(ks);
-      }
-      x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.f;
-#pragma unroll
-      for (int gr = 0; gr < NG; ++gr) {
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t b[4];
-        if constexpr (sizeof(T) == 2 && QT == 1 && PT == 2) {
-          b[0] = codes_f16<0>(w[gr]); b[1] = codes_f16<1>(w[gr]); b[2] = codes_f16<2>(w[gr]); b[3] = codes_f16<3>(w[gr]);
-          mma_f16(s, qa[2 * gr], b[0], b[1]);
-          mma_f16(s, qa[2 * gr + 1], b[2], b[3]);
-        } else {
-          b[0] = codes_bf16<0>(w[gr]); b[1] = codes_bf16<1>(w[gr]); b[2] = codes_bf16<2>(w[gr]); b[3] = codes_bf16<3>(w[gr]);
-#pragma unroll
-          for (int term = QT - 1; term >= 0; --term) {      // small terms first
-            const uint4 a0 = QT == 1 ? qa[QT == 1 ? 2 * gr : 0] : q_smem[(term * NG * 2 + 2 * gr) * 32 + lane];
-            const uint4 a1 = QT == 1 ? qa[QT == 1 ? 2 * gr + 1 : 0] : q_smem[(term * NG * 2 + 2 * gr + 1) * 32 + lane];
-            mma_bf16(s, a0, b[0], b[1]);
-            mma_bf16(s, a1, b[2], b[3]);
-          }
-        }
-        // scales of position 2 c: halves gr of the first NG, of 2 c + 1: of the second
-        const float s0 = gr & 1 ? bf16_high(sc[gr >> 1]) : bf16_low(sc[gr >> 1]);
-        const float s1 = gr & 1 ? bf16_high(sc[NG / 2 + (gr >> 1)]) : bf16_low(sc[NG / 2 + (gr >> 1)]);
-        x[j][0] = fmaf(s[0], s0, x[j][0]);
-        x[j][1] = fmaf(s[1], s1, x[j][1]);
-        x[j][2] = fmaf(s[2], s0, x[j][2]);
-        x[j][3] = fmaf(s[3], s1, x[j][3]);
-      }
-    }
-    if (a.cap > 0.f) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[j][e] = cap_log2 * tanh_of<T>(x[j][e] * to_log2);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[j][e] *= to_log2;
-    }
-    if (a.slope) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[j][e] -= slope[e >> 1] * fabsf((float)(pos + 8 * j + 2 * c + (e & 1)) - centre[e >> 1]);
-    }
-    const bool edge = pos < all_lo || pos + pages4::kTile > all_hi;
-    if (edge) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int p = pos + 8 * j + 2 * c + (e & 1);
-          if (p < lo[e >> 1] || p >= hi[e >> 1]) x[j][e] = -INFINITY;
-        }
-    }
-    float top[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      top[e] = fmaxf(fmaxf(x[0][2 * e], x[0][2 * e + 1]), fmaxf(x[1][2 * e], x[1][2 * e + 1]));
-      top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], 1));
-      top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], 2));
-    }
-    const bool up0 = top[0] > m[0] + kSlack || (m[0] == -INFINITY && top[0] > -INFINITY), up1 = top[1] > m[1] + kSlack || (m[1] == -INFINITY && top[1] > -INFINITY);
-    if (__any_sync(~0u, up0 || up1)) {
-      const float f0 = up0 ? exp2_of(m[0] - top[0]) : 1.f, f1 = up1 ? exp2_of(m[1] - top[1]) : 1.f;
-      if (up0) m[0] = top[0];
-      if (up1) m[1] = top[1];
-      l[0] *= f0;
-      l[1] *= f1;
-#pragma unroll
-      for (int gr = 0; gr < NG; ++gr)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          o[gr][e][0] *= f0; o[gr][e][1] *= f0;
-          o[gr][e][2] *= f1; o[gr][e][3] *= f1;
-        }
-    }
-    const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      x[j][0] = exp2_of(x[j][0] - m0);
-      x[j][1] = exp2_of(x[j][1] - m0);
-      x[j][2] = exp2_of(x[j][2] - m1);
-      x[j][3] = exp2_of(x[j][3] - m1);
-      l[0] += x[j][0] + x[j][1];
-      l[1] += x[j][2] + x[j][3];
-    }
-
-    // out += weights . values, a group of 32 components a time: its scales go into the weights
-    uint32_t vs[2][NG];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const unsigned char* const at = tile + pages4::value_scales(D) + (8 * j + 2 * c) * (2 * NG);
-      if constexpr (NG == 4) *reinterpret_cast<uint4*>(vs[j]) = *reinterpret_cast<const uint4*>(at);
-      else *reinterpret_cast<uint2*>(vs[j]) = *reinterpret_cast<const uint2*>(at);
-      if (edge) {            // a position that nobody sees may hold anything: 0 times its scale has to be 0
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (x[j][e] == 0.f && x[j][e + 2] == 0.f) {
-#pragma unroll
-            for (int i2 = 0; i2 < NG / 2; ++i2) vs[j][e * (NG / 2) + i2] = 0u;
-          }
-      }
-    }
-#pragma unroll
-    for (int i2 = 0; i2 < NG / 2; ++i2) {
-      const uint4 u = *reinterpret_cast<const uint4*>(tile + pages4::value_codes(D) + 16 * (i2 * 32 + lane));
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int gr = 2 * i2 + h;
-        const uint32_t w0 = h ? u.y : u.x, w1 = h ? u.w : u.z;
-        float p[2][4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float s0 = h ? bf16_high(vs[j][i2]) : bf16_low(vs[j][i2]), s1 = h ? bf16_high(vs[j][NG / 2 + i2]) : bf16_low(vs[j][NG / 2 + i2]);
-          p[j][0] = x[j][0] * s0;
-          p[j][1] = x[j][1] * s1;
-          p[j][2] = x[j][2] * s0;
-          p[j][3] = x[j][3] * s1;
-        }
-        uint4 pa[PT];
-#pragma unroll
-        for (int term = 0; term < PT; ++term) {
-          pa[term] = make_uint4(pack_bf16(p[0][0], p[0][1]), pack_bf16(p[0][2], p[0][3]), pack_bf16(p[1][0], p[1][1]), pack_bf16(p[1][2], p[1][3]));
-          if (term + 1 < PT) {
-            p[0][0] -= bf16_low(pa[term].x); p[0][1] -= bf16_high(pa[term].x);
-            p[0][2] -= bf16_low(pa[term].y); p[0][3] -= bf16_high(pa[term].y);
-            p[1][0] -= bf16_low(pa[term].z); p[1][1] -= bf16_high(pa[term].z);
-            p[1][2] -= bf16_low(pa[term].w); p[1][3] -= bf16_high(pa[term].w);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t b0 = e == 0 ? codes_bf16<0>(w0) : e == 1 ? codes_bf16<1>(w0) : e == 2 ? codes_bf16<2>(w0) : codes_bf16<3>(w0);
-          const uint32_t b1 = e == 0 ? codes_bf16<0>(w1) : e == 1 ? codes_bf16<1>(w1) : e == 2 ? codes_bf16<2>(w1) : codes_bf16<3>(w1);
-#pragma unroll
-          for (int term = PT - 1; term >= 0; --term) mma_bf16(o[gr][e], pa[term], b0, b1);
-        }
-      }
-    }
-  }
-
-  // The warps' parts, joined: their rings are free once all have come here.
+// The CTA's warps' parts, joined and written: sums o (o[group][e][2 r + i] = row gid + 8 r, component 32 group + 8 c + 4 i + e), relative to 2^m, and weights l.
+template <class T, int D>
+__device__ __forceinline__ void join_warps(const AttendParams& a, const Piece& p, const Job& job, unsigned char* smem, const float (&o)[D / 32][4][4], const float (&m)[2], float (&l)[2]) {
+  constexpr int NG = D / 32;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, c = lane & 3;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     l[e] += __shfl_xor_sync(~0u, l[e], 1);
     l[e] += __shfl_xor_sync(~0u, l[e], 2);
   }
   copy_wait<0>();
-  __syncthreads();
+  __syncthreads();                    // the rings are free
   float* const part = reinterpret_cast<float*>(smem);              // [warp][row][D]
   __shared__ float part_m[kWarps][kRows], part_l[kWarps][kRows];
   if (c == 0) {
@@ -401,16 +305,17 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
   for (int gr = 0; gr < NG; ++gr)
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      // columns 2 c and 2 c + 1 of product e are components 8 c + e and 8 c + 4 + e of the group
       float4* const to = reinterpret_cast<float4*>(part + (warp * kRows + gid + 8 * r) * D + 32 * gr + 8 * c);
       to[0] = make_float4(o[gr][0][2 * r], o[gr][1][2 * r], o[gr][2][2 * r], o[gr][3][2 * r]);
       to[1] = make_float4(o[gr][0][2 * r + 1], o[gr][1][2 * r + 1], o[gr][2][2 * r + 1], o[gr][3][2 * r + 1]);
     }
   __syncthreads();
-  float* const ws = a.splits > 1 ? a.ws + (out_tile * a.splits + split) * (kRows * (D + 2)) : nullptr;   // [row][D] sums, [row] maximum, [row] weight
-  for (int i = tid; i < kRows * (D / 4); i += kWarps * 32) {
-    const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-    if (r >= n_rows) break;
+  const bool whole = p.p0 == 0 && p.p1 == p.pairs;
+  // a part of the workspace: [row][D] sums, [row] maximum, [row] weight.  A CTA's first is of the segment that it has from the CTA before, its second
+  // of the one that the next CTA goes on with.
+  float* const ws = a.ws + ((int64_t)blockIdx.x * 2 + (p.p0 == 0)) * (kRows * (D + 2));
+  const int d = tid % (D / 4) * 4;
+  for (int r = tid / (D / 4); r < job.n_rows; r += kWarps * 32 / (D / 4)) {
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) top = fmaxf(top, part_m[w][r]);
@@ -424,74 +329,611 @@ __global__ void __launch_bounds__(kWarps * 32) attend_kernel(const __grid_consta
       sum.x += f * v.x; sum.y += f * v.y; sum.z += f * v.z; sum.w += f * v.w;
       weight += f * part_l[w][r];
     }
-    if (ws) {
+    if (whole) {
+      write_row<T>(a, p.sent, p.kvh, p.rt * kRows + r, d, sum, top, weight);
+    } else {
       *reinterpret_cast<float4*>(ws + r * D + d) = sum;
       if (d == 0) { ws[kRows * D + r] = top; ws[kRows * D + kRows + r] = weight; }
-    } else {
-      const int at = rt * kRows + r, g = at / a.rep, h = kvh * a.rep + at % a.rep;
-      const float f = weight > 0.f ? 1.f / weight : 0.f;
-      T* const to = static_cast<T*>(a.out) + sent * a.o_n + g * a.o_g + h * a.o_h + d;
-      to[0] = from_float<T>(sum.x * f); to[1] = from_float<T>(sum.y * f); to[2] = from_float<T>(sum.z * f); to[3] = from_float<T>(sum.w * f);
-      if (d == 0 && a.lse) a.lse[((int64_t)sent * a.g + g) * a.heads + h] = weight > 0.f ? (top + log2f(weight)) * 0.69314718055994531f : -INFINITY;
     }
+  }
+  __syncthreads();                    // (before the next piece's tiles come in)
+}
+
+template <int D>
+__global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend32_kernel(const __grid_constant__ AttendParams a) {
+  constexpr int NG = D / 32, kTileBytes = pages4::tile_bytes(D), QT = kTerms, PT = kTerms;
+  extern __shared__ __align__(16) unsigned char smem[];
+  launch_next();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, c = lane & 3;
+  Share share = share_of(a, gridDim.x);
+  Piece piece;
+  while (next_piece(a, share, piece)) {
+    const float* q_row[2];
+    const Job job = job_of<float>(a, piece, q_row);
+    const int t0 = job.t0, t1 = job.t1, all_lo = job.all_lo, all_hi = job.all_hi;
+    const int (&lo)[2] = job.lo, (&hi)[2] = job.hi;
+    const float (&slope)[2] = job.slope, (&centre)[2] = job.centre;
+
+    // Queries as left operands: step (group, half) takes components 32 group + 8 c + 2 half + {0, 4 | 1, 5}.
+    uint4* const q_smem = reinterpret_cast<uint4*>(smem + kWarps * kStages * kTileBytes);
+    for (int s = warp; s < QT * NG * 2; s += kWarps) {
+      const int term = s / (NG * 2), d = 32 * ((s % (NG * 2)) >> 1) + 8 * c + 2 * (s & 1);
+      q_smem[s * 32 + lane] = make_uint4(query_pair(q_row[0], d, term), query_pair(q_row[1], d, term), query_pair(q_row[0], d + 1, term), query_pair(q_row[1], d + 1, term));
+    }
+    __syncthreads();
+
+    float o[NG][4][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    const float to_log2 = a.cap > 0.f ? a.scale / a.cap : a.scale * kLog2e, cap_log2 = a.cap * kLog2e;
+    unsigned char* const ring = smem + warp * kStages * kTileBytes;
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+    const int32_t* const table = a.table + piece.sent * a.table_stride;
+    const unsigned char* const head = a.data + piece.kvh * a.stride_head;
+    const int tiles_per_page = a.page / pages4::kTile;
+    const int mine = t1 - t0 > warp ? (t1 - t0 - warp + kWarps - 1) / kWarps : 0;        // this warp's tiles: t0 + warp + kWarps i
+
+    // Where this warp's tiles are: looked up 32 at a time, one by each lane, a batch ahead of their use.
+    int64_t where = -1;
+    uint32_t bad = 0;                // bit of a stage: it holds no tile of the pool
+    auto fetch = [&](int i) {
+      if ((i & 31) == 0) {
+        where = -1;
+        if (i + lane < mine) where = pages4::tile_offset(table, t0 + warp + kWarps * (i + lane), tiles_per_page, a.n_pages, a.stride_page, D);
+      }
+      const int64_t at = __shfl_sync(~0u, where, i & 31);
+      const int stage = i % kStages;
+      if (i < mine && at >= 0) {
+        bad &= ~(1u << stage);
+#pragma unroll
+        for (int b = 0; b < (kTileBytes + 511) / 512; ++b) {
+          const int byte = b * 512 + lane * 16;
+          if (byte < kTileBytes) copy16(ring_at + stage * kTileBytes + byte, head + at + byte);
+        }
+      } else {
+        bad |= 1u << stage;
+      }
+      copy_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) fetch(i);
+
+    for (int i = 0; i < mine; ++i) {
+      copy_wait<kStages - 2>();
+      __syncwarp();                       // every lane's part of tile i is there, and tile i - 1 has been read by all
+      fetch(i + kStages - 1);
+      if ((bad >> (i % kStages)) & 1) continue;
+      const unsigned char* const tile = ring + (i % kStages) * kTileBytes;
+      const int pos = (t0 + warp + kWarps * i) * pages4::kTile;
+
+      // scores: x[j][0..3] = rows gid, gid, gid + 8, gid + 8 at positions pos + 8 j + 2 c + {0, 1, 0, 1}
+      float x[2][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t w[NG], sc[NG];
+        const unsigned char* const kw = tile + (8 * j + gid) * (D / 2) + c * (4 * NG);
+        const unsigned char* const ks = tile + pages4::key_scales(D) + (8 * j + 2 * c) * (2 * NG);
+        if constexpr (NG == 4) {
+          *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(kw);
+          *reinterpret_cast<uint4*>(sc) = *reinterpret_cast<const uint4*>(ks);
+        } else {
+          *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(kw);
+          *reinterpret_cast<uint2*>(sc) = *reinterpret_cast<const uint2*>(ks);
+        }
+        x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.f;
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          float s[4] = {0.f, 0.f, 0.f, 0.f};
+          uint32_t b[4];
+          b[0] = codes_bf16<0>(w[gr]); b[1] = codes_bf16<1>(w[gr]); b[2] = codes_bf16<2>(w[gr]); b[3] = codes_bf16<3>(w[gr]);
+#pragma unroll
+          for (int term = QT - 1; term >= 0; --term) {      // small terms first
+            mma_bf16(s, q_smem[(term * NG * 2 + 2 * gr) * 32 + lane], b[0], b[1]);
+            mma_bf16(s, q_smem[(term * NG * 2 + 2 * gr + 1) * 32 + lane], b[2], b[3]);
+          }
+          // scales of position 2 c: halves gr of the first NG, of 2 c + 1: of the second
+          const float s0 = gr & 1 ? bf16_high(sc[gr >> 1]) : bf16_low(sc[gr >> 1]);
+          const float s1 = gr & 1 ? bf16_high(sc[NG / 2 + (gr >> 1)]) : bf16_low(sc[NG / 2 + (gr >> 1)]);
+          x[j][0] = fmaf(s[0], s0, x[j][0]);
+          x[j][1] = fmaf(s[1], s1, x[j][1]);
+          x[j][2] = fmaf(s[2], s0, x[j][2]);
+          x[j][3] = fmaf(s[3], s1, x[j][3]);
+        }
+      }
+      if (a.cap > 0.f) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[j][e] = cap_log2 * tanhf(x[j][e] * to_log2);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[j][e] *= to_log2;
+      }
+      if (a.slope) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[j][e] -= slope[e >> 1] * fabsf((float)(pos + 8 * j + 2 * c + (e & 1)) - centre[e >> 1]);
+      }
+      const bool edge = pos < all_lo || pos + pages4::kTile > all_hi;
+      if (edge) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int p = pos + 8 * j + 2 * c + (e & 1);
+            if (p < lo[e >> 1] || p >= hi[e >> 1]) x[j][e] = -INFINITY;
+          }
+      }
+      float top[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        top[e] = fmaxf(fmaxf(x[0][2 * e], x[0][2 * e + 1]), fmaxf(x[1][2 * e], x[1][2 * e + 1]));
+        top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], 1));
+        top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], 2));
+      }
+      const bool up0 = top[0] > m[0] + kSlack || (m[0] == -INFINITY && top[0] > -INFINITY), up1 = top[1] > m[1] + kSlack || (m[1] == -INFINITY && top[1] > -INFINITY);
+      if (__any_sync(~0u, up0 || up1)) {
+        const float f0 = up0 ? exp2_of(m[0] - top[0]) : 1.f, f1 = up1 ? exp2_of(m[1] - top[1]) : 1.f;
+        if (up0) m[0] = top[0];
+        if (up1) m[1] = top[1];
+        l[0] *= f0;
+        l[1] *= f1;
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            o[gr][e][0] *= f0; o[gr][e][1] *= f0;
+            o[gr][e][2] *= f1; o[gr][e][3] *= f1;
+          }
+      }
+      const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        x[j][0] = exp2_of(x[j][0] - m0);
+        x[j][1] = exp2_of(x[j][1] - m0);
+        x[j][2] = exp2_of(x[j][2] - m1);
+        x[j][3] = exp2_of(x[j][3] - m1);
+        l[0] += x[j][0] + x[j][1];
+        l[1] += x[j][2] + x[j][3];
+      }
+
+      // out += weights . values, a group of 32 components a time: its scales go into the weights
+      uint32_t vs[2][NG];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const unsigned char* const at = tile + pages4::value_scales(D) + (8 * j + 2 * c) * (2 * NG);
+        if constexpr (NG == 4) *reinterpret_cast<uint4*>(vs[j]) = *reinterpret_cast<const uint4*>(at);
+        else *reinterpret_cast<uint2*>(vs[j]) = *reinterpret_cast<const uint2*>(at);
+        if (edge) {            // a position that nobody sees may hold anything: 0 times its scale has to be 0
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (x[j][e] == 0.f && x[j][e + 2] == 0.f) {
+#pragma unroll
+              for (int i2 = 0; i2 < NG / 2; ++i2) vs[j][e * (NG / 2) + i2] = 0u;
+            }
+        }
+      }
+#pragma unroll
+      for (int i2 = 0; i2 < NG / 2; ++i2) {
+        const uint4 u = *reinterpret_cast<const uint4*>(tile + pages4::value_codes(D) + 16 * (i2 * 32 + lane));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int gr = 2 * i2 + h;
+          const uint32_t w0 = h ? u.y : u.x, w1 = h ? u.w : u.z;
+          float p[2][4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float s0 = h ? bf16_high(vs[j][i2]) : bf16_low(vs[j][i2]), s1 = h ? bf16_high(vs[j][NG / 2 + i2]) : bf16_low(vs[j][NG / 2 + i2]);
+            p[j][0] = x[j][0] * s0;
+            p[j][1] = x[j][1] * s1;
+            p[j][2] = x[j][2] * s0;
+            p[j][3] = x[j][3] * s1;
+          }
+          uint4 pa[PT];
+#pragma unroll
+          for (int term = 0; term < PT; ++term) {
+            pa[term] = make_uint4(pack_bf16(p[0][0], p[0][1]), pack_bf16(p[0][2], p[0][3]), pack_bf16(p[1][0], p[1][1]), pack_bf16(p[1][2], p[1][3]));
+            if (term + 1 < PT) {
+              p[0][0] -= bf16_low(pa[term].x); p[0][1] -= bf16_high(pa[term].x);
+              p[0][2] -= bf16_low(pa[term].y); p[0][3] -= bf16_high(pa[term].y);
+              p[1][0] -= bf16_low(pa[term].z); p[1][1] -= bf16_high(pa[term].z);
+              p[1][2] -= bf16_low(pa[term].w); p[1][3] -= bf16_high(pa[term].w);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t b0 = e == 0 ? codes_bf16<0>(w0) : e == 1 ? codes_bf16<1>(w0) : e == 2 ? codes_bf16<2>(w0) : codes_bf16<3>(w0);
+            const uint32_t b1 = e == 0 ? codes_bf16<0>(w1) : e == 1 ? codes_bf16<1>(w1) : e == 2 ? codes_bf16<2>(w1) : codes_bf16<3>(w1);
+#pragma unroll
+            for (int term = PT - 1; term >= 0; --term) mma_bf16(o[gr][e], pa[term], b0, b1);
+          }
+        }
+      }
+    }
+
+    join_warps<float, D>(a, piece, job, smem, o, m, l);
   }
 }
 
-// Joins the parts of a row tile: one CTA for each.
 template <class T, int D>
-__global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant__ AttendParams a) {
-  const int64_t out_tile = blockIdx.x;
-  const int rt = (int)(out_tile % a.row_tiles), kvh = (int)(out_tile / a.row_tiles % a.pool_heads), sent = (int)(out_tile / a.row_tiles / a.pool_heads);
-  const int n_rows = min(kRows, a.g * a.rep - rt * kRows);
-  const float* const ws = a.ws + out_tile * a.splits * (kRows * (D + 2));
-  for (int i = threadIdx.x; i < n_rows * (D / 4); i += 128) {
-    const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+__global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(const __grid_constant__ AttendParams a) {
+  constexpr int NG = D / 32, kTileBytes = pages4::tile_bytes(D), PT = sizeof(T) == 2 && Fp16<T>::value ? 2 : 1;
+  constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;
+  extern __shared__ __align__(16) unsigned char smem[];
+  launch_next();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, c = lane & 3;
+  Share share = share_of(a, gridDim.x);
+  Piece piece;
+  while (next_piece(a, share, piece)) {
+    const T* q_row[2];
+    const Job job = job_of<T>(a, piece, q_row);
+
+    unsigned char* const ring = smem + warp * kPairStages * 2 * kTileBytes;
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+    const int32_t* const table = a.table + piece.sent * a.table_stride;
+    const unsigned char* const head = a.data + piece.kvh * a.stride_head;
+    const int tiles_per_page = a.page / pages4::kTile;
+    const int pairs = (job.t1 - job.t0 + 1) / 2, mine = pairs > warp ? (pairs - warp + kWarps - 1) / kWarps : 0;      // this warp's: warp + kWarps i
+
+    // Where this warp's tiles are: looked up 32 at a time, one by each lane.
+    int64_t where = -1;
+    uint32_t bad = 0;                // bits of a stage: no tile of the pool
+    int fetch_stage = 0;
+    auto fetch = [&](int i) {
+      if ((i & 15) == 0) {
+        const int t = job.t0 + 2 * (warp + kWarps * (i + (lane >> 1))) + (lane & 1);
+        where = i + (lane >> 1) < mine && t < job.t1 ? pages4::tile_offset(table, t, tiles_per_page, a.n_pages, a.stride_page, D) : -1;
+      }
+      const int64_t at0 = __shfl_sync(~0u, where, 2 * (i & 15)), at1 = __shfl_sync(~0u, where, 2 * (i & 15) + 1);
+      const int stage = fetch_stage;
+      fetch_stage = fetch_stage + 1 == kPairStages ? 0 : fetch_stage + 1;
+      bad &= ~(3u << (2 * stage));
+      if (i >= mine || at0 < 0) bad |= 1u << (2 * stage);
+      if (i >= mine || at1 < 0) bad |= 2u << (2 * stage);
+      if (i < mine) {
+        const uint32_t to = ring_at + stage * 2 * kTileBytes + lane * 16;
+        const unsigned char *const from0 = head + at0 + lane * 16, *const from1 = head + at1 + lane * 16;
+        constexpr int kWhole = kTileBytes / 512, kRest = (kTileBytes % 512) / 16;      // D = 128: four of 32 lanes and one of 16 for each tile; 64: two and one of 8
+        if (at0 >= 0) {
+#pragma unroll
+          for (int b = 0; b < kWhole; ++b) copy16(to + b * 512, from0 + b * 512);
+          if (lane < kRest) copy16(to + kWhole * 512, from0 + kWhole * 512);
+        }
+        if (at1 >= 0) {
+#pragma unroll
+          for (int b = 0; b < kWhole; ++b) copy16(to + kTileBytes + b * 512, from1 + b * 512);
+          if (lane < kRest) copy16(to + kTileBytes + kWhole * 512, from1 + kWhole * 512);
+        }
+      }
+      copy_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kPairStages - 1; ++i) fetch(i);
+
+    // Queries as left operands in fp16: step (group, half) takes components 32 group + 8 c + 2 half + {0, 4 | 1, 5}, the latter over 16.  A row is scaled
+    // so that its largest component is 2^9 to 2^10; what a group's codes carry too much, 8 times the sum of its components, in three bf16
+    // terms for a product with the keys' scales: place k of it belongs to group k % 4, term k / 4.
+    uint4 qa[NG * 2], over;
+    float mul[2];                  // from a sum of products to a power of 2 (or, with a cap, to what tanh takes)
+    {
+      uint32_t f[2][NG][4];        // [row][group]: components 0 and 4, 1 and 5, 2 and 6, 3 and 7 of the lane's eight
+      uint32_t ov[2][2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float x[NG][8], most = 0.f;
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          if (q_row[r] && a.q_wide) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(q_row[r] + 32 * gr + 8 * c));
+            const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[gr][i] = to_float(e[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[gr][i] = q_row[r] ? to_float(q_row[r][32 * gr + 8 * c + i]) : 0.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[gr][i]));
+        }
+        most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
+        const int up = most > 0.f && most < INFINITY ? 9 - max(-100, ilogbf(most)) : 0;      // -118 .. 109
+        const float by = (a.scale < 0.f ? -1.f : 1.f) * exp2f((float)up);
+        mul[r] = ldexpf(fabsf(a.scale) * (a.cap > 0.f ? 1.f / a.cap : kLog2e), 24 - up);
+        float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const __half2 h = __floats2half2_rn(x[gr][i] * by * (i & 1 ? 0.0625f : 1.f), x[gr][i + 4] * by * (i & 1 ? 0.0625f : 1.f));
+            f[r][gr][i] = *reinterpret_cast<const uint32_t*>(&h);
+            const float2 back = __half22float2(h);
+            sums[gr] += (back.x + back.y) * (i & 1 ? 16.f : 1.f);
+          }
+          sums[gr] += __shfl_xor_sync(~0u, sums[gr], 1);
+          sums[gr] += __shfl_xor_sync(~0u, sums[gr], 2);
+        }
+        float s0 = (c & 1 ? sums[2] : sums[0]) * (-8.f / 16777216.f), s1 = (c & 1 ? sums[3] : sums[1]) * (-8.f / 16777216.f);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {          // terms c / 2 and 2 + c / 2
+          float u0 = s0, u1 = s1;
+          const int term = 2 * h + (c >> 1);
+          for (int i = 0; i < term; ++i) {
+            u0 -= __bfloat162float(__float2bfloat16_rn(u0));
+            u1 -= __bfloat162float(__float2bfloat16_rn(u1));
+          }
+          ov[r][h] = term < 3 ? pack_bf16(u0, u1) : 0u;
+        }
+      }
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) qa[2 * gr + h] = make_uint4(f[0][gr][2 * h], f[1][gr][2 * h], f[0][gr][2 * h + 1], f[1][gr][2 * h + 1]);
+      over = make_uint4(ov[0][0], ov[1][0], ov[0][1], ov[1][1]);
+    }
+    const bool plain = a.cap == 0.f && !a.slope && a.scale != 0.f;       // scores are products times mul
+    const float cap_log2 = a.cap * kLog2e;
+
+    // Sums are kept times 2^up (a weight p is p 2^up), and those of values times 2^-133 as the codes are.
+    float o[NG][4][4] = {}, extra[4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, up = 0.f;
+    bool begun = false;
+    int stage = 0;
+    for (int i = 0; i < mine; ++i) {
+      copy_wait<kPairStages - 2>();
+      __syncwarp();                       // every lane's part of pair i is there, and pair i - 1 has been read by all
+      fetch(i + kPairStages - 1);
+      const unsigned char* const pair = ring + stage * 2 * kTileBytes;
+      const uint32_t gone = (bad >> (2 * stage)) & 3;
+      stage = stage + 1 == kPairStages ? 0 : stage + 1;
+      if (gone == 3) continue;
+      const int pos = (job.t0 + 2 * (warp + kWarps * i)) * pages4::kTile;
+
+      // scores: x[j][0..3] = rows gid, gid, gid + 8, gid + 8 at positions pos + 8 j + 2 c + {0, 1, 0, 1}
+      float x[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned char* const tile = pair + (j >> 1) * kTileBytes;
+        const int j1 = j & 1;
+        uint32_t w[NG], sc[NG];
+        const unsigned char* const kw = tile + (8 * j1 + gid) * (D / 2) + c * (4 * NG);
+        const unsigned char* const ks = tile + pages4::key_scales(D) + (8 * j1 + 2 * c) * (2 * NG);
+        if constexpr (NG == 4) {
+          *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(kw);
+          *reinterpret_cast<uint4*>(sc) = *reinterpret_cast<const uint4*>(ks);
+        } else {
+          *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(kw);
+          *reinterpret_cast<uint2*>(sc) = *reinterpret_cast<const uint2*>(ks);
+        }
+        const uint32_t mine2 = *reinterpret_cast<const uint32_t*>(tile + pages4::key_scales(D) + (8 * j1 + gid) * (2 * NG) + (NG == 4 ? 4 * (c & 1) : 0));
+        mma_bf16_first(x[j], over, mine2, mine2);
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          float s[4];
+          mma_f16_first(s, qa[2 * gr], w[gr] & kEven, w[gr] & kOdd);
+          mma_f16(s, qa[2 * gr + 1], (w[gr] >> 8) & kEven, (w[gr] >> 8) & kOdd);
+          // scales of position 2 c: halves gr of the first NG, of 2 c + 1: of the second
+          const float s0 = gr & 1 ? bf16_high(sc[gr >> 1]) : bf16_low(sc[gr >> 1]);
+          const float s1 = gr & 1 ? bf16_high(sc[NG / 2 + (gr >> 1)]) : bf16_low(sc[NG / 2 + (gr >> 1)]);
+          x[j][0] = fmaf(s[0], s0, x[j][0]);
+          x[j][1] = fmaf(s[1], s1, x[j][1]);
+          x[j][2] = fmaf(s[2], s0, x[j][2]);
+          x[j][3] = fmaf(s[3], s1, x[j][3]);
+        }
+      }
+      float r0 = mul[0], r1 = mul[1];
+      if (!plain) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float v = x[j][e] * (e < 2 ? r0 : r1);
+            if (a.cap > 0.f) v = cap_log2 * tanh_of(v);
+            if (a.slope) v -= job.slope[e >> 1] * fabsf((float)(pos + 8 * j + 2 * c + (e & 1)) - job.centre[e >> 1]);
+            x[j][e] = v;
+          }
+        r0 = r1 = 1.f;
+      }
+      const bool edge = gone || pos < job.all_lo || pos + 2 * pages4::kTile > job.all_hi;
+      if (edge) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int p = pos + 8 * j + 2 * c + (e & 1);
+            if (p < job.lo[e >> 1] || p >= job.hi[e >> 1] || ((gone >> (j >> 1)) & 1)) x[j][e] = -INFINITY;
+          }
+      }
+      float top[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        top[e] = fmaxf(fmaxf(fmaxf(x[0][2 * e], x[0][2 * e + 1]), fmaxf(x[1][2 * e], x[1][2 * e + 1])), fmaxf(fmaxf(x[2][2 * e], x[2][2 * e + 1]), fmaxf(x[3][2 * e], x[3][2 * e + 1])));
+        top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], 1));
+        top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], 2));
+        top[e] *= e ? r1 : r0;
+      }
+      const bool up0 = top[0] > m[0] + kSlack || (m[0] == -INFINITY && top[0] > -INFINITY), up1 = top[1] > m[1] + kSlack || (m[1] == -INFINITY && top[1] > -INFINITY);
+      if (__any_sync(~0u, up0 || up1)) {
+        const float f0 = up0 ? exp2_of(m[0] - top[0]) : 1.f, f1 = up1 ? exp2_of(m[1] - top[1]) : 1.f;
+        if (up0) m[0] = top[0];
+        if (up1) m[1] = top[1];
+        l[0] *= f0;
+        l[1] *= f1;
+        extra[0] *= f0; extra[2] *= f1;
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            o[gr][e][0] *= f0; o[gr][e][1] *= f0;
+            o[gr][e][2] *= f1; o[gr][e][3] *= f1;
+          }
+      }
+
+      // values' scales of the lane's positions, two words for each of the four
+      uint32_t vs[4][NG];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned char* const at = pair + (j >> 1) * kTileBytes + pages4::value_scales(D) + (8 * (j & 1) + 2 * c) * (2 * NG);
+        if constexpr (NG == 4) *reinterpret_cast<uint4*>(vs[j]) = *reinterpret_cast<const uint4*>(at);
+        else *reinterpret_cast<uint2*>(vs[j]) = *reinterpret_cast<const uint2*>(at);
+        if (edge) {            // a position that the lane's rows do not see may hold anything: 0 times its scale has to be 0
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (x[j][e] == -INFINITY && x[j][e + 2] == -INFINITY) {
+#pragma unroll
+              for (int i2 = 0; i2 < NG / 2; ++i2) vs[j][e * (NG / 2) + i2] = 0u;
+            }
+        }
+      }
+      if (!begun) {            // the power of 2 that brings weights times these scales to some 2^50
+        begun = true;
+        int most = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i2 = 0; i2 < NG; ++i2) most = max(most, max((int)(vs[j][i2] >> 7) & 255, (int)(vs[j][i2] >> 23) & 255));
+        most = __reduce_max_sync(~0u, most);
+        up = (float)min(90, max(-60, 50 - (most ? most - 127 : 0)));
+      }
+      const float m0 = (m[0] == -INFINITY ? 0.f : m[0]) - up, m1 = (m[1] == -INFINITY ? 0.f : m[1]) - up;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j][0] = exp2_of(fmaf(x[j][0], r0, -m0));
+        x[j][1] = exp2_of(fmaf(x[j][1], r0, -m0));
+        x[j][2] = exp2_of(fmaf(x[j][2], r1, -m1));
+        x[j][3] = exp2_of(fmaf(x[j][3], r1, -m1));
+        l[0] += x[j][0] + x[j][1];
+        l[1] += x[j][2] + x[j][3];
+      }
+
+      // out += weights . values, a group of 32 components a time: its scales go into the weights
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt) {
+#pragma unroll
+        for (int i2 = 0; i2 < NG / 2; ++i2) {
+          const uint4 u = *reinterpret_cast<const uint4*>(pair + tt * kTileBytes + pages4::value_codes(D) + 16 * (i2 * 32 + lane));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int gr = 2 * i2 + h;
+            const uint32_t w0 = h ? u.y : u.x, w1 = h ? u.w : u.z;
+            float p[2][4];
+#pragma unroll
+            for (int j1 = 0; j1 < 2; ++j1) {
+              const int j = 2 * tt + j1;
+              const float s0 = h ? bf16_high(vs[j][i2]) : bf16_low(vs[j][i2]), s1 = h ? bf16_high(vs[j][NG / 2 + i2]) : bf16_low(vs[j][NG / 2 + i2]);
+              p[j1][0] = x[j][0] * s0;
+              p[j1][1] = x[j][1] * s1;
+              p[j1][2] = x[j][2] * s0;
+              p[j1][3] = x[j][3] * s1;
+            }
+            uint4 pa[PT];
+#pragma unroll
+            for (int term = 0; term < PT; ++term) {
+              pa[term] = make_uint4(pack_bf16(p[0][0], p[0][1]), pack_bf16(p[0][2], p[0][3]), pack_bf16(p[1][0], p[1][1]), pack_bf16(p[1][2], p[1][3]));
+              if (term + 1 < PT) {
+                p[0][0] -= bf16_low(pa[term].x); p[0][1] -= bf16_high(pa[term].x);
+                p[0][2] -= bf16_low(pa[term].y); p[0][3] -= bf16_high(pa[term].y);
+                p[1][0] -= bf16_low(pa[term].z); p[1][1] -= bf16_high(pa[term].z);
+                p[1][2] -= bf16_low(pa[term].w); p[1][3] -= bf16_high(pa[term].w);
+              }
+            }
+            const uint32_t eight = (gid >> 1) == gr ? 0x00080008u : 0u;       // columns 2 gr and 2 gr + 1: 8 times the weights' sum
+#pragma unroll
+            for (int term = PT - 1; term >= 0; --term) {
+              mma_bf16(o[gr][0], pa[term], w0 & kEven, w1 & kEven);
+              mma_bf16(o[gr][1], pa[term], w0 & kOdd, w1 & kOdd);
+              mma_bf16(o[gr][2], pa[term], (w0 >> 8) & kEven, (w1 >> 8) & kEven);
+              mma_bf16(o[gr][3], pa[term], (w0 >> 8) & kOdd, (w1 >> 8) & kOdd);
+              mma_bf16(extra, pa[term], eight, eight);
+            }
+          }
+        }
+      }
+    }
+
+    // From the sums as they are kept to sums relative to 2^m: less 8 for each code, times 2^133 / 2^up.
+    const float fa = exp2f(66.f - up * 0.5f), fb = exp2f(67.f - up * 0.5f), back = exp2f(-up);
+#pragma unroll
+    for (int gr = 0; gr < NG; ++gr) {
+      const float e0 = __shfl_sync(~0u, extra[0], (lane & ~3) | gr), e1 = __shfl_sync(~0u, extra[2], (lane & ~3) | gr);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[gr][e][i] = (o[gr][e][i] * fa * (e & 1 ? 0.0625f : 1.f) - (i < 2 ? e0 : e1) * fa) * fb;
+    }
+    l[0] *= back;
+    l[1] *= back;
+    join_warps<T, D>(a, piece, job, smem, o, m, l);
+  }
+}
+
+// Joins the parts of the segment that ends in a CTA's share and began in one before: a CTA for each of attend's.
+template <class T, int D>
+__global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant__ AttendParams a, int blocks) {
+  Share share = share_of(a, blocks);
+  Piece p;
+  const int64_t per = share.per;
+  const bool ends = next_piece(a, share, p) && p.p0 > 0 && p.p1 == p.pairs;
+  wait_for_last();
+  if (!ends) return;
+  const int from = (int)(p.start / per), n_parts = (int)blockIdx.x - from + 1;
+  constexpr int kPart = kRows * (D + 2);
+  auto part = [&](int i) { return a.ws + ((int64_t)(from + i) * 2 + (i == 0)) * kPart; };
+  const int n_rows = min(kRows, a.g * a.rep - p.rt * kRows), d = threadIdx.x % (D / 4) * 4;
+  for (int r = threadIdx.x / (D / 4); r < n_rows; r += 128 / (D / 4)) {
     float top = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, ws[(int64_t)s * (kRows * (D + 2)) + kRows * D + r]);
+#pragma unroll 4
+    for (int i = 0; i < n_parts; ++i) top = fmaxf(top, part(i)[kRows * D + r]);
     const float base = top == -INFINITY ? 0.f : top;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     float weight = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-      const float* const p = ws + (int64_t)s * (kRows * (D + 2));
-      const float f = exp2_of(p[kRows * D + r] - base);
-      const float4 v = *reinterpret_cast<const float4*>(p + r * D + d);
+#pragma unroll 4
+    for (int i = 0; i < n_parts; ++i) {
+      const float* const w = part(i);
+      const float f = exp2_of(w[kRows * D + r] - base);
+      const float4 v = *reinterpret_cast<const float4*>(w + r * D + d);
       sum.x += f * v.x; sum.y += f * v.y; sum.z += f * v.z; sum.w += f * v.w;
-      weight += f * p[kRows * D + kRows + r];
+      weight += f * w[kRows * D + kRows + r];
     }
-    const int at = rt * kRows + r, g = at / a.rep, h = kvh * a.rep + at % a.rep;
-    const float f = weight > 0.f ? 1.f / weight : 0.f;
-    T* const to = static_cast<T*>(a.out) + sent * a.o_n + g * a.o_g + h * a.o_h + d;
-    to[0] = from_float<T>(sum.x * f); to[1] = from_float<T>(sum.y * f); to[2] = from_float<T>(sum.z * f); to[3] = from_float<T>(sum.w * f);
-    if (d == 0 && a.lse) a.lse[((int64_t)sent * a.g + g) * a.heads + h] = weight > 0.f ? (top + log2f(weight)) * 0.69314718055994531f : -INFINITY;
+    write_row<T>(a, p.sent, p.kvh, p.rt * kRows + r, d, sum, top, weight);
   }
 }
 
 template <class T, int D>
-cudaError_t launch_attend(const AttendParams& p, int device, cudaStream_t st) {
+cudaError_t launch_attend(const AttendParams& p, int blocks, int device, cudaStream_t st) {
   constexpr int smem = attend_smem<T, D>();
+  void (*kernel)(AttendParams);
+  if constexpr (sizeof(T) == 2) kernel = attend16_kernel<T, D>; else kernel = attend32_kernel<D>;
   static std::atomic<bool> opted_in[kOpMaxDevices] = {};
   if (smem + 1024 > 48 << 10 && !opted_in[device].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(attend_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     opted_in[device].store(true, std::memory_order_release);
   }
-  const int64_t tiles = (int64_t)p.n * p.pool_heads * p.row_tiles;
-  attend_kernel<T, D><<<(unsigned)(tiles * p.splits), kWarps * 32, smem, st>>>(p);
+  kernel<<<(unsigned)blocks, kWarps * 32, smem, st>>>(p);
   cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || p.splits == 1) return e;
-  attend_join_kernel<T, D><<<(unsigned)tiles, 128, 0, st>>>(p);
-  return cudaGetLastError();
+  if (e != cudaSuccess || !p.ws) return e;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, attend_join_kernel<T, D>, p, blocks);
+  return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
 int row_tiles_of(const linmt_attend_pages4_args* g) { return (int)(((int64_t)g->g * (g->heads / g->pages.heads) + kRows - 1) / kRows); }
 
-// CTAs that share a row tile's positions: as many as give the GPU three rounds of the four CTAs that an SM holds, but 16 tiles (256
-// positions) at least for each.
-int splits_of(const linmt_attend_pages4_args* g) {
-  const int64_t tiles = (int64_t)g->n * g->pages.heads * row_tiles_of(g), most = ((int64_t)g->width * (g->pages.page / pages4::kTile) + 15) / 16;
-  if (tiles == 0 || most <= 1) return 1;
-  const int64_t want = (3 * 4 * 148 + tiles - 1) / tiles;
-  return (int)(want < most ? want : most);
+int64_t pairs_at_most(const linmt_attend_pages4_args* g) { const int64_t p = ((int64_t)g->width * g->pages.page + 31) / 32; return p < 1 ? 1 : p; }
+// CTAs: as many as fit on the GPU at once (three on an SM with 128 components, four with 64), or as the longest possible sentences
+// give kLeast pairs each.
+int blocks_of(const linmt_attend_pages4_args* g) {
+  const int64_t segments = (int64_t)g->n * g->pages.heads * row_tiles_of(g), most = segments * ((pairs_at_most(g) + kLeast - 1) / kLeast), fit = 148 * (g->pages.dim == 64 ? 4 : 3);
+  return (int)(most < fit ? most : fit);
 }
 
 int check(const linmt_attend_pages4_args* g) {
@@ -511,9 +953,9 @@ int check(const linmt_attend_pages4_args* g) {
   return LINMT_OK;
 }
 
+// Two parts for each CTA: of the segments that it shares with the CTAs before and behind it.  None where no segment can be long enough to be cut.
 int64_t workspace_of(const linmt_attend_pages4_args* g) {
-  const int splits = splits_of(g);
-  return splits == 1 ? 0 : (int64_t)g->n * g->pages.heads * row_tiles_of(g) * splits * (kRows * (g->pages.dim + 2)) * 4;
+  return pairs_at_most(g) <= kLeast ? 0 : (int64_t)blocks_of(g) * 2 * (kRows * (g->pages.dim + 2)) * 4;
 }
 
 }  // namespace
@@ -540,14 +982,16 @@ int linmt_attend_pages4(const linmt_attend_pages4_args* g) {
   if (on.err != cudaSuccess) return op_cuda(on.err, "attend_pages4");
   AttendParams p{static_cast<const unsigned char*>(g->pages.data), g->pages.stride_page, g->pages.stride_head, g->pages.n_pages, g->pages.heads, g->pages.page,
                  g->q, g->q_stride_n, g->q_stride_g, g->q_stride_h, g->out, g->out_stride_n, g->out_stride_g, g->out_stride_h, g->lse, g->table, g->table_stride, g->len,
-                 g->slope, g->centre, g->first, g->last, static_cast<float*>(g->workspace), g->n, g->g, g->heads, g->heads / g->pages.heads, g->width, row_tiles_of(g), splits_of(g),
-                 g->scale, g->cap};
+                 g->slope, g->centre, g->first, g->last, need ? static_cast<float*>(g->workspace) : nullptr, g->n, g->g, g->heads, g->heads / g->pages.heads, g->width, row_tiles_of(g),
+                 g->scale, g->cap, aligned(g->q, 16) && (g->q_stride_n | g->q_stride_g | g->q_stride_h) % (16 / dtype_bytes(g->dtype)) == 0,
+                 aligned(g->out, 4 * dtype_bytes(g->dtype)) && (g->out_stride_n | g->out_stride_g | g->out_stride_h) % 4 == 0};
+  const int blocks = blocks_of(g);
   const cudaStream_t st = static_cast<cudaStream_t>(g->stream);
   cudaError_t e;
   if (g->pages.dim == 64)
-    e = g->dtype == LINMT_F32 ? launch_attend<float, 64>(p, g->device, st) : g->dtype == LINMT_BF16 ? launch_attend<__nv_bfloat16, 64>(p, g->device, st) : launch_attend<__half, 64>(p, g->device, st);
+    e = g->dtype == LINMT_F32 ? launch_attend<float, 64>(p, blocks, g->device, st) : g->dtype == LINMT_BF16 ? launch_attend<__nv_bfloat16, 64>(p, blocks, g->device, st) : launch_attend<__half, 64>(p, blocks, g->device, st);
   else
-    e = g->dtype == LINMT_F32 ? launch_attend<float, 128>(p, g->device, st) : g->dtype == LINMT_BF16 ? launch_attend<__nv_bfloat16, 128>(p, g->device, st) : launch_attend<__half, 128>(p, g->device, st);
+    e = g->dtype == LINMT_F32 ? launch_attend<float, 128>(p, blocks, g->device, st) : g->dtype == LINMT_BF16 ? launch_attend<__nv_bfloat16, 128>(p, blocks, g->device, st) : launch_attend<__half, 128>(p, blocks, g->device, st);
   return e == cudaSuccess ? LINMT_OK : op_cuda(e, "attend_pages4");
 }
 

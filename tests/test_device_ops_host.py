@@ -108,10 +108,10 @@ def test_attend_refuses(cuda_lib, code, word, kw):
 
 def test_attend_workspace(cuda_lib):
     size = lambda **kw: cuda_lib.linmt_attend_pages4_workspace(_pack("linmt_attend_pages4_args", **kw))
-    assert size(width=16) == 0 and size(n=0, width=4096) == 0 and size(heads=3) == -1
-    need = size(width=4096)
-    assert need > 0 and need % (16 * 66 * 4 * 2 * 2) == 0        # [sentence][head of the pool][part][16 rows][64 sums, maximum, weight]
-    assert size(width=4096, n=4000) == 0                       # enough sentences: their positions are not split
+    assert size(width=16) == 0 and size(n=0, width=4096) == 0 and size(heads=3) == -1     # sentences of up to 256 positions are not cut
+    part = 16 * 66 * 4                                         # 16 rows: 64 sums, a maximum and a weight
+    assert size(width=4096) == 592 * 2 * part and size(width=4096, n=4000) == 592 * 2 * part
+    assert size(width=32) == 2 * 2 * 2 * 2 * part               # 2 sentences, 2 heads, 16 pairs of tiles in parts of 8
 
 
 def test_nothing_to_do_reaches_no_device(cuda_lib):

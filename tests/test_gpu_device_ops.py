@@ -446,10 +446,11 @@ def test_write_extremes_and_strides(ops):
 # ---- attention
 
 def attend_ref(q, k, v, table, lens, page, scale, cap, slope, centre, first, last, n_pages):
-    """In 64 bits.  k, v [n_pages * page, heads, dim].  Returns out, lse, the sum of w |v|, and the largest sum |q||k| scale."""
+    """In 64 bits.  k, v [n_pages * page, heads, dim].  Returns out, lse, the sum of w |v|, the largest sum |q||k| scale, and the sum of w times the values' scales."""
     n, g, heads, dim = q.shape
     rep = heads // k.shape[1]
     out, lse, wv, big = np.zeros((n, g, heads, dim)), np.full((n, g, heads), -INF), np.zeros((n, g, heads, dim)), 0.0
+    ws = np.zeros((n, g, heads, dim))
     for i in range(n):
         length = min(max(int(lens[i]), 0), table.shape[1] * page)
         at = np.arange(length)
@@ -474,7 +475,10 @@ def attend_ref(q, k, v, table, lens, page, scale, cap, slope, centre, first, las
                 m = s.max()
                 e = np.exp(s - m)
                 out[i, a, h], wv[i, a, h], lse[i, a, h] = e @ vv / e.sum(), e @ np.abs(vv) / e.sum(), m + np.log(e.sum())
-    return out, lse, wv, big
+                # a scale is an eighth of the group's largest component, but for its rounding to bf16
+                step = np.abs(vv).reshape(len(vv), -1, 32).max(-1).repeat(32, -1) / 8 * (1 + 2.0 ** -7)
+                ws[i, a, h] = e @ step / e.sum()
+    return out, lse, wv, big, ws
 
 
 def _memory(ops, rng, lens, heads, dim, page, width=None, spare=2, fill=0xFF):
@@ -507,7 +511,7 @@ def attend_check(ops, q, pages, table, lens, kk, vv, page, scale=None, cap=0.0, 
     got, lse = ops.attend_pages4(q, pages, _cuda(table), _cuda(np.asarray(lens, np.int32)), scale=scale, cap=cap, slope=dev(slope), centre=dev(centre), first=dev(first), last=dev(last), want_lse=True, out=out)
     dim = q.shape[3]
     scale = dim ** -0.5 if scale is None else scale
-    want, wlse, wv, big = attend_ref(q.double().cpu().numpy(), kk, vv, table, lens, page, scale, cap, slope, centre, first, last, pages.shape[0])
+    want, wlse, wv, big, ws = attend_ref(q.double().cpu().numpy(), kk, vv, table, lens, page, scale, cap, slope, centre, first, last, pages.shape[0])
     # A score: products of exact values added in 32 bits, at most dim + 8 additions and products; the cap's tanh to 2e-7 of the cap (16-bit queries) and the bias
     # and the change to powers of two a few roundings of their own size.  Queries in 32 bits are exact to 2^-24 in three terms.
     bias = 0.0 if slope is None else float(np.max(slope)) * (max(lens) + float(np.max(np.abs(centre))))
@@ -517,7 +521,11 @@ def attend_check(ops, q, pages, table, lens, kk, vv, page, scale=None, cap=0.0, 
     # weights: exp2 2^-22 and sums of up to 2^12 additions a lane would be 2^-12 at worst, but each is of positive terms rounded to nearest: 64 warps' and lanes' partial
     # sums of some hundreds, 2^-24 * 300; the rounding of the weight to its terms, the output's own
     weight = {BF16: 2.0 ** -8, F16: 2.0 ** -16, F32: 2.0 ** -24}[q.dtype]
-    tol = HALF_STEP[q.dtype] * np.abs(want) + (weight + 2 * score + 2.0 ** -15) * wv + (2.0 ** -25 if q.dtype == F16 else 0)
+    # 16-bit queries: codes go into the products as 0 .. 15 and 8 for each comes off at the end, so that the sums on the way are up to 15 sum(w scale) in size whatever
+    # the values are.  A warp adds a product of 16 positions (of the CTA's 64) a time to them, each addition off by 2^-23 of the sum at most (the matrix unit may cut off),
+    # and some 8 more join the parts: a component whose values cancel, or whose codes are all near 8, is off by that and not by a share of itself.
+    shift = 0.0 if q.dtype == F32 else (max(lens) / 64 + 8) * 2.0 ** -23 * 15 * ws
+    tol = HALF_STEP[q.dtype] * np.abs(want) + (weight + 2 * score + 2.0 ** -15) * wv + shift + (2.0 ** -25 if q.dtype == F16 else 0)
     assert np.isfinite(g).all()
     assert (np.abs(g - want) <= tol).all(), float((np.abs(g - want) / np.maximum(tol, 1e-300)).max())
     l = lse.double().cpu().numpy()
@@ -580,6 +588,19 @@ def test_attend_long_and_split(ops, dtype):
     first = np.array([[0, 8999, 4000, 10, 16, 2000]] * 3, np.int32)
     last = np.array([[9000, 9000, 4001, 8000, 32, 2048]] * 3, np.int32)
     attend_check(ops, q, pages, table, lens, kk, vv, 64, first=first, last=last)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("lens", [[5000, 1, 1, 1, 4000, 0, 0, 700], [33] * 150, [3] * 40 + [6000] + [50] * 30, [0, 0, 0], [129, 130, 8000, 257]])
+def test_attend_shares_of_uneven_sentences(ops, lens, dtype):
+    """Segments that several CTAs share, that share a CTA, and both: long sentences before, between and behind short ones."""
+    rng = _rng(sum(lens), len(lens))
+    pages, table, kk, vv = _memory(ops, rng, lens, 2, 64, 16)
+    n, g = len(lens), 9
+    q = _q(rng, n, g, 4, 64, dtype)                    # 18 rows a head of the pool: two row tiles
+    attend_check(ops, q, pages, table, lens, kk, vv, 16)
+    a, b = rng.integers(0, max(lens) + 1, (2, n, g)).astype(np.int32)
+    attend_check(ops, q, pages, table, lens, kk, vv, 16, first=np.minimum(a, b), last=np.maximum(a, b))
 
 
 def test_attend_strides(ops):
@@ -695,7 +716,7 @@ def _decode(ops, toy, lens, keys, values, steps, page=16, reference=False):
                 s = table[i, at // page].long() * page + at % page
                 rk, rv = ops.read_pages4(pages, s)
                 kk[s.cpu()], vv[s.cpu()] = rk.cpu(), rv.cpu()
-            c, _, _, _ = attend_ref(q.double().cpu().numpy(), kk.numpy(), vv.numpy(), table.cpu().numpy(), lens, page, toy.dim ** -0.5, 0.0, None, None, None, None, pages.shape[0])
+            c, _, _, _, _ = attend_ref(q.double().cpu().numpy(), kk.numpy(), vv.numpy(), table.cpu().numpy(), lens, page, toy.dim ** -0.5, 0.0, None, None, None, None, pages.shape[0])
             context = _cuda(c.astype(np.float32))
         else:
             context = ops.attend_pages4(q, pages, table, new)
