@@ -12,8 +12,8 @@
 //   code, goes off by a product of its own: the queries' sums with the keys' scales, and the weights' sums.  That is 5
 //   instructions for 8 codes where a code minus 8 in normal form takes 11, in a kernel bound by what it can issue.  Queries are scaled to
 //   fp16's upper range by a power of 2 for each row, weights by one for each warp (after the first values' scale), so that nothing that matters
-//   falls out of range.  Weights are rounded to bf16 once for bf16 queries (2^-8 each at most, on average over the positions far less, and the output's
-//   own rounding is as large); for fp16 they are taken as two bf16 terms (2^-16).
+//   falls out of range.  For bf16 queries weights are rounded to bf16, and once more when a scale is multiplied in there (2^-7 at most, on average over the
+//   positions far less, and the output's own rounding is 2^-8); for fp16 they are taken as two bf16 terms (2^-16).
 //   32-bit queries (attend32_kernel) are three bf16 terms, the weights too (2^-24), the codes minus 8 in normal form.
 // Every warp has a ring of tiles of its own (cp.async, no barrier among warps) and its own maximum and sums; the CTA's four are
 // joined through shared memory at the end of a piece of work, and where a sentence's positions are shared by CTAs a second kernel joins those.
@@ -91,6 +91,12 @@ __device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {
   const uint32_t b = lop_and_or(w >> (4 * I), 0x000f000fu, 0x43004300u), off = 0x43084308u;      // 128 + code, 136
   __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&off));
   return *reinterpret_cast<uint32_t*>(&r);
+}
+// The low (or high) halves of two words, side by side.
+__device__ __forceinline__ uint32_t pair_of(uint32_t a, uint32_t b, int high) { return __byte_perm(a, b, high ? 0x7632 : 0x5410); }
+__device__ __forceinline__ uint32_t mul_bf16(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ float bf16_low(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float bf16_high(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
@@ -229,7 +235,7 @@ __device__ __forceinline__ bool next_piece(const AttendParams& a, Share& s, Piec
 
 template <class T, int D>
 constexpr int attend_smem() {
-  if constexpr (sizeof(T) == 2) return kWarps * kPairStages * 2 * 18 * D;
+  if constexpr (sizeof(T) == 2) return kWarps * kPairStages * 2 * 18 * D + (D / 16) * 512;
   else return kWarps * kStages * 18 * D + kTerms * (D / 16) * 512;
 }
 
@@ -570,6 +576,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
     const Job job = job_of<T>(a, piece, q_row);
 
     unsigned char* const ring = smem + warp * kPairStages * 2 * kTileBytes;
+    uint4* const q_smem = reinterpret_cast<uint4*>(smem + kWarps * kPairStages * 2 * kTileBytes);
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
     const int32_t* const table = a.table + piece.sent * a.table_stride;
     const unsigned char* const head = a.data + piece.kvh * a.stride_head;
@@ -613,63 +620,78 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
 
     // Queries as left operands in fp16: step (group, half) takes components 32 group + 8 c + 2 half + {0, 4 | 1, 5}, the latter over 16.  A row is scaled
     // so that its largest component is 2^9 to 2^10; what a group's codes carry too much, 8 times the sum of its components, in three bf16
-    // terms for a product with the keys' scales: place k of it belongs to group k % 4, term k / 4.
-    uint4 qa[NG * 2], over;
+    // terms for a product with the keys' scales: place k of it belongs to group k % 4, term k / 4.  A warp prepares one group.
+    uint4 over;
     float mul[2];                  // from a sum of products to a power of 2 (or, with a cap, to what tanh takes)
     {
-      uint32_t f[2][NG][4];        // [row][group]: components 0 and 4, 1 and 5, 2 and 6, 3 and 7 of the lane's eight
+      __shared__ float s_most[NG][kRows], s_sum[4][kRows];
+      float x[2][8];
+      if (warp < NG) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          if (q_row[r] && a.q_wide) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(q_row[r] + 32 * warp + 8 * c));
+            const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[r][i] = to_float(e[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[r][i] = q_row[r] ? to_float(q_row[r][32 * warp + 8 * c + i]) : 0.f;
+          }
+          float most = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[r][i]));
+          most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
+          most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
+          if (c == 0) s_most[warp][gid + 8 * r] = most;
+        }
+      } else if (c == 0) {         // (64 components: groups 2 and 3 are none)
+        s_sum[warp][gid] = s_sum[warp][gid + 8] = 0.f;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float most = s_most[0][gid + 8 * r];
+#pragma unroll
+        for (int gr = 1; gr < NG; ++gr) most = fmaxf(most, s_most[gr][gid + 8 * r]);
+        const int up = most > 0.f && most < INFINITY ? 9 - max(-100, ilogbf(most)) : 0;      // -118 .. 109
+        const float by = ldexpf(a.scale < 0.f ? -1.f : 1.f, up);
+        mul[r] = ldexpf(fabsf(a.scale) * (a.cap > 0.f ? 1.f / a.cap : kLog2e), 24 - up);
+        if (warp < NG) {
+          float sum = 0.f;
+          uint32_t f[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const __half2 h = __floats2half2_rn(x[r][i] * by * (i & 1 ? 0.0625f : 1.f), x[r][i + 4] * by * (i & 1 ? 0.0625f : 1.f));
+            f[i] = *reinterpret_cast<const uint32_t*>(&h);
+            const float2 back = __half22float2(h);
+            sum += (back.x + back.y) * (i & 1 ? 16.f : 1.f);
+          }
+          sum += __shfl_xor_sync(~0u, sum, 1);
+          sum += __shfl_xor_sync(~0u, sum, 2);
+          if (c == 0) s_sum[warp][gid + 8 * r] = sum * (-8.f / 16777216.f);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(q_smem + (2 * warp + (i >> 1)) * 32 + lane)[2 * (i & 1) + r] = f[i];
+        }
+      }
+      __syncthreads();
       uint32_t ov[2][2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        float x[NG][8], most = 0.f;
-#pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-          if (q_row[r] && a.q_wide) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(q_row[r] + 32 * gr + 8 * c));
-            const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[gr][i] = to_float(e[i]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[gr][i] = q_row[r] ? to_float(q_row[r][32 * gr + 8 * c + i]) : 0.f;
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[gr][i]));
-        }
-        most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
-        most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
-        const int up = most > 0.f && most < INFINITY ? 9 - max(-100, ilogbf(most)) : 0;      // -118 .. 109
-        const float by = (a.scale < 0.f ? -1.f : 1.f) * exp2f((float)up);
-        mul[r] = ldexpf(fabsf(a.scale) * (a.cap > 0.f ? 1.f / a.cap : kLog2e), 24 - up);
-        float sums[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const __half2 h = __floats2half2_rn(x[gr][i] * by * (i & 1 ? 0.0625f : 1.f), x[gr][i + 4] * by * (i & 1 ? 0.0625f : 1.f));
-            f[r][gr][i] = *reinterpret_cast<const uint32_t*>(&h);
-            const float2 back = __half22float2(h);
-            sums[gr] += (back.x + back.y) * (i & 1 ? 16.f : 1.f);
-          }
-          sums[gr] += __shfl_xor_sync(~0u, sums[gr], 1);
-          sums[gr] += __shfl_xor_sync(~0u, sums[gr], 2);
-        }
-        float s0 = (c & 1 ? sums[2] : sums[0]) * (-8.f / 16777216.f), s1 = (c & 1 ? sums[3] : sums[1]) * (-8.f / 16777216.f);
+        const float s0 = s_sum[2 * (c & 1)][gid + 8 * r], s1 = s_sum[2 * (c & 1) + 1][gid + 8 * r];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {          // terms c / 2 and 2 + c / 2
           float u0 = s0, u1 = s1;
           const int term = 2 * h + (c >> 1);
-          for (int i = 0; i < term; ++i) {
-            u0 -= __bfloat162float(__float2bfloat16_rn(u0));
-            u1 -= __bfloat162float(__float2bfloat16_rn(u1));
-          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (i < term) {
+              u0 -= __bfloat162float(__float2bfloat16_rn(u0));
+              u1 -= __bfloat162float(__float2bfloat16_rn(u1));
+            }
           ov[r][h] = term < 3 ? pack_bf16(u0, u1) : 0u;
         }
       }
-#pragma unroll
-      for (int gr = 0; gr < NG; ++gr)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) qa[2 * gr + h] = make_uint4(f[0][gr][2 * h], f[1][gr][2 * h], f[0][gr][2 * h + 1], f[1][gr][2 * h + 1]);
       over = make_uint4(ov[0][0], ov[1][0], ov[0][1], ov[1][1]);
     }
     const bool plain = a.cap == 0.f && !a.slope && a.scale != 0.f;       // scores are products times mul
@@ -691,30 +713,34 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
 
       // scores: x[j][0..3] = rows gid, gid, gid + 8, gid + 8 at positions pos + 8 j + 2 c + {0, 1, 0, 1}
       float x[4][4];
+      uint32_t w[4][NG], sc[4][NG];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const unsigned char* const tile = pair + (j >> 1) * kTileBytes;
         const int j1 = j & 1;
-        uint32_t w[NG], sc[NG];
         const unsigned char* const kw = tile + (8 * j1 + gid) * (D / 2) + c * (4 * NG);
         const unsigned char* const ks = tile + pages4::key_scales(D) + (8 * j1 + 2 * c) * (2 * NG);
         if constexpr (NG == 4) {
-          *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(kw);
-          *reinterpret_cast<uint4*>(sc) = *reinterpret_cast<const uint4*>(ks);
+          *reinterpret_cast<uint4*>(w[j]) = *reinterpret_cast<const uint4*>(kw);
+          *reinterpret_cast<uint4*>(sc[j]) = *reinterpret_cast<const uint4*>(ks);
         } else {
-          *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(kw);
-          *reinterpret_cast<uint2*>(sc) = *reinterpret_cast<const uint2*>(ks);
+          *reinterpret_cast<uint2*>(w[j]) = *reinterpret_cast<const uint2*>(kw);
+          *reinterpret_cast<uint2*>(sc[j]) = *reinterpret_cast<const uint2*>(ks);
         }
-        const uint32_t mine2 = *reinterpret_cast<const uint32_t*>(tile + pages4::key_scales(D) + (8 * j1 + gid) * (2 * NG) + (NG == 4 ? 4 * (c & 1) : 0));
-        mma_bf16_first(x[j], over, mine2, mine2);
+        const uint32_t own = *reinterpret_cast<const uint32_t*>(tile + pages4::key_scales(D) + (8 * j1 + gid) * (2 * NG) + (NG == 4 ? 4 * (c & 1) : 0));
+        mma_bf16_first(x[j], over, own, own);
+      }
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
+      for (int gr = 0; gr < NG; ++gr) {
+        const uint4 qa = q_smem[2 * gr * 32 + lane], qb = q_smem[(2 * gr + 1) * 32 + lane];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
           float s[4];
-          mma_f16_first(s, qa[2 * gr], w[gr] & kEven, w[gr] & kOdd);
-          mma_f16(s, qa[2 * gr + 1], (w[gr] >> 8) & kEven, (w[gr] >> 8) & kOdd);
+          mma_f16_first(s, qa, w[j][gr] & kEven, w[j][gr] & kOdd);
+          mma_f16(s, qb, (w[j][gr] >> 8) & kEven, (w[j][gr] >> 8) & kOdd);
           // scales of position 2 c: halves gr of the first NG, of 2 c + 1: of the second
-          const float s0 = gr & 1 ? bf16_high(sc[gr >> 1]) : bf16_low(sc[gr >> 1]);
-          const float s1 = gr & 1 ? bf16_high(sc[NG / 2 + (gr >> 1)]) : bf16_low(sc[NG / 2 + (gr >> 1)]);
+          const float s0 = gr & 1 ? bf16_high(sc[j][gr >> 1]) : bf16_low(sc[j][gr >> 1]);
+          const float s1 = gr & 1 ? bf16_high(sc[j][NG / 2 + (gr >> 1)]) : bf16_low(sc[j][NG / 2 + (gr >> 1)]);
           x[j][0] = fmaf(s[0], s0, x[j][0]);
           x[j][1] = fmaf(s[1], s1, x[j][1]);
           x[j][2] = fmaf(s[2], s0, x[j][2]);
@@ -807,6 +833,14 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
       }
 
       // out += weights . values, a group of 32 components a time: its scales go into the weights
+      uint32_t pb[4][2];             // one term: the weights in bf16, rows gid and gid + 8
+      if constexpr (PT == 1) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          pb[j][0] = pack_bf16(x[j][0], x[j][1]);
+          pb[j][1] = pack_bf16(x[j][2], x[j][3]);
+        }
+      }
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
@@ -816,25 +850,31 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
           for (int h = 0; h < 2; ++h) {
             const int gr = 2 * i2 + h;
             const uint32_t w0 = h ? u.y : u.x, w1 = h ? u.w : u.z;
-            float p[2][4];
-#pragma unroll
-            for (int j1 = 0; j1 < 2; ++j1) {
-              const int j = 2 * tt + j1;
-              const float s0 = h ? bf16_high(vs[j][i2]) : bf16_low(vs[j][i2]), s1 = h ? bf16_high(vs[j][NG / 2 + i2]) : bf16_low(vs[j][NG / 2 + i2]);
-              p[j1][0] = x[j][0] * s0;
-              p[j1][1] = x[j][1] * s1;
-              p[j1][2] = x[j][2] * s0;
-              p[j1][3] = x[j][3] * s1;
-            }
             uint4 pa[PT];
+            if constexpr (PT == 1) {
+              // rounded to bf16 and multiplied by the scale there: positions 2 c and 2 c + 1 side by side
+              const uint32_t sa = pair_of(vs[2 * tt][i2], vs[2 * tt][NG / 2 + i2], h), sb = pair_of(vs[2 * tt + 1][i2], vs[2 * tt + 1][NG / 2 + i2], h);
+              pa[0] = make_uint4(mul_bf16(pb[2 * tt][0], sa), mul_bf16(pb[2 * tt][1], sa), mul_bf16(pb[2 * tt + 1][0], sb), mul_bf16(pb[2 * tt + 1][1], sb));
+            } else {
+              float p[2][4];
 #pragma unroll
-            for (int term = 0; term < PT; ++term) {
-              pa[term] = make_uint4(pack_bf16(p[0][0], p[0][1]), pack_bf16(p[0][2], p[0][3]), pack_bf16(p[1][0], p[1][1]), pack_bf16(p[1][2], p[1][3]));
-              if (term + 1 < PT) {
-                p[0][0] -= bf16_low(pa[term].x); p[0][1] -= bf16_high(pa[term].x);
-                p[0][2] -= bf16_low(pa[term].y); p[0][3] -= bf16_high(pa[term].y);
-                p[1][0] -= bf16_low(pa[term].z); p[1][1] -= bf16_high(pa[term].z);
-                p[1][2] -= bf16_low(pa[term].w); p[1][3] -= bf16_high(pa[term].w);
+              for (int j1 = 0; j1 < 2; ++j1) {
+                const int j = 2 * tt + j1;
+                const float s0 = h ? bf16_high(vs[j][i2]) : bf16_low(vs[j][i2]), s1 = h ? bf16_high(vs[j][NG / 2 + i2]) : bf16_low(vs[j][NG / 2 + i2]);
+                p[j1][0] = x[j][0] * s0;
+                p[j1][1] = x[j][1] * s1;
+                p[j1][2] = x[j][2] * s0;
+                p[j1][3] = x[j][3] * s1;
+              }
+#pragma unroll
+              for (int term = 0; term < PT; ++term) {
+                pa[term] = make_uint4(pack_bf16(p[0][0], p[0][1]), pack_bf16(p[0][2], p[0][3]), pack_bf16(p[1][0], p[1][1]), pack_bf16(p[1][2], p[1][3]));
+                if (term + 1 < PT) {
+                  p[0][0] -= bf16_low(pa[term].x); p[0][1] -= bf16_high(pa[term].x);
+                  p[0][2] -= bf16_low(pa[term].y); p[0][3] -= bf16_high(pa[term].y);
+                  p[1][0] -= bf16_low(pa[term].z); p[1][1] -= bf16_high(pa[term].z);
+                  p[1][2] -= bf16_low(pa[term].w); p[1][3] -= bf16_high(pa[term].w);
+                }
               }
             }
             const uint32_t eight = (gid >> 1) == gr ? 0x00080008u : 0u;       // columns 2 gr and 2 gr + 1: 8 times the weights' sum

@@ -520,7 +520,8 @@ def attend_check(ops, q, pages, table, lens, kk, vv, page, scale=None, cap=0.0, 
     g = got.double().cpu().numpy()
     # weights: exp2 2^-22 and sums of up to 2^12 additions a lane would be 2^-12 at worst, but each is of positive terms rounded to nearest: 64 warps' and lanes' partial
     # sums of some hundreds, 2^-24 * 300; the rounding of the weight to its terms, the output's own
-    weight = {BF16: 2.0 ** -8, F16: 2.0 ** -16, F32: 2.0 ** -24}[q.dtype]
+    # (bf16: the weight is rounded to 8 bits, and its product with a value's scale once more: twice 2^-8)
+    weight = {BF16: 2.0 ** -7, F16: 2.0 ** -16, F32: 2.0 ** -24}[q.dtype]
     # 16-bit queries: codes go into the products as 0 .. 15 and 8 for each comes off at the end, so that the sums on the way are up to 15 sum(w scale) in size whatever
     # the values are.  A warp adds a product of 16 positions (of the CTA's 64) a time to them, each addition off by 2^-23 of the sum at most (the matrix unit may cut off),
     # and some 8 more join the parts: a component whose values cancel, or whose codes are all near 8, is off by that and not by a share of itself.
