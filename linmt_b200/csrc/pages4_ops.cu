@@ -137,9 +137,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams a) 
 
 // ---- rows in and out of a pool -------------------------------------------------------------------
 //
-// A thread has eight components of one position and head, four neighbours the 32 of a scale.  Bound by the bytes moved.
-constexpr int kRowThreads = 256;
-
+// A CTA has 16 neighbours of the call's positions and some heads in turn, a thread eight components of one position (four neighbours share a scale).  Where positions fill
+// a tile one after the other, as in a text that is written at once, the CTA that has the tile's first does all 16 through shared memory: a
+// value's codes lie two bytes at a time among those of the positions beside it, and two-byte stores of many CTAs to the same sectors cost four times
+// what the bytes do.  Other positions go one by one.  Bound by the bytes moved (a text), by latency (a step's positions).
 struct RowsParams {
   unsigned char* data;
   int64_t stride_page, stride_head;
@@ -148,15 +149,20 @@ struct RowsParams {
   void* k;
   void* v;
   int64_t k_t, k_h, v_t, v_h;
-  int64_t words;            // t * heads * dim / 8
+  int32_t t, heads_each;
 };
 
+template <class T> struct Raw8 { uint4 r[sizeof(T) / 2]; };
 template <class T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  uint4 r[sizeof(T) / 2];
+__device__ __forceinline__ Raw8<T> load8(const T* p) {
+  Raw8<T> x;
 #pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-  const T* e = reinterpret_cast<const T*>(r);
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) x.r[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  return x;
+}
+template <class T>
+__device__ __forceinline__ void floats_of(const Raw8<T>& raw, float (&x)[8]) {
+  const T* e = reinterpret_cast<const T*>(raw.r);
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = to_float(e[i]);
 }
@@ -170,15 +176,43 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
   for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r[i];
 }
 
-// Codes and scale of the thread's eight components, the scale that of 32 in four neighbouring threads.
-__device__ __forceinline__ uint32_t quantise(float (&x)[8], __nv_bfloat16& scale) {
-  constexpr float kMost = 3.3895313892515355e38f;      // largest finite bf16
-  float hi = -INFINITY, lo = INFINITY;
+// Largest and smallest of the eight; NaN if one of them is.
+__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+template <class T, class T2>
+__device__ __forceinline__ void extremes16(const uint4& r, float& hi, float& lo) {
+  const T2* p = reinterpret_cast<const T2*>(&r);
+  const T2 a = __hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3])), b = __hmin2_nan(__hmin2_nan(p[0], p[1]), __hmin2_nan(p[2], p[3]));
+  hi = max_nan(to_float(T(a.x)), to_float(T(a.y)));
+  lo = min_nan(to_float(T(b.x)), to_float(T(b.y)));
+}
+__device__ __forceinline__ void extremes(const Raw8<__nv_bfloat16>& r, const float (&)[8], float& hi, float& lo) { extremes16<__nv_bfloat16, __nv_bfloat162>(r.r[0], hi, lo); }
+__device__ __forceinline__ void extremes(const Raw8<__half>& r, const float (&)[8], float& hi, float& lo) { extremes16<__half, __half2>(r.r[0], hi, lo); }
+__device__ __forceinline__ void extremes(const Raw8<float>&, const float (&x)[8], float& hi, float& lo) {
+  hi = lo = x[0];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -kMost), kMost);
-    hi = fmaxf(hi, x[i]);
-    lo = fminf(lo, x[i]);
+  for (int i = 1; i < 8; ++i) {
+    hi = max_nan(hi, x[i]);
+    lo = min_nan(lo, x[i]);
+  }
+}
+
+// Codes and scale of the thread's eight components, the scale that of 32 in four neighbouring threads; every lane of the warp calls it.
+template <class T>
+__device__ __forceinline__ uint32_t quantise(const Raw8<T>& raw, __nv_bfloat16& scale) {
+  constexpr float kMost = 3.3895313892515355e38f;      // largest finite bf16
+  float x[8], hi, lo;
+  floats_of(raw, x);
+  extremes(raw, x, hi, lo);
+  if (!(hi <= kMost && lo >= -kMost)) {
+    hi = -INFINITY;
+    lo = INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -kMost), kMost);
+      hi = fmaxf(hi, x[i]);
+      lo = fminf(lo, x[i]);
+    }
   }
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
@@ -187,76 +221,189 @@ __device__ __forceinline__ uint32_t quantise(float (&x)[8], __nv_bfloat16& scale
   }
   scale = __float2bfloat16_rn((hi >= -lo ? hi : lo) * -0.125f);
   const float s = __bfloat162float(scale);
-  uint32_t codes = 0;
+  if (s == 0.f) return 0x88888888u;
+  // A code is the quotient in 32 bits, rounded.  With the rounded reciprocal y of s, q = x y is one unit off at most and q + (x - q s) y, each a
+  // fused multiply-add, is the correctly rounded quotient (P. Markstein, IBM J. Res. Dev. 34, 1990), as long as nothing underflows on the way.
+  // 1.5 * 2^23 + 8 makes a float's last bits the code; a component is at most 8 (1 + 2^-8) scales in size, so only 8 itself has to be held to 7.
+  const float magic = 12582920.f;
+  float t[8];
+  if (fabsf(s) > 1e-30f && fabsf(s) < 1e30f) {
+    const float y = 1.f / s;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    // (a true quotient: a product with 1 / scale would round some components to the other neighbour)
-    const float c = s == 0.f ? 0.f : fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -8.f), 7.f);
-    codes |= (uint32_t)((int)c + 8) << (4 * i);
+    for (int i = 0; i < 8; ++i) {
+      const float q = x[i] * y;
+      t[i] = fminf(fmaf(fmaf(-q, s, x[i]), y, q), 7.f) + magic;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = fminf(fmaxf(__fdiv_rn(x[i], s), -8.f), 7.f) + magic;
   }
-  return codes;
+  uint32_t b[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(t[i]);
+  const uint32_t even = __byte_perm(__byte_perm(b[0], b[2], 0x0040), __byte_perm(b[4], b[6], 0x0040), 0x5410);
+  const uint32_t odds = __byte_perm(__byte_perm(b[1], b[3], 0x0040), __byte_perm(b[5], b[7], 0x0040), 0x5410);
+  return even | odds << 4;
+}
+
+// Where the CTA's 16 positions go: which are part of a tile that is filled in order (and done by the CTA that has its first), and the tile that begins here.
+struct Rows {
+  int64_t slot;            // of position threadIdx.x / W; -1 where there is none, or it has nothing to do
+  int64_t at;              // its tile's place in the pool (head 0)
+  int lead;                // 0..15: the position whose tile the CTA does; -1: none
+  int64_t lead_at;
+};
+template <int W, int BYTES>
+__device__ __forceinline__ Rows rows_of_cta(const RowsParams& a) {
+  constexpr int kReach = 15, kMine = 16 + kReach;
+  __shared__ int64_t slots[16 + 2 * kReach];
+  __shared__ int gap[kMine];               // no tile's 16 begin at position first - 15 + i
+  __shared__ int lead;
+  __shared__ int64_t lead_at;
+  const int tid = threadIdx.x;
+  const int64_t first = (int64_t)blockIdx.x * 16, most = (int64_t)a.n_pages * a.page;
+  auto place = [&](int64_t slot) {
+    const int64_t page = slot / a.page;
+    return page * a.stride_page + (int)(slot - page * a.page) / pages4::kTile * (int64_t)BYTES;
+  };
+  if (tid < 16 + 2 * kReach) {
+    const int64_t t = first - kReach + tid;
+    const int64_t s = t >= 0 && t < a.t ? __ldg(a.slots + t) : -1;
+    slots[tid] = s >= 0 && s < most ? s : -1;
+  }
+  if (tid < kMine) gap[tid] = 0;
+  if (tid == 0) lead = -1;
+  __syncthreads();
+  for (int i = tid; i < kMine * 16; i += 16 * W) {
+    const int64_t s = slots[i / 16];
+    if (s < 0 || (s & (pages4::kTile - 1)) || slots[i / 16 + i % 16] != s + i % 16) gap[i / 16] = 1;
+  }
+  __syncthreads();
+  if (tid >= kReach && tid < kMine && !gap[tid]) {     // one at most: two that overlap could not both go on by ones
+    lead = tid - kReach;
+    lead_at = place(slots[tid]);
+  }
+  const int j = kReach + tid / W;
+  Rows r;
+  r.slot = slots[j];
+  if (r.slot >= 0 && !gap[j - (int)(r.slot & (pages4::kTile - 1))]) r.slot = -1;
+  r.at = r.slot >= 0 ? place(r.slot) : 0;
+  __syncthreads();
+  r.lead = lead;
+  r.lead_at = lead_at;
+  return r;
 }
 
 template <class T, int D>
-__global__ void __launch_bounds__(kRowThreads) write_kernel(const RowsParams a) {
-  constexpr int W = D / 8;
-  const int64_t at = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
-  const int64_t th = min(at, a.words - 1) / W;                 // (the last warp's idle lanes repeat the last word: the shuffles need them)
-  const int w = (int)(min(at, a.words - 1) % W), h = (int)(th % a.heads);
-  const int64_t t = th / a.heads, slot = __ldg(a.slots + t), page = pages4::slot_page(slot, a.n_pages, a.page);
-  float x[8];
+__global__ void __launch_bounds__(2 * D) write_kernel(const RowsParams a) {
+  constexpr int W = D / 8, kBytes = pages4::tile_bytes(D);
+  __shared__ __align__(16) unsigned char tile[2][kBytes];
+  const int tid = threadIdx.x, j = tid / W, w = tid % W, h0 = blockIdx.y * a.heads_each, h1 = min(a.heads, h0 + a.heads_each);
+  const Rows rows = rows_of_cta<W, kBytes>(a);
+  auto put = [&](unsigned char* to, int r, uint32_t kc, uint32_t vc, __nv_bfloat16 ks, __nv_bfloat16 vs) {
+    *reinterpret_cast<uint32_t*>(to + pages4::key_word(r, w, D)) = kc;
+    *reinterpret_cast<uint16_t*>(to + pages4::value_four(r, 2 * w, D)) = (uint16_t)vc;
+    *reinterpret_cast<uint16_t*>(to + pages4::value_four(r, 2 * w + 1, D)) = (uint16_t)(vc >> 16);
+    if ((w & 3) == 0) {
+      *reinterpret_cast<__nv_bfloat16*>(to + pages4::key_scales(D) + pages4::scale_at(r, w >> 2, D)) = ks;
+      *reinterpret_cast<__nv_bfloat16*>(to + pages4::value_scales(D) + pages4::scale_at(r, w >> 2, D)) = vs;
+    }
+  };
   __nv_bfloat16 ks, vs;
-  load8(static_cast<const T*>(a.k) + t * a.k_t + h * a.k_h + 8 * w, x);
-  const uint32_t kc = quantise(x, ks);
-  load8(static_cast<const T*>(a.v) + t * a.v_t + h * a.v_h + 8 * w, x);
-  const uint32_t vc = quantise(x, vs);
-  if (page < 0 || at >= a.words) return;
-  const int pos = (int)(slot - page * a.page), r = pos % pages4::kTile;
-  unsigned char* tile = a.data + page * a.stride_page + h * a.stride_head + (int64_t)(pos / pages4::kTile) * pages4::tile_bytes(D);
-  *reinterpret_cast<uint32_t*>(tile + pages4::key_word(r, w, D)) = kc;
-  *reinterpret_cast<uint16_t*>(tile + pages4::value_four(r, 2 * w, D)) = (uint16_t)vc;
-  *reinterpret_cast<uint16_t*>(tile + pages4::value_four(r, 2 * w + 1, D)) = (uint16_t)(vc >> 16);
-  if ((w & 3) == 0) {
-    *reinterpret_cast<__nv_bfloat16*>(tile + pages4::key_scales(D) + pages4::scale_at(r, w >> 2, D)) = ks;
-    *reinterpret_cast<__nv_bfloat16*>(tile + pages4::value_scales(D) + pages4::scale_at(r, w >> 2, D)) = vs;
+  if (rows.lead >= 0) {
+    const int64_t t = (int64_t)blockIdx.x * 16 + rows.lead + j;
+    const T *k = static_cast<const T*>(a.k) + t * a.k_t + h0 * a.k_h + 8 * w, *v = static_cast<const T*>(a.v) + t * a.v_t + h0 * a.v_h + 8 * w;
+    Raw8<T> rk = load8(k), rv = load8(v);
+    for (int h = h0; h < h1; ++h) {
+      Raw8<T> nk = rk, nv = rv;
+      k += a.k_h;
+      v += a.v_h;
+      if (h + 1 < h1) { nk = load8(k); nv = load8(v); }
+      const uint32_t kc = quantise(rk, ks), vc = quantise(rv, vs);
+      unsigned char* const here = tile[h & 1];
+      put(here, j, kc, vc, ks, vs);
+      __syncthreads();              // (one for each head: the other tile's readers have come here too)
+      unsigned char* const to = a.data + rows.lead_at + h * a.stride_head;
+      for (int i = tid; i < kBytes / 16; i += 2 * D) reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(here)[i];
+      rk = nk;
+      rv = nv;
+    }
+  }
+  if (__any_sync(~0u, rows.slot >= 0)) {
+    const int64_t t = min((int64_t)blockIdx.x * 16 + j, (int64_t)a.t - 1);      // (lanes without a position take part in the scales' exchange)
+    for (int h = h0; h < h1; ++h) {
+      const Raw8<T> rk = load8(static_cast<const T*>(a.k) + t * a.k_t + h * a.k_h + 8 * w), rv = load8(static_cast<const T*>(a.v) + t * a.v_t + h * a.v_h + 8 * w);
+      const uint32_t kc = quantise(rk, ks), vc = quantise(rv, vs);
+      if (rows.slot >= 0) put(a.data + rows.at + h * a.stride_head, (int)(rows.slot & (pages4::kTile - 1)), kc, vc, ks, vs);
+    }
   }
 }
 
 template <class T, int D>
-__global__ void __launch_bounds__(kRowThreads) read_kernel(const RowsParams a) {
-  constexpr int W = D / 8;
-  const int64_t at = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
-  if (at >= a.words) return;
-  const int64_t th = at / W, t = th / a.heads, slot = __ldg(a.slots + t), page = pages4::slot_page(slot, a.n_pages, a.page);
-  const int w = (int)(at % W), h = (int)(th % a.heads);
-  uint32_t kc = 0, vc = 0;
-  float ks = 0.f, vs = 0.f;
-  if (page >= 0) {
-    const int pos = (int)(slot - page * a.page), r = pos % pages4::kTile;
-    const unsigned char* tile = a.data + page * a.stride_page + h * a.stride_head + (int64_t)(pos / pages4::kTile) * pages4::tile_bytes(D);
-    kc = *reinterpret_cast<const uint32_t*>(tile + pages4::key_word(r, w, D));
-    vc = *reinterpret_cast<const uint16_t*>(tile + pages4::value_four(r, 2 * w, D)) |
-         (uint32_t) * reinterpret_cast<const uint16_t*>(tile + pages4::value_four(r, 2 * w + 1, D)) << 16;
-    ks = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(tile + pages4::key_scales(D) + pages4::scale_at(r, w >> 2, D)));
-    vs = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(tile + pages4::value_scales(D) + pages4::scale_at(r, w >> 2, D)));
+__global__ void __launch_bounds__(2 * D) read_kernel(const RowsParams a) {
+  constexpr int W = D / 8, kBytes = pages4::tile_bytes(D);
+  static_assert(kBytes / 16 <= 2 * D, "a tile is one vector a thread");
+  __shared__ __align__(16) unsigned char tile[2][2][kBytes];
+  const int tid = threadIdx.x, j = tid / W, w = tid % W, h0 = blockIdx.y * a.heads_each, h1 = min(a.heads, h0 + a.heads_each);
+  const Rows rows = rows_of_cta<W, kBytes>(a);
+  auto get = [&](const unsigned char* from, int r, int64_t t, int h) {
+    const uint32_t kc = *reinterpret_cast<const uint32_t*>(from + pages4::key_word(r, w, D));
+    const uint32_t vc = *reinterpret_cast<const uint16_t*>(from + pages4::value_four(r, 2 * w, D)) |
+                        (uint32_t) * reinterpret_cast<const uint16_t*>(from + pages4::value_four(r, 2 * w + 1, D)) << 16;
+    const float ks = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(from + pages4::key_scales(D) + pages4::scale_at(r, w >> 2, D)));
+    const float vs = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(from + pages4::value_scales(D) + pages4::scale_at(r, w >> 2, D)));
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)((int)((kc >> (4 * i)) & 15) - 8) * ks;
+    store8(static_cast<T*>(a.k) + t * a.k_t + h * a.k_h + 8 * w, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)((int)((vc >> (4 * i)) & 15) - 8) * vs;
+    store8(static_cast<T*>(a.v) + t * a.v_t + h * a.v_h + 8 * w, x);
+  };
+  const int64_t own = (int64_t)blockIdx.x * 16 + j;
+  if (rows.lead >= 0) {
+    const unsigned char* const from = a.data + rows.lead_at + tid * 16;
+    const bool has = tid < kBytes / 16;
+    auto fetch = [&](int h) { return has && h < h1 ? __ldg(reinterpret_cast<const uint4*>(from + h * a.stride_head)) : make_uint4(0, 0, 0, 0); };
+    uint4 r0 = fetch(h0), r1 = fetch(h0 + 1);
+    for (int h = h0, at = 0; h < h1; h += 2, at ^= 1) {        // two heads a turn
+      if (has) {
+        reinterpret_cast<uint4*>(tile[at][0])[tid] = r0;
+        reinterpret_cast<uint4*>(tile[at][1])[tid] = r1;
+      }
+      r0 = fetch(h + 2);
+      r1 = fetch(h + 3);
+      __syncthreads();
+      get(tile[at][0], j, own + rows.lead, h);
+      if (h + 1 < h1) get(tile[at][1], j, own + rows.lead, h + 1);
+    }
   }
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = page < 0 ? 0.f : (float)((int)((kc >> (4 * i)) & 15) - 8) * ks;
-  store8(static_cast<T*>(a.k) + t * a.k_t + h * a.k_h + 8 * w, x);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = page < 0 ? 0.f : (float)((int)((vc >> (4 * i)) & 15) - 8) * vs;
-  store8(static_cast<T*>(a.v) + t * a.v_t + h * a.v_h + 8 * w, x);
+  if (rows.slot >= 0) {
+    for (int h = h0; h < h1; ++h) get(a.data + rows.at + h * a.stride_head, (int)(rows.slot & (pages4::kTile - 1)), own, h);
+  } else if (own < a.t) {
+    const int64_t s = __ldg(a.slots + own);
+    if (s < 0 || s >= (int64_t)a.n_pages * a.page) {
+      const float none[8] = {};
+      for (int h = h0; h < h1; ++h) {
+        store8(static_cast<T*>(a.k) + own * a.k_t + h * a.k_h + 8 * w, none);
+        store8(static_cast<T*>(a.v) + own * a.v_t + h * a.v_h + 8 * w, none);
+      }
+    }
+  }
 }
 
 template <bool WRITE, class T>
-void launch_rows(const RowsParams& p, int dim, unsigned blocks, cudaStream_t st) {
+void launch_rows(RowsParams p, int dim, cudaStream_t st) {
+  // Heads in turn where that leaves some 16 CTAs for each SM all the same: looking at the slots takes as long as a head.
+  const int64_t rows = ((int64_t)p.t + 15) / 16, each = rows * p.heads / (16 * 148);
+  p.heads_each = (int)(each < 1 ? 1 : each > p.heads ? p.heads : each);
+  const dim3 grid((unsigned)rows, (unsigned)((p.heads + p.heads_each - 1) / p.heads_each));
   if (WRITE) {
-    if (dim == 64) write_kernel<T, 64><<<blocks, kRowThreads, 0, st>>>(p);
-    else write_kernel<T, 128><<<blocks, kRowThreads, 0, st>>>(p);
+    if (dim == 64) write_kernel<T, 64><<<grid, 128, 0, st>>>(p);
+    else write_kernel<T, 128><<<grid, 256, 0, st>>>(p);
   } else {
-    if (dim == 64) read_kernel<T, 64><<<blocks, kRowThreads, 0, st>>>(p);
-    else read_kernel<T, 128><<<blocks, kRowThreads, 0, st>>>(p);
+    if (dim == 64) read_kernel<T, 64><<<grid, 128, 0, st>>>(p);
+    else read_kernel<T, 128><<<grid, 256, 0, st>>>(p);
   }
 }
 
@@ -272,15 +419,14 @@ int rows(const linmt_pages4_rows_args* g, const char* what) {
     return op_fail(LINMT_EINVAL, "%s: keys, values and their strides have to be multiples of 16 bytes", what);
   const linmt_pages4& pg = g->pages;
   RowsParams p{static_cast<unsigned char*>(pg.data), pg.stride_page, pg.stride_head, pg.n_pages, pg.heads, pg.page, g->slots, g->k, g->v,
-               g->k_stride_t, g->k_stride_h, g->v_stride_t, g->v_stride_h, (int64_t)g->t * pg.heads * (pg.dim / 8)};
-  const int64_t blocks = (p.words + kRowThreads - 1) / kRowThreads;
-  if (blocks > INT32_MAX) return op_fail(LINMT_ELIMIT, "%s: %lld components in one call", what, (long long)p.words * 8);
+               g->k_stride_t, g->k_stride_h, g->v_stride_t, g->v_stride_h, g->t, 1};
+  if (pg.heads > 65535) return op_fail(LINMT_ELIMIT, "%s: %d heads (at most 65535)", what, pg.heads);
   OnDevice on(g->device);
   if (on.err != cudaSuccess) return op_cuda(on.err, what);
   const cudaStream_t st = static_cast<cudaStream_t>(g->stream);
-  if (g->dtype == LINMT_F32) launch_rows<WRITE, float>(p, pg.dim, (unsigned)blocks, st);
-  else if (g->dtype == LINMT_BF16) launch_rows<WRITE, __nv_bfloat16>(p, pg.dim, (unsigned)blocks, st);
-  else launch_rows<WRITE, __half>(p, pg.dim, (unsigned)blocks, st);
+  if (g->dtype == LINMT_F32) launch_rows<WRITE, float>(p, pg.dim, st);
+  else if (g->dtype == LINMT_BF16) launch_rows<WRITE, __nv_bfloat16>(p, pg.dim, st);
+  else launch_rows<WRITE, __half>(p, pg.dim, st);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? LINMT_OK : op_cuda(e, what);
 }

@@ -424,6 +424,42 @@ def test_write_and_read(ops, t, heads, dim, page, dtype):
             assert torch.equal(r.cpu(), want.to(out))
 
 
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 48)])
+def test_write_and_read_of_texts(ops, dim, page):
+    """Positions one after the other, as a text's are: whole tiles that begin anywhere among the call's positions, beginnings and ends of tiles, tiles with a gap or two
+    places exchanged, and quotients that lie in the middle of two codes."""
+    rng = _rng(dim, page)
+    heads, n_pages = 3, 40
+    runs = [(0, 16), (33, 40), (96, 7), (112, 17), (160, 48), (223, 1), (240, 16), (258, 30), (304, 200)]
+    slots = np.concatenate([np.arange(a, a + n) for a, n in runs]).astype(np.int64)
+    at = int(np.nonzero(slots == 176)[0][0])
+    slots[at + 3], slots[at + 4] = slots[at + 4], slots[at + 3]
+    slots[np.nonzero(slots == 245)[0]] = -1
+    t = len(slots)
+    x = rng.normal(0, 1, (2, t, heads, dim)).astype(np.float32)
+    x[:, ::3] = rng.integers(-16, 17, (2, len(x[0, ::3]), heads, dim)) / 2          # halves of a scale of 1, where the largest is 8
+    x[:, ::3, :, ::32] = 8
+    k, v = _cuda(x[0]), _cuda(x[1])
+    pages = ops.new_pages4(n_pages, heads, dim, page)
+    pages.fill_(0x5A)
+    ops.write_pages4(pages, _cuda(slots), k, v)
+    (kc, vc), (ks, vs) = tile_ref(pages.cpu().numpy(), n_pages, heads, page, dim)
+    ok = slots >= 0
+    rest = np.ones(n_pages * page, bool)
+    rest[slots[ok]] = False
+    for y, got_c, got_s in ((x[0], kc, ks), (x[1], vc, vs)):
+        c, s, value = codes_ref(y)
+        got_c, got_s = got_c.reshape(-1, heads, dim), got_s.reshape(-1, heads, dim // 32)
+        assert (got_c[slots[ok]] == c.reshape(t, heads, dim)[ok]).all()
+        assert (got_s[slots[ok]] == s.view(torch.int16).numpy().view(np.uint16)[ok]).all()
+        assert (got_c[rest] == np.tile([10, 5], dim // 2)).all() and (got_s[rest] == 0x5A5A).all()
+    rk, rv = ops.read_pages4(pages, _cuda(slots))
+    for y, r in ((x[0], rk), (x[1], rv)):
+        want = codes_ref(y)[2].reshape(t, heads, dim)
+        want[~ok] = 0
+        assert torch.equal(r.cpu(), torch.from_numpy(want))
+
+
 def test_write_extremes_and_strides(ops):
     rng = _rng(9)
     t, heads, dim, page = 6, 2, 64, 16
