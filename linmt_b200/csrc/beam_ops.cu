@@ -161,31 +161,38 @@ struct Row {
   __device__ static uint4 nothing() { return make_uint4(Packed<T>::kNegInf, Packed<T>::kNegInf, Packed<T>::kNegInf, Packed<T>::kNegInf); }
   // Vector v as it lies there, if all of it belongs to the row.
   __device__ uint4 raw(int v) const { return __ldg(reinterpret_cast<const uint4*>(p + ((int64_t)v * E - shift))); }
-  // The same with -inf for what lies outside the row or is not allowed.
+  // Bits of a whole vector's elements that are allowed.
+  __device__ uint32_t bits_of(int v) const {
+    const int first = v * E - shift;
+    if (shift == 0) return __ldg(reinterpret_cast<const uint8_t*>(allowed) + (first >> 3)) >> (first & 7);
+    const int at = first >> 5;
+    return __funnelshift_r(__ldg(allowed + at), (first & 31) + E > 32 ? __ldg(allowed + at + 1) : 0u, first & 31);
+  }
+  // -inf for the elements whose bit is not set.
+  __device__ static uint4 keep(uint32_t bits, uint4 r) {
+    uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int h = 0; h < E / 4; ++h) {
+      // four bits to the tops of four bytes, and those over the elements' width
+      const uint32_t tops = ((bits >> (4 * h)) & 15) * 0x10204080u;
+#pragma unroll
+      for (int i = 0; i < 4 / P; ++i) {
+        const uint32_t all = top_bits(tops, P == 1 ? 0x8888 + 0x1111 * i : 0x9988 + 0x2222 * i);
+        uint32_t& x = w[h * (4 / P) + i];
+        x = (x & all) | (Packed<T>::kNegInf & ~all);
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // Vector v with -inf for what lies outside the row or is not allowed.
   __device__ uint4 clean(int v, bool is_whole, uint4 r) const {
     uint32_t w[4] = {r.x, r.y, r.z, r.w};
     const int first = v * E - shift;
     if (is_whole) {
       if (!allowed) return r;
-      uint32_t bits;
-      if (shift == 0) {
-        bits = __ldg(reinterpret_cast<const uint8_t*>(allowed) + (first >> 3)) >> (first & 7);
-      } else {
-        const int at = first >> 5;
-        bits = __funnelshift_r(__ldg(allowed + at), (first & 31) + E > 32 ? __ldg(allowed + at + 1) : 0u, first & 31);
-      }
-#pragma unroll
-      for (int h = 0; h < E / 4; ++h) {
-        // four bits to the tops of four bytes, and those over the elements' width
-        const uint32_t tops = ((bits >> (4 * h)) & 15) * 0x10204080u;
-#pragma unroll
-        for (int i = 0; i < 4 / P; ++i) {
-          const uint32_t keep = top_bits(tops, P == 1 ? 0x8888 + 0x1111 * i : 0x9988 + 0x2222 * i);
-          uint32_t& x = w[h * (4 / P) + i];
-          x = (x & keep) | (Packed<T>::kNegInf & ~keep);
-        }
-      }
-    } else {
+      return keep(bits_of(v), r);
+    }
+    {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         w[i] = Packed<T>::kNegInf;
@@ -257,15 +264,26 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
   const int most_chunks = ((a.vocab / E + 2) / per_row + kChunkVecs) / kChunkVecs;      // of any stretch of the sentence
   int group = 0;                         // chunks of a kept maximum, as a power of 2
   while ((most_chunks - 1) >> group >= kMaxima) ++group;
+  // (The next chunk is on its way while one is added up, where it lies in the row from end to end.)
+  uint4 ahead[4];
+  uint32_t ahead_bits[4];
+  auto inside = [&](int vb) { return vb >= r.whole0 && vb + kChunkVecs <= min(v1, r.whole1); };
+  auto fetch = [&](int vb) {
+    if (!inside(vb)) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      ahead[j] = r.raw(vb + lane + 32 * j);
+      if (r.allowed) ahead_bits[j] = r.bits_of(vb + lane + 32 * j);
+    }
+  };
+  fetch(v0);
   for (int c = 0; c < n_chunks; ++c) {
     const int vb = v0 + c * kChunkVecs;
     uint4 raw[4];
     float m;
-    if (vb >= r.whole0 && vb + kChunkVecs <= min(v1, r.whole1)) {
+    if (inside(vb)) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) raw[j] = r.raw(vb + lane + 32 * j);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) raw[j] = r.clean(vb + lane + 32 * j, true, raw[j]);
+      for (int j = 0; j < 4; ++j) raw[j] = r.allowed ? r.keep(ahead_bits[j], ahead[j]) : ahead[j];
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -275,6 +293,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
         if (v < v1) raw[j] = r.clean(v, whole, raw[j]);
       }
     }
+    fetch(vb + kChunkVecs);
     m = fmaxf(fmaxf(Packed<T>::max4(raw[0]), Packed<T>::max4(raw[1])), fmaxf(Packed<T>::max4(raw[2]), Packed<T>::max4(raw[3])));
     const int chunk_max = __reduce_max_sync(~0u, ordered(m));
     if (lane == 0) {
