@@ -210,6 +210,9 @@ struct Row {
   }
 };
 
+// Where part `part` of `parts` equal ones begins (the first n % parts are one longer).
+__device__ __forceinline__ int cut(int n, int part, int parts) { return part * (int)((uint32_t)n / (uint32_t)parts) + min(part, (int)((uint32_t)n % (uint32_t)parts)); }
+
 // A float as an integer that is ordered alike.
 __device__ __forceinline__ int ordered(float x) {
   const int b = __float_as_int(x + 0.f);
@@ -224,8 +227,8 @@ __device__ __forceinline__ float exp2_of(float x) {
 
 // Bound on the error of a row's log of its sum as a lane adds it up in `chunks` steps: two roundings of an exponent's argument
 // (2^-24 of it, on average at most log2(vocab) + 1), exp2's own 2^-22, 20 additions deep inside and across lanes, and for each chunk one
-// addition and one change of the maximum.
-__device__ __forceinline__ double row_error(int chunks) { return 4.2e-6 + 4.5e-7 * chunks; }
+// addition and one change of the maximum; the same once more where the stretches' sums are joined, and the logarithm's last place, 2^-20 below 16.
+__device__ __forceinline__ double row_error(int chunks) { return 7e-6 + 4.5e-7 * chunks; }
 
 template <class T, int C>
 __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectParams<T> a) {
@@ -255,7 +258,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
   const bool busy = unit < per_row * n_live;
   const int row = busy ? s.live[unit / per_row] : 0, part = busy ? unit % per_row : 0;
   const Row<T> r(a.logits + sent * a.stride_n + row * a.stride_k, a.vocab, a.allowed ? a.allowed + sent * a.allowed_stride : nullptr);
-  const int v0 = (int)((int64_t)r.n_vecs * part / per_row), v1 = busy ? (int)((int64_t)r.n_vecs * (part + 1) / per_row) : v0;
+  const int v0 = cut(r.n_vecs, part, per_row), v1 = busy ? cut(r.n_vecs, part + 1, per_row) : v0;
 
   // 1. the stretch, once
   float top = -INFINITY, sum = 0.f;
@@ -360,14 +363,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
     for (int u = lane; u < per_row; u += 32) m = fmaxf(m, s.unit_max[i * per_row + u]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    double t = 0.0;
+    float t = 0.f;
     for (int u = i * per_row + lane; u < (i + 1) * per_row; u += 32)
-      t += s.unit_max[u] == -INFINITY ? s.unit_sum[u] : s.unit_sum[u] * exp((double)s.unit_max[u] - (double)m);
+      t += s.unit_max[u] == -INFINITY ? (float)s.unit_sum[u] : (float)s.unit_sum[u] * exp2_of((s.unit_max[u] - m) * kLog2e);
 #pragma unroll
     for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
     if (lane == 0) {
       s.row_max[s.live[i]] = m;
-      s.row_lse[s.live[i]] = m == -INFINITY ? (double)NAN : log(t);
+      s.row_lse[s.live[i]] = m == -INFINITY ? (double)NAN : (double)logf(t);
     }
   }
   __syncthreads();
@@ -464,7 +467,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
       for (int i = warp; i < n_todo; i += kWarps) {
         const int w = s.todo[i] / kMaxima, g = s.todo[i] % kMaxima, u = w * C + cta, rw = s.live[u / per_row], pt = u % per_row;
         const Row<T> q(a.logits + sent * a.stride_n + rw * a.stride_k, a.vocab, r.allowed);
-        const int q0 = (int)((int64_t)q.n_vecs * pt / per_row), q1 = (int)((int64_t)q.n_vecs * (pt + 1) / per_row);
+        const int q0 = cut(q.n_vecs, pt, per_row), q1 = cut(q.n_vecs, pt + 1, per_row);
         const double sc = s.score[rw], bs = s.row_max[rw], ls = s.row_lse[rw];
         const float floor_x = floor_of(sc, ls, bs);
         const int c1 = min((g + 1) << group, (q1 - q0 + kChunkVecs - 1) / kChunkVecs);
@@ -610,8 +613,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
     // equal sums and their ties stay ties.
     if (busy && ((ask >> row) & 1)) {
       double t = 0.0;
-      const int e1 = (int)((int64_t)a.vocab * (part + 1) / per_row);
-      for (int at = (int)((int64_t)a.vocab * part / per_row) + lane; at < e1; at += 32)
+      const int e1 = cut(a.vocab, part + 1, per_row);
+      for (int at = cut(a.vocab, part, per_row) + lane; at < e1; at += 32)
         if (r.may(at)) t += exp((double)to_float(r.p[at]) - base);
 #pragma unroll
       for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
@@ -635,9 +638,13 @@ template <class T>
 cudaError_t launch_select(const linmt_beam_select_args& g) {
   SelectParams<T> p{static_cast<const T*>(g.logits), g.stride_n, g.stride_k, g.scores, g.done, g.allowed, g.allowed_stride,
                     g.out_tokens, g.out_parents, g.out_scores, g.out_done, g.k, g.vocab, g.eos};
-  // As many CTAs for a sentence as leave every sentence on the GPU at once (two CTAs on an SM, clusters of 8 only reach 33): a second
-  // round of clusters costs its latencies, some 6 us, again.  24 warps of 2 CTAs have a row each for 24 beams at most.
-  const int c = g.n <= 33 ? 8 : g.n <= 74 || g.k > 2 * kWarps ? 4 : 2;
+  // As many CTAs for a sentence as leave all of them on the GPU at once (two on an SM; clusters of 8 only reach 33), since a second round of
+  // clusters costs its latencies again, and as have 16k logits each: exchanges among more take longer (64 x 12 x 30k fp32: 40, 30 and 51 us
+  // with 2, 4 and 8; 128 x 12 x 80k bf16: 82, 95 and 141; 1 x 4 x 1000: 10.2, 10.6 and 12.4).  A warp needs a row at most: 12 beams for one CTA.
+  const int64_t logits = (int64_t)g.k * g.vocab;
+  int c = g.n <= 33 ? 8 : g.n <= 74 ? 4 : g.n <= 148 ? 2 : 1;
+  while (c > 1 && logits < (int64_t)(c / 2 + 1) * 16384) c /= 2;
+  while (c * kWarps < g.k) c *= 2;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -648,7 +655,7 @@ cudaError_t launch_select(const linmt_beam_select_args& g) {
   cfg.stream = static_cast<cudaStream_t>(g.stream);
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, c == 8 ? select_kernel<T, 8> : c == 4 ? select_kernel<T, 4> : select_kernel<T, 2>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, c == 8 ? select_kernel<T, 8> : c == 4 ? select_kernel<T, 4> : c == 2 ? select_kernel<T, 2> : select_kernel<T, 1>, p);
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
