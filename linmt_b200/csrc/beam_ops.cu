@@ -57,10 +57,11 @@ __device__ __forceinline__ bool bid_before(Key s, int32_t at, int i, Key s2, int
 }
 
 struct SelectSmem {
-  float unit_max[kMaxC * kWarps];
-  double unit_sum[kMaxC * kWarps];
+  float unit_max[kMaxC * kWarps], unit_sum[kMaxC * kWarps];
+  int32_t unit_changes[kMaxC * kWarps];      // most often that a lane's maximum changed
   double row_lse[kMaxK];         // log of the row's sum, relative to row_max
   float row_max[kMaxK];
+  int32_t row_changes[kMaxK];
   float score[kMaxK];
   int32_t live[kMaxK];           // rows that are read, in order
   uint32_t done_bits, finite_bits, exact_bits, ask_bits;   // per row: finished; score is finite; summed in 64 bits; to be summed so
@@ -225,10 +226,11 @@ __device__ __forceinline__ float exp2_of(float x) {
   return y;
 }
 
-// Bound on the error of a row's log of its sum as a lane adds it up in `chunks` steps: two roundings of an exponent's argument
-// (2^-24 of it, on average at most log2(vocab) + 1), exp2's own 2^-22, 20 additions deep inside and across lanes, and for each chunk one
-// addition and one change of the maximum; the same once more where the stretches' sums are joined, and the logarithm's last place, 2^-20 below 16.
-__device__ __forceinline__ double row_error(int chunks) { return 7e-6 + 4.5e-7 * chunks; }
+// Bound on the error of a row's log of its sum, where a lane adds it up in `chunks` steps and changes its maximum `changes` times: two roundings of
+// an exponent's argument (2^-24 of it, on average at most log2(vocab) + 1 in size: 1.5e-6 below a vocabulary of 2^17), exp2's own 2^-22, 20 additions
+// deep inside and across lanes, the same where stretches are joined, the logarithm's last place (2^-20 below 16); an addition
+// for each chunk, and an exp2 and a product for each change.
+__device__ __forceinline__ double row_error(int chunks, int changes) { return 6e-6 + 6e-8 * chunks + 4.5e-7 * changes; }
 
 template <class T, int C>
 __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectParams<T> a) {
@@ -262,7 +264,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
 
   // 1. the stretch, once
   float top = -INFINITY, sum = 0.f;
-  int top_vec = 0;                       // first vector of the warp's chunk that the lane's maximum is in
+  int changes = 0, top_vec = 0;          // first vector of the warp's chunk that the lane's maximum is in
   const int n_chunks = (v1 - v0 + kChunkVecs - 1) / kChunkVecs;
   const int most_chunks = ((a.vocab / E + 2) / per_row + kChunkVecs) / kChunkVecs;      // of any stretch of the sentence
   int group = 0;                         // chunks of a kept maximum, as a power of 2
@@ -308,6 +310,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
       sum *= exp2_of((top - m) * kLog2e);
       top = m;
       top_vec = vb;
+      ++changes;
     }
     const float base = top == -INFINITY ? 0.f : top;     // (nothing allowed yet: every term is exp2(-inf), or a NaN, which stays one)
     float part_sum[4];
@@ -332,11 +335,13 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
   float wsum = top == -INFINITY ? sum : sum * exp2_of((top - wtop) * kLog2e);
 #pragma unroll
   for (int o = 16; o; o >>= 1) wsum += __shfl_xor_sync(~0u, wsum, o);
+  const int wchanges = __reduce_max_sync(~0u, changes);
   cluster.barrier_wait();
   if (busy && lane < C) {
     SelectSmem* to = cluster.map_shared_rank(&s, lane);
     to->unit_max[unit] = wtop;
-    to->unit_sum[unit] = (double)wsum;
+    to->unit_sum[unit] = wsum;
+    to->unit_changes[unit] = wchanges;
   }
   cluster.sync();
 
@@ -354,7 +359,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
     }
   const int best_bits = (int)((uint32_t)(lane_bid >> 32) ^ 0x80000000u), best_at = (int)~(uint32_t)lane_bid;
   const float best = __int_as_float(best_bits ^ ((best_bits >> 31) & 0x7fffffff));
-  const double near = 2 * row_error((a.vocab / E + 2) / (per_row * kChunkVecs) + 2);
   SelectSmem* const lead = cluster.map_shared_rank(&s, 0);
 
   // The rows' normalisers from the units' sums, a warp for each.
@@ -364,13 +368,18 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
     float t = 0.f;
-    for (int u = i * per_row + lane; u < (i + 1) * per_row; u += 32)
-      t += s.unit_max[u] == -INFINITY ? (float)s.unit_sum[u] : (float)s.unit_sum[u] * exp2_of((s.unit_max[u] - m) * kLog2e);
+    int most = 0;
+    for (int u = i * per_row + lane; u < (i + 1) * per_row; u += 32) {
+      t += s.unit_max[u] == -INFINITY ? s.unit_sum[u] : s.unit_sum[u] * exp2_of((s.unit_max[u] - m) * kLog2e);
+      most = max(most, s.unit_changes[u]);
+    }
+    most = __reduce_max_sync(~0u, most);
 #pragma unroll
     for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
     if (lane == 0) {
       s.row_max[s.live[i]] = m;
       s.row_lse[s.live[i]] = m == -INFINITY ? (double)NAN : (double)logf(t);
+      s.row_changes[i] = most;
     }
   }
   __syncthreads();
@@ -567,6 +576,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
       if (warp == 0) {
         // Pair i = sorted i and i + 1.  The first pair from the k-th on that is not near closes the order: what comes behind it cannot be
         // among the k best.  A near pair of two rows before that, one of them summed in 32 bits, has to be settled.
+        const int changes_most = __reduce_max_sync(~0u, lane < n_live ? s.row_changes[lane] : 0);
+        const double near = 2 * row_error(most_chunks, changes_most);
         uint32_t near_bits[2], unsure_bits[2], ask = 0;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -609,25 +620,36 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
       }
       return;
     }
-    // The rows that are asked for, in 64 bits: cut and added up by the words' own numbers, wherever the row begins, so that equal rows get
-    // equal sums and their ties stay ties.
-    if (busy && ((ask >> row) & 1)) {
-      double t = 0.0;
-      const int e1 = cut(a.vocab, part + 1, per_row);
-      for (int at = cut(a.vocab, part, per_row) + lane; at < e1; at += 32)
-        if (r.may(at)) t += exp((double)to_float(r.p[at]) - base);
+    // The rows that are asked for, in 64 bits, a part by each of the cluster's warps: cut and added up by the words' own numbers, wherever
+    // the row begins, so that equal rows get equal sums and their ties stay ties.  (The list's place is free.)
+    constexpr int kRowsAtOnce = kMaxList / (kMaxC * kWarps);
+    for (uint32_t left = ask; left;) {
+      uint32_t now = 0;
+      for (int i = 0; i < kRowsAtOnce && left; ++i) { now |= left & (0u - left); left &= left - 1; }
+      int i = 0;
+      for (uint32_t rows = now; rows; rows &= rows - 1, ++i) {
+        const int rw = __ffs(rows) - 1;
+        const T* const p = a.logits + sent * a.stride_n + rw * a.stride_k;
+        const double m = s.row_max[rw];
+        double t = 0.0;
+        const int e1 = cut(a.vocab, unit + 1, kUnits);
+        for (int at = cut(a.vocab, unit, kUnits) + lane; at < e1; at += 32)
+          if (r.may(at)) t += exp((double)to_float(p[at]) - m);
 #pragma unroll
-      for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
-      if (lane < C) cluster.map_shared_rank(&s, lane)->unit_sum[unit] = t;
-    }
-    cluster.sync();
-    for (int i = warp; i < n_live; i += kWarps) {
-      if (!((ask >> s.live[i]) & 1)) continue;
-      double t = 0.0;
-      for (int u = lane; u < per_row; u += 32) t += s.unit_sum[i * per_row + u];
+        for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
+        if (lane < C) reinterpret_cast<double*>(cluster.map_shared_rank(&s, lane)->list)[i * kUnits + unit] = t;
+      }
+      cluster.sync();
+      i = 0;
+      for (uint32_t rows = now; rows; rows &= rows - 1, ++i) {
+        if (i % kWarps != warp) continue;
+        double t = 0.0;
+        for (int u = lane; u < kUnits; u += 32) t += reinterpret_cast<const double*>(s.list)[i * kUnits + u];
 #pragma unroll
-      for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
-      if (lane == 0) s.row_lse[s.live[i]] = log(t);
+        for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
+        if (lane == 0) s.row_lse[__ffs(rows) - 1] = log(t);
+      }
+      cluster.sync();              // (before the next rows' parts are written, or the next list)
     }
     if (tid == 0) s.exact_bits |= ask;
     __syncthreads();

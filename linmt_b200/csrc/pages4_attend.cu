@@ -6,14 +6,13 @@
 // operand of mma.m16n8k16, so every code is loaded and unpacked once for all of them.  (tcgen05.mma wants both operands of at least 64
 // rows, and codes unpacked into shared memory first; with 16 rows the unpacking, not the product, is what takes the time.)
 //   Scales stay out of the products: a key's is multiplied onto its group's sum, a value's into the weight on the left.
-//   16-bit queries (attend16_kernel).  A word's codes become matrix operands with one AND each: an integer in the low bits of a
-//   bf16 or fp16 number is a subnormal one, that integer times 2^-133 or 2^-24, and stays so up to 255 and 2047, so every second
+//   16-bit queries (attend16_kernel).  A word's codes become matrix operands with one AND each: an integer in the low bits of an
+//   fp16 number is a subnormal one, that integer times 2^-24, and stays so up to 2047, so every second
 //   code may be left four bits up and its 16 taken out elsewhere (of the queries before, of the output's columns after).  What is then too much, 8 for each
 //   code, goes off by a product of its own: the queries' sums with the keys' scales, and the weights' sums.  That is 5
 //   instructions for 8 codes where a code minus 8 in normal form takes 11, in a kernel bound by what it can issue.  Queries are scaled to
-//   fp16's upper range by a power of 2 for each row, weights by one for each warp (after the first values' scale), so that nothing that matters
-//   falls out of range.  For bf16 queries weights are rounded to bf16, and once more when a scale is multiplied in there (2^-7 at most, on average over the
-//   positions far less, and the output's own rounding is 2^-8); for fp16 they are taken as two bf16 terms (2^-16).
+//   fp16's upper range by a power of 2 for each row.  Weights are multiplied by their values' scales and rounded to fp16 (2^-11 each at most), with a power of 2
+//   that follows the scales, as the maximum follows the scores: the largest scale lies 2^3 above 1, and a weight 2^28 below the largest still counts.
 //   32-bit queries (attend32_kernel) are three bf16 terms, the weights too (2^-24), the codes minus 8 in normal form.
 // Every warp has a ring of tiles of its own (cp.async, no barrier among warps) and its own maximum and sums; the CTA's four are
 // joined through shared memory at the end of a piece of work, and where a sentence's positions are shared by CTAs a second kernel joins those.
@@ -28,14 +27,11 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kStages = 4;         // of attend32_kernel: tiles
-constexpr int kPairStages = 3;     // of attend16_kernel: pairs of tiles
+constexpr int kPairStages = 2;     // of attend16_kernel: pairs of tiles (three: 2 % longer)
 constexpr int kRows = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTerms = 3;          // bf16 terms of a 32-bit query and weight
 constexpr float kSlack = 8.f;      // the reference maximum follows the true one only when it lags by 2^8: few tiles rescale the sums
-
-template <class T> struct Fp16 { static constexpr bool value = false; };
-template <> struct Fp16<__half> { static constexpr bool value = true; };
 
 struct AttendParams {
   const unsigned char* data;
@@ -92,11 +88,10 @@ __device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {
   __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&off));
   return *reinterpret_cast<uint32_t*>(&r);
 }
-// The low (or high) halves of two words, side by side.
-__device__ __forceinline__ uint32_t pair_of(uint32_t a, uint32_t b, int high) { return __byte_perm(a, b, high ? 0x7632 : 0x5410); }
-__device__ __forceinline__ uint32_t mul_bf16(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ __nv_bfloat162 bf16_pair(uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); }
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 __device__ __forceinline__ float bf16_low(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float bf16_high(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
@@ -564,7 +559,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend32_kernel(
 
 template <class T, int D>
 __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(const __grid_constant__ AttendParams a) {
-  constexpr int NG = D / 32, kTileBytes = pages4::tile_bytes(D), PT = sizeof(T) == 2 && Fp16<T>::value ? 2 : 1;
+  constexpr int NG = D / 32, kTileBytes = pages4::tile_bytes(D);
   constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;
   extern __shared__ __align__(16) unsigned char smem[];
   launch_next();
@@ -697,9 +692,9 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
     const bool plain = a.cap == 0.f && !a.slope && a.scale != 0.f;       // scores are products times mul
     const float cap_log2 = a.cap * kLog2e;
 
-    // Sums are kept times 2^up (a weight p is p 2^up), and those of values times 2^-133 as the codes are.
-    float o[NG][4][4] = {}, extra[4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, up = 0.f;
-    bool begun = false;
+    // The values' sums are kept times 2^-24, as the codes are, and times the power of 2 that brings their scales into fp16's range.
+    float o[NG][4][4] = {}, extra[4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, size = 1.f;   // size: that power
+    uint32_t limit = 0;              // bits of the bf16 that no scale may reach with `size` as it is
     int stage = 0;
     for (int i = 0; i < mine; ++i) {
       copy_wait<kPairStages - 2>();
@@ -811,17 +806,27 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
             }
         }
       }
-      if (!begun) {            // the power of 2 that brings weights times these scales to some 2^50
-        begun = true;
-        int most = 0;
+      // The power of 2 that takes the largest scale to 2^3 .. 2^4; it changes with a scale 2^3 larger (a weight's 2^8 and that leave 2^15 at most).
+      __nv_bfloat162 most2 = __habs2(bf16_pair(vs[0][0]));
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int i2 = 0; i2 < NG; ++i2) most = max(most, max((int)(vs[j][i2] >> 7) & 255, (int)(vs[j][i2] >> 23) & 255));
-        most = __reduce_max_sync(~0u, most);
-        up = (float)min(90, max(-60, 50 - (most ? most - 127 : 0)));
+        for (int i2 = 0; i2 < NG; ++i2) most2 = __hmax2(most2, __habs2(bf16_pair(vs[j][i2])));
+      const uint32_t most = max(*reinterpret_cast<const uint32_t*>(&most2) & 0xffffu, *reinterpret_cast<const uint32_t*>(&most2) >> 16);
+      if (__any_sync(~0u, most >= limit)) {
+        const int e = min(max((int)(__reduce_max_sync(~0u, most) >> 7) - 127, -97), 103);
+        const float now = exp2_of((float)(3 - e)), f = limit ? now / size : 1.f;
+        size = now;
+        limit = (uint32_t)min(e + 127 + 4, 255) << 7;
+        extra[0] *= f; extra[2] *= f;
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+          for (int e4 = 0; e4 < 4; ++e4)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) o[gr][e4][i4] *= f;
       }
-      const float m0 = (m[0] == -INFINITY ? 0.f : m[0]) - up, m1 = (m[1] == -INFINITY ? 0.f : m[1]) - up;
+      const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         x[j][0] = exp2_of(fmaf(x[j][0], r0, -m0));
@@ -830,17 +835,11 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
         x[j][3] = exp2_of(fmaf(x[j][3], r1, -m1));
         l[0] += x[j][0] + x[j][1];
         l[1] += x[j][2] + x[j][3];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[j][e] *= size;
       }
 
       // out += weights . values, a group of 32 components a time: its scales go into the weights
-      uint32_t pb[4][2];             // one term: the weights in bf16, rows gid and gid + 8
-      if constexpr (PT == 1) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          pb[j][0] = pack_bf16(x[j][0], x[j][1]);
-          pb[j][1] = pack_bf16(x[j][2], x[j][3]);
-        }
-      }
 #pragma unroll
       for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
@@ -850,59 +849,36 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
           for (int h = 0; h < 2; ++h) {
             const int gr = 2 * i2 + h;
             const uint32_t w0 = h ? u.y : u.x, w1 = h ? u.w : u.z;
-            uint4 pa[PT];
-            if constexpr (PT == 1) {
-              // rounded to bf16 and multiplied by the scale there: positions 2 c and 2 c + 1 side by side
-              const uint32_t sa = pair_of(vs[2 * tt][i2], vs[2 * tt][NG / 2 + i2], h), sb = pair_of(vs[2 * tt + 1][i2], vs[2 * tt + 1][NG / 2 + i2], h);
-              pa[0] = make_uint4(mul_bf16(pb[2 * tt][0], sa), mul_bf16(pb[2 * tt][1], sa), mul_bf16(pb[2 * tt + 1][0], sb), mul_bf16(pb[2 * tt + 1][1], sb));
-            } else {
-              float p[2][4];
+            uint32_t pa[2][2];       // [half of the positions][row gid, row gid + 8]
 #pragma unroll
-              for (int j1 = 0; j1 < 2; ++j1) {
-                const int j = 2 * tt + j1;
-                const float s0 = h ? bf16_high(vs[j][i2]) : bf16_low(vs[j][i2]), s1 = h ? bf16_high(vs[j][NG / 2 + i2]) : bf16_low(vs[j][NG / 2 + i2]);
-                p[j1][0] = x[j][0] * s0;
-                p[j1][1] = x[j][1] * s1;
-                p[j1][2] = x[j][2] * s0;
-                p[j1][3] = x[j][3] * s1;
-              }
-#pragma unroll
-              for (int term = 0; term < PT; ++term) {
-                pa[term] = make_uint4(pack_bf16(p[0][0], p[0][1]), pack_bf16(p[0][2], p[0][3]), pack_bf16(p[1][0], p[1][1]), pack_bf16(p[1][2], p[1][3]));
-                if (term + 1 < PT) {
-                  p[0][0] -= bf16_low(pa[term].x); p[0][1] -= bf16_high(pa[term].x);
-                  p[0][2] -= bf16_low(pa[term].y); p[0][3] -= bf16_high(pa[term].y);
-                  p[1][0] -= bf16_low(pa[term].z); p[1][1] -= bf16_high(pa[term].z);
-                  p[1][2] -= bf16_low(pa[term].w); p[1][3] -= bf16_high(pa[term].w);
-                }
-              }
+            for (int j1 = 0; j1 < 2; ++j1) {
+              const int j = 2 * tt + j1;
+              const float s0 = h ? bf16_high(vs[j][i2]) : bf16_low(vs[j][i2]), s1 = h ? bf16_high(vs[j][NG / 2 + i2]) : bf16_low(vs[j][NG / 2 + i2]);
+              pa[j1][0] = pack_f16(x[j][0] * s0, x[j][1] * s1);
+              pa[j1][1] = pack_f16(x[j][2] * s0, x[j][3] * s1);
             }
+            const uint4 weights = make_uint4(pa[0][0], pa[0][1], pa[1][0], pa[1][1]);
             const uint32_t eight = (gid >> 1) == gr ? 0x00080008u : 0u;       // columns 2 gr and 2 gr + 1: 8 times the weights' sum
-#pragma unroll
-            for (int term = PT - 1; term >= 0; --term) {
-              mma_bf16(o[gr][0], pa[term], w0 & kEven, w1 & kEven);
-              mma_bf16(o[gr][1], pa[term], w0 & kOdd, w1 & kOdd);
-              mma_bf16(o[gr][2], pa[term], (w0 >> 8) & kEven, (w1 >> 8) & kEven);
-              mma_bf16(o[gr][3], pa[term], (w0 >> 8) & kOdd, (w1 >> 8) & kOdd);
-              mma_bf16(extra, pa[term], eight, eight);
-            }
+            mma_f16(o[gr][0], weights, w0 & kEven, w1 & kEven);
+            mma_f16(o[gr][1], weights, w0 & kOdd, w1 & kOdd);
+            mma_f16(o[gr][2], weights, (w0 >> 8) & kEven, (w1 >> 8) & kEven);
+            mma_f16(o[gr][3], weights, (w0 >> 8) & kOdd, (w1 >> 8) & kOdd);
+            mma_f16(extra, weights, eight, eight);
           }
         }
       }
     }
 
-    // From the sums as they are kept to sums relative to 2^m: less 8 for each code, times 2^133 / 2^up.
-    const float fa = exp2f(66.f - up * 0.5f), fb = exp2f(67.f - up * 0.5f), back = exp2f(-up);
+    // From the sums as they are kept to sums of values: less 8 for each code, times 2^24 / size.
+    const float by = 16777216.f / size;
 #pragma unroll
     for (int gr = 0; gr < NG; ++gr) {
       const float e0 = __shfl_sync(~0u, extra[0], (lane & ~3) | gr), e1 = __shfl_sync(~0u, extra[2], (lane & ~3) | gr);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[gr][e][i] = (o[gr][e][i] * fa * (e & 1 ? 0.0625f : 1.f) - (i < 2 ? e0 : e1) * fa) * fb;
+        for (int i = 0; i < 4; ++i) o[gr][e][i] = fmaf(o[gr][e][i], e & 1 ? 0.0625f : 1.f, -(i < 2 ? e0 : e1)) * by;
     }
-    l[0] *= back;
-    l[1] *= back;
     join_warps<T, D>(a, piece, job, smem, o, m, l);
   }
 }

@@ -80,9 +80,9 @@ def select_check(ops, logits, scores, done=None, allowed=None, eos=1):
     g = got[2].cpu().numpy().astype(np.float64)
     assert (np.isneginf(g) == np.isneginf(sc)).all()
     ok = np.isfinite(sc)
-    # the bound of a 32-bit normaliser: 7e-6 (exponents' arguments 2^-23 log2(vocab) twice, exp2 2^-22 twice, 40 additions of 2^-24, the logarithm 2^-20) and 4.5e-7 (an
-    # addition and an exp2) for each of a lane's steps (at most ceil(vocab / 512) + 2 of them), and the result's own rounding
-    tol = 7e-6 + 4.5e-7 * (-(-logits.shape[2] // 512) + 2)
+    # the bound of a 32-bit normaliser: 6e-6 (exponents' arguments 2^-23 log2(vocab), exp2 2^-22 twice, 40 additions of 2^-24, the logarithm 2^-20) and 5.1e-7 (an addition, an
+    # exp2 and a product) for each of a lane's steps (at most ceil(vocab / 512) + 2 of them), and the result's own rounding
+    tol = 6e-6 + 5.1e-7 * (-(-logits.shape[2] // 512) + 2)
     assert (np.abs(g[ok] - sc[ok]) <= tol + 2.0 ** -24 * np.abs(sc[ok])).all()
     return got
 
@@ -548,6 +548,7 @@ def attend_check(ops, q, pages, table, lens, kk, vv, page, scale=None, cap=0.0, 
     got, lse = ops.attend_pages4(q, pages, _cuda(table), _cuda(np.asarray(lens, np.int32)), scale=scale, cap=cap, slope=dev(slope), centre=dev(centre), first=dev(first), last=dev(last), want_lse=True, out=out)
     dim = q.shape[3]
     scale = dim ** -0.5 if scale is None else scale
+    big_scale = float(np.abs(vv).max()) / 7
     want, wlse, wv, big, ws = attend_ref(q.double().cpu().numpy(), kk, vv, table, lens, page, scale, cap, slope, centre, first, last, pages.shape[0])
     # A score: products of exact values added in 32 bits, at most dim + 8 additions and products; the cap's tanh to 2e-7 of the cap (16-bit queries) and the bias
     # and the change to powers of two a few roundings of their own size.  Queries in 32 bits are exact to 2^-24 in three terms.
@@ -557,12 +558,14 @@ def attend_check(ops, q, pages, table, lens, kk, vv, page, scale=None, cap=0.0, 
     g = got.double().cpu().numpy()
     # weights: exp2 2^-22 and sums of up to 2^12 additions a lane would be 2^-12 at worst, but each is of positive terms rounded to nearest: 64 warps' and lanes' partial
     # sums of some hundreds, 2^-24 * 300; the rounding of the weight to its terms, the output's own
-    # (bf16: the weight is rounded to 8 bits, and its product with a value's scale once more: twice 2^-8)
-    weight = {BF16: 2.0 ** -7, F16: 2.0 ** -16, F32: 2.0 ** -24}[q.dtype]
+    # (16-bit queries: the product of a weight and a value's scale is rounded to fp16)
+    weight = {BF16: 2.0 ** -11, F16: 2.0 ** -11, F32: 2.0 ** -24}[q.dtype]
     # 16-bit queries: codes go into the products as 0 .. 15 and 8 for each comes off at the end, so that the sums on the way are up to 15 sum(w scale) in size whatever
-    # the values are.  A warp adds a product of 16 positions (of the CTA's 64) a time to them, each addition off by 2^-23 of the sum at most (the matrix unit may cut off),
-    # and some 8 more join the parts: a component whose values cancel, or whose codes are all near 8, is off by that and not by a share of itself.
-    shift = 0.0 if q.dtype == F32 else (max(lens) / 64 + 8) * 2.0 ** -23 * 15 * ws
+    # the values are.  A warp adds a product of 16 positions (of the CTA's 64) a time to them; the matrix unit lays its 17 addends side by side and cuts each off below
+    # the largest one's 24th bit, 17 * 2^-23 in all, and some 8 additions join the parts: a component whose values cancel, or whose codes are all near 8, is off by that
+    # and not by a share of itself.  A weight times its scale is kept in fp16 below 2^4 times the largest scale: 2^-25 / 8 of the largest scale at least.
+    steps = max(lens) / 64 + 1
+    shift = 0.0 if q.dtype == F32 else (steps * 17 + 8) * 2.0 ** -23 * 15 * ws + 8 * 2.0 ** -28 * big_scale * max(lens)
     tol = HALF_STEP[q.dtype] * np.abs(want) + (weight + 2 * score + 2.0 ** -15) * wv + shift + (2.0 ** -25 if q.dtype == F16 else 0)
     assert np.isfinite(g).all()
     assert (np.abs(g - want) <= tol).all(), float((np.abs(g - want) / np.maximum(tol, 1e-300)).max())
@@ -639,6 +642,32 @@ def test_attend_shares_of_uneven_sentences(ops, lens, dtype):
     attend_check(ops, q, pages, table, lens, kk, vv, 16)
     a, b = rng.integers(0, max(lens) + 1, (2, n, g)).astype(np.int32)
     attend_check(ops, q, pages, table, lens, kk, vv, 16, first=np.minimum(a, b), last=np.maximum(a, b))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_attend_values_of_all_sizes(ops, dtype):
+    """Values that grow and shrink along the positions by 2^16, and values and queries that are small or large throughout: the result is as exact as its largest parts
+    allow, whatever came first."""
+    rng = _rng(21)
+    lens, heads, dim, page = [700, 333, 64], 2, 128, 32
+    n_pages, width = 40, 22
+    table = rng.permutation(n_pages)[:3 * 13].reshape(3, 13)
+    table = np.concatenate([table, np.full((3, width - 13), -1)], 1).astype(np.int32)
+    table[0] = rng.permutation(n_pages)[:width]
+    lens[1], lens[2] = 333, 64
+    table[1:] = np.array([[i for i in range(n_pages) if i not in table[0]][:11] + [-1] * 11, [i for i in range(n_pages) if i not in table[0]][11:13] + [-1] * 20])
+    slots = np.concatenate([table[i, np.arange(x) // page].astype(np.int64) * page + np.arange(x) % page for i, x in enumerate(lens)])
+    at = np.concatenate([np.arange(x) for x in lens])
+    top = {BF16: 1e30, F16: 1e4, F32: 1e20}[dtype]
+    for sizes, q_size in ((2.0 ** (at % 17 - 8), 1.0), (2.0 ** -(at / 50), 1.0), (2.0 ** (at / 50), 1.0), (np.full(len(at), 1e-9 if dtype != F16 else 1e-3), 1e-3), (np.full(len(at), top), 1e2)):
+        k, v = rng.normal(0, 1, (len(slots), heads, dim)), rng.normal(0, 1, (len(slots), heads, dim)) * sizes[:, None, None]
+        pages = ops.new_pages4(n_pages, heads, dim, page)
+        ops.write_pages4(pages, _cuda(slots), _cuda(k.astype(np.float32)), _cuda(v.astype(np.float32)))
+        rk, rv = ops.read_pages4(pages, _cuda(slots))
+        kk, vv = np.zeros((n_pages * page, heads, dim), np.float32), np.zeros((n_pages * page, heads, dim), np.float32)
+        kk[slots], vv[slots] = rk.cpu().numpy(), rv.cpu().numpy()
+        q = _q(rng, 3, 4, 4, dim, F32).mul_(q_size).to(dtype)
+        attend_check(ops, q, pages, table, lens, kk, vv, page, scale=dim ** -0.5 / q_size)
 
 
 def test_attend_strides(ops):
