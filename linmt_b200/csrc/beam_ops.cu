@@ -30,7 +30,7 @@ namespace {
 // Sums are compared in 64 bits (as integers of the same order: a comparison of two doubles costs several times one of two integers), but
 // exponentials cost five instructions in 32 bits and twenty in 64, and the logits arrive at a rate that allows for the former.  So the
 // normaliser is summed in 32 bits with a bound on its error (row_error); where two neighbours of the final order come from different rows and
-// lie closer than twice that, their rows' normalisers are summed once more in 64 bits and the steps from 2 on repeat.
+// lie closer than twice that, their rows' normalisers are summed once more to 2^-36 (PairSum) and the steps from 2 on repeat.
 constexpr int kMaxC = 8;
 constexpr int kMaxK = 32;
 constexpr int kWarps = 12;                       // 96 of a cluster of 8: 12 beams leave none without a stretch, 5, 7, 16, 31 few
@@ -56,6 +56,36 @@ __device__ __forceinline__ bool bid_before(Key s, int32_t at, int i, Key s2, int
   return (s > s2) | ((s == s2) & ((at < at2) | ((at == at2) & (i < i2))));
 }
 
+// ---- a sum of exponentials in pairs of 32-bit numbers
+//
+// Near ties are settled with sums that are good to 2^-36, which 64-bit arithmetic would give too, but at an eighth of the rate: exp(d) = 2^(j / 64) exp(r) with j the
+// nearest integer of 64 d / ln 2 and |r| <= ln 2 / 128 (the table-driven method of P. T. P. Tang, ACM TOMS 15, 1989), the reduction, the table's value and the sum
+// each as a number and its rest.
+constexpr double kStep = 0.6931471805599453094 / 64;
+struct ExpTable { float hi[64], lo[64]; };
+struct PairSum {
+  float hi = 0.f, lo = 0.f;
+  // Adds exp(x - m).
+  __device__ __forceinline__ void add(const ExpTable& table, float x, float m) {
+    constexpr float step_hi = (float)kStep, step_lo = (float)(kStep - (double)step_hi);
+    const float d = x - m;
+    if (!(d > -86.f)) return;                                          // (below 2^-124 of the largest; -inf)
+    const float back = d + m, d_lo = (x - back) - (m + (d - back));    // d + d_lo = x - m
+    const float jf = rintf(d * (float)(1.0 / kStep));
+    const int j = (int)jf;
+    const float p = jf * step_hi, p_lo = fmaf(jf, step_hi, -p);
+    const float a = d - p, r = a - p_lo, r_lo = ((a - r) - p_lo) + fmaf(-jf, step_lo, d_lo);
+    const float rest = fmaf(r * r, fmaf(r, fmaf(r, 1.f / 24, 1.f / 6), 0.5f), fmaf(r, r_lo, r_lo));      // exp(r) = 1 + r + rest
+    const float t = table.hi[j & 63], t_lo = table.lo[j & 63];
+    const float b = t * r, b_lo = fmaf(t, r, -b);
+    const float h = t + b, l = (b - (h - t)) + (b_lo + fmaf(t, rest, fmaf(t_lo, r, t_lo)));
+    const float scale = __int_as_float(((j >> 6) + 127) << 23);
+    const float y = h * scale, s = hi + y, z = s - hi;
+    lo += ((hi - (s - z)) + (y - z)) + l * scale;
+    hi = s;
+  }
+};
+
 struct SelectSmem {
   float unit_max[kMaxC * kWarps], unit_sum[kMaxC * kWarps];
   int32_t unit_changes[kMaxC * kWarps];      // most often that a lane's maximum changed
@@ -64,7 +94,7 @@ struct SelectSmem {
   int32_t row_changes[kMaxK];
   float score[kMaxK];
   int32_t live[kMaxK];           // rows that are read, in order
-  uint32_t done_bits, finite_bits, exact_bits, ask_bits;   // per row: finished; score is finite; summed in 64 bits; to be summed so
+  uint32_t done_bits, finite_bits, exact_bits, ask_bits;   // per row: finished; score is finite; summed exactly; to be summed so
   int32_t n_live;
   Key bid[kWarps * 32];                      // each warp's, in order
   int32_t bid_at[kWarps * 32];
@@ -84,6 +114,7 @@ struct SelectSmem {
   int32_t list_at[kMaxList];
   Key sorted[kSorted];
   int32_t sorted_at[kSorted];
+  ExpTable exps;
 };
 
 template <class T>
@@ -620,9 +651,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
       }
       return;
     }
-    // The rows that are asked for, in 64 bits, a part by each of the cluster's warps: cut and added up by the words' own numbers, wherever
+    // The rows that are asked for once more, exactly, a part by each of the cluster's warps: cut and added up by the words' own numbers, wherever
     // the row begins, so that equal rows get equal sums and their ties stay ties.  (The list's place is free.)
     constexpr int kRowsAtOnce = kMaxList / (kMaxC * kWarps);
+    if (tid < 64) {
+      const double e = exp2(tid / 64.0);
+      s.exps.hi[tid] = (float)e;
+      s.exps.lo[tid] = (float)(e - (double)(float)e);
+    }
+    __syncthreads();
     for (uint32_t left = ask; left;) {
       uint32_t now = 0;
       for (int i = 0; i < kRowsAtOnce && left; ++i) { now |= left & (0u - left); left &= left - 1; }
@@ -630,11 +667,22 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
       for (uint32_t rows = now; rows; rows &= rows - 1, ++i) {
         const int rw = __ffs(rows) - 1;
         const T* const p = a.logits + sent * a.stride_n + rw * a.stride_k;
-        const double m = s.row_max[rw];
-        double t = 0.0;
+        const float m = s.row_max[rw];
+        PairSum sums;
         const int e1 = cut(a.vocab, unit + 1, kUnits);
-        for (int at = cut(a.vocab, unit, kUnits) + lane; at < e1; at += 32)
-          if (r.may(at)) t += exp((double)to_float(p[at]) - m);
+        for (int at = cut(a.vocab, unit, kUnits) + lane; at < e1; at += 8 * 32) {
+          T x[8];                          // (eight on their way at once: loaded whether they count or not)
+          uint32_t word[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int i = min(at + 32 * j, e1 - 1);
+            x[j] = p[i];
+            word[j] = r.allowed ? __ldg(r.allowed + (i >> 5)) >> (i & 31) : 1u;
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sums.add(s.exps, at + 32 * j < e1 && (word[j] & 1) ? to_float(x[j]) : -INFINITY, m);
+        }
+        double t = (double)sums.hi + (double)sums.lo;
 #pragma unroll
         for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
         if (lane < C) reinterpret_cast<double*>(cluster.map_shared_rank(&s, lane)->list)[i * kUnits + unit] = t;
