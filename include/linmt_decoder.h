@@ -323,8 +323,8 @@ const char* linmt_op_error(void);
  *   a live beam b      offers every word v with score_b + x_v - log sum_u exp(x_u) over its allowed logits x
  *   a finished beam    offers `eos` alone, with its score as it is; its logits are not read
  *   a beam whose score is not finite, and one with a NaN or +inf at an allowed place, offers nothing
- * Equal sums go to the lowest b * vocab + v.  The order is that of 64-bit arithmetic: sums of two beams that lie closer than
- * 32 bits can tell apart are compared again with 64-bit normalisers.  Words that are not allowed may hold anything;
+ * Equal sums go to the lowest b * vocab + v.  The order is that of 64-bit arithmetic as far as 2^-36: sums of two beams that lie closer
+ * than 32 bits can tell apart are compared again with normalisers that are good to that.  Words that are not allowed may hold anything;
  * one whose logit is -inf is never chosen.  Slots that nothing is left for get token eos, parent = the slot itself, score -inf, done 1.
  * out_* may be the arrays `scores` and `done`. */
 typedef struct linmt_beam_select_args {
@@ -341,12 +341,12 @@ typedef struct linmt_beam_select_args {
   int32_t* out_parents;      /* [n][k], 0 .. k-1 */
   float* out_scores;         /* [n][k] */
   uint8_t* out_done;         /* [n][k]: parent was finished, or the token is eos */
-  int32_t n, k, vocab, eos, dtype;   /* k <= 32, k * vocab < 2^31 */
+  int32_t n, k, vocab, eos, dtype;   /* k <= 32, k * vocab <= 2^31 - 4096 */
 } linmt_beam_select_args;
 int linmt_beam_select(const linmt_beam_select_args* args);
 
 /* Rows of states follow their beams: dst[l][i][j] = src[l][i][parents[i][j]] for every state, one launch for up to 16 of them.
- * dst may be src (the same pointer and strides); otherwise the two must not overlap.  A parent outside 0 .. k-1 takes the row's own. */
+ * dst may be src (the same pointer and strides); otherwise the two must not overlap, nor may a dst and another state.  A parent outside 0 .. k-1 takes the row's own. */
 typedef struct linmt_beam_state {
   const void* src;
   void* dst;
@@ -427,7 +427,9 @@ int linmt_read_pages4(const linmt_pages4_rows_args* args);
  *   s = scale * q . k_t;  cap > 0: s = cap * tanh(s / cap);  slope: s -= slope[h] * |t - centre[i][row]|
  *   seen: first[i][row] <= t < last[i][row] (NULL: all), 0 <= t < len[i], and the table names a page of the pool
  *   out = sum over seen of softmax(s) * v_t; lse = log sum over seen of exp(s).  Nothing seen: 0 and -inf.
- * `len` beyond width * page is taken as that.  Sums are held in 32 bits; 32-bit queries are multiplied as three bf16 terms.
+ * `len` beyond width * page is taken as that.  Sums are held in 32 bits.  16-bit queries: weights times
+ * scales are rounded to fp16, with a power of 2 that follows the largest scale so far (scales of 2^-97 to 2^103).  32-bit queries and weights are
+ * multiplied as three bf16 terms each.
  * `workspace`: linmt_attend_pages4_workspace bytes, 16-byte aligned, the call's own until it has run; NULL where that is 0. */
 typedef struct linmt_attend_pages4_args {
   uint32_t size;

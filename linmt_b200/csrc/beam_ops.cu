@@ -743,7 +743,7 @@ struct ReorderState {
 };
 struct ReorderParams {
   const int32_t* parents;
-  int32_t n, k, n_states;
+  int32_t n, k, n_states, narrow;        // narrow: every state's columns can be counted in 32 bits
   ReorderState state[16];
 };
 constexpr int kReorderThreads = 128;
@@ -770,8 +770,9 @@ __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const __grid_c
   int i = 0;
   while (i + 1 < a.n_states && (int64_t)blockIdx.x >= a.state[i + 1].first_block) ++i;
   const ReorderState& st = a.state[i];
-  const int64_t at = ((int64_t)blockIdx.x - st.first_block) * kReorderThreads + threadIdx.x, ln = at / st.cols, col = at - ln * st.cols;
-  const int64_t l = ln / a.n, n = ln - l * a.n;
+  const int64_t at = ((int64_t)blockIdx.x - st.first_block) * kReorderThreads + threadIdx.x;
+  const int64_t ln = a.narrow ? (int64_t)((uint32_t)at / (uint32_t)st.cols) : at / st.cols, col = at - ln * st.cols;
+  const int64_t l = a.narrow ? (int64_t)((uint32_t)ln / (uint32_t)a.n) : ln / a.n, n = ln - l * a.n;
   if (l >= st.layers) return;
   switch (st.vec_bytes) {
     case 16: move_column<uint4, K>(st, a.parents, a.k, l, n, col); break;
@@ -798,8 +799,8 @@ int linmt_beam_select(const linmt_beam_select_args* g) {
   if (g->eos < 0 || g->eos >= g->vocab) return op_fail(LINMT_EINVAL, "beam_select: eos = %d is not in a vocabulary of %d", g->eos, g->vocab);
   if (!aligned(g->logits, dtype_bytes(g->dtype)) || !aligned(g->scores, 4) || !aligned(g->allowed, 4) || !aligned(g->out_tokens, 4) || !aligned(g->out_parents, 4) || !aligned(g->out_scores, 4))
     return op_fail(LINMT_EINVAL, "beam_select: an array is not aligned to its type");
-  if (g->k > kMaxK || (int64_t)g->k * g->vocab >= INT32_MAX || g->n > (1 << 27))
-    return op_fail(LINMT_ELIMIT, "beam_select: k = %d (at most %d), k * vocab = %lld (below 2^31), n = %d", g->k, kMaxK, (long long)g->k * g->vocab, g->n);
+  if (g->k > kMaxK || (int64_t)g->k * g->vocab > INT32_MAX - 4095 || g->n > (1 << 27))
+    return op_fail(LINMT_ELIMIT, "beam_select: k = %d (at most %d), k * vocab = %lld (at most 2^31 - 4096), n = %d", g->k, kMaxK, (long long)g->k * g->vocab, g->n);
   if (g->n == 0) return LINMT_OK;
   OnDevice on(g->device);
   if (on.err != cudaSuccess) return op_cuda(on.err, "beam_select");
@@ -814,7 +815,7 @@ int linmt_beam_reorder(const linmt_beam_reorder_args* g) {
     return op_fail(LINMT_EINVAL, "beam_reorder: n = %d, k = %d, %d states (at most 16), parents %p", g->n, g->k, g->n_states, (const void*)g->parents);
   if (g->k > kMaxK) return op_fail(LINMT_ELIMIT, "beam_reorder: k = %d (at most %d)", g->k, kMaxK);
   ReorderParams p{};
-  p.parents = g->parents; p.n = g->n; p.k = g->k;
+  p.parents = g->parents; p.n = g->n; p.k = g->k; p.narrow = 1;
   int64_t blocks = 0;
   for (int i = 0; i < g->n_states; ++i) {
     const linmt_beam_state& s = g->state[i];
@@ -830,6 +831,7 @@ int linmt_beam_reorder(const linmt_beam_reorder_args* g) {
     ReorderState& d = p.state[p.n_states++];
     d = ReorderState{static_cast<const unsigned char*>(s.src), static_cast<unsigned char*>(s.dst), s.src_stride_l, s.src_stride_n, s.src_stride_k,
                      s.dst_stride_l, s.dst_stride_n, s.dst_stride_k, s.row_bytes / vec, blocks, s.layers, vec};
+    if (s.layers * g->n * d.cols > INT32_MAX - kReorderThreads) p.narrow = 0;
     blocks += (s.layers * g->n * d.cols + kReorderThreads - 1) / kReorderThreads;
   }
   if (!blocks) return LINMT_OK;

@@ -148,7 +148,11 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-struct Strides { int64_t layers, l, n, k, row; };      // in bytes; row: bytes of one
+struct Strides {
+  int64_t layers, l, n, k, row;      // in bytes; row: bytes of one
+  const char* p;
+  const char* end;                   // behind the last byte
+};
 
 Strides strides_of(const Tensor& x, int64_t n, int64_t k, const char* what, Py_ssize_t i) {
   const int64_t d = x.dim(), size = x.element_size();
@@ -157,14 +161,29 @@ Strides strides_of(const Tensor& x, int64_t n, int64_t k, const char* what, Py_s
   NEED(x.size(f) == n && x.size(f + 1) == k, what, "[", i, "] has to have the sentences and beams of parents, not ", x.sizes());
   const int64_t width = d == 2 ? 1 : x.size(d - 1);
   NEED(d == 2 || width <= 1 || x.stride(d - 1) == 1, "the rows of ", what, "[", i, "] have to be contiguous");
-  return {f ? x.size(0) : 1, f ? x.stride(0) * size : 0, x.stride(f) * size, x.stride(f + 1) * size, width * size};
+  Strides s{f ? x.size(0) : 1, f ? x.stride(0) * size : 0, x.stride(f) * size, x.stride(f + 1) * size, width * size, static_cast<const char*>(x.data_ptr()), nullptr};
+  s.end = s.p + (s.layers - 1) * s.l + (n - 1) * s.n + (k - 1) * s.k + s.row;
+  return s;
 }
-// First byte, and the one behind the last.
-std::pair<const char*, const char*> span(const Tensor& x) {
-  int64_t last = 0;
-  for (int64_t i = 0; i < x.dim(); ++i) last += (x.size(i) - 1) * x.stride(i);
-  const char* p = static_cast<const char*>(x.data_ptr());
-  return {p, p + (last + 1) * x.element_size()};
+// Whether two states share no byte, as far as can be told: one lies behind the other, or they are columns of the same rows.
+bool disjoint(const Strides& a, const Strides& b, int64_t n, int64_t k) {
+  if (a.end <= b.p || b.end <= a.p) return true;
+  const Strides &x = a.p <= b.p ? a : b, &y = a.p <= b.p ? b : a;
+  const int64_t d = y.p - x.p;
+  int64_t room = INT64_MAX;
+  if (x.layers > 1 || y.layers > 1) {
+    if (x.layers != y.layers || x.l != y.l) return false;
+    room = std::min(room, x.l);
+  }
+  if (n > 1) {
+    if (x.n != y.n) return false;
+    room = std::min(room, x.n);
+  }
+  if (k > 1) {
+    if (x.k != y.k) return false;
+    room = std::min(room, x.k);
+  }
+  return d >= x.row && d + y.row <= room;
 }
 
 PyObject* beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
@@ -186,7 +205,13 @@ PyObject* beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   g.reserved = 0;
   const Py_ssize_t all = PyList_GET_SIZE(a[0]);
   std::vector<linmt_beam_state> states;
+  std::vector<Strides> from, to;
   states.reserve((size_t)all);
+  from.reserve((size_t)all);
+  to.reserve((size_t)all);
+  Strides by{};
+  by.p = static_cast<const char*>(parents.data_ptr());
+  by.end = by.p + n * k * 4;
   for (Py_ssize_t i = 0; i < all; ++i) {
     PyObject *ox = PyList_GET_ITEM(a[0], i), *oy = PyList_GET_ITEM(a[2], i);
     const Tensor &x = on_device(ox, "states", dev), &y = on_device(oy, "out", dev);
@@ -198,14 +223,14 @@ PyObject* beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     }
     if (x.numel() == 0) continue;
     NEED(apart(y), "out[", i, "] has rows that share memory");
-    if (oy != ox) {
-      const auto from = span(x), to = span(y);
-      NEED(to.first >= from.second || from.first >= to.second || (from == to && s.l == d.l && s.n == d.n && s.k == d.k), "out[", i, "] overlaps states[", i, "]");
-    }
-    const auto to = span(y), by = span(parents);
-    NEED(to.first >= by.second || by.first >= to.second, "out[", i, "] overlaps parents");
-    for (const linmt_beam_state& before : states) NEED(before.dst != y.data_ptr(), "out[", i, "] is written twice");
+    const bool in_place = s.p == d.p && s.l == d.l && s.n == d.n && s.k == d.k;
+    NEED(in_place || disjoint(s, d, n, k), "out[", i, "] overlaps states[", i, "]");
+    NEED(d.end <= by.p || by.end <= d.p, "out[", i, "] overlaps parents");
+    for (size_t j = 0; j < states.size(); ++j)
+      NEED(disjoint(d, to[j], n, k) && disjoint(d, from[j], n, k) && disjoint(s, to[j], n, k), "out[", i, "] or an out before it overlaps another state");
     states.push_back({x.data_ptr(), y.data_ptr(), s.l, s.n, s.k, d.l, d.n, d.k, s.row, s.layers});
+    from.push_back(s);
+    to.push_back(d);
   }
   for (size_t i = 0; i < states.size(); i += 16) {
     g.n_states = (int)std::min<size_t>(16, states.size() - i);

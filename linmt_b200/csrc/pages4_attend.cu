@@ -143,51 +143,60 @@ struct Share {
   int sent, whole;         // sentence of `begin`; segments of up to `whole` pairs are not cut
 };
 __device__ __forceinline__ int length_of(const AttendParams& a, int sent) {
-  return min(max(__ldg(a.len + sent), 0), (int)min((int64_t)a.width * a.page, (int64_t)0x7fffffff));
+  return min(max(__ldg(a.len + sent), 0), (int)min((int64_t)a.width * a.page, (int64_t)0x7fffffff - 64));
 }
 __device__ __forceinline__ int pairs_of(const AttendParams& a, int sent) { return max(kLeast, (int)(((int64_t)length_of(a, sent) + 31) / 32)); }
 
-// Share of block `blockIdx.x` of `blocks`; all threads of the CTA (a multiple of 32, at most 128) call it.
+// Share of block `blockIdx.x` of `blocks`; all threads of the CTA (a multiple of 32, at most 128) call it.  The sentences are added up by all
+// threads, then those of the thread that has the first pair, until one is left.
 __device__ __forceinline__ Share share_of(const AttendParams& a, int blocks) {
-  __shared__ int64_t sums[4];
-  __shared__ int64_t found_first;
-  __shared__ int found_sent;
+  __shared__ int64_t sums[4], found_first;
+  __shared__ int found_lo, found_hi;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, segments = a.pool_heads * a.row_tiles;
-  const int each = (a.n + threads - 1) / threads, i0 = min(a.n, tid * each), i1 = min(a.n, i0 + each);
-  int64_t mine = 0;
-  for (int i = i0; i < i1; ++i) mine += pairs_of(a, i);
-  int64_t upto = mine;
+  Share s{};
+  int lo = 0, hi = a.n;
+  bool all = true;
+  for (;;) {
+    const int each = (hi - lo + threads - 1) / threads, i0 = min(hi, lo + tid * each), i1 = min(hi, i0 + each);
+    int64_t mine = 0;
+#pragma unroll 8
+    for (int i = i0; i < i1; ++i) mine += pairs_of(a, i);
+    int64_t upto = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t x = __shfl_up_sync(~0u, upto, o);
-    if (lane >= o) upto += x;
-  }
-  if (lane == 31) sums[warp] = upto;
-  __syncthreads();
-  int64_t total = 0;
-  for (int w = 0; w < threads / 32; ++w) {
-    if (w == warp) upto += total;
-    total += sums[w];
-  }
-  Share s;
-  s.per = max((int64_t)kLeast, (total * segments + blocks - 1) / blocks);
-  s.begin = min(total * segments, blockIdx.x * s.per);
-  s.end = min(total * segments, s.begin + s.per);
-  s.whole = (int)min((int64_t)0x7fffffff, max((int64_t)kLeast, s.per / 8));
-  if (i0 < i1 && s.begin >= (upto - mine) * segments && s.begin < upto * segments) {
-    int64_t before = (upto - mine) * segments;
-    int i = i0;
-    for (;; ++i) {
-      const int64_t next = before + (int64_t)pairs_of(a, i) * segments;
-      if (s.begin < next) break;
-      before = next;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(~0u, upto, o);
+      if (lane >= o) upto += x;
     }
-    found_first = before;
-    found_sent = i;
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    int64_t total = 0;
+    for (int w = 0; w < threads / 32; ++w) {
+      if (w == warp) upto += total;
+      total += sums[w];
+    }
+    if (all) {
+      all = false;
+      total *= segments;
+      s.per = max((int64_t)kLeast, (total + blocks - 1) / blocks);
+      s.begin = min(total, blockIdx.x * s.per);
+      s.end = min(total, s.begin + s.per);
+      s.whole = (int)min((int64_t)0x7fffffff, max((int64_t)kLeast, s.per / 8));
+    }
+    if (s.begin >= s.end) return s;
+    const int64_t before = s.first + (upto - mine) * segments;
+    if (s.begin >= before && s.begin < s.first + upto * segments) {
+      found_first = before;
+      found_lo = i0;
+      found_hi = i1;
+    }
+    __syncthreads();
+    s.first = found_first;
+    lo = found_lo;
+    hi = found_hi;
+    if (hi - lo == 1) break;
+    __syncthreads();                     // (before these are written again)
   }
-  __syncthreads();
-  s.first = found_first;
-  s.sent = found_sent;
+  s.sent = lo;
   return s;
 }
 
@@ -958,6 +967,7 @@ int check(const linmt_attend_pages4_args* g) {
   if (g->n < 0 || g->g < 0 || g->heads < 1 || g->heads % g->pages.heads || g->width < 0 || !dtype_ok(g->dtype))
     return op_fail(LINMT_EINVAL, "attend_pages4: n = %d, g = %d, heads = %d (a multiple of the pool's %d), width = %d, dtype = %d", g->n, g->g, g->heads, g->pages.heads, g->width, g->dtype);
   if (!(g->scale - g->scale == 0.f) || !(g->cap >= 0.f) || !(g->cap - g->cap == 0.f)) return op_fail(LINMT_EINVAL, "attend_pages4: scale and cap have to be finite, cap not negative");
+  if (g->cap > 0.f && (g->cap < 1e-18f || !(g->scale / g->cap - g->scale / g->cap == 0.f))) return op_fail(LINMT_EINVAL, "attend_pages4: cap = %g is too small (0: none)", (double)g->cap);
   if (g->n == 0 || g->g == 0) return LINMT_OK;
   if (!g->q || !g->out || !g->len || (g->width && !g->table)) return op_fail(LINMT_EINVAL, "attend_pages4: an array is missing");
   if (!g->slope != !g->centre || !g->first != !g->last) return op_fail(LINMT_EINVAL, "attend_pages4: slope goes with centre, first with last");

@@ -56,7 +56,7 @@ def beam_reorder(states, parents, *, out=None):
     """Rows of states follow their beams: ``out[...][.., i, j, :] = states[...][.., i, parents[i, j], :]``, all states in one launch (for each 16).
 
     ``states``: tensors [n, k], [n, k, width] or [layers, n, k, width] of any type, rows contiguous.  ``parents`` [n, k] int32; one outside 0 .. k-1 is taken as the
-    row's own.  ``out``: tensors like them, each either the state itself or one that it does not overlap; without it the states are reordered in place.
+    row's own.  ``out``: tensors like them, each either the state itself or one that overlaps no state; without it the states are reordered in place.
     Returns the list of the tensors written."""
     states = list(states)
     return _front.beam_reorder(states, parents, states if out is None else list(out))

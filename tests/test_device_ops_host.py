@@ -100,7 +100,7 @@ def test_rows_refuse(cuda_lib, fn, code, word, kw):
 
 @pytest.mark.parametrize("code,word,kw", [
     (EINVAL, "struct", dict(size=8)), (EINVAL, "multiple of the pool", dict(heads=3)), (EINVAL, "heads = 0", dict(heads=0)), (EINVAL, "missing", dict(q=0)), (EINVAL, "missing", dict(len=0)),
-    (EINVAL, "slope goes with", dict(slope=PTR)), (EINVAL, "first with last", dict(last=PTR)), (EINVAL, "finite", dict(scale=float("nan"))), (EINVAL, "finite", dict(cap=float("inf"))), (EINVAL, "finite", dict(cap=-1.0)),
+    (EINVAL, "slope goes with", dict(slope=PTR)), (EINVAL, "first with last", dict(last=PTR)), (EINVAL, "finite", dict(scale=float("nan"))), (EINVAL, "finite", dict(cap=float("inf"))), (EINVAL, "finite", dict(cap=-1.0)), (EINVAL, "too small", dict(cap=1e-30)),
     (EINVAL, "aligned", dict(q=PTR + 1)), (ELIMIT, "dim = 32", dict(dim=32)), (EINVAL, "workspace", dict(width=4096)), (EINVAL, "workspace", dict(width=4096, workspace=PTR, workspace_bytes=64)), (ELIMIT, "too many", dict(n=1 << 24))])
 def test_attend_refuses(cuda_lib, code, word, kw):
     _refused(cuda_lib, "linmt_attend_pages4", "linmt_attend_pages4_args", code, word, **kw)

@@ -270,6 +270,21 @@ def test_reorder_strides_many_states_and_parents_outside(ops):
     assert ops.beam_reorder([empty, torch.zeros(n, k, 0, device="cuda")], parents)[0] is empty
 
 
+def test_reorder_columns_of_one_buffer(ops):
+    """h and c side by side in one buffer, each a state of its own."""
+    rng = _rng(30)
+    hc = _cuda(rng.normal(0, 1, (2, 5, 6, 48)).astype(np.float32))
+    parents = _cuda(rng.integers(0, 6, (5, 6)).astype(np.int32))
+    want = _reordered(hc.clone(), parents)
+    ops.beam_reorder([hc[..., :20], hc[..., 20:44], hc[..., 44:]], parents)
+    assert torch.equal(hc, want)
+    a, b = _cuda(rng.normal(0, 1, (5, 6, 8)).astype(np.float32)), _cuda(rng.normal(0, 1, (5, 6, 8)).astype(np.float32))
+    for bad in (lambda: ops.beam_reorder([a, b], parents, out=[b, a]), lambda: ops.beam_reorder([hc[..., :20], hc[..., 19:]], parents), lambda: ops.beam_reorder([a, a], parents, out=[b, b]),
+                lambda: ops.beam_reorder([a, b], parents, out=[torch.empty_like(a), a])):
+        with pytest.raises(ValueError):
+            bad()
+
+
 def test_reorder_refuses(ops):
     x, parents = torch.zeros(2, 8, 64, device="cuda"), torch.zeros(2, 4, dtype=torch.int32, device="cuda")
     a = x[:, :4]
@@ -632,7 +647,7 @@ def test_attend_long_and_split(ops, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("lens", [[5000, 1, 1, 1, 4000, 0, 0, 700], [33] * 150, [3] * 40 + [6000] + [50] * 30, [0, 0, 0], [129, 130, 8000, 257]])
+@pytest.mark.parametrize("lens", [[5000, 1, 1, 1, 4000, 0, 0, 700], [33] * 150, [3] * 40 + [6000] + [50] * 30, [0, 0, 0], [1] * 700 + [900] + [2] * 300, [129, 130, 8000, 257]])
 def test_attend_shares_of_uneven_sentences(ops, lens, dtype):
     """Segments that several CTAs share, that share a CTA, and both: long sentences before, between and behind short ones."""
     rng = _rng(sum(lens), len(lens))
