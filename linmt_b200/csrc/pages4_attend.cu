@@ -147,10 +147,10 @@ __device__ __forceinline__ int length_of(const AttendParams& a, int sent) {
 }
 __device__ __forceinline__ int pairs_of(const AttendParams& a, int sent) { return max(kLeast, (int)(((int64_t)length_of(a, sent) + 31) / 32)); }
 
-// Share of block `blockIdx.x` of `blocks`; all threads of the CTA (a multiple of 32, at most 128) call it.  The sentences are added up by all
+// Share of block `blockIdx.x` of `blocks`; all threads of the CTA (a multiple of 32, at most 512) call it.  The sentences are added up by all
 // threads, then those of the thread that has the first pair, until one is left.
 __device__ __forceinline__ Share share_of(const AttendParams& a, int blocks) {
-  __shared__ int64_t sums[4], found_first;
+  __shared__ int64_t sums[16], found_first;
   __shared__ int found_lo, found_hi;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, segments = a.pool_heads * a.row_tiles;
   Share s{};
@@ -892,36 +892,53 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
   }
 }
 
-// Joins the parts of the segment that ends in a CTA's share and began in one before: a CTA for each of attend's.
+// Joins the parts of the segment that ends in a CTA's share and began in one before: a CTA for each of attend's, a thread for four components of a
+// row.  Shares are found while attend still runs.
 template <class T, int D>
-__global__ void __launch_bounds__(128) attend_join_kernel(const __grid_constant__ AttendParams a, int blocks) {
+__global__ void __launch_bounds__(kRows * D / 4) attend_join_kernel(const __grid_constant__ AttendParams a, int blocks) {
   Share share = share_of(a, blocks);
   Piece p;
   const int64_t per = share.per;
   const bool ends = next_piece(a, share, p) && p.p0 > 0 && p.p1 == p.pairs;
-  wait_for_last();
-  if (!ends) return;
-  const int from = (int)(p.start / per), n_parts = (int)blockIdx.x - from + 1;
+  const int from = ends ? (int)(p.start / per) : 0, n_parts = (int)blockIdx.x - from + 1;
   constexpr int kPart = kRows * (D + 2);
+  const int d = threadIdx.x % (D / 4) * 4, r = threadIdx.x / (D / 4);
+  wait_for_last();
+  if (!ends || r >= a.g * a.rep - p.rt * kRows) return;
   auto part = [&](int i) { return a.ws + ((int64_t)(from + i) * 2 + (i == 0)) * kPart; };
-  const int n_rows = min(kRows, a.g * a.rep - p.rt * kRows), d = threadIdx.x % (D / 4) * 4;
-  for (int r = threadIdx.x / (D / 4); r < n_rows; r += 128 / (D / 4)) {
-    float top = -INFINITY;
-#pragma unroll 4
-    for (int i = 0; i < n_parts; ++i) top = fmaxf(top, part(i)[kRows * D + r]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    float weight = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < n_parts; ++i) {
-      const float* const w = part(i);
-      const float f = exp2_of(w[kRows * D + r] - base);
-      const float4 v = *reinterpret_cast<const float4*>(w + r * D + d);
-      sum.x += f * v.x; sum.y += f * v.y; sum.z += f * v.z; sum.w += f * v.w;
-      weight += f * w[kRows * D + kRows + r];
+  // The maximum so far goes along, so that every part is waited for once: eight of them at a time are on their way.
+  float top = -INFINITY, weight = 0.f;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < n_parts; i0 += 8) {
+    float m[8], l[8];
+    float4 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      m[j] = -INFINITY;
+      if (i0 + j < n_parts) {
+        const float* const w = part(i0 + j);
+        m[j] = w[kRows * D + r];
+        l[j] = w[kRows * D + kRows + r];
+        v[j] = *reinterpret_cast<const float4*>(w + r * D + d);
+      }
     }
-    write_row<T>(a, p.sent, p.kvh, p.rt * kRows + r, d, sum, top, weight);
+    float now = top;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) now = fmaxf(now, m[j]);
+    if (now == -INFINITY) continue;
+    const float f0 = exp2_of(top - now);
+    top = now;
+    weight *= f0;
+    sum.x *= f0; sum.y *= f0; sum.z *= f0; sum.w *= f0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (i0 + j >= n_parts) break;
+      const float f = exp2_of(m[j] - now);
+      sum.x += f * v[j].x; sum.y += f * v[j].y; sum.z += f * v[j].z; sum.w += f * v[j].w;
+      weight += f * l[j];
+    }
   }
+  write_row<T>(a, p.sent, p.kvh, p.rt * kRows + r, d, sum, top, weight);
 }
 
 template <class T, int D>
@@ -943,7 +960,7 @@ cudaError_t launch_attend(const AttendParams& p, int blocks, int device, cudaStr
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3(128);
+  cfg.blockDim = dim3(kRows * D / 4);
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
