@@ -50,7 +50,7 @@ struct AttendParams {
   const int32_t* first;
   const int32_t* last;
   float* ws;
-  int32_t n, g, heads, rep, width, row_tiles;
+  int32_t n, g, heads, rep, width, row_tiles, by_window;
   float scale, cap;
   int32_t q_wide, o_wide;    // the rows of q are 16-byte aligned; fours of components of out are aligned to their size
 };
@@ -100,8 +100,12 @@ __device__ __forceinline__ float exp2_of(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// tanh as 1 - 2 / (e^2x + 1), good to 2e-7 of 1: what a 16-bit result can see of it.
-__device__ __forceinline__ float tanh_of(float x) { return 1.f - __fdividef(2.f, exp2_of(x * (2 * kLog2e)) + 1.f); }
+// cap tanh(x) as cap - 2 cap / (2^y + 1), y = 2 x log2(e): good to 3e-7 of the cap, what a 16-bit result can see of it.
+__device__ __forceinline__ float capped(float y, float cap) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(exp2_of(y) + 1.f));
+  return fmaf(-2.f * cap, r, cap);
+}
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -131,7 +135,8 @@ __device__ __forceinline__ void write_row(const AttendParams& a, int sent, int k
 // ---- who does what
 //
 // The work is a list of pairs of tiles (32 positions): sentence by sentence, in each by head of the pool and row tile (a segment), a segment's
-// pairs in order.  It is cut into as many equal parts as CTAs fit on the GPU at once, each of at least kLeast pairs: a segment
+// pairs in order, from the first that a row of the sentence sees to the last (where there are windows, and not so many that looking at them takes
+// longer than the pairs that they leave out).  It is cut into as many equal parts as CTAs fit on the GPU at once, each of at least kLeast pairs: a segment
 // longer than a part is then shared by several CTAs, whose parts the join kernel adds up, and a CTA may have several short ones.  Lengths
 // are known on the device only, so every CTA adds them up itself.  A short segment counts as kLeast pairs, its fixed costs being as large, and
 // segments of up to kLeast pairs or an eighth of a part are not cut: the CTA that has their first pair takes them whole.
@@ -145,7 +150,33 @@ struct Share {
 __device__ __forceinline__ int length_of(const AttendParams& a, int sent) {
   return min(max(__ldg(a.len + sent), 0), (int)min((int64_t)a.width * a.page, (int64_t)0x7fffffff - 64));
 }
-__device__ __forceinline__ int pairs_of(const AttendParams& a, int sent) { return max(kLeast, (int)(((int64_t)length_of(a, sent) + 31) / 32)); }
+// The pairs of a sentence that any of its rows sees: from pair `from` on; `a.by_window`: its rows are few enough to look at.
+struct Seen { int from, pairs; };
+__device__ __forceinline__ Seen seen_between(int lo, int hi) {
+  if (lo >= hi) return {0, kLeast};
+  return {lo / 32, max(kLeast, (hi + 31) / 32 - lo / 32)};
+}
+__device__ __forceinline__ Seen seen_of(const AttendParams& a, int sent) {             // by one thread
+  const int len = length_of(a, sent);
+  if (!a.by_window) return seen_between(0, len);
+  int lo = 0x7fffffff, hi = 0;
+#pragma unroll 4
+  for (int g = 0; g < a.g; ++g) {
+    const int f = max(__ldg(a.first + (int64_t)sent * a.g + g), 0), l = min(__ldg(a.last + (int64_t)sent * a.g + g), len);
+    if (f < l) { lo = min(lo, f); hi = max(hi, l); }
+  }
+  return seen_between(lo, hi);
+}
+__device__ __forceinline__ Seen seen_by_warp(const AttendParams& a, int sent) {        // by a warp
+  const int len = length_of(a, sent);
+  if (!a.by_window) return seen_between(0, len);
+  int lo = 0x7fffffff, hi = 0;
+  for (int g = threadIdx.x & 31; g < a.g; g += 32) {
+    const int f = max(__ldg(a.first + (int64_t)sent * a.g + g), 0), l = min(__ldg(a.last + (int64_t)sent * a.g + g), len);
+    if (f < l) { lo = min(lo, f); hi = max(hi, l); }
+  }
+  return seen_between(__reduce_min_sync(~0u, lo), __reduce_max_sync(~0u, hi));
+}
 
 // Share of block `blockIdx.x` of `blocks`; all threads of the CTA (a multiple of 32, at most 512) call it.  The sentences are added up by all
 // threads, then those of the thread that has the first pair, until one is left.
@@ -160,7 +191,7 @@ __device__ __forceinline__ Share share_of(const AttendParams& a, int blocks) {
     const int each = (hi - lo + threads - 1) / threads, i0 = min(hi, lo + tid * each), i1 = min(hi, i0 + each);
     int64_t mine = 0;
 #pragma unroll 8
-    for (int i = i0; i < i1; ++i) mine += pairs_of(a, i);
+    for (int i = i0; i < i1; ++i) mine += seen_of(a, i).pairs;
     int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -203,14 +234,17 @@ __device__ __forceinline__ Share share_of(const AttendParams& a, int blocks) {
 // One CTA's piece of a segment.
 struct Piece {
   int sent, kvh, rt;
+  int from;                // its first pair is that of positions 32 from on
   int p0, p1, pairs;       // pairs p0 .. p1 - 1 of the segment's
   int64_t start;           // number of the segment's first pair
 };
-// The piece that begins at s.begin; false where the CTA has none left.  Moves s on behind it.
+// The piece that begins at s.begin; false where the CTA has none left.  Moves s on behind it.  All lanes of a warp call it.
 __device__ __forceinline__ bool next_piece(const AttendParams& a, Share& s, Piece& p) {
   const int segments = a.pool_heads * a.row_tiles;
   while (s.begin < s.end) {
-    p.pairs = pairs_of(a, s.sent);
+    const Seen seen = seen_by_warp(a, s.sent);
+    p.from = seen.from;
+    p.pairs = seen.pairs;
     const int64_t in = s.begin - s.first, seg = in / p.pairs;
     if (seg >= segments) {
       s.first += (int64_t)p.pairs * segments;
@@ -288,8 +322,8 @@ __device__ __forceinline__ Job job_of(const AttendParams& a, const Piece& p, con
   j.all_lo = __reduce_max_sync(~0u, j.all_lo);
   j.all_hi = __reduce_min_sync(~0u, j.all_hi);
   const bool any = any_lo < any_hi;
-  j.t0 = max(2 * p.p0, any ? any_lo / pages4::kTile & ~1 : 0);
-  j.t1 = max(j.t0, min(2 * p.p1, any ? (any_hi - 1) / pages4::kTile + 1 : 0));
+  j.t0 = max(2 * (p.from + p.p0), any ? any_lo / pages4::kTile & ~1 : 0);
+  j.t1 = max(j.t0, min(2 * (p.from + p.p1), any ? (any_hi - 1) / pages4::kTile + 1 : 0));
   return j;
 }
 
@@ -566,7 +600,8 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend32_kernel(
   }
 }
 
-template <class T, int D>
+// PLAIN: no cap, no bias, and a scale: scores are products times mul.
+template <class T, int D, bool PLAIN>
 __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(const __grid_constant__ AttendParams a) {
   constexpr int NG = D / 32, kTileBytes = pages4::tile_bytes(D);
   constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;
@@ -626,7 +661,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
     // so that its largest component is 2^9 to 2^10; what a group's codes carry too much, 8 times the sum of its components, in three bf16
     // terms for a product with the keys' scales: place k of it belongs to group k % 4, term k / 4.  A warp prepares one group.
     uint4 over;
-    float mul[2];                  // from a sum of products to a power of 2 (or, with a cap, to what tanh takes)
+    float mul[2];                  // from a sum of products to a power of 2 (or, with a cap, to what capped() takes)
     {
       __shared__ float s_most[NG][kRows], s_sum[4][kRows];
       float x[2][8];
@@ -660,7 +695,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
         for (int gr = 1; gr < NG; ++gr) most = fmaxf(most, s_most[gr][gid + 8 * r]);
         const int up = most > 0.f && most < INFINITY ? 9 - max(-100, ilogbf(most)) : 0;      // -118 .. 109
         const float by = ldexpf(a.scale < 0.f ? -1.f : 1.f, up);
-        mul[r] = ldexpf(fabsf(a.scale) * (a.cap > 0.f ? 1.f / a.cap : kLog2e), 24 - up);
+        mul[r] = ldexpf(fabsf(a.scale) * kLog2e * (a.cap > 0.f ? 2.f / a.cap : 1.f), 24 - up);
         if (warp < NG) {
           float sum = 0.f;
           uint32_t f[4];
@@ -698,7 +733,6 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
       }
       over = make_uint4(ov[0][0], ov[1][0], ov[0][1], ov[1][1]);
     }
-    const bool plain = a.cap == 0.f && !a.slope && a.scale != 0.f;       // scores are products times mul
     const float cap_log2 = a.cap * kLog2e;
 
     // The values' sums are kept times 2^-24, as the codes are, and times the power of 2 that brings their scales into fp16's range.
@@ -752,27 +786,35 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
         }
       }
       float r0 = mul[0], r1 = mul[1];
-      if (!plain) {
+      if constexpr (!PLAIN) {
+        const float at0 = (float)(pos + 2 * c) - job.centre[0], at1 = (float)(pos + 2 * c) - job.centre[1];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float v = x[j][e] * (e < 2 ? r0 : r1);
-            if (a.cap > 0.f) v = cap_log2 * tanh_of(v);
-            if (a.slope) v -= job.slope[e >> 1] * fabsf((float)(pos + 8 * j + 2 * c + (e & 1)) - job.centre[e >> 1]);
+            if (a.cap > 0.f) v = capped(v, cap_log2);
+            if (a.slope) v = fmaf(-job.slope[e >> 1], fabsf((e < 2 ? at0 : at1) + (float)(8 * j + (e & 1))), v);
             x[j][e] = v;
           }
         r0 = r1 = 1.f;
       }
       const bool edge = gone || pos < job.all_lo || pos + 2 * pages4::kTile > job.all_hi;
       if (edge) {
+        const int from0 = pos + 2 * c - job.lo[0], from1 = pos + 2 * c - job.lo[1];
+        const uint32_t n0 = job.lo[0] < job.hi[0] ? job.hi[0] - job.lo[0] : 0, n1 = job.lo[1] < job.hi[1] ? job.hi[1] - job.lo[1] : 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int p = pos + 8 * j + 2 * c + (e & 1);
-            if (p < job.lo[e >> 1] || p >= job.hi[e >> 1] || ((gone >> (j >> 1)) & 1)) x[j][e] = -INFINITY;
-          }
+          for (int e = 0; e < 4; ++e)
+            if ((uint32_t)((e < 2 ? from0 : from1) + 8 * j + (e & 1)) >= (e < 2 ? n0 : n1)) x[j][e] = -INFINITY;
+        if (gone) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if ((gone >> (j >> 1)) & 1) x[j][e] = -INFINITY;
+        }
       }
       float top[2];
 #pragma unroll
@@ -944,13 +986,15 @@ __global__ void __launch_bounds__(kRows * D / 4) attend_join_kernel(const __grid
 template <class T, int D>
 cudaError_t launch_attend(const AttendParams& p, int blocks, int device, cudaStream_t st) {
   constexpr int smem = attend_smem<T, D>();
+  const bool plain = p.cap == 0.f && !p.slope && p.scale != 0.f;
   void (*kernel)(AttendParams);
-  if constexpr (sizeof(T) == 2) kernel = attend16_kernel<T, D>; else kernel = attend32_kernel<D>;
-  static std::atomic<bool> opted_in[kOpMaxDevices] = {};
-  if (smem + 1024 > 48 << 10 && !opted_in[device].load(std::memory_order_acquire)) {
+  if constexpr (sizeof(T) == 2) kernel = plain ? attend16_kernel<T, D, true> : attend16_kernel<T, D, false>;
+  else kernel = attend32_kernel<D>;
+  static std::atomic<bool> opted_in[kOpMaxDevices][2] = {};
+  if (smem + 1024 > 48 << 10 && !opted_in[device][plain].load(std::memory_order_acquire)) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    opted_in[device].store(true, std::memory_order_release);
+    opted_in[device][plain].store(true, std::memory_order_release);
   }
   kernel<<<(unsigned)blocks, kWarps * 32, smem, st>>>(p);
   cudaError_t e = cudaGetLastError();
@@ -1025,7 +1069,7 @@ int linmt_attend_pages4(const linmt_attend_pages4_args* g) {
   if (on.err != cudaSuccess) return op_cuda(on.err, "attend_pages4");
   AttendParams p{static_cast<const unsigned char*>(g->pages.data), g->pages.stride_page, g->pages.stride_head, g->pages.n_pages, g->pages.heads, g->pages.page,
                  g->q, g->q_stride_n, g->q_stride_g, g->q_stride_h, g->out, g->out_stride_n, g->out_stride_g, g->out_stride_h, g->lse, g->table, g->table_stride, g->len,
-                 g->slope, g->centre, g->first, g->last, need ? static_cast<float*>(g->workspace) : nullptr, g->n, g->g, g->heads, g->heads / g->pages.heads, g->width, row_tiles_of(g),
+                 g->slope, g->centre, g->first, g->last, need ? static_cast<float*>(g->workspace) : nullptr, g->n, g->g, g->heads, g->heads / g->pages.heads, g->width, row_tiles_of(g), g->first && g->g <= 32 && (int64_t)g->n * g->g <= 65536,
                  g->scale, g->cap, aligned(g->q, 16) && (g->q_stride_n | g->q_stride_g | g->q_stride_h) % (16 / dtype_bytes(g->dtype)) == 0,
                  aligned(g->out, 4 * dtype_bytes(g->dtype)) && (g->out_stride_n | g->out_stride_g | g->out_stride_h) % 4 == 0};
   const int blocks = blocks_of(g);
