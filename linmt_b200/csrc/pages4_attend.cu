@@ -138,23 +138,25 @@ __device__ __forceinline__ void write_row(const AttendParams& a, int sent, int k
 // pairs in order, from the first that a row of the sentence sees to the last (where there are windows, and not so many that looking at them takes
 // longer than the pairs that they leave out).  It is cut into as many equal parts as CTAs fit on the GPU at once, each of at least kLeast pairs: a segment
 // longer than a part is then shared by several CTAs, whose parts the join kernel adds up, and a CTA may have several short ones.  Lengths
-// are known on the device only, so every CTA adds them up itself.  A short segment counts as kLeast pairs, its fixed costs being as large, and
-// segments of up to kLeast pairs or an eighth of a part are not cut: the CTA that has their first pair takes them whole.
+// are known on the device only, so every CTA adds them up itself.  A segment counts as kFixed units more than it has pairs, its fixed costs being as large,
+// and as kLeast at least; one of up to kLeast + kFixed units or an eighth of a part is not cut: the CTA that has its first unit takes it whole.
 constexpr int kLeast = 8;
+constexpr int kFixed = 4;
 struct Share {
-  int64_t begin, end;      // the CTA's pairs
-  int64_t first;           // number of the first pair of sentence `sent`
-  int64_t per;             // pairs of a part
-  int sent, whole;         // sentence of `begin`; segments of up to `whole` pairs are not cut
+  int64_t begin, end;      // the CTA's units
+  int64_t first;           // number of the first unit of sentence `sent`
+  int64_t per;             // units of a part
+  int sent, whole;         // sentence of `begin`; segments of up to `whole` units are not cut
 };
 __device__ __forceinline__ int length_of(const AttendParams& a, int sent) {
   return min(max(__ldg(a.len + sent), 0), (int)min((int64_t)a.width * a.page, (int64_t)0x7fffffff - 64));
 }
-// The pairs of a sentence that any of its rows sees: from pair `from` on; `a.by_window`: its rows are few enough to look at.
-struct Seen { int from, pairs; };
+// The pairs of a sentence that any of its rows sees, from pair `from` on, and the units that they count; `a.by_window`: its rows are few enough to look at.
+struct Seen { int from, pairs, units; };
 __device__ __forceinline__ Seen seen_between(int lo, int hi) {
-  if (lo >= hi) return {0, kLeast};
-  return {lo / 32, max(kLeast, (hi + 31) / 32 - lo / 32)};
+  if (lo >= hi) return {0, 0, kLeast};
+  const int pairs = (hi + 31) / 32 - lo / 32;
+  return {lo / 32, pairs, max(kLeast, pairs + kFixed)};
 }
 __device__ __forceinline__ Seen seen_of(const AttendParams& a, int sent) {             // by one thread
   const int len = length_of(a, sent);
@@ -191,7 +193,7 @@ __device__ __forceinline__ Share share_of(const AttendParams& a, int blocks) {
     const int each = (hi - lo + threads - 1) / threads, i0 = min(hi, lo + tid * each), i1 = min(hi, i0 + each);
     int64_t mine = 0;
 #pragma unroll 8
-    for (int i = i0; i < i1; ++i) mine += seen_of(a, i).pairs;
+    for (int i = i0; i < i1; ++i) mine += seen_of(a, i).units;
     int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -211,7 +213,7 @@ __device__ __forceinline__ Share share_of(const AttendParams& a, int blocks) {
       s.per = max((int64_t)kLeast, (total + blocks - 1) / blocks);
       s.begin = min(total, blockIdx.x * s.per);
       s.end = min(total, s.begin + s.per);
-      s.whole = (int)min((int64_t)0x7fffffff, max((int64_t)kLeast, s.per / 8));
+      s.whole = (int)min((int64_t)0x7fffffff, max((int64_t)(kLeast + kFixed), s.per / 8));
     }
     if (s.begin >= s.end) return s;
     const int64_t before = s.first + (upto - mine) * segments;
@@ -234,37 +236,36 @@ __device__ __forceinline__ Share share_of(const AttendParams& a, int blocks) {
 // One CTA's piece of a segment.
 struct Piece {
   int sent, kvh, rt;
-  int from;                // its first pair is that of positions 32 from on
-  int p0, p1, pairs;       // pairs p0 .. p1 - 1 of the segment's
-  int64_t start;           // number of the segment's first pair
+  int u0, u1, units;       // units u0 .. u1 - 1 of the segment's
+  int64_t start;           // number of the segment's first unit
+  int from, fixed;         // unit u >= fixed is the pair of positions 32 (from + u - fixed) on
+  __device__ __forceinline__ bool whole() const { return u0 == 0 && u1 == units; }
 };
 // The piece that begins at s.begin; false where the CTA has none left.  Moves s on behind it.  All lanes of a warp call it.
 __device__ __forceinline__ bool next_piece(const AttendParams& a, Share& s, Piece& p) {
   const int segments = a.pool_heads * a.row_tiles;
   while (s.begin < s.end) {
     const Seen seen = seen_by_warp(a, s.sent);
+    p.units = seen.units;
     p.from = seen.from;
-    p.pairs = seen.pairs;
-    const int64_t in = s.begin - s.first, seg = in / p.pairs;
+    p.fixed = seen.units - seen.pairs;
+    const int64_t in = s.begin - s.first, seg = in / p.units;
     if (seg >= segments) {
-      s.first += (int64_t)p.pairs * segments;
+      s.first += (int64_t)p.units * segments;
       ++s.sent;
       continue;
     }
     p.sent = s.sent;
     p.kvh = (int)seg / a.row_tiles;
     p.rt = (int)seg - p.kvh * a.row_tiles;
-    p.start = s.first + seg * p.pairs;
-    p.p0 = (int)(s.begin - p.start);
-    p.p1 = (int)min((int64_t)p.pairs, s.end - p.start);
-    s.begin = p.start + p.p1;
-    if (p.pairs <= s.whole) {
-      if (p.p0 > 0) {           // the CTA before has all of it
-        s.begin = p.start + p.pairs;
-        continue;
-      }
-      p.p1 = p.pairs;
-      s.begin = p.start + p.pairs;
+    p.start = s.first + seg * p.units;
+    p.u0 = (int)(s.begin - p.start);
+    p.u1 = (int)min((int64_t)p.units, s.end - p.start);
+    s.begin = p.start + p.u1;
+    if (p.units <= s.whole) {
+      s.begin = p.start + p.units;
+      if (p.u0 > 0) continue;            // the CTA before has all of it
+      p.u1 = p.units;
     }
     return true;
   }
@@ -322,8 +323,8 @@ __device__ __forceinline__ Job job_of(const AttendParams& a, const Piece& p, con
   j.all_lo = __reduce_max_sync(~0u, j.all_lo);
   j.all_hi = __reduce_min_sync(~0u, j.all_hi);
   const bool any = any_lo < any_hi;
-  j.t0 = max(2 * (p.from + p.p0), any ? any_lo / pages4::kTile & ~1 : 0);
-  j.t1 = max(j.t0, min(2 * (p.from + p.p1), any ? (any_hi - 1) / pages4::kTile + 1 : 0));
+  j.t0 = max(2 * (p.from + max(p.u0 - p.fixed, 0)), any ? any_lo / pages4::kTile & ~1 : 0);
+  j.t1 = max(j.t0, min(2 * (p.from + max(p.u1 - p.fixed, 0)), any ? (any_hi - 1) / pages4::kTile + 1 : 0));
   return j;
 }
 
@@ -354,10 +355,10 @@ __device__ __forceinline__ void join_warps(const AttendParams& a, const Piece& p
       to[1] = make_float4(o[gr][0][2 * r + 1], o[gr][1][2 * r + 1], o[gr][2][2 * r + 1], o[gr][3][2 * r + 1]);
     }
   __syncthreads();
-  const bool whole = p.p0 == 0 && p.p1 == p.pairs;
+  const bool whole = p.whole();
   // a part of the workspace: [row][D] sums, [row] maximum, [row] weight.  A CTA's first is of the segment that it has from the CTA before, its second
   // of the one that the next CTA goes on with.
-  float* const ws = a.ws + ((int64_t)blockIdx.x * 2 + (p.p0 == 0)) * (kRows * (D + 2));
+  float* const ws = a.ws + ((int64_t)blockIdx.x * 2 + (p.u0 == 0)) * (kRows * (D + 2));
   const int d = tid % (D / 4) * 4;
   for (int r = tid / (D / 4); r < job.n_rows; r += kWarps * 32 / (D / 4)) {
     float top = -INFINITY;
@@ -941,7 +942,7 @@ __global__ void __launch_bounds__(kRows * D / 4) attend_join_kernel(const __grid
   Share share = share_of(a, blocks);
   Piece p;
   const int64_t per = share.per;
-  const bool ends = next_piece(a, share, p) && p.p0 > 0 && p.p1 == p.pairs;
+  const bool ends = next_piece(a, share, p) && p.u0 > 0 && p.u1 == p.units;
   const int from = ends ? (int)(p.start / per) : 0, n_parts = (int)blockIdx.x - from + 1;
   constexpr int kPart = kRows * (D + 2);
   const int d = threadIdx.x % (D / 4) * 4, r = threadIdx.x / (D / 4);
@@ -1018,7 +1019,7 @@ int64_t pairs_at_most(const linmt_attend_pages4_args* g) { const int64_t p = ((i
 // CTAs: as many as fit on the GPU at once (three on an SM with 128 components, four with 64), or as the longest possible sentences
 // give kLeast pairs each.
 int blocks_of(const linmt_attend_pages4_args* g) {
-  const int64_t segments = (int64_t)g->n * g->pages.heads * row_tiles_of(g), most = segments * ((pairs_at_most(g) + kLeast - 1) / kLeast), fit = 148 * (g->pages.dim == 64 ? 4 : 3);
+  const int64_t segments = (int64_t)g->n * g->pages.heads * row_tiles_of(g), most = segments * ((pairs_at_most(g) + kFixed + kLeast - 1) / kLeast), fit = 148 * (g->pages.dim == 64 ? 4 : 3);
   return (int)(most < fit ? most : fit);
 }
 
