@@ -111,7 +111,7 @@ def test_attend_workspace(cuda_lib):
     assert size(width=16) == 0 and size(n=0, width=4096) == 0 and size(heads=3) == -1     # sentences of up to 256 positions are not cut
     part = 16 * 66 * 4                                         # 16 rows: 64 sums, a maximum and a weight
     assert size(width=4096) == 592 * 2 * part and size(width=4096, n=4000) == 592 * 2 * part
-    assert size(width=32) == 2 * 2 * 3 * 2 * part               # 2 sentences, 2 heads, 16 pairs of tiles that count as 20 units, in parts of 8
+    assert size(width=32) == 2 * 2 * 4 * 2 * part               # 2 sentences, 2 heads, 16 pairs of tiles that count as 28 units, in parts of 8
 
 
 def test_nothing_to_do_reaches_no_device(cuda_lib):
