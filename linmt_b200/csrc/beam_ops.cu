@@ -37,8 +37,8 @@ constexpr int kWarps = 12;                       // 96 of a cluster of 8: 12 bea
 constexpr int kBeyond = 8;                       // candidates past the k-th that the order is checked on
 constexpr int kChunkVecs = 128;                  // a warp's step: four 16-byte vectors a lane
 constexpr int kMaxima = 64;                      // maxima that a warp keeps: of one chunk each, of more where its stretch has more
-constexpr int kMany = 200;                       // candidates of a CTA that are listed as they are found; of more the best `need`
-constexpr int kMaxList = kMaxC * kMany + kMaxK;  // finished rows add one each
+constexpr int kMany = 128;                       // candidates of a CTA that are listed as they are found; of more the best `need`
+constexpr int kMaxList = kMaxC * kMany + kMaxK;  // kMany places for each CTA; finished rows add one each
 constexpr int kSorted = 64;                      // of them that are put in order (>= need)
 constexpr float kLog2e = 1.4426950408889634f;
 typedef long long Key;                           // a sum, as an integer that is ordered alike
@@ -92,6 +92,7 @@ struct SelectSmem {
   double row_lse[kMaxK];         // log of the row's sum, relative to row_max
   float row_max[kMaxK];
   int32_t row_changes[kMaxK];
+  float row_floor[kMaxK];        // what an element has to be to come near the bar
   float score[kMaxK];
   int32_t live[kMaxK];           // rows that are read, in order
   uint32_t done_bits, finite_bits, exact_bits, ask_bits;   // per row: finished; score is finite; summed exactly; to be summed so
@@ -103,15 +104,15 @@ struct SelectSmem {
   int32_t top_at[kMaxC * 32];
   Key bar;
   int32_t bar_at;
-  int32_t n_list;
+  int32_t n_listed[kMaxC];       // candidates that each CTA has put into the list
   int32_t n_todo, n_found;
   uint16_t todo[kWarps * kMaxima];           // chunks to be read again: warp * kMaxima + kept maximum
   Key found[kMany];
   int32_t found_at[kMany];
   Key most[kWarps];
   int32_t most_at[kWarps];
-  Key list[kMaxList];
-  int32_t list_at[kMaxList];
+  Key list[kMaxC * kMany], packed[kMaxList];
+  int32_t list_at[kMaxC * kMany], packed_at[kMaxList];
   Key sorted[kSorted];
   int32_t sorted_at[kSorted];
   ExpTable exps;
@@ -455,7 +456,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
         }
       }
     }
-    if (tid == 0) s.n_list = s.n_todo = s.n_found = 0;
+    if (tid == 0) s.n_todo = s.n_found = 0;
     if (warp == 0) {
 #pragma unroll
       for (int c = 0; c < C; ++c) {
@@ -493,6 +494,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
     };
     if (__shfl_sync(~0u, bid, 0) != kNone) {           // (a warp's best bid is its best candidate's sum)
       const float floor_x = floor_of(score, lse, base);
+      if (lane == 0) s.row_floor[row] = floor_x;         // (all its warps say the same)
 #pragma unroll
       for (int h = 0; h < kMaxima / 32; ++h) {
         const int g = lane + 32 * h;
@@ -509,7 +511,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
         const Row<T> q(a.logits + sent * a.stride_n + rw * a.stride_k, a.vocab, r.allowed);
         const int q0 = cut(q.n_vecs, pt, per_row), q1 = cut(q.n_vecs, pt + 1, per_row);
         const double sc = s.score[rw], bs = s.row_max[rw], ls = s.row_lse[rw];
-        const float floor_x = floor_of(sc, ls, bs);
+        const float floor_x = s.row_floor[rw];
         const int c1 = min((g + 1) << group, (q1 - q0 + kChunkVecs - 1) / kChunkVecs);
         for (int c = g << group; c < c1; ++c) {
           const int vb = q0 + c * kChunkVecs + lane;
@@ -544,13 +546,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
     });
     __syncthreads();
     const int n_found = s.n_found;
+    Key* const list = lead->list + cta * kMany;
+    int32_t* const list_at = lead->list_at + cta * kMany;
+    if (tid == 0) lead->n_listed[cta] = min(n_found, n_found <= kMany ? kMany : need);
     if (n_found <= kMany) {
-      if (warp == 0) {
-        int first = 0;
-        if (lane == 0 && n_found) first = atomicAdd(&lead->n_list, n_found);
-        first = __shfl_sync(~0u, first, 0);
-        for (int i = lane; i < n_found; i += 32) { lead->list[first + i] = s.found[i]; lead->list_at[first + i] = s.found_at[i]; }
-      }
+      for (int i = tid; i < n_found; i += kWarps * 32) { list[i] = s.found[i]; list_at[i] = s.found_at[i]; }
     } else {
       Key prev = kNone;                      // many (equal or sorted logits): the best `need` of them, one by one
       int prev_at = 0;
@@ -570,11 +570,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
         __syncthreads();
         for (int w = 0; w < kWarps; ++w)
           if (before(s.most[w], s.most_at[w], most, most_at)) { most = s.most[w]; most_at = s.most_at[w]; }
-        if (tid == 0) {
-          const int slot = atomicAdd(&lead->n_list, 1);
-          lead->list[slot] = most;
-          lead->list_at[slot] = most_at;
-        }
+        if (tid == 0) { list[turn] = most; list_at[turn] = most_at; }
         prev = most;
         prev_at = most_at;
         __syncthreads();
@@ -585,22 +581,29 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
     // 4. the order
     int n_sorted = 0;
     if (cta == 0) {
-      const int n_listed = s.n_list;
+      // the CTAs' candidates one after the other, then one for each finished beam
       const uint32_t ended = s.done_bits & s.finite_bits;
-      const int n = n_listed + __popc(ended);
+      int before_cta = 0;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int m = s.n_listed[c];
+        for (int i = tid; i < m; i += kWarps * 32) { s.packed[before_cta + i] = s.list[c * kMany + i]; s.packed_at[before_cta + i] = s.list_at[c * kMany + i]; }
+        before_cta += m;
+      }
+      const int n = before_cta + __popc(ended);
       if (warp == 0 && ((ended >> lane) & 1)) {
-        const int slot = n_listed + __popc(ended & ((1u << lane) - 1));
-        s.list[slot] = key_of((double)s.score[lane]);
-        s.list_at[slot] = lane * a.vocab + a.eos;
+        const int slot = before_cta + __popc(ended & ((1u << lane) - 1));
+        s.packed[slot] = key_of((double)s.score[lane]);
+        s.packed_at[slot] = lane * a.vocab + a.eos;
       }
       __syncthreads();
       n_sorted = min(n, kSorted);
       for (int i = tid; i < n; i += kWarps * 32) {
-        const Key ck = s.list[i];
-        const int ca = s.list_at[i];
+        const Key ck = s.packed[i];
+        const int ca = s.packed_at[i];
         int rank = 0;
 #pragma unroll 4
-        for (int j = 0; j < n; ++j) rank += before(s.list[j], s.list_at[j], ck, ca);
+        for (int j = 0; j < n; ++j) rank += before(s.packed[j], s.packed_at[j], ck, ca);
         if (rank < kSorted) { s.sorted[rank] = ck; s.sorted_at[rank] = ca; }
       }
       __syncthreads();
@@ -653,7 +656,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
     }
     // The rows that are asked for once more, exactly, a part by each of the cluster's warps: cut and added up by the words' own numbers, wherever
     // the row begins, so that equal rows get equal sums and their ties stay ties.  (The list's place is free.)
-    constexpr int kRowsAtOnce = kMaxList / (kMaxC * kWarps);
+    constexpr int kRowsAtOnce = kMany / kWarps;
     if (tid < 64) {
       const double e = exp2(tid / 64.0);
       s.exps.hi[tid] = (float)e;

@@ -2,6 +2,7 @@
 // what was not given, and calls.  In C++ because a step's calls are shorter than the same checks in Python take (20 to 40 us a call there, 3 to 7
 // here).  What each function takes and returns is described in linmt_b200/device_ops.py, which passes its arguments on in order.
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -26,7 +27,8 @@ const Tensor& tensor(PyObject* o, const char* name) {
 }
 const Tensor& on_cuda(PyObject* o, const char* name) {
   const Tensor& t = tensor(o, name);
-  NEED(t.is_cuda() && t.layout() == at::kStrided, name, " has to be a CUDA tensor");
+  NEED(t.is_cuda() && t.layout() == at::kStrided && !t.is_neg(), name, " has to be a CUDA tensor");
+  NEED(!t.requires_grad() || !at::GradMode::is_enabled(), name, " requires a gradient, and there is no backward pass: call under torch.no_grad()");
   return t;
 }
 const Tensor& on_device(PyObject* o, const char* name, int dev) {
@@ -324,6 +326,7 @@ PyObject* write_pages4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   g.device = dev;
   g.stream = stream_of(dev);
   g.pages = pool_of(a[0], dev);
+  NEED(apart(THPVariable_Unpack(a[0])), "pages have places that share memory");
   slots_of(a[1], dev, g);
   const Tensor &k = on_device(a[2], "k", dev), &v = on_device(a[3], "v", dev);
   g.dtype = dtype_of(k);

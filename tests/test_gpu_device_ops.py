@@ -750,6 +750,17 @@ def test_attend_refuses(ops):
             bad()
 
 
+def test_gradients_are_refused(ops):
+    """No backward pass: a call that would drop a gradient does not go through."""
+    x, s = torch.zeros(1, 2, 50, device="cuda", requires_grad=True), torch.zeros(1, 2, device="cuda")
+    h, parents = torch.zeros(1, 2, 8, device="cuda", requires_grad=True), torch.zeros(1, 2, dtype=torch.int32, device="cuda")
+    for call in (lambda: ops.beam_select(x, s), lambda: ops.beam_reorder([h], parents)):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+
+
 # ---- together
 
 class Toy:
