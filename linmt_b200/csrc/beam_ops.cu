@@ -2,6 +2,7 @@
 #include <cooperative_groups.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "device_ops.h"
 
@@ -88,7 +89,7 @@ struct PairSum {
 
 struct SelectSmem {
   float unit_max[kMaxC * kWarps], unit_sum[kMaxC * kWarps];
-  int32_t unit_changes[kMaxC * kWarps];      // most often that a lane's maximum changed
+  int32_t unit_changes[kMaxC * kWarps];      // how often its sum was scaled by other than a power of 2
   double row_lse[kMaxK];         // log of the row's sum, relative to row_max
   float row_max[kMaxK];
   int32_t row_changes[kMaxK];
@@ -258,10 +259,10 @@ __device__ __forceinline__ float exp2_of(float x) {
   return y;
 }
 
-// Bound on the error of a row's log of its sum, where a lane adds it up in `chunks` steps and changes its maximum `changes` times: two roundings of
-// an exponent's argument (2^-24 of it, on average at most log2(vocab) + 1 in size: 1.5e-6 below a vocabulary of 2^17), exp2's own 2^-22, 20 additions
-// deep inside and across lanes, the same where stretches are joined, the logarithm's last place (2^-20 below 16); an addition
-// for each chunk, and an exp2 and a product for each change.
+// Bound on the error of a row's log of its sum, where a lane adds it up in `chunks` steps and scales it by other than a power of 2 `changes` times: two roundings
+// of an exponent's argument (2^-24 of it, on average at most log2(vocab) + 1 in size: 1.5e-6 below a vocabulary of 2^17; or one, and log2 e's of logits
+// below 64), exp2's own 2^-22, 20 additions deep inside and across lanes, the same where stretches are joined, the logarithm's last place (2^-20 below
+// 16); an addition for each chunk, and an exp2 and a product for each change.
 __device__ __forceinline__ double row_error(int chunks, int changes) { return 6e-6 + 6e-8 * chunks + 4.5e-7 * changes; }
 
 template <class T, int C>
@@ -295,8 +296,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
   const int v0 = cut(r.n_vecs, part, per_row), v1 = busy ? cut(r.n_vecs, part + 1, per_row) : v0;
 
   // 1. the stretch, once
-  float top = -INFINITY, sum = 0.f;
-  int changes = 0, top_vec = 0;          // first vector of the warp's chunk that the lane's maximum is in
+  float top = -INFINITY;                 // the lane's maximum
+  float wtop = -INFINITY, sum = 0.f, ref = 0.f;      // the warp's; the lane's sum, relative to it
+  int changes = 0, top_vec = 0;          // top_vec: first vector of the warp's chunk that the lane's maximum is in
   const int n_chunks = (v1 - v0 + kChunkVecs - 1) / kChunkVecs;
   const int most_chunks = ((a.vocab / E + 2) / per_row + kChunkVecs) / kChunkVecs;      // of any stretch of the sentence
   int group = 0;                         // chunks of a kept maximum, as a power of 2
@@ -313,67 +315,82 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
       if (r.allowed) ahead_bits[j] = r.bits_of(vb + lane + 32 * j);
     }
   };
-  fetch(v0);
-  for (int c = 0; c < n_chunks; ++c) {
-    const int vb = v0 + c * kChunkVecs;
-    uint4 raw[4];
-    float m;
-    if (inside(vb)) {
+  // Terms are exp2(x log2 e - ref), ref the whole number next to the warp's maximum in these units: one instruction for the exponent, and a new maximum
+  // scales the sum by an exact power of 2.  FAR: the maximum is 64 or more in size, where log2 e's own rounding (1.4e-8 of x) would tell:
+  // the stretch is read again with differences to the maximum itself.
+  auto scan = [&](auto is_far) {
+    constexpr bool FAR = decltype(is_far)::value;
+    top = wtop = -INFINITY;
+    sum = ref = 0.f;
+    fetch(v0);
+    for (int c = 0; c < n_chunks; ++c) {
+      const int vb = v0 + c * kChunkVecs;
+      uint4 raw[4];
+      if (inside(vb)) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) raw[j] = r.allowed ? r.keep(ahead_bits[j], ahead[j]) : ahead[j];
-    } else {
+        for (int j = 0; j < 4; ++j) raw[j] = r.allowed ? r.keep(ahead_bits[j], ahead[j]) : ahead[j];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int v = vb + lane + 32 * j;
+          const bool whole = v < v1 && r.whole(v);
+          raw[j] = whole ? r.raw(v) : r.nothing();
+          if (v < v1) raw[j] = r.clean(v, whole, raw[j]);
+        }
+      }
+      fetch(vb + kChunkVecs);
+      const float m = fmaxf(fmaxf(Packed<T>::max4(raw[0]), Packed<T>::max4(raw[1])), fmaxf(Packed<T>::max4(raw[2]), Packed<T>::max4(raw[3])));
+      if (m > top) {
+        top = m;
+        top_vec = vb;
+      }
+      const int most = __reduce_max_sync(~0u, ordered(m));
+      const float chunk_max = __int_as_float(most ^ ((most >> 31) & 0x7fffffff));
+      if (lane == 0) {
+        float* const slot = &s.chunk_max[warp][c >> group];
+        *slot = c & ((1 << group) - 1) ? fmaxf(*slot, chunk_max) : chunk_max;
+      }
+      if (chunk_max > wtop) {
+        if (FAR) {
+          sum *= exp2_of((wtop - chunk_max) * kLog2e);
+          ++changes;
+        } else {
+          const float now = rintf(chunk_max * kLog2e);
+          sum *= ref - now < -126.f ? 0.f : __int_as_float((127 + (int)(ref - now)) << 23);
+          ref = now;
+        }
+        wtop = chunk_max;
+      }
+      const float base = wtop == -INFINITY ? 0.f : wtop;     // (nothing allowed yet: every term is exp2(-inf), or a NaN, which stays one)
+      float part_sum[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int v = vb + lane + 32 * j;
-        const bool whole = v < v1 && r.whole(v);
-        raw[j] = whole ? r.raw(v) : r.nothing();
-        if (v < v1) raw[j] = r.clean(v, whole, raw[j]);
+        const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+        part_sum[j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x[Packed<T>::kPer];
+          Packed<T>::get(w[i], x);
+#pragma unroll
+          for (int e = 0; e < Packed<T>::kPer; ++e) part_sum[j] += exp2_of(FAR ? (x[e] - base) * kLog2e : fmaf(x[e], kLog2e, -ref));
+        }
       }
+      sum += (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
     }
-    fetch(vb + kChunkVecs);
-    m = fmaxf(fmaxf(Packed<T>::max4(raw[0]), Packed<T>::max4(raw[1])), fmaxf(Packed<T>::max4(raw[2]), Packed<T>::max4(raw[3])));
-    const int chunk_max = __reduce_max_sync(~0u, ordered(m));
-    if (lane == 0) {
-      float* const slot = &s.chunk_max[warp][c >> group];
-      const float cm = __int_as_float(chunk_max ^ ((chunk_max >> 31) & 0x7fffffff));
-      *slot = c & ((1 << group) - 1) ? fmaxf(*slot, cm) : cm;
-    }
-    if (m > top) {
-      sum *= exp2_of((top - m) * kLog2e);
-      top = m;
-      top_vec = vb;
-      ++changes;
-    }
-    const float base = top == -INFINITY ? 0.f : top;     // (nothing allowed yet: every term is exp2(-inf), or a NaN, which stays one)
-    float part_sum[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
-      part_sum[j] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x[Packed<T>::kPer];
-        Packed<T>::get(w[i], x);
-#pragma unroll
-        for (int e = 0; e < Packed<T>::kPer; ++e) part_sum[j] += exp2_of((x[e] - base) * kLog2e);
-      }
-    }
-    sum += (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
-  }
-  // (fmaxf passes over NaN: the sum has it.  +inf: its own term is a NaN.)
-  float wtop = top;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) wtop = fmaxf(wtop, __shfl_xor_sync(~0u, wtop, o));
-  float wsum = top == -INFINITY ? sum : sum * exp2_of((top - wtop) * kLog2e);
+    if (!FAR && wtop > -INFINITY) sum *= exp2_of(fmaf(-wtop, kLog2e, ref));      // relative to exp(wtop)
+  };
+  scan(std::false_type{});
+  if (wtop > -INFINITY && !(fabsf(wtop) < 64.f)) scan(std::true_type{});
+  // (Maxima pass over NaN: the sum has it.  +inf: its own term is a NaN.)
+  float wsum = sum;
 #pragma unroll
   for (int o = 16; o; o >>= 1) wsum += __shfl_xor_sync(~0u, wsum, o);
-  const int wchanges = __reduce_max_sync(~0u, changes);
   cluster.barrier_wait();
   if (busy && lane < C) {
     SelectSmem* to = cluster.map_shared_rank(&s, lane);
     to->unit_max[unit] = wtop;
     to->unit_sum[unit] = wsum;
-    to->unit_changes[unit] = wchanges;
+    to->unit_changes[unit] = changes;
   }
   cluster.sync();
 
