@@ -38,7 +38,8 @@ constexpr int kWarps = 12;                       // 96 of a cluster of 8: 12 bea
 constexpr int kBeyond = 8;                       // candidates past the k-th that the order is checked on
 constexpr int kChunkVecs = 128;                  // a warp's step: four 16-byte vectors a lane
 constexpr int kMaxima = 64;                      // maxima that a warp keeps: of one chunk each, of more where its stretch has more
-constexpr int kMany = 128;                       // candidates of a CTA that are listed as they are found; of more the best `need`
+constexpr int kMany = 128;                       // candidates of a CTA that are listed as they are found; of more the best `need`:
+constexpr int kFound = 512;                      // of up to so many by ranking them, of more one by one
 constexpr int kMaxList = kMaxC * kMany + kMaxK;  // kMany places for each CTA; finished rows add one each
 constexpr int kSorted = 64;                      // of them that are put in order (>= need)
 constexpr float kLog2e = 1.4426950408889634f;
@@ -108,8 +109,8 @@ struct SelectSmem {
   int32_t n_listed[kMaxC];       // candidates that each CTA has put into the list
   int32_t n_todo, n_found;
   uint16_t todo[kWarps * kMaxima];           // chunks to be read again: warp * kMaxima + kept maximum
-  Key found[kMany];
-  int32_t found_at[kMany];
+  Key found[kFound];
+  int32_t found_at[kFound];
   Key most[kWarps];
   int32_t most_at[kWarps];
   Key list[kMaxC * kMany], packed[kMaxList];
@@ -559,7 +560,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
     };
     sweep([&](Key key, int at) {
       const int slot = atomicAdd(&s.n_found, 1);
-      if (slot < kMany) { s.found[slot] = key; s.found_at[slot] = at; }
+      if (slot < kFound) { s.found[slot] = key; s.found_at[slot] = at; }
     });
     __syncthreads();
     const int n_found = s.n_found;
@@ -568,6 +569,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
     if (tid == 0) lead->n_listed[cta] = min(n_found, n_found <= kMany ? kMany : need);
     if (n_found <= kMany) {
       for (int i = tid; i < n_found; i += kWarps * 32) { list[i] = s.found[i]; list_at[i] = s.found_at[i]; }
+    } else if (n_found <= kFound) {
+      for (int i = tid; i < n_found; i += kWarps * 32) {
+        const Key fk = s.found[i];
+        const int fa = s.found_at[i];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < n_found; ++j) rank += before(s.found[j], s.found_at[j], fk, fa);
+        if (rank < need) { list[rank] = fk; list_at[rank] = fa; }
+      }
     } else {
       Key prev = kNone;                      // many (equal or sorted logits): the best `need` of them, one by one
       int prev_at = 0;
@@ -730,11 +740,12 @@ cudaError_t launch_select(const linmt_beam_select_args& g) {
                     g.out_tokens, g.out_parents, g.out_scores, g.out_done, g.k, g.vocab, g.eos};
   // As many CTAs for a sentence as leave all of them on the GPU at once (two on an SM; clusters of 8 only reach 33), since a second round of
   // clusters costs its latencies again, and as have 16k logits each: exchanges among more take longer (64 x 12 x 30k fp32: 40, 30 and 51 us
-  // with 2, 4 and 8; 128 x 12 x 80k bf16: 82, 95 and 141; 1 x 4 x 1000: 10.2, 10.6 and 12.4).  A warp needs a row at most: 12 beams for one CTA.
+  // with 2, 4 and 8; 128 x 12 x 80k bf16: 82, 95 and 141; 1 x 4 x 1000: 10.2, 10.6 and 12.4).  A row needs as many warps as have
+  // four thirds of `need` lanes, or the bar falls below what its best candidates are when one beam is ahead (139 x 30 x 5.9k fp16 with one warp a row: 480 us).
   const int64_t logits = (int64_t)g.k * g.vocab;
   int c = g.n <= 33 ? 8 : g.n <= 74 ? 4 : g.n <= 148 ? 2 : 1;
   while (c > 1 && logits < (int64_t)(c / 2 + 1) * 16384) c /= 2;
-  while (c * kWarps < g.k) c *= 2;
+  while (g.k + kBeyond > 24 * (c * kWarps / g.k)) c *= 2;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;

@@ -131,7 +131,7 @@ def test_select_ties_go_to_the_lowest_index(ops, k, v, dtype):
             select_check(ops, x, scores)
 
 
-@pytest.mark.parametrize("n,k,v", [(1, 12, 30000), (80, 5, 9001), (50, 9, 4003), (80, 31, 1500), (160, 12, 3001), (160, 13, 3001)])
+@pytest.mark.parametrize("n,k,v", [(1, 12, 30000), (80, 5, 9001), (50, 9, 4003), (80, 31, 1500), (160, 12, 3001), (160, 13, 3001), (3, 17, 9000), (140, 24, 2500), (90, 32, 2100)])
 def test_select_one_beam_ahead(ops, n, k, v):
     """All that is chosen lies in one row, in few of its places, or in logits too small to tell apart; for one sentence and for so many that each has few CTAs."""
     rng = _rng(n, k, v, 3)
