@@ -427,9 +427,9 @@ int linmt_read_pages4(const linmt_pages4_rows_args* args);
  *   s = scale * q . k_t;  cap > 0: s = cap * tanh(s / cap);  slope: s -= slope[h] * |t - centre[i][row]|
  *   seen: first[i][row] <= t < last[i][row] (NULL: all), 0 <= t < len[i], and the table names a page of the pool
  *   out = sum over seen of softmax(s) * v_t; lse = log sum over seen of exp(s).  Nothing seen: 0 and -inf.
- * `len` beyond width * page is taken as that.  Sums are held in 32 bits.  16-bit queries: weights times
- * scales are rounded to fp16, with a power of 2 that follows the largest scale so far (scales of 2^-97 to 2^103).  32-bit queries and weights are
- * multiplied as three bf16 terms each.
+ * `len` beyond width * page is taken as that.  Sums are held in 32 bits.  Weights times scales are
+ * rounded to fp16, with a power of 2 that follows the largest scale so far (scales of 2^-97 to 2^103); for 32-bit queries, which are multiplied as two fp16
+ * terms, they are two such terms too.
  * `workspace`: linmt_attend_pages4_workspace bytes, 16-byte aligned, the call's own until it has run; NULL where that is 0. */
 typedef struct linmt_attend_pages4_args {
   uint32_t size;

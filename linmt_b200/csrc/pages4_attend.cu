@@ -6,14 +6,17 @@
 // operand of mma.m16n8k16, so every code is loaded and unpacked once for all of them.  (tcgen05.mma wants both operands of at least 64
 // rows, and codes unpacked into shared memory first; with 16 rows the unpacking, not the product, is what takes the time.)
 //   Scales stay out of the products: a key's is multiplied onto its group's sum, a value's into the weight on the left.
-//   16-bit queries (attend16_kernel).  A word's codes become matrix operands with one AND each: an integer in the low bits of an
+//   A word's codes become matrix operands with one AND each: an integer in the low bits of an
 //   fp16 number is a subnormal one, that integer times 2^-24, and stays so up to 2047, so every second
 //   code may be left four bits up and its 16 taken out elsewhere (of the queries before, of the output's columns after).  What is then too much, 8 for each
 //   code, goes off by a product of its own: the queries' sums with the keys' scales, and the weights' sums.  That is 5
 //   instructions for 8 codes where a code minus 8 in normal form takes 11, in a kernel bound by what it can issue.  Queries are scaled to
 //   fp16's upper range by a power of 2 for each row.  Weights are multiplied by their values' scales and rounded to fp16 (2^-11 each at most), with a power of 2
 //   that follows the scales, as the maximum follows the scores: the largest scale lies 2^3 above 1, and a weight 2^28 below the largest still counts.
-//   32-bit queries (attend32_kernel) are three bf16 terms, the weights too (2^-24), the codes minus 8 in normal form.
+//   32-bit queries are two fp16 terms, and so are their weights: 2^-22 of each, or 2^-34 of the largest.  Their codes are made normal numbers less 8 (9
+//   instructions for 8 codes): the matrix unit cuts addends off at a place that goes by their exponents, and subnormal operands lose up to 10 bits there, which
+//   an output rounded to 16 bits does not see but one of 32 does (2^-14 of a scale was seen).  (Three bf16 terms of each, exact to 2^-24: 18 sentences of
+//   6068 to 8725 positions with 10 beams and 28 heads of 64 in 168 us, not 155.)
 // Every warp has a ring of tiles of its own (cp.async, no barrier among warps) and its own maximum and sums; the CTA's four are
 // joined through shared memory at the end of a piece of work, and where a sentence's positions are shared by CTAs a second kernel joins those.
 #include <atomic>
@@ -26,12 +29,13 @@ namespace ops {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kStages = 4;         // of attend32_kernel: tiles
-constexpr int kPairStages = 2;     // of attend16_kernel: pairs of tiles (three: 2 % longer)
+constexpr int kPairStages = 2;     // pairs of tiles in a warp's ring (three: 2 % longer)
 constexpr int kRows = 16;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kTerms = 3;          // bf16 terms of a 32-bit query and weight
-constexpr float kSlack = 8.f;      // the reference maximum follows the true one only when it lags by 2^8: few tiles rescale the sums
+
+template <class T> constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;           // fp16 terms of a query and of a weight
+template <class T> constexpr float kSlack = sizeof(T) == 4 ? 2.f : 8.f;     // the reference maximum follows the true one only when it lags by 2^8 (2^2): few tiles rescale the sums
+template <class T> constexpr int kAbove = sizeof(T) == 4 ? 9 : 3;           // the largest scale, in powers of 2 above 1: with the slack and 2^4 of its own growth 2^15 at most
 
 struct AttendParams {
   const unsigned char* data;
@@ -55,15 +59,11 @@ struct AttendParams {
   int32_t q_wide, o_wide;    // the rows of q are 16-byte aligned; fours of components of out are aligned to their size
 };
 
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-// The same onto nothing.
+// The products onto nothing.
 __device__ __forceinline__ void mma_bf16_first(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
@@ -76,22 +76,19 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
 }
-__device__ __forceinline__ uint32_t lop_and_or(uint32_t x, uint32_t m, uint32_t o) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(m), "r"(o));
-  return r;
-}
-// Codes i (low half) and i + 4 (high half) of a word, minus 8.  An integer below 128 laid into the low bits of 128.0 adds itself to it.
-template <int I>
-__device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {
-  const uint32_t b = lop_and_or(w >> (4 * I), 0x000f000fu, 0x43004300u), off = 0x43084308u;      // 128 + code, 136
-  __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&off));
-  return *reinterpret_cast<uint32_t*>(&r);
-}
 __device__ __forceinline__ __nv_bfloat162 bf16_pair(uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Every second code of a word as matrix operands: `odd`, those four bits up.  16-bit queries: 0 .. 15 (odd: times 16) times 2^-24.  32-bit: less 8, in normal form.
+template <class T>
+__device__ __forceinline__ uint32_t operand(uint32_t word, bool odd) {
+  const uint32_t v = word & (odd ? 0x00f000f0u : 0x000f000fu);
+  if constexpr (sizeof(T) == 2) return v;
+  const uint32_t up = v | 0x64006400u;      // 1024 more
+  const __half2 x = *reinterpret_cast<const __half2*>(&up), y = odd ? __hfma2(x, __float2half2_rn(0.0625f), __float2half2_rn(-72.f)) : __hsub2(x, __float2half2_rn(1032.f));
+  return *reinterpret_cast<const uint32_t*>(&y);
 }
 __device__ __forceinline__ float bf16_low(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float bf16_high(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
@@ -274,19 +271,7 @@ __device__ __forceinline__ bool next_piece(const AttendParams& a, Share& s, Piec
 
 template <class T, int D>
 constexpr int attend_smem() {
-  if constexpr (sizeof(T) == 2) return kWarps * kPairStages * 2 * 18 * D + (D / 16) * 512;
-  else return kWarps * kStages * 18 * D + kTerms * (D / 16) * 512;
-}
-
-// The pair of query components that a lane's 32 bits of the left operand hold, as term `term` of their bf16 expansion.
-__device__ __forceinline__ uint32_t query_pair(const float* row, int d, int term) {
-  if (!row) return 0u;
-  float lo = __ldg(row + d), hi = __ldg(row + d + 4);
-  for (int i = 0; i < term; ++i) {
-    lo -= __bfloat162float(__float2bfloat16_rn(lo));
-    hi -= __bfloat162float(__float2bfloat16_rn(hi));
-  }
-  return pack_bf16(lo, hi);
+  return kWarps * kPairStages * 2 * 18 * D + kTerms<T> * (D / 16) * 512;
 }
 
 // What a piece's rows see.
@@ -384,234 +369,19 @@ __device__ __forceinline__ void join_warps(const AttendParams& a, const Piece& p
   __syncthreads();                    // (before the next piece's tiles come in)
 }
 
-template <int D>
-__global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend32_kernel(const __grid_constant__ AttendParams a) {
-  constexpr int NG = D / 32, kTileBytes = pages4::tile_bytes(D), QT = kTerms, PT = kTerms;
-  extern __shared__ __align__(16) unsigned char smem[];
-  launch_next();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, c = lane & 3;
-  Share share = share_of(a, gridDim.x);
-  Piece piece;
-  while (next_piece(a, share, piece)) {
-    const float* q_row[2];
-    const Job job = job_of<float>(a, piece, q_row);
-    const int t0 = job.t0, t1 = job.t1, all_lo = job.all_lo, all_hi = job.all_hi;
-    const int (&lo)[2] = job.lo, (&hi)[2] = job.hi;
-    const float (&slope)[2] = job.slope, (&centre)[2] = job.centre;
-
-    // Queries as left operands: step (group, half) takes components 32 group + 8 c + 2 half + {0, 4 | 1, 5}.
-    uint4* const q_smem = reinterpret_cast<uint4*>(smem + kWarps * kStages * kTileBytes);
-    for (int s = warp; s < QT * NG * 2; s += kWarps) {
-      const int term = s / (NG * 2), d = 32 * ((s % (NG * 2)) >> 1) + 8 * c + 2 * (s & 1);
-      q_smem[s * 32 + lane] = make_uint4(query_pair(q_row[0], d, term), query_pair(q_row[1], d, term), query_pair(q_row[0], d + 1, term), query_pair(q_row[1], d + 1, term));
-    }
-    __syncthreads();
-
-    float o[NG][4][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    const float to_log2 = a.cap > 0.f ? a.scale / a.cap : a.scale * kLog2e, cap_log2 = a.cap * kLog2e;
-    unsigned char* const ring = smem + warp * kStages * kTileBytes;
-    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-    const int32_t* const table = a.table + piece.sent * a.table_stride;
-    const unsigned char* const head = a.data + piece.kvh * a.stride_head;
-    const int tiles_per_page = a.page / pages4::kTile;
-    const int mine = t1 - t0 > warp ? (t1 - t0 - warp + kWarps - 1) / kWarps : 0;        // this warp's tiles: t0 + warp + kWarps i
-
-    // Where this warp's tiles are: looked up 32 at a time, one by each lane, a batch ahead of their use.
-    int64_t where = -1;
-    uint32_t bad = 0;                // bit of a stage: it holds no tile of the pool
-    auto fetch = [&](int i) {
-      if ((i & 31) == 0) {
-        where = -1;
-        if (i + lane < mine) where = pages4::tile_offset(table, t0 + warp + kWarps * (i + lane), tiles_per_page, a.n_pages, a.stride_page, D);
-      }
-      const int64_t at = __shfl_sync(~0u, where, i & 31);
-      const int stage = i % kStages;
-      if (i < mine && at >= 0) {
-        bad &= ~(1u << stage);
-#pragma unroll
-        for (int b = 0; b < (kTileBytes + 511) / 512; ++b) {
-          const int byte = b * 512 + lane * 16;
-          if (byte < kTileBytes) copy16(ring_at + stage * kTileBytes + byte, head + at + byte);
-        }
-      } else {
-        bad |= 1u << stage;
-      }
-      copy_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) fetch(i);
-
-    for (int i = 0; i < mine; ++i) {
-      copy_wait<kStages - 2>();
-      __syncwarp();                       // every lane's part of tile i is there, and tile i - 1 has been read by all
-      fetch(i + kStages - 1);
-      if ((bad >> (i % kStages)) & 1) continue;
-      const unsigned char* const tile = ring + (i % kStages) * kTileBytes;
-      const int pos = (t0 + warp + kWarps * i) * pages4::kTile;
-
-      // scores: x[j][0..3] = rows gid, gid, gid + 8, gid + 8 at positions pos + 8 j + 2 c + {0, 1, 0, 1}
-      float x[2][4];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        uint32_t w[NG], sc[NG];
-        const unsigned char* const kw = tile + (8 * j + gid) * (D / 2) + c * (4 * NG);
-        const unsigned char* const ks = tile + pages4::key_scales(D) + (8 * j + 2 * c) * (2 * NG);
-        if constexpr (NG == 4) {
-          *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(kw);
-          *reinterpret_cast<uint4*>(sc) = *reinterpret_cast<const uint4*>(ks);
-        } else {
-          *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(kw);
-          *reinterpret_cast<uint2*>(sc) = *reinterpret_cast<const uint2*>(ks);
-        }
-        x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.f;
-#pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-          float s[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t b[4];
-          b[0] = codes_bf16<0>(w[gr]); b[1] = codes_bf16<1>(w[gr]); b[2] = codes_bf16<2>(w[gr]); b[3] = codes_bf16<3>(w[gr]);
-#pragma unroll
-          for (int term = QT - 1; term >= 0; --term) {      // small terms first
-            mma_bf16(s, q_smem[(term * NG * 2 + 2 * gr) * 32 + lane], b[0], b[1]);
-            mma_bf16(s, q_smem[(term * NG * 2 + 2 * gr + 1) * 32 + lane], b[2], b[3]);
-          }
-          // scales of position 2 c: halves gr of the first NG, of 2 c + 1: of the second
-          const float s0 = gr & 1 ? bf16_high(sc[gr >> 1]) : bf16_low(sc[gr >> 1]);
-          const float s1 = gr & 1 ? bf16_high(sc[NG / 2 + (gr >> 1)]) : bf16_low(sc[NG / 2 + (gr >> 1)]);
-          x[j][0] = fmaf(s[0], s0, x[j][0]);
-          x[j][1] = fmaf(s[1], s1, x[j][1]);
-          x[j][2] = fmaf(s[2], s0, x[j][2]);
-          x[j][3] = fmaf(s[3], s1, x[j][3]);
-        }
-      }
-      if (a.cap > 0.f) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[j][e] = cap_log2 * tanhf(x[j][e] * to_log2);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[j][e] *= to_log2;
-      }
-      if (a.slope) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[j][e] -= slope[e >> 1] * fabsf((float)(pos + 8 * j + 2 * c + (e & 1)) - centre[e >> 1]);
-      }
-      const bool edge = pos < all_lo || pos + pages4::kTile > all_hi;
-      if (edge) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int p = pos + 8 * j + 2 * c + (e & 1);
-            if (p < lo[e >> 1] || p >= hi[e >> 1]) x[j][e] = -INFINITY;
-          }
-      }
-      float top[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        top[e] = fmaxf(fmaxf(x[0][2 * e], x[0][2 * e + 1]), fmaxf(x[1][2 * e], x[1][2 * e + 1]));
-        top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], 1));
-        top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], 2));
-      }
-      const bool up0 = top[0] > m[0] + kSlack || (m[0] == -INFINITY && top[0] > -INFINITY), up1 = top[1] > m[1] + kSlack || (m[1] == -INFINITY && top[1] > -INFINITY);
-      if (__any_sync(~0u, up0 || up1)) {
-        const float f0 = up0 ? exp2_of(m[0] - top[0]) : 1.f, f1 = up1 ? exp2_of(m[1] - top[1]) : 1.f;
-        if (up0) m[0] = top[0];
-        if (up1) m[1] = top[1];
-        l[0] *= f0;
-        l[1] *= f1;
-#pragma unroll
-        for (int gr = 0; gr < NG; ++gr)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            o[gr][e][0] *= f0; o[gr][e][1] *= f0;
-            o[gr][e][2] *= f1; o[gr][e][3] *= f1;
-          }
-      }
-      const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        x[j][0] = exp2_of(x[j][0] - m0);
-        x[j][1] = exp2_of(x[j][1] - m0);
-        x[j][2] = exp2_of(x[j][2] - m1);
-        x[j][3] = exp2_of(x[j][3] - m1);
-        l[0] += x[j][0] + x[j][1];
-        l[1] += x[j][2] + x[j][3];
-      }
-
-      // out += weights . values, a group of 32 components a time: its scales go into the weights
-      uint32_t vs[2][NG];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const unsigned char* const at = tile + pages4::value_scales(D) + (8 * j + 2 * c) * (2 * NG);
-        if constexpr (NG == 4) *reinterpret_cast<uint4*>(vs[j]) = *reinterpret_cast<const uint4*>(at);
-        else *reinterpret_cast<uint2*>(vs[j]) = *reinterpret_cast<const uint2*>(at);
-        if (edge) {            // a position that nobody sees may hold anything: 0 times its scale has to be 0
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (x[j][e] == 0.f && x[j][e + 2] == 0.f) {
-#pragma unroll
-              for (int i2 = 0; i2 < NG / 2; ++i2) vs[j][e * (NG / 2) + i2] = 0u;
-            }
-        }
-      }
-#pragma unroll
-      for (int i2 = 0; i2 < NG / 2; ++i2) {
-        const uint4 u = *reinterpret_cast<const uint4*>(tile + pages4::value_codes(D) + 16 * (i2 * 32 + lane));
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int gr = 2 * i2 + h;
-          const uint32_t w0 = h ? u.y : u.x, w1 = h ? u.w : u.z;
-          float p[2][4];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float s0 = h ? bf16_high(vs[j][i2]) : bf16_low(vs[j][i2]), s1 = h ? bf16_high(vs[j][NG / 2 + i2]) : bf16_low(vs[j][NG / 2 + i2]);
-            p[j][0] = x[j][0] * s0;
-            p[j][1] = x[j][1] * s1;
-            p[j][2] = x[j][2] * s0;
-            p[j][3] = x[j][3] * s1;
-          }
-          uint4 pa[PT];
-#pragma unroll
-          for (int term = 0; term < PT; ++term) {
-            pa[term] = make_uint4(pack_bf16(p[0][0], p[0][1]), pack_bf16(p[0][2], p[0][3]), pack_bf16(p[1][0], p[1][1]), pack_bf16(p[1][2], p[1][3]));
-            if (term + 1 < PT) {
-              p[0][0] -= bf16_low(pa[term].x); p[0][1] -= bf16_high(pa[term].x);
-              p[0][2] -= bf16_low(pa[term].y); p[0][3] -= bf16_high(pa[term].y);
-              p[1][0] -= bf16_low(pa[term].z); p[1][1] -= bf16_high(pa[term].z);
-              p[1][2] -= bf16_low(pa[term].w); p[1][3] -= bf16_high(pa[term].w);
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t b0 = e == 0 ? codes_bf16<0>(w0) : e == 1 ? codes_bf16<1>(w0) : e == 2 ? codes_bf16<2>(w0) : codes_bf16<3>(w0);
-            const uint32_t b1 = e == 0 ? codes_bf16<0>(w1) : e == 1 ? codes_bf16<1>(w1) : e == 2 ? codes_bf16<2>(w1) : codes_bf16<3>(w1);
-#pragma unroll
-            for (int term = PT - 1; term >= 0; --term) mma_bf16(o[gr][e], pa[term], b0, b1);
-          }
-        }
-      }
-    }
-
-    join_warps<float, D>(a, piece, job, smem, o, m, l);
-  }
-}
-
 // PLAIN: no cap, no bias, and a scale: scores are products times mul.
 template <class T, int D, bool PLAIN>
-__global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(const __grid_constant__ AttendParams a) {
-  constexpr int NG = D / 32, kTileBytes = pages4::tile_bytes(D);
-  constexpr uint32_t kEven = 0x000f000fu, kOdd = 0x00f000f0u;
+__global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend_kernel(const __grid_constant__ AttendParams a) {
+  constexpr int NG = D / 32, kTileBytes = pages4::tile_bytes(D), QT = kTerms<T>, PT = kTerms<T>;
+  constexpr bool kOver = sizeof(T) == 2;      // codes are operands as they are: 8 for each, and every second's 16, come off apart
   extern __shared__ __align__(16) unsigned char smem[];
   launch_next();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, c = lane & 3;
   Share share = share_of(a, gridDim.x);
   Piece piece;
+  int4 ends = make_int4(-1, 0, 0, 0);      // for the join: the segment that ends here and began in a CTA before, and which
   while (next_piece(a, share, piece)) {
+    if (piece.u0 > 0 && piece.u1 == piece.units) ends = make_int4(piece.sent, piece.kvh, piece.rt, (int)(piece.start / share.per));
     const T* q_row[2];
     const Job job = job_of<T>(a, piece, q_row);
 
@@ -655,6 +425,23 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
       }
       copy_commit();
     };
+    float x[2][8];                   // the lane's part of two rows of queries: on its way while the table is looked at
+    if (warp < NG) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        if (q_row[r] && a.q_wide) {
+          uint4 v[sizeof(T) / 2];
+#pragma unroll
+          for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(q_row[r] + 32 * warp + 8 * c) + i);
+          const T* e = reinterpret_cast<const T*>(v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[r][i] = to_float(e[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[r][i] = q_row[r] ? to_float(q_row[r][32 * warp + 8 * c + i]) : 0.f;
+        }
+      }
+    }
 #pragma unroll
     for (int i = 0; i < kPairStages - 1; ++i) fetch(i);
 
@@ -665,19 +452,9 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
     float mul[2];                  // from a sum of products to a power of 2 (or, with a cap, to what capped() takes)
     {
       __shared__ float s_most[NG][kRows], s_sum[4][kRows];
-      float x[2][8];
       if (warp < NG) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          if (q_row[r] && a.q_wide) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(q_row[r] + 32 * warp + 8 * c));
-            const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[r][i] = to_float(e[i]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[r][i] = q_row[r] ? to_float(q_row[r][32 * warp + 8 * c + i]) : 0.f;
-          }
           float most = 0.f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[r][i]));
@@ -696,47 +473,54 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
         for (int gr = 1; gr < NG; ++gr) most = fmaxf(most, s_most[gr][gid + 8 * r]);
         const int up = most > 0.f && most < INFINITY ? 9 - max(-100, ilogbf(most)) : 0;      // -118 .. 109
         const float by = ldexpf(a.scale < 0.f ? -1.f : 1.f, up);
-        mul[r] = ldexpf(fabsf(a.scale) * kLog2e * (a.cap > 0.f ? 2.f / a.cap : 1.f), 24 - up);
+        mul[r] = ldexpf(fabsf(a.scale) * kLog2e * (a.cap > 0.f ? 2.f / a.cap : 1.f), (kOver ? 24 : 0) - up);
         if (warp < NG) {
           float sum = 0.f;
-          uint32_t f[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const __half2 h = __floats2half2_rn(x[r][i] * by * (i & 1 ? 0.0625f : 1.f), x[r][i + 4] * by * (i & 1 ? 0.0625f : 1.f));
-            f[i] = *reinterpret_cast<const uint32_t*>(&h);
-            const float2 back = __half22float2(h);
-            sum += (back.x + back.y) * (i & 1 ? 16.f : 1.f);
-          }
-          sum += __shfl_xor_sync(~0u, sum, 1);
-          sum += __shfl_xor_sync(~0u, sum, 2);
-          if (c == 0) s_sum[warp][gid + 8 * r] = sum * (-8.f / 16777216.f);
+            float lo = x[r][i] * by * (kOver && (i & 1) ? 0.0625f : 1.f), hi = x[r][i + 4] * by * (kOver && (i & 1) ? 0.0625f : 1.f);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(q_smem + (2 * warp + (i >> 1)) * 32 + lane)[2 * (i & 1) + r] = f[i];
+            for (int term = 0; term < QT; ++term) {
+              const __half2 h = __floats2half2_rn(lo, hi);
+              reinterpret_cast<uint32_t*>(q_smem + (term * NG * 2 + 2 * warp + (i >> 1)) * 32 + lane)[2 * (i & 1) + r] = *reinterpret_cast<const uint32_t*>(&h);
+              const float2 back = __half22float2(h);
+              sum += (back.x + back.y) * (i & 1 ? 16.f : 1.f);
+              lo -= back.x;
+              hi -= back.y;
+            }
+          }
+          if constexpr (kOver) {
+            sum += __shfl_xor_sync(~0u, sum, 1);
+            sum += __shfl_xor_sync(~0u, sum, 2);
+            if (c == 0) s_sum[warp][gid + 8 * r] = sum * (-8.f / 16777216.f);
+          }
         }
       }
       __syncthreads();
-      uint32_t ov[2][2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float s0 = s_sum[2 * (c & 1)][gid + 8 * r], s1 = s_sum[2 * (c & 1) + 1][gid + 8 * r];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {          // terms c / 2 and 2 + c / 2
-          float u0 = s0, u1 = s1;
-          const int term = 2 * h + (c >> 1);
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (i < term) {
-              u0 -= __bfloat162float(__float2bfloat16_rn(u0));
-              u1 -= __bfloat162float(__float2bfloat16_rn(u1));
-            }
-          ov[r][h] = term < 3 ? pack_bf16(u0, u1) : 0u;
+      if constexpr (kOver) {
+        uint32_t ov[2][2];
+  #pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float s0 = s_sum[2 * (c & 1)][gid + 8 * r], s1 = s_sum[2 * (c & 1) + 1][gid + 8 * r];
+  #pragma unroll
+          for (int h = 0; h < 2; ++h) {          // terms c / 2 and 2 + c / 2
+            float u0 = s0, u1 = s1;
+            const int term = 2 * h + (c >> 1);
+  #pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (i < term) {
+                u0 -= __bfloat162float(__float2bfloat16_rn(u0));
+                u1 -= __bfloat162float(__float2bfloat16_rn(u1));
+              }
+            ov[r][h] = term < 3 ? pack_bf16(u0, u1) : 0u;
+          }
         }
+        over = make_uint4(ov[0][0], ov[1][0], ov[0][1], ov[1][1]);
       }
-      over = make_uint4(ov[0][0], ov[1][0], ov[0][1], ov[1][1]);
     }
     const float cap_log2 = a.cap * kLog2e;
 
-    // The values' sums are kept times 2^-24, as the codes are, and times the power of 2 that brings their scales into fp16's range.
+    // The values' sums are kept times 2^-24 where the codes are, and times the power of 2 that brings their scales into fp16's range.
     float o[NG][4][4] = {}, extra[4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, size = 1.f;   // size: that power
     uint32_t limit = 0;              // bits of the bf16 that no scale may reach with `size` as it is
     int stage = 0;
@@ -766,17 +550,31 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
           *reinterpret_cast<uint2*>(w[j]) = *reinterpret_cast<const uint2*>(kw);
           *reinterpret_cast<uint2*>(sc[j]) = *reinterpret_cast<const uint2*>(ks);
         }
-        const uint32_t own = *reinterpret_cast<const uint32_t*>(tile + pages4::key_scales(D) + (8 * j1 + gid) * (2 * NG) + (NG == 4 ? 4 * (c & 1) : 0));
-        mma_bf16_first(x[j], over, own, own);
+        if constexpr (kOver) {
+          const uint32_t own = *reinterpret_cast<const uint32_t*>(tile + pages4::key_scales(D) + (8 * j1 + gid) * (2 * NG) + (NG == 4 ? 4 * (c & 1) : 0));
+          mma_bf16_first(x[j], over, own, own);
+        } else {
+          x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.f;
+        }
       }
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
-        const uint4 qa = q_smem[2 * gr * 32 + lane], qb = q_smem[(2 * gr + 1) * 32 + lane];
+        uint4 qa[QT], qb[QT];
+#pragma unroll
+        for (int term = 0; term < QT; ++term) {
+          qa[term] = q_smem[(term * NG * 2 + 2 * gr) * 32 + lane];
+          qb[term] = q_smem[(term * NG * 2 + 2 * gr + 1) * 32 + lane];
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float s[4];
-          mma_f16_first(s, qa, w[j][gr] & kEven, w[j][gr] & kOdd);
-          mma_f16(s, qb, (w[j][gr] >> 8) & kEven, (w[j][gr] >> 8) & kOdd);
+          const uint32_t even0 = operand<T>(w[j][gr], false), odd0 = operand<T>(w[j][gr], true), even1 = operand<T>(w[j][gr] >> 8, false), odd1 = operand<T>(w[j][gr] >> 8, true);
+          mma_f16_first(s, qa[QT - 1], even0, odd0);         // small terms first
+          mma_f16(s, qb[QT - 1], even1, odd1);
+          if constexpr (QT == 2) {
+            mma_f16(s, qa[0], even0, odd0);
+            mma_f16(s, qb[0], even1, odd1);
+          }
           // scales of position 2 c: halves gr of the first NG, of 2 c + 1: of the second
           const float s0 = gr & 1 ? bf16_high(sc[j][gr >> 1]) : bf16_low(sc[j][gr >> 1]);
           const float s1 = gr & 1 ? bf16_high(sc[j][NG / 2 + (gr >> 1)]) : bf16_low(sc[j][NG / 2 + (gr >> 1)]);
@@ -794,7 +592,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float v = x[j][e] * (e < 2 ? r0 : r1);
-            if (a.cap > 0.f) v = capped(v, cap_log2);
+            if (a.cap > 0.f) v = sizeof(T) == 4 ? cap_log2 * tanhf(v * (0.5f / kLog2e)) : capped(v, cap_log2);
             if (a.slope) v = fmaf(-job.slope[e >> 1], fabsf((e < 2 ? at0 : at1) + (float)(8 * j + (e & 1))), v);
             x[j][e] = v;
           }
@@ -825,7 +623,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
         top[e] = fmaxf(top[e], __shfl_xor_sync(~0u, top[e], 2));
         top[e] *= e ? r1 : r0;
       }
-      const bool up0 = top[0] > m[0] + kSlack || (m[0] == -INFINITY && top[0] > -INFINITY), up1 = top[1] > m[1] + kSlack || (m[1] == -INFINITY && top[1] > -INFINITY);
+      const bool up0 = top[0] > m[0] + kSlack<T> || (m[0] == -INFINITY && top[0] > -INFINITY), up1 = top[1] > m[1] + kSlack<T> || (m[1] == -INFINITY && top[1] > -INFINITY);
       if (__any_sync(~0u, up0 || up1)) {
         const float f0 = up0 ? exp2_of(m[0] - top[0]) : 1.f, f1 = up1 ? exp2_of(m[1] - top[1]) : 1.f;
         if (up0) m[0] = top[0];
@@ -858,7 +656,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
             }
         }
       }
-      // The power of 2 that takes the largest scale to 2^3 .. 2^4; it changes with a scale 2^3 larger (a weight's 2^8 and that leave 2^15 at most).
+      // The power of 2 that takes the largest scale to 2^kAbove and up to twice that; it changes with a scale 2^4 times 2^kAbove.
       __nv_bfloat162 most2 = __habs2(bf16_pair(vs[0][0]));
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -867,7 +665,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
       const uint32_t most = max(*reinterpret_cast<const uint32_t*>(&most2) & 0xffffu, *reinterpret_cast<const uint32_t*>(&most2) >> 16);
       if (__any_sync(~0u, most >= limit)) {
         const int e = min(max((int)(__reduce_max_sync(~0u, most) >> 7) - 127, -97), 103);
-        const float now = exp2_of((float)(3 - e)), f = limit ? now / size : 1.f;
+        const float now = exp2_of((float)(kAbove<T> - e)), f = limit ? now / size : 1.f;
         size = now;
         limit = (uint32_t)min(e + 127 + 4, 255) << 7;
         extra[0] *= f; extra[2] *= f;
@@ -901,65 +699,78 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend16_kernel(
           for (int h = 0; h < 2; ++h) {
             const int gr = 2 * i2 + h;
             const uint32_t w0 = h ? u.y : u.x, w1 = h ? u.w : u.z;
-            uint32_t pa[2][2];       // [half of the positions][row gid, row gid + 8]
+            uint32_t pa[PT][2][2];   // [term][half of the positions][row gid, row gid + 8]
 #pragma unroll
             for (int j1 = 0; j1 < 2; ++j1) {
               const int j = 2 * tt + j1;
               const float s0 = h ? bf16_high(vs[j][i2]) : bf16_low(vs[j][i2]), s1 = h ? bf16_high(vs[j][NG / 2 + i2]) : bf16_low(vs[j][NG / 2 + i2]);
-              pa[j1][0] = pack_f16(x[j][0] * s0, x[j][1] * s1);
-              pa[j1][1] = pack_f16(x[j][2] * s0, x[j][3] * s1);
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                float p0 = x[j][2 * r] * s0, p1 = x[j][2 * r + 1] * s1;
+#pragma unroll
+                for (int term = 0; term < PT; ++term) {
+                  pa[term][j1][r] = pack_f16(p0, p1);
+                  if (term + 1 < PT) {
+                    const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&pa[term][j1][r]));
+                    p0 -= back.x;
+                    p1 -= back.y;
+                  }
+                }
+              }
             }
-            const uint4 weights = make_uint4(pa[0][0], pa[0][1], pa[1][0], pa[1][1]);
             const uint32_t eight = (gid >> 1) == gr ? 0x00080008u : 0u;       // columns 2 gr and 2 gr + 1: 8 times the weights' sum
-            mma_f16(o[gr][0], weights, w0 & kEven, w1 & kEven);
-            mma_f16(o[gr][1], weights, w0 & kOdd, w1 & kOdd);
-            mma_f16(o[gr][2], weights, (w0 >> 8) & kEven, (w1 >> 8) & kEven);
-            mma_f16(o[gr][3], weights, (w0 >> 8) & kOdd, (w1 >> 8) & kOdd);
-            mma_f16(extra, weights, eight, eight);
+#pragma unroll
+            for (int term = PT - 1; term >= 0; --term) {
+              const uint4 weights = make_uint4(pa[term][0][0], pa[term][0][1], pa[term][1][0], pa[term][1][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) mma_f16(o[gr][e], weights, operand<T>(w0 >> (e & 2) * 4, e & 1), operand<T>(w1 >> (e & 2) * 4, e & 1));
+              if constexpr (kOver) mma_f16(extra, weights, eight, eight);
+            }
           }
         }
       }
     }
 
-    // From the sums as they are kept to sums of values: less 8 for each code, times 2^24 / size.
-    const float by = 16777216.f / size;
+    // From the sums as they are kept to sums of values: times 1 / size, and with codes as they are less 8 for each and times 2^24.
+    const float by = (kOver ? 16777216.f : 1.f) / size;
 #pragma unroll
     for (int gr = 0; gr < NG; ++gr) {
-      const float e0 = __shfl_sync(~0u, extra[0], (lane & ~3) | gr), e1 = __shfl_sync(~0u, extra[2], (lane & ~3) | gr);
+      const float e0 = kOver ? __shfl_sync(~0u, extra[0], (lane & ~3) | gr) : 0.f, e1 = kOver ? __shfl_sync(~0u, extra[2], (lane & ~3) | gr) : 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[gr][e][i] = fmaf(o[gr][e][i], e & 1 ? 0.0625f : 1.f, -(i < 2 ? e0 : e1)) * by;
+        for (int i = 0; i < 4; ++i) o[gr][e][i] = fmaf(o[gr][e][i], kOver && (e & 1) ? 0.0625f : 1.f, -(i < 2 ? e0 : e1)) * by;
     }
     join_warps<T, D>(a, piece, job, smem, o, m, l);
   }
+  if (a.ws && threadIdx.x == 0) reinterpret_cast<int4*>(a.ws + (int64_t)gridDim.x * 2 * (kRows * (D + 2)))[blockIdx.x] = ends;
 }
 
-// Joins the parts of the segment that ends in a CTA's share and began in one before: a CTA for each of attend's, a thread for four components of a
-// row.  Shares are found while attend still runs.
+// Joins the parts of the segment that ends in a CTA's share and began in one before: a CTA for each of attend's.  A thread has four components of a row, in one of kBy
+// parts in turn.  (Four CTAs with four rows each: 64 paragraphs of 1 to 4001 positions in 87 us, not 79.)
+constexpr int kJoinThreads = 512;
 template <class T, int D>
-__global__ void __launch_bounds__(kRows * D / 4) attend_join_kernel(const __grid_constant__ AttendParams a, int blocks) {
-  Share share = share_of(a, blocks);
-  Piece p;
-  const int64_t per = share.per;
-  const bool ends = next_piece(a, share, p) && p.u0 > 0 && p.u1 == p.units;
-  const int from = ends ? (int)(p.start / per) : 0, n_parts = (int)blockIdx.x - from + 1;
-  constexpr int kPart = kRows * (D + 2);
-  const int d = threadIdx.x % (D / 4) * 4, r = threadIdx.x / (D / 4);
+__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_constant__ AttendParams a, int blocks) {
+  constexpr int kPart = kRows * (D + 2), kBy = kJoinThreads / (kRows * D / 4);
+  __shared__ float s_top[kBy][kRows], s_weight[kBy][kRows];
+  __shared__ float4 s_sum[kBy][kRows * D / 4];
+  const int at = threadIdx.x % (kRows * D / 4), by = threadIdx.x / (kRows * D / 4), r = at / (D / 4), d = at % (D / 4) * 4;
   wait_for_last();
-  if (!ends || r >= a.g * a.rep - p.rt * kRows) return;
+  const int4 ends = reinterpret_cast<const int4*>(a.ws + (int64_t)blocks * 2 * kPart)[blockIdx.x];
+  if (ends.x < 0) return;
+  const int from = ends.w, n_parts = (int)blockIdx.x - from + 1;
   auto part = [&](int i) { return a.ws + ((int64_t)(from + i) * 2 + (i == 0)) * kPart; };
   // The maximum so far goes along, so that every part is waited for once: eight of them at a time are on their way.
   float top = -INFINITY, weight = 0.f;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < n_parts; i0 += 8) {
+  for (int i0 = by; i0 < n_parts; i0 += 8 * kBy) {
     float m[8], l[8];
     float4 v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       m[j] = -INFINITY;
-      if (i0 + j < n_parts) {
-        const float* const w = part(i0 + j);
+      if (i0 + j * kBy < n_parts) {
+        const float* const w = part(i0 + j * kBy);
         m[j] = w[kRows * D + r];
         l[j] = w[kRows * D + kRows + r];
         v[j] = *reinterpret_cast<const float4*>(w + r * D + d);
@@ -975,13 +786,29 @@ __global__ void __launch_bounds__(kRows * D / 4) attend_join_kernel(const __grid
     sum.x *= f0; sum.y *= f0; sum.z *= f0; sum.w *= f0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if (i0 + j >= n_parts) break;
+      if (i0 + j * kBy >= n_parts) break;
       const float f = exp2_of(m[j] - now);
       sum.x += f * v[j].x; sum.y += f * v[j].y; sum.z += f * v[j].z; sum.w += f * v[j].w;
       weight += f * l[j];
     }
   }
-  write_row<T>(a, p.sent, p.kvh, p.rt * kRows + r, d, sum, top, weight);
+  s_sum[by][at] = sum;
+  if (d == 0) { s_top[by][r] = top; s_weight[by][r] = weight; }
+  __syncthreads();
+  if (by || r >= a.g * a.rep - ends.z * kRows) return;
+#pragma unroll
+  for (int i = 1; i < kBy; ++i) top = fmaxf(top, s_top[i][r]);
+  const float base = top == -INFINITY ? 0.f : top;
+  sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  weight = 0.f;
+#pragma unroll
+  for (int i = 0; i < kBy; ++i) {
+    const float f = exp2_of(s_top[i][r] - base);
+    const float4 v = s_sum[i][at];
+    sum.x += f * v.x; sum.y += f * v.y; sum.z += f * v.z; sum.w += f * v.w;
+    weight += f * s_weight[i][r];
+  }
+  write_row<T>(a, ends.x, ends.y, ends.z * kRows + r, d, sum, top, weight);
 }
 
 template <class T, int D>
@@ -989,8 +816,7 @@ cudaError_t launch_attend(const AttendParams& p, int blocks, int device, cudaStr
   constexpr int smem = attend_smem<T, D>();
   const bool plain = p.cap == 0.f && !p.slope && p.scale != 0.f;
   void (*kernel)(AttendParams);
-  if constexpr (sizeof(T) == 2) kernel = plain ? attend16_kernel<T, D, true> : attend16_kernel<T, D, false>;
-  else kernel = attend32_kernel<D>;
+  kernel = plain ? attend_kernel<T, D, true> : attend_kernel<T, D, false>;
   static std::atomic<bool> opted_in[kOpMaxDevices][2] = {};
   if (smem + 1024 > 48 << 10 && !opted_in[device][plain].load(std::memory_order_acquire)) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -1005,7 +831,7 @@ cudaError_t launch_attend(const AttendParams& p, int blocks, int device, cudaStr
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3(kRows * D / 4);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
@@ -1041,9 +867,9 @@ int check(const linmt_attend_pages4_args* g) {
   return LINMT_OK;
 }
 
-// Two parts for each CTA: of the segments that it shares with the CTAs before and behind it.  None where no segment can be long enough to be cut.
+// Two parts for each CTA, of the segments that it shares with the CTAs before and behind it, and what the join has to know.  None where no segment can be long enough to be cut.
 int64_t workspace_of(const linmt_attend_pages4_args* g) {
-  return pairs_at_most(g) <= kLeast ? 0 : (int64_t)blocks_of(g) * 2 * (kRows * (g->pages.dim + 2)) * 4;
+  return pairs_at_most(g) <= kLeast ? 0 : (int64_t)blocks_of(g) * (2 * (kRows * (g->pages.dim + 2)) * 4 + 16);
 }
 
 }  // namespace

@@ -109,7 +109,7 @@ def test_attend_refuses(cuda_lib, code, word, kw):
 def test_attend_workspace(cuda_lib):
     size = lambda **kw: cuda_lib.linmt_attend_pages4_workspace(_pack("linmt_attend_pages4_args", **kw))
     assert size(width=16) == 0 and size(n=0, width=4096) == 0 and size(heads=3) == -1     # sentences of up to 256 positions are not cut
-    part = 16 * 66 * 4                                         # 16 rows: 64 sums, a maximum and a weight
+    part = 16 * 66 * 4 + 8                                     # 16 rows: 64 sums, a maximum and a weight; two of them and 16 bytes for each CTA
     assert size(width=4096) == 592 * 2 * part and size(width=4096, n=4000) == 592 * 2 * part
     assert size(width=32) == 2 * 2 * 4 * 2 * part               # 2 sentences, 2 heads, 16 pairs of tiles that count as 28 units, in parts of 8
 

@@ -566,21 +566,22 @@ def attend_check(ops, q, pages, table, lens, kk, vv, page, scale=None, cap=0.0, 
     big_scale = float(np.abs(vv).max()) / 7
     want, wlse, wv, big, ws = attend_ref(q.double().cpu().numpy(), kk, vv, table, lens, page, scale, cap, slope, centre, first, last, pages.shape[0])
     # A score: products of exact values added in 32 bits, at most dim + 8 additions and products; the cap's tanh to 2e-7 of the cap (16-bit queries) and the bias
-    # and the change to powers of two a few roundings of their own size.  Queries in 32 bits are exact to 2^-24 in three terms.
+    # and the change to powers of two a few roundings of their own size.  Queries in 32 bits are exact to 2^-22 in two fp16 terms.
     bias = 0.0 if slope is None else float(np.max(slope)) * (max(lens) + float(np.max(np.abs(centre))))
     lo = np.where(np.isneginf(wlse), 0, wlse)
-    score = (dim + 12) * 2.0 ** -24 * big + 4e-7 * cap + 6 * 2.0 ** -24 * (bias + np.abs(lo).max() + 32)
+    score = ((dim + 12) * 2.0 ** -24 + (2.0 ** -22 if q.dtype == F32 else 0)) * big + 4e-7 * cap + 6 * 2.0 ** -24 * (bias + np.abs(lo).max() + 32)
     g = got.double().cpu().numpy()
     # weights: exp2 2^-22 and sums of up to 2^12 additions a lane would be 2^-12 at worst, but each is of positive terms rounded to nearest: 64 warps' and lanes' partial
     # sums of some hundreds, 2^-24 * 300; the rounding of the weight to its terms, the output's own
-    # (16-bit queries: the product of a weight and a value's scale is rounded to fp16)
-    weight = {BF16: 2.0 ** -11, F16: 2.0 ** -11, F32: 2.0 ** -24}[q.dtype]
+    # (the product of a weight and a value's scale is rounded to fp16, for 32-bit queries to two terms)
+    weight = {BF16: 2.0 ** -11, F16: 2.0 ** -11, F32: 2.0 ** -22}[q.dtype]
     # 16-bit queries: codes go into the products as 0 .. 15 and 8 for each comes off at the end, so that the sums on the way are up to 15 sum(w scale) in size whatever
     # the values are.  A warp adds a product of 16 positions (of the CTA's 64) a time to them; the matrix unit lays its 17 addends side by side and cuts each off below
     # the largest one's 24th bit, 17 * 2^-23 in all, and some 8 additions join the parts: a component whose values cancel, or whose codes are all near 8, is off by that
     # and not by a share of itself.  A weight times its scale is kept in fp16 below 2^4 times the largest scale: 2^-25 / 8 of the largest scale at least.
     steps = max(lens) / 64 + 1
-    shift = 0.0 if q.dtype == F32 else (steps * 17 + 8) * 2.0 ** -23 * 15 * ws + 8 * 2.0 ** -28 * big_scale * max(lens)
+    # 32-bit queries: codes are less 8 already; a weight's second term is kept to 2^-25 below 2^9 times the largest scale, and goes with codes of up to 8.
+    shift = 8 * 2.0 ** -34 * big_scale * max(lens) if q.dtype == F32 else (steps * 17 + 8) * 2.0 ** -23 * 15 * ws + 8 * 2.0 ** -28 * big_scale * max(lens)
     tol = HALF_STEP[q.dtype] * np.abs(want) + (weight + 2 * score + 2.0 ** -15) * wv + shift + (2.0 ** -25 if q.dtype == F16 else 0)
     assert np.isfinite(g).all()
     assert (np.abs(g - want) <= tol).all(), float((np.abs(g - want) / np.maximum(tol, 1e-300)).max())
