@@ -740,12 +740,15 @@ cudaError_t launch_select(const linmt_beam_select_args& g) {
                     g.out_tokens, g.out_parents, g.out_scores, g.out_done, g.k, g.vocab, g.eos};
   // As many CTAs for a sentence as leave all of them on the GPU at once (two on an SM; clusters of 8 only reach 33), since a second round of
   // clusters costs its latencies again, and as have 16k logits each: exchanges among more take longer (64 x 12 x 30k fp32: 40, 30 and 51 us
-  // with 2, 4 and 8; 128 x 12 x 80k bf16: 82, 95 and 141; 1 x 4 x 1000: 10.2, 10.6 and 12.4).  A row needs as many warps as have
-  // four thirds of `need` lanes, or the bar falls below what its best candidates are when one beam is ahead (139 x 30 x 5.9k fp16 with one warp a row: 480 us).
+  // with 2, 4 and 8; 128 x 12 x 80k bf16: 82, 95 and 141; 1 x 4 x 1000: 10.2, 10.6 and 12.4).  A row has a warp at
+  // least, and as many as have 8 / 7 of `need` lanes, or the bar falls below what its best candidates are when one beam is ahead (139 x 30 x 5.9k fp16
+  // with one warp a row: 480 us; 300 x 20 x 4000 with two a row, not one: 77, not 50).  A row so short that all of it can be ranked needs no more than one
+  // (300 x 27 x 300: 81 us; 208 with three).
   const int64_t logits = (int64_t)g.k * g.vocab;
   int c = g.n <= 33 ? 8 : g.n <= 74 ? 4 : g.n <= 148 ? 2 : 1;
   while (c > 1 && logits < (int64_t)(c / 2 + 1) * 16384) c /= 2;
-  while (g.k + kBeyond > 24 * (c * kWarps / g.k)) c *= 2;
+  const int need = g.k + kBeyond;
+  while (c * kWarps < g.k || (need > 28 * (c * kWarps / g.k) && g.vocab + need > kFound)) c *= 2;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;

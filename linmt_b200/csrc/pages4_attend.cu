@@ -138,7 +138,7 @@ __device__ __forceinline__ void write_row(const AttendParams& a, int sent, int k
 // are known on the device only, so every CTA adds them up itself.  A segment counts as kFixed units more than it has pairs, its fixed costs being as large,
 // and as kLeast at least; one of up to kLeast + kFixed units or an eighth of a part is not cut: the CTA that has its first unit takes it whole.
 constexpr int kLeast = 8;
-constexpr int kFixed = 12;      // (64 paragraphs of 1 to 4001 positions: 97, 89, 82, 84 us with 4, 8, 12, 16)
+constexpr int kFixed = 12;      // (64 paragraphs of 1 to 4001 positions: 93, 86, 82, 78 us with 6, 8, 10, 12)
 struct Share {
   int64_t begin, end;      // the CTA's units
   int64_t first;           // number of the first unit of sentence `sent`
