@@ -326,7 +326,7 @@ const char* linmt_op_error(void);
  * Equal sums go to the lowest b * vocab + v.  The order is that of 64-bit arithmetic as far as 2^-36: sums of two beams that lie closer
  * than 32 bits can tell apart are compared again with normalisers that are good to that.  Words that are not allowed may hold anything;
  * one whose logit is -inf is never chosen.  Slots that nothing is left for get token eos, parent = the slot itself, score -inf, done 1.
- * out_* may be the arrays `scores` and `done`. */
+ * out_scores and out_done may be the arrays `scores` and `done`; nothing else that is written may overlap what is read. */
 typedef struct linmt_beam_select_args {
   uint32_t size;
   int32_t device;
@@ -438,7 +438,7 @@ typedef struct linmt_attend_pages4_args {
   linmt_pages4 pages;
   const void* q;             /* [n][g][heads][dim], components contiguous, rows 4-byte aligned */
   int64_t q_stride_n, q_stride_g, q_stride_h;
-  void* out;                 /* as q, strides of its own */
+  void* out;                 /* as q, strides of its own; q itself with q's strides, or apart from it */
   int64_t out_stride_n, out_stride_g, out_stride_h;
   float* lse;                /* [n][g][heads]; may be NULL */
   const int32_t* table;      /* [n][width], rows `table_stride` apart */

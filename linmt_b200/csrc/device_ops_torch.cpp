@@ -129,7 +129,17 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     t[2] = dense(PyTuple_GET_ITEM(a[5], 2), "out[2]", dev, at::kFloat, shape);
     flags(PyTuple_GET_ITEM(a[5], 3), "out[3]", dev, shape);
     t[3] = THPVariable_Unpack(PyTuple_GET_ITEM(a[5], 3));
-    NEED(n * k == 0 || t[0].data_ptr() != t[1].data_ptr(), "out[0] and out[1] are one tensor");
+    // A sentence's results are written while others are still read: each has to lie apart from all that is read, or be it, place for place.
+    struct Span { const char *p, *end; };
+    auto span = [](const void* p, int64_t bytes) { return Span{static_cast<const char*>(p), static_cast<const char*>(p) + bytes}; };
+    auto meet = [](const Span& x, const Span& y) { return x.p < y.end && y.p < x.end; };
+    const Span outs[4] = {span(t[0].data_ptr(), n * k * 4), span(t[1].data_ptr(), n * k * 4), span(t[2].data_ptr(), n * k * 4), span(t[3].data_ptr(), n * k)};
+    const Span reads[4] = {span(g.scores, n * k * 4), span(g.done, g.done ? n * k : 0), span(g.allowed, g.allowed ? (g.allowed_stride ? n : 1) * ((v + 31) / 32) * 4 : 0),
+                           span(g.logits, n * k ? ((n - 1) * g.stride_n + (k - 1) * g.stride_k + v) * (int64_t)logits.element_size() : 0)};
+    for (int i = 0; i < 4 && n * k; ++i) {
+      for (int j = 0; j < i; ++j) NEED(!meet(outs[i], outs[j]), "out[", j, "] and out[", i, "] overlap");
+      for (int j = 0; j < 4; ++j) NEED(!meet(outs[i], reads[j]) || (i == j + 2 && outs[i].p == reads[j].p), "out[", i, "] overlaps what the call reads");
+    }
   }
   g.out_tokens = static_cast<int32_t*>(t[0].data_ptr());
   g.out_parents = static_cast<int32_t*>(t[1].data_ptr());
@@ -408,6 +418,16 @@ PyObject* attend_pages4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     out = on_device(a[10], "out", dev);
     NEED(out.scalar_type() == q.scalar_type() && out.sizes() == q.sizes() && out.stride(3) == 1, "out has to be like q, its components contiguous");
     NEED(apart(out), "out has rows that share memory");
+    const bool flat = q.stride(2) == q.size(3) && out.stride(2) == q.size(3);      // heads one behind the other: a row of all of them
+    auto places = [&](const Tensor& x) {
+      const int64_t e = x.element_size();
+      Strides s{n, x.stride(0) * e, x.stride(1) * e, x.stride(2) * e, (flat ? heads : 1) * x.size(3) * e, static_cast<const char*>(x.data_ptr()), nullptr};
+      s.end = s.p + (n - 1) * s.l + (rows - 1) * s.n + (flat ? 0 : heads - 1) * s.k + s.row;
+      return s;
+    };
+    const Strides from = places(q), to = places(out);
+    const bool same = from.p == to.p && from.l == to.l && from.n == to.n && from.k == to.k;
+    NEED(q.numel() == 0 || same || disjoint(from, to, rows, flat ? 1 : heads), "out overlaps q");
   }
   g.out = out.data_ptr();
   g.out_stride_n = out.stride(0);

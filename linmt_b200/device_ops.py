@@ -48,7 +48,7 @@ def beam_select(logits, scores, *, done=None, allowed=None, eos=1, out=None):
 
     Returns ``tokens``, ``parents`` [n, k] int32, ``scores`` [n, k] float32 and ``done`` [n, k] bool (the parent was finished, or the token is
     ``eos``).  A slot for which nothing is left has token eos, itself as the parent, -inf and True.  ``out``: a tuple of four such tensors to
-    write into; they may be ``scores`` and ``done`` themselves."""
+    write into; they may be ``scores`` and ``done`` themselves, and overlap nothing else that the call reads."""
     return _front.beam_select(logits, scores, done, allowed, eos, None if out is None else tuple(out))
 
 
@@ -101,5 +101,5 @@ def attend_pages4(q, pages, table, lens, *, scale=None, cap=0.0, slope=None, cen
     [heads] with ``centre`` [n, g], float32: scores lose slope * |position - centre|.  ``first``, ``last`` [n, g] int32: a row sees positions
     first <= t < last only.  Positions in a column that names no page of the pool are not seen.  A row that sees nothing gets zeros and lse -inf.
 
-    Returns ``out`` like q, and with ``want_lse`` also the log of the row's sum of exponentials, [n, g, heads] float32."""
+    Returns ``out`` like q (it may be q itself, or overlap nothing of it), and with ``want_lse`` also the log of the row's sum of exponentials, [n, g, heads] float32."""
     return _front.attend_pages4(q, pages, table, lens, scale, cap, slope, centre, first, last, out, want_lse)

@@ -751,6 +751,39 @@ def test_attend_refuses(ops):
             bad()
 
 
+def test_results_that_lie_upon_what_is_read(ops):
+    """Results may take the place of scores, finished flags and queries, or lie between the queries; whatever would be written while it is still read is refused."""
+    rng = _rng(77)
+    n, k, v = 4, 6, 300
+    x = _logits(rng, n, k, v, F32)
+    pool = torch.zeros(5 * n * k, dtype=torch.int32, device="cuda")
+    ints = lambda at: pool[at:at + n * k].view(n, k)
+    tokens, parents, scores = ints(0), ints(n * k), pool[2 * n * k:3 * n * k].view(F32).view(n, k)
+    scores.copy_(_cuda(rng.normal(-10, 3, (n, k)).astype(np.float32)))
+    flags = torch.zeros(2 * n * k, dtype=torch.bool, device="cuda")
+    done = flags[:n * k].view(n, k)
+    later = pool[2 * n * k + k:3 * n * k + k].view(F32).view(n, k)
+    for out in ((tokens, tokens, scores, done), (tokens, ints(k), scores, done), (tokens, parents, later, done), (scores.view(torch.int32), parents, later, done),
+                (tokens, parents, scores, flags[k:k + n * k].view(n, k)), (x.view(-1)[:n * k].view(torch.int32).view(n, k), parents, scores, done)):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.beam_select(x, scores, done=done, out=out)
+    want = ops.beam_select(x, scores, done=done)
+    got = ops.beam_select(x, scores, done=done, out=(tokens, parents, scores, done))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+    for lens in ([40, 3], [3000, 700]):
+        pages, table, kk, vv = _memory(ops, rng, lens, 2, 64, 16)
+        fused = torch.zeros(2, 5, 3, 4, 64, dtype=BF16, device="cuda")
+        q, beside = fused[:, :, 0], fused[:, :, 1]
+        q.copy_(_q(rng, 2, 5, 4, 64, BF16))
+        at = lambda **kw: ops.attend_pages4(q, pages, _cuda(table), _cuda(np.asarray(lens, np.int32)), **kw)
+        want = at()
+        for out in (fused.view(2, 5, 12, 64)[:, :, 2:6], fused.view(-1)[64:64 + 2 * 5 * 12 * 64 - 128].as_strided((2, 5, 4, 64), (5 * 768, 768, 64, 1))):
+            with pytest.raises(ValueError, match="overlaps"):
+                at(out=out)
+        assert torch.equal(at(out=beside), want) and torch.equal(beside, want) and torch.equal(at(out=q), want) and torch.equal(q, want)
+
+
 def test_gradients_are_refused(ops):
     """No backward pass: a call that would drop a gradient does not go through."""
     x, s = torch.zeros(1, 2, 50, device="cuda", requires_grad=True), torch.zeros(1, 2, device="cuda")
