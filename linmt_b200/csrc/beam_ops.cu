@@ -43,6 +43,7 @@ constexpr int kFound = 512;                      // of up to so many by ranking 
 constexpr int kMaxList = kMaxC * kMany + kMaxK;  // kMany places for each CTA; finished rows add one each
 constexpr int kSorted = 64;                      // of them that are put in order (>= need)
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLeastRef = -92.f;               // -64 log2 e, rounded
 typedef long long Key;                           // a sum, as an integer that is ordered alike
 constexpr Key kNone = -0x7fffffffffffffffll - 1; // below every sum
 
@@ -317,12 +318,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
     }
   };
   // Terms are exp2(x log2 e - ref), ref the whole number next to the warp's maximum in these units: one instruction for the exponent, and a new maximum
-  // scales the sum by an exact power of 2.  FAR: the maximum is 64 or more in size, where log2 e's own rounding (1.4e-8 of x) would tell:
+  // scales the sum by an exact power of 2.  A maximum below -64 (words masked by a finite value, before the ordinary ones) counts as -64: what lies far below makes terms
+  // of 0, and the factors stay within 1.  FAR: the stretch's maximum is 64 or more in size, where log2 e's own rounding (1.4e-8 of x) would tell:
   // the stretch is read again with differences to the maximum itself.
   auto scan = [&](auto is_far) {
     constexpr bool FAR = decltype(is_far)::value;
     top = wtop = -INFINITY;
-    sum = ref = 0.f;
+    sum = 0.f;
+    ref = kLeastRef;
     fetch(v0);
     for (int c = 0; c < n_chunks; ++c) {
       const int vb = v0 + c * kChunkVecs;
@@ -356,7 +359,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
           sum *= exp2_of((wtop - chunk_max) * kLog2e);
           ++changes;
         } else {
-          const float now = rintf(chunk_max * kLog2e);
+          const float now = fmaxf(rintf(chunk_max * kLog2e), kLeastRef);
           sum *= ref - now < -126.f ? 0.f : __int_as_float((127 + (int)(ref - now)) << 23);
           ref = now;
         }

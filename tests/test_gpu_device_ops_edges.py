@@ -1,0 +1,48 @@
+"""Operators on device tensors at the values, overlaps and orders where they can go wrong, against plain implementations in 64 bits."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from test_gpu_device_ops import (BF16, F16, F32, HALF_STEP, INF, _cuda, _logits, _memory, _q, _reordered, _rng, attend_check, attend_ref, plan_ref, select_check)
+
+
+@pytest.fixture(scope="module")
+def ops(cuda_lib):
+    from linmt_b200 import device_ops
+    return device_ops
+
+
+NAN = float("nan")
+
+
+# ---- selection
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,k,v", [(1, 4, 12000), (64, 3, 6100), (200, 12, 5300)])
+def test_select_low_values_before_ordinary_ones(ops, n, k, v, dtype):
+    """Words masked by a finite value, the first of every row among them, so that a warp's maximum comes from there to the ordinary words."""
+    rng = _rng(n, k, v, 40)
+    x = _logits(rng, n, k, v, dtype)
+    scores = _cuda(rng.normal(-10, 3, (n, k)).astype(np.float32))
+    least = torch.finfo(dtype).min
+    lows = [-88.7, -266.2, -443.6, -1e9, -1e10, -1e18, -1e30, least] if n < 100 else [-1e9, least]
+    for low in [x for x in lows if x >= least]:
+        for words in (512, 1024, 5000, v - 100) if n < 100 else (1024,):
+            y = x.clone()
+            y[:, :, :words] = low
+            select_check(ops, y, scores)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,k,v", [(2, 5, 9001), (70, 4, 3000)])
+def test_select_logits_far_from_zero(ops, n, k, v, dtype):
+    """Logits of 64 and more in size that differ: far up, far down, spread wide, and rows that cross 64."""
+    rng = _rng(n, k, v, 41)
+    x = _logits(rng, n, k, v, F32)
+    scores = _cuda(rng.normal(-10, 3, (n, k)).astype(np.float32))
+    ramp = torch.linspace(-150, 150, v, device="cuda")
+    for y in (x + 100, x - 100, x * 40, x + ramp, x - ramp, torch.where(ramp < 0, x - 1000, x + 64), torch.where(ramp < 0, x + 70, x)):
+        select_check(ops, y.to(dtype), scores)
