@@ -666,7 +666,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
         }
         ask = __reduce_or_sync(~0u, ask);
         if (close >= n_sorted - 1 && n_sorted >= k && bar != kNone) ask = ~0u;      // the list ends before the order is closed
-        ask &= s.finite_bits & ~s.exact_bits;
+        // (a row whose sum is NaN offers nothing, and the sums in pairs pass over NaN)
+        ask &= s.finite_bits & ~s.exact_bits & __ballot_sync(~0u, ((s.finite_bits & ~s.done_bits) >> lane) & 1 && !isnan(s.row_lse[lane]));
         if (lane < C) cluster.map_shared_rank(&s, lane)->ask_bits = ask;
       }
     }

@@ -46,3 +46,29 @@ def test_select_logits_far_from_zero(ops, n, k, v, dtype):
     ramp = torch.linspace(-150, 150, v, device="cuda")
     for y in (x + 100, x - 100, x * 40, x + ramp, x - ramp, torch.where(ramp < 0, x - 1000, x + 64), torch.where(ramp < 0, x + 70, x)):
         select_check(ops, y.to(dtype), scores)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,k,v", [(1, 4, 1000), (3, 6, 20000), (80, 13, 1500)])
+def test_select_nan_beside_ties(ops, n, k, v, dtype):
+    """A beam with a NaN offers nothing, whatever ties the others are in: flat rows, a flat row beside a better one with a NaN, and more equal best words than are kept."""
+    rng = _rng(n, k, v, 42)
+    flat = torch.zeros(n, k, v, dtype=dtype, device="cuda")
+    flat[:, 1, v // 3] = NAN
+    select_check(ops, flat, torch.full((n, k), -2.0, device="cuda"))
+    scores = torch.full((n, k), -10.0, device="cuda")
+    scores[:, 1] = -1
+    select_check(ops, flat, scores)
+    x = _logits(rng, n, k, v, dtype)
+    x[:, 0] = 0
+    x[:, 2, 5] = x[:, 2, v - 1] = NAN
+    scores = torch.full((n, k), -200.0, device="cuda")
+    scores[:, 0], scores[:, 2] = -10, -1
+    select_check(ops, x, scores)
+    x[:, 3, ::7] = 30
+    x[:, 3, 1] = INF
+    scores[:, 3] = 0
+    select_check(ops, x, scores)
+    done = torch.zeros(n, k, dtype=torch.bool, device="cuda")
+    done[:, 1] = True
+    select_check(ops, x, scores, done=done)
