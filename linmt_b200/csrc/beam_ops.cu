@@ -108,6 +108,7 @@ struct SelectSmem {
   Key bar;
   int32_t bar_at;
   int32_t n_listed[kMaxC];       // candidates that each CTA has put into the list
+  int32_t n_had[kMaxC];          // candidates that it had: of more than it has put there only the best `need`
   int32_t n_todo, n_found;
   uint16_t todo[kWarps * kMaxima];           // chunks to be read again: warp * kMaxima + kept maximum
   Key found[kFound];
@@ -569,7 +570,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
     const int n_found = s.n_found;
     Key* const list = lead->list + cta * kMany;
     int32_t* const list_at = lead->list_at + cta * kMany;
-    if (tid == 0) lead->n_listed[cta] = min(n_found, n_found <= kMany ? kMany : need);
+    if (tid == 0) {
+      lead->n_listed[cta] = min(n_found, n_found <= kMany ? kMany : need);
+      lead->n_had[cta] = n_found;
+    }
     if (n_found <= kMany) {
       for (int i = tid; i < n_found; i += kWarps * 32) { list[i] = s.found[i]; list_at[i] = s.found_at[i]; }
     } else if (n_found <= kFound) {
@@ -613,11 +617,13 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
     if (cta == 0) {
       // the CTAs' candidates one after the other, then one for each finished beam
       const uint32_t ended = s.done_bits & s.finite_bits;
+      Key rest = bar;              // no candidate that is not in order at the end has a larger key
       int before_cta = 0;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int m = s.n_listed[c];
         for (int i = tid; i < m; i += kWarps * 32) { s.packed[before_cta + i] = s.list[c * kMany + i]; s.packed_at[before_cta + i] = s.list_at[c * kMany + i]; }
+        if (s.n_had[c] > m) rest = max(rest, s.list[c * kMany + m - 1]);
         before_cta += m;
       }
       const int n = before_cta + __popc(ended);
@@ -638,26 +644,31 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
       }
       __syncthreads();
       if (warp == 0) {
-        // Pair i = sorted i and i + 1.  The first pair from the k-th on that is not near closes the order: what comes behind it cannot be
-        // among the k best.  A near pair of two rows before that, one of them summed in 32 bits, has to be settled.
+        // Pair i = sorted i and i + 1.  It is open where i + 1, or what is not in order, is near: the first from the k-th on that is not closes the order, and what comes
+        // behind it cannot be among the k best.  A near pair of two rows before that, one of them summed in 32 bits, has to be settled.
         const int changes_most = __reduce_max_sync(~0u, lane < n_live ? s.row_changes[lane] : 0);
         const double near = 2 * row_error(most_chunks, changes_most);
-        uint32_t near_bits[2], unsure_bits[2], ask = 0;
+        if (n > kSorted) rest = max(rest, s.sorted[kSorted - 1]);
+        uint32_t open_bits[2], unsure_bits[2], ask = 0;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int i = lane + 32 * h;
-          bool is_near = false, unsure = false;
-          if (i + 1 < n_sorted) {
-            const uint32_t r1 = s.sorted_at[i] / a.vocab, r2 = s.sorted_at[i + 1] / a.vocab;
-            is_near = sum_of_key(s.sorted[i]) - sum_of_key(s.sorted[i + 1]) < near;
-            unsure = is_near && r1 != r2 && !((s.exact_bits >> r1) & (s.exact_bits >> r2) & 1);
+          bool is_open = false, unsure = false;
+          if (i < n_sorted) {
+            const double sum = sum_of_key(s.sorted[i]);
+            is_open = rest != kNone && sum - sum_of_key(rest) < near;
+            if (i + 1 < n_sorted && sum - sum_of_key(s.sorted[i + 1]) < near) {
+              const uint32_t r1 = s.sorted_at[i] / a.vocab, r2 = s.sorted_at[i + 1] / a.vocab;
+              is_open = true;
+              unsure = r1 != r2 && !((s.exact_bits >> r1) & (s.exact_bits >> r2) & 1);
+            }
           }
-          near_bits[h] = __ballot_sync(~0u, is_near);
+          open_bits[h] = __ballot_sync(~0u, is_open);
           unsure_bits[h] = __ballot_sync(~0u, unsure);
         }
-        const uint64_t is_near = near_bits[0] | (uint64_t)near_bits[1] << 32, unsure = unsure_bits[0] | (uint64_t)unsure_bits[1] << 32;
-        const uint64_t from_k = ~is_near & ~((1ull << (k - 1)) - 1);
-        const int close = __ffsll((long long)from_k) - 1;                     // (pair kSorted - 1 is never near)
+        const uint64_t is_open = open_bits[0] | (uint64_t)open_bits[1] << 32, unsure = unsure_bits[0] | (uint64_t)unsure_bits[1] << 32;
+        const uint64_t from_k = ~is_open & ~((1ull << (k - 1)) - 1);
+        const int close = from_k ? __ffsll((long long)from_k) - 1 : kSorted - 1;
         const uint64_t matter = unsure & ((2ull << close) - 1);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -665,7 +676,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) select_kernel(const SelectPara
           if ((matter >> i) & 1) ask |= (1u << (s.sorted_at[i] / a.vocab)) | (1u << (s.sorted_at[i + 1] / a.vocab));
         }
         ask = __reduce_or_sync(~0u, ask);
-        if (close >= n_sorted - 1 && n_sorted >= k && bar != kNone) ask = ~0u;      // the list ends before the order is closed
+        if (!from_k || close >= n_sorted) ask = rest == kNone ? ask : ~0u;      // the list ends before the order is closed
         // (a row whose sum is NaN offers nothing, and the sums in pairs pass over NaN)
         ask &= s.finite_bits & ~s.exact_bits & __ballot_sync(~0u, ((s.finite_bits & ~s.done_bits) >> lane) & 1 && !isnan(s.row_lse[lane]));
         if (lane < C) cluster.map_shared_rank(&s, lane)->ask_bits = ask;

@@ -72,3 +72,46 @@ def test_select_nan_beside_ties(ops, n, k, v, dtype):
     done = torch.zeros(n, k, dtype=torch.bool, device="cuda")
     done[:, 1] = True
     select_check(ops, x, scores, done=done)
+
+
+def _two_rows(rng, n, k, pattern, dtype, size=8.0, steps=256):
+    """Rows 0 and 1 of each sentence are one pattern, moved by a number of each row's own that leaves every difference exact: the definition has them tie, a normaliser in 32
+    bits puts either ahead.  The other beams are empty."""
+    x = torch.zeros(n, k, len(pattern), device="cuda")
+    moved = _cuda(rng.integers(-size * steps, size * steps, (n, 2)).astype(np.float32) / steps)
+    x[:, :2] = _cuda(pattern.astype(np.float32)) + moved[..., None]
+    assert torch.equal(x.to(dtype).float(), x)
+    scores = torch.full((n, k), -INF, device="cuda")
+    scores[:, :2] = -3
+    return x.to(dtype), scores
+
+
+@pytest.mark.parametrize("n,k,v", [(64, 4, 1000), (40, 4, 12000), (100, 12, 3000)])
+def test_select_ties_above_a_finished_beam(ops, n, k, v):
+    """The last candidate that is kept is a finished beam's, far below; what ties with the others is not among them."""
+    x, scores = _two_rows(_rng(n, k, v, 43), n, k, np.zeros(v), F32)
+    scores[:, 2] = -60
+    done = torch.zeros(n, k, dtype=torch.bool, device="cuda")
+    done[:, 2] = True
+    select_check(ops, x, scores, done=done)
+
+
+def test_select_ties_of_more_words_than_are_kept_in_one_part(ops):
+    """The first words of both rows tie, more of them than a part of the row hands on, but lie in so few places that the parts behind hand on theirs too, which are far below."""
+    n, k, v = 148, 12, 9600
+    for seed in range(20):
+        rng = _rng(seed, 3)
+        pattern = rng.integers(-9 * 256, -8 * 256, v) / 256
+        for vec in range(200):                 # of the first steps' 16-byte vectors those of three lanes
+            if vec % 128 % 32 < 3:
+                pattern[4 * vec:4 * vec + 4] = 0
+        x, scores = _two_rows(rng, n, k, pattern, F32)
+        tokens, parents, _, _ = ops.beam_select(x, scores)
+        assert not parents.any() and (tokens.cpu().numpy() == np.nonzero(pattern == 0)[0][:k]).all(), seed      # ties go to the lowest index
+
+
+@pytest.mark.parametrize("v", [120, 152])
+def test_select_ties_where_every_word_is_a_candidate(ops, v):
+    """Two flat rows of so few words that all of them are ranked, and more of them tie than are put in order."""
+    x, scores = _two_rows(_rng(v, 45), 40, 32, np.zeros(v), F16, size=8.0, steps=64)
+    select_check(ops, x, scores)
