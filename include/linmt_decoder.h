@@ -426,7 +426,8 @@ int linmt_read_pages4(const linmt_pages4_rows_args* args);
  * h / (heads / pages.heads) of the pool; position t of sentence i is row t % page of page table[i][t / page].
  *   s = scale * q . k_t;  cap > 0: s = cap * tanh(s / cap);  slope: s -= slope[h] * |t - centre[i][row]|
  *   seen: first[i][row] <= t < last[i][row] (NULL: all), 0 <= t < len[i], and the table names a page of the pool
- *   out = sum over seen of softmax(s) * v_t; lse = log sum over seen of exp(s).  Nothing seen: 0 and -inf.
+ *   out = sum over seen of softmax(s) * v_t; lse = log sum over seen of exp(s).  Nothing seen: 0 and -inf.  A query with a NaN or an infinity that
+ *   sees something: NaN and NaN.
  * `len` beyond width * page is taken as that.  Sums are held in 32 bits.  Weights times scales are
  * rounded to fp16, with a power of 2 that follows the largest scale so far (scales of 2^-97 to 2^103); for 32-bit queries, which are multiplied as two fp16
  * terms, they are two such terms too.

@@ -112,11 +112,11 @@ template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.
 __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// Four components of row `at` of a sentence's head of the pool, and with the first the log of its weight.
+// Four components of row `at` of a sentence's head of the pool, and with the first the log of its weight.  A weight of 0: nothing was seen; of NaN (a query that is not finite): so are the row and the log.
 template <class T>
 __device__ __forceinline__ void write_row(const AttendParams& a, int sent, int kvh, int at, int d, const float4& sum, float top, float weight) {
   const int g = at / a.rep, h = kvh * a.rep + at - g * a.rep;
-  const float f = weight > 0.f ? 1.f / weight : 0.f;
+  const float f = weight == 0.f ? 0.f : 1.f / weight;
   T* const to = static_cast<T*>(a.out) + sent * a.o_n + g * a.o_g + h * a.o_h + d;
   struct alignas(4 * sizeof(T)) Four { T v[4]; };
   const Four v{{from_float<T>(sum.x * f), from_float<T>(sum.y * f), from_float<T>(sum.z * f), from_float<T>(sum.w * f)}};
@@ -126,7 +126,7 @@ __device__ __forceinline__ void write_row(const AttendParams& a, int sent, int k
 #pragma unroll
     for (int i = 0; i < 4; ++i) to[i] = v.v[i];
   }
-  if (d == 0 && a.lse) a.lse[((int64_t)sent * a.g + g) * a.heads + h] = weight > 0.f ? (top + log2f(weight)) * 0.69314718055994531f : -INFINITY;
+  if (d == 0 && a.lse) a.lse[((int64_t)sent * a.g + g) * a.heads + h] = weight == 0.f ? -INFINITY : (top + log2f(weight)) * 0.69314718055994531f;
 }
 
 // ---- who does what
@@ -779,15 +779,15 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
     float now = top;
 #pragma unroll
     for (int j = 0; j < 8; ++j) now = fmaxf(now, m[j]);
-    if (now == -INFINITY) continue;
-    const float f0 = exp2_of(top - now);
+    const float base = now == -INFINITY ? 0.f : now;      // (a part without a maximum has a weight of 0, or of NaN, which stays one)
+    const float f0 = exp2_of(top - base);
     top = now;
     weight *= f0;
     sum.x *= f0; sum.y *= f0; sum.z *= f0; sum.w *= f0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if (i0 + j * kBy >= n_parts) break;
-      const float f = exp2_of(m[j] - now);
+      const float f = exp2_of(m[j] - base);
       sum.x += f * v[j].x; sum.y += f * v[j].y; sum.z += f * v[j].z; sum.w += f * v[j].w;
       weight += f * l[j];
     }

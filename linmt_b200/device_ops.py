@@ -99,7 +99,8 @@ def attend_pages4(q, pages, table, lens, *, scale=None, cap=0.0, slope=None, cen
     ``q`` [n, g, heads, dim] (float32, bfloat16 or float16, components contiguous); query head h reads head h // (heads / pool heads).  ``table`` [n, width] int32
     names each sentence's pages, ``lens`` [n] int32 its positions.  ``scale``: dim ** -0.5 if None.  ``cap`` > 0: scores are cap * tanh(s / cap).  ``slope``
     [heads] with ``centre`` [n, g], float32: scores lose slope * |position - centre|.  ``first``, ``last`` [n, g] int32: a row sees positions
-    first <= t < last only.  Positions in a column that names no page of the pool are not seen.  A row that sees nothing gets zeros and lse -inf.
+    first <= t < last only.  Positions in a column that names no page of the pool are not seen.  A row that sees nothing gets zeros and lse -inf,
+    one whose query has a NaN or an infinity gets NaN in both.
 
     Returns ``out`` like q (it may be q itself, or overlap nothing of it), and with ``want_lse`` also the log of the row's sum of exponentials, [n, g, heads] float32."""
     return _front.attend_pages4(q, pages, table, lens, scale, cap, slope, centre, first, last, out, want_lse)

@@ -115,3 +115,34 @@ def test_select_ties_where_every_word_is_a_candidate(ops, v):
     """Two flat rows of so few words that all of them are ranked, and more of them tie than are put in order."""
     x, scores = _two_rows(_rng(v, 45), 40, 32, np.zeros(v), F16, size=8.0, steps=64)
     select_check(ops, x, scores)
+
+
+# ---- attention
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("lens", [[40, 17], [3000, 700], [20000, 1]])
+def test_attend_queries_that_are_not_finite(ops, lens, dtype):
+    """A row whose query has a NaN or an infinity gets NaN and says so in its lse, in a sentence that one CTA has and in one that several share; it gets 0 and -inf where it
+    sees nothing; the other rows are as they were."""
+    rng = _rng(sum(lens), 46)
+    pages, table, kk, vv = _memory(ops, rng, lens, 2, 64, 16)
+    n, g, heads = 2, 5, 4
+    q = _q(rng, n, g, heads, 64, dtype)
+    tab, ln = _cuda(table), _cuda(np.array(lens, np.int32))
+    first = torch.zeros(n, g, dtype=torch.int32, device="cuda")
+    last = torch.full((n, g), 2 ** 31 - 1, dtype=torch.int32, device="cuda")
+    first[:, 4] = last[:, 4] = 3
+    bad = q.clone()
+    bad[0, 1, 2, 7] = bad[1, 0, 0, 63] = bad[:, 4] = NAN
+    bad[0, 2, 1, 0] = INF
+    bad[1, 3, 3, 40] = -INF
+    broken = ~torch.isfinite(bad).all(-1)
+    broken[:, 4] = False
+    centre, slope = torch.zeros(n, g, device="cuda"), torch.full((heads,), 0.01, device="cuda")
+    for kw in (dict(), dict(cap=20.0), dict(slope=slope, centre=centre)):
+        want, wl = ops.attend_pages4(q, pages, tab, ln, first=first, last=last, want_lse=True, **kw)
+        got, lse = ops.attend_pages4(bad, pages, tab, ln, first=first, last=last, want_lse=True, **kw)
+        assert torch.isnan(got[broken]).all() and torch.isnan(lse[broken]).all()
+        assert torch.equal(got[~broken], want[~broken]) and torch.equal(lse[~broken], wl[~broken])
+        assert not got[:, 4].any() and torch.isneginf(lse[:, 4]).all()
