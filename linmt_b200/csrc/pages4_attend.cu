@@ -20,6 +20,7 @@
 // Every warp has a ring of tiles of its own (cp.async, no barrier among warps) and its own maximum and sums; the CTA's four are
 // joined through shared memory at the end of a piece of work, and where a sentence's positions are shared by CTAs a second kernel joins those.
 #include <atomic>
+#include <cmath>
 
 #include "device_ops.h"
 #include "pages4.h"
@@ -56,6 +57,8 @@ struct AttendParams {
   float* ws;
   int32_t n, g, heads, rep, width, row_tiles, by_window;
   float scale, cap;
+  float mul;                 // mul 2^mul_up = |scale| log2(e); with a cap times 2 / cap, and with one above kHugeCap times kHugeUp
+  int32_t mul_up;
   int32_t q_wide, o_wide;    // the rows of q are 16-byte aligned; fours of components of out are aligned to their size
 };
 
@@ -97,7 +100,9 @@ __device__ __forceinline__ float exp2_of(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// cap tanh(x) as cap - 2 cap / (2^y + 1), y = 2 x log2(e): good to 3e-7 of the cap, what a 16-bit result can see of it.
+// cap tanh(x) as cap - 2 cap / (2^y + 1), y = 2 x log2(e): good to 3e-7 of the cap.  With a cap of up to kQuickCap that is 2e-5 of a score, which a 16-bit result does not
+// see (2^-11 of a weight is rounded away besides); the difference of two such numbers has nothing left of scores that are small beside a cap of millions.
+constexpr float kQuickCap = 64.f, kHugeCap = 1e30f, kHugeUp = 1.2676506002282294e30f;      // (the last: 2^100)
 __device__ __forceinline__ float capped(float y, float cap) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(exp2_of(y) + 1.f));
@@ -369,8 +374,9 @@ __device__ __forceinline__ void join_warps(const AttendParams& a, const Piece& p
   __syncthreads();                    // (before the next piece's tiles come in)
 }
 
-// PLAIN: no cap, no bias, and a scale: scores are products times mul.
-template <class T, int D, bool PLAIN>
+// What is done to scores.  kPlain: no cap, no bias, and a scale: they are products times mul.  kQuick: caps of up to kQuickCap for 16-bit queries.  kExact: tanhf.
+enum Scores { kPlain, kQuick, kExact };
+template <class T, int D, Scores HOW>
 __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend_kernel(const __grid_constant__ AttendParams a) {
   constexpr int NG = D / 32, kTileBytes = pages4::tile_bytes(D), QT = kTerms<T>, PT = kTerms<T>;
   constexpr bool kOver = sizeof(T) == 2;      // codes are operands as they are: 8 for each, and every second's 16, come off apart
@@ -473,7 +479,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend_kernel(co
         for (int gr = 1; gr < NG; ++gr) most = fmaxf(most, s_most[gr][gid + 8 * r]);
         const int up = most > 0.f && most < INFINITY ? 9 - max(-100, ilogbf(most)) : 0;      // -118 .. 109
         const float by = ldexpf(a.scale < 0.f ? -1.f : 1.f, up);
-        mul[r] = ldexpf(fabsf(a.scale) * kLog2e * (a.cap > 0.f ? 2.f / a.cap : 1.f), (kOver ? 24 : 0) - up);
+        mul[r] = ldexpf(a.mul, a.mul_up + (kOver ? 24 : 0) - up);
         if (warp < NG) {
           float sum = 0.f;
 #pragma unroll
@@ -518,7 +524,9 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend_kernel(co
         over = make_uint4(ov[0][0], ov[1][0], ov[0][1], ov[1][1]);
       }
     }
-    const float cap_log2 = a.cap * kLog2e;
+    // A cap near the largest 32-bit number: its product with log2(e), and one over it, are kept within the normal ones by a power of 2 each.
+    const bool huge = HOW == kExact && a.cap > kHugeCap;
+    const float cap_by = huge ? 256.f : 1.f, cap_log2 = a.cap / cap_by * kLog2e, tanh_by = 0.5f / kLog2e * (huge ? 1.f / kHugeUp : 1.f);
 
     // The values' sums are kept times 2^-24 where the codes are, and times the power of 2 that brings their scales into fp16's range.
     float o[NG][4][4] = {}, extra[4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, size = 1.f;   // size: that power
@@ -585,14 +593,14 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend_kernel(co
         }
       }
       float r0 = mul[0], r1 = mul[1];
-      if constexpr (!PLAIN) {
+      if constexpr (HOW != kPlain) {
         const float at0 = (float)(pos + 2 * c) - job.centre[0], at1 = (float)(pos + 2 * c) - job.centre[1];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             float v = x[j][e] * (e < 2 ? r0 : r1);
-            if (a.cap > 0.f) v = sizeof(T) == 4 ? cap_log2 * tanhf(v * (0.5f / kLog2e)) : capped(v, cap_log2);
+            if (a.cap > 0.f) v = HOW == kExact ? cap_log2 * tanhf(v * tanh_by) * cap_by : capped(v, cap_log2);
             if (a.slope) v = fmaf(-job.slope[e >> 1], fabsf((e < 2 ? at0 : at1) + (float)(8 * j + (e & 1))), v);
             x[j][e] = v;
           }
@@ -814,14 +822,16 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
 template <class T, int D>
 cudaError_t launch_attend(const AttendParams& p, int blocks, int device, cudaStream_t st) {
   constexpr int smem = attend_smem<T, D>();
-  const bool plain = p.cap == 0.f && !p.slope && p.scale != 0.f;
-  void (*kernel)(AttendParams);
-  kernel = plain ? attend_kernel<T, D, true> : attend_kernel<T, D, false>;
-  static std::atomic<bool> opted_in[kOpMaxDevices][2] = {};
-  if (smem + 1024 > 48 << 10 && !opted_in[device][plain].load(std::memory_order_acquire)) {
+  const Scores how = p.cap == 0.f && !p.slope && p.scale != 0.f ? kPlain : sizeof(T) == 4 || p.cap > kQuickCap ? kExact : kQuick;
+  void (*kernel)(AttendParams) = how == kPlain ? attend_kernel<T, D, kPlain> : attend_kernel<T, D, kExact>;
+  if constexpr (sizeof(T) == 2) {
+    if (how == kQuick) kernel = attend_kernel<T, D, kQuick>;
+  }
+  static std::atomic<bool> opted_in[kOpMaxDevices][3] = {};
+  if (smem + 1024 > 48 << 10 && !opted_in[device][how].load(std::memory_order_acquire)) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    opted_in[device][plain].store(true, std::memory_order_release);
+    opted_in[device][how].store(true, std::memory_order_release);
   }
   kernel<<<(unsigned)blocks, kWarps * 32, smem, st>>>(p);
   cudaError_t e = cudaGetLastError();
@@ -897,8 +907,10 @@ int linmt_attend_pages4(const linmt_attend_pages4_args* g) {
   AttendParams p{static_cast<const unsigned char*>(g->pages.data), g->pages.stride_page, g->pages.stride_head, g->pages.n_pages, g->pages.heads, g->pages.page,
                  g->q, g->q_stride_n, g->q_stride_g, g->q_stride_h, g->out, g->out_stride_n, g->out_stride_g, g->out_stride_h, g->lse, g->table, g->table_stride, g->len,
                  g->slope, g->centre, g->first, g->last, need ? static_cast<float*>(g->workspace) : nullptr, g->n, g->g, g->heads, g->heads / g->pages.heads, g->width, row_tiles_of(g), g->first && g->g <= 32 && (int64_t)g->n * g->g <= 65536,
-                 g->scale, g->cap, aligned(g->q, 16) && (g->q_stride_n | g->q_stride_g | g->q_stride_h) % (16 / dtype_bytes(g->dtype)) == 0,
+                 g->scale, g->cap, std::fabs(g->scale) * kLog2e * (g->cap > 0.f ? 2.f / g->cap : 1.f), 0, aligned(g->q, 16) && (g->q_stride_n | g->q_stride_g | g->q_stride_h) % (16 / dtype_bytes(g->dtype)) == 0,
                  aligned(g->out, 4 * dtype_bytes(g->dtype)) && (g->out_stride_n | g->out_stride_g | g->out_stride_h) % 4 == 0};
+  if (g->cap > kQuickCap) p.mul = (float)std::frexp(std::fabs((double)g->scale) * 1.4426950408889634 * 2 / g->cap, &p.mul_up);
+  if (g->cap > kHugeCap) p.mul_up += 100;
   const int blocks = blocks_of(g);
   const cudaStream_t st = static_cast<cudaStream_t>(g->stream);
   cudaError_t e;

@@ -146,3 +146,25 @@ def test_attend_queries_that_are_not_finite(ops, lens, dtype):
         assert torch.isnan(got[broken]).all() and torch.isnan(lse[broken]).all()
         assert torch.equal(got[~broken], want[~broken]) and torch.equal(lse[~broken], wl[~broken])
         assert not got[:, 4].any() and torch.isneginf(lse[:, 4]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("cap", [64.0, 65.0, 1e3, 1e4, 1e6, 1e9, 1e20, 3e38])
+def test_attend_caps_of_all_sizes(ops, cap, dtype):
+    """A large cap leaves the scores nearly as they are: to 2^-20 of a score, however large the cap."""
+    rng = _rng(int(np.log2(cap) * 100), 47)
+    lens, dim = [33, 500], 64
+    pages, table, kk, vv = _memory(ops, rng, lens, 2, dim, 16)
+    q = _q(rng, 2, 3, 4, dim, dtype).mul_(4)
+    got, lse = ops.attend_pages4(q, pages, _cuda(table), _cuda(np.array(lens, np.int32)), cap=cap, want_lse=True)
+    want, wlse, wv, big, ws = attend_ref(q.double().cpu().numpy(), kk, vv, table, lens, 16, dim ** -0.5, cap, None, None, None, None, pages.shape[0])
+    # A score as in attend_check, with 3e-7 of a cap of up to 64 and, above that, tanh and its argument's products to 2^-21 of the score (four roundings and tanh's 2^-22).
+    score = ((dim + 12) * 2.0 ** -24 + 2.0 ** -21 + (2.0 ** -22 if dtype == F32 else 0)) * big + (4e-7 * cap if cap <= 64 else 0) + 6 * 2.0 ** -24 * (np.abs(wlse).max() + 32)
+    weight = {BF16: 2.0 ** -11, F16: 2.0 ** -11, F32: 2.0 ** -22}[dtype]
+    steps, big_scale = max(lens) / 64 + 1, float(np.abs(vv).max()) / 7
+    shift = 8 * 2.0 ** -34 * big_scale * max(lens) if dtype == F32 else (steps * 17 + 8) * 2.0 ** -23 * 15 * ws + 8 * 2.0 ** -28 * big_scale * max(lens)
+    tol = HALF_STEP[dtype] * np.abs(want) + (weight + 2 * score + 2.0 ** -15) * wv + shift + (2.0 ** -25 if dtype == F16 else 0)
+    g, l = got.double().cpu().numpy(), lse.double().cpu().numpy()
+    assert np.isfinite(g).all() and np.isfinite(l).all()
+    assert (np.abs(l - wlse) <= score + 2.0 ** -15 + 2.0 ** -23 * np.abs(wlse)).all(), float(np.abs(l - wlse).max())
+    assert (np.abs(g - want) <= tol).all(), float((np.abs(g - want) / np.maximum(tol, 1e-300)).max())
