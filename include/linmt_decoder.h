@@ -370,7 +370,8 @@ int linmt_beam_reorder(const linmt_beam_reorder_args* args);
  * ceil(old / page) <= p < ceil(new / page) gets the next entry of `free_pages`, sentence by sentence, and every new position its
  * slot = table[i][pos / page] * page + pos % page, sentence by sentence.  Lengths are taken as 0 .. width * page, a shorter new length as the
  * old one.  Where the free list has run out a column gets -1; a position in a column that holds none of the pool's pages gets slot -1;
- * so do slots behind the last new position.  out_used = used + the pages that were wanted (more than n_free: the list ran out). */
+ * so do slots behind the last new position.  out_used = used + the pages that were wanted (more than n_free: the list ran out).
+ * Nothing that is written, the table among it, may overlap the lengths, the free pages or `used`. */
 typedef struct linmt_plan_pages_args {
   uint32_t size;
   int32_t device;

@@ -8,6 +8,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 #include <vector>
@@ -86,6 +87,51 @@ bool apart(const Tensor& t) {
   return true;
 }
 
+// The bytes from a tensor's first to its last.
+struct Span { const char *p, *end; };
+Span span_of(const Tensor& t) {
+  const char* const p = static_cast<const char*>(t.data_ptr());
+  if (t.numel() == 0) return {p, p};
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+  return {p, p + (last + 1) * (int64_t)t.element_size()};
+}
+// Whether the bytes p .. end - 1 meet elements of `bytes` bytes at `base` and `dims` strides from it, the widest first.
+bool meets(const char* base, const int64_t* size, const int64_t* stride, int dims, int64_t bytes, const char* p, const char* end) {
+  int64_t extent = bytes;
+  for (int i = 0; i < dims; ++i) extent += (size[i] - 1) * stride[i];
+  if (end <= base || p >= base + extent) return false;
+  if (dims == 0) return true;
+  if (extent - (size[0] - 1) * stride[0] > stride[0]) return true;      // (strides that do not nest: as far as can be told)
+  const int64_t first = p <= base ? 0 : (p - base) / stride[0], last = std::min((end - 1 - base) / stride[0], size[0] - 1);
+  for (int64_t i = first; i <= last; ++i)
+    if (i > first && i < last) return true;
+    else if (meets(base + i * stride[0], size + 1, stride + 1, dims - 1, bytes, p, end)) return true;
+  return false;
+}
+bool meets(const Tensor& t, const Span& s) {
+  const Span all = span_of(t);
+  if (s.p == s.end || all.end <= s.p || s.end <= all.p) return false;
+  int64_t size[8], stride[8];
+  int dims = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    if (t.size(i) == 1) continue;
+    if (dims == 8) return true;
+    const int64_t by = t.stride(i) * (int64_t)t.element_size();
+    int j = dims++;
+    for (; j > 0 && stride[j - 1] < by; --j) { size[j] = size[j - 1]; stride[j] = stride[j - 1]; }
+    size[j] = t.size(i);
+    stride[j] = by;
+  }
+  return meets(all.p, size, stride, dims, (int64_t)t.element_size(), s.p, s.end);
+}
+// A tensor that is written while `read` is still read has to lie apart from it, or in the gaps between its places.
+void lie_apart(const Tensor& written, const char* name, PyObject* read, const char* of) {
+  if (read == Py_None) return;
+  const Tensor& r = THPVariable_Unpack(read);
+  NEED(!meets(written, span_of(r)) || !meets(r, span_of(written)), name, " overlaps ", of);
+}
+
 PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
   arguments(n_args, 6);
@@ -130,7 +176,6 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     flags(PyTuple_GET_ITEM(a[5], 3), "out[3]", dev, shape);
     t[3] = THPVariable_Unpack(PyTuple_GET_ITEM(a[5], 3));
     // A sentence's results are written while others are still read: each has to lie apart from all that is read, or be it, place for place.
-    struct Span { const char *p, *end; };
     auto span = [](const void* p, int64_t bytes) { return Span{static_cast<const char*>(p), static_cast<const char*>(p) + bytes}; };
     auto meet = [](const Span& x, const Span& y) { return x.p < y.end && y.p < x.end; };
     const Span outs[4] = {span(t[0].data_ptr(), n * k * 4), span(t[1].data_ptr(), n * k * 4), span(t[2].data_ptr(), n * k * 4), span(t[3].data_ptr(), n * k)};
@@ -283,6 +328,11 @@ PyObject* plan_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   NEED(free.dim() == 1, "free has to be [n_free]");
   g.free_pages = static_cast<const int32_t*>(dense(a[3], "free", dev, at::kInt, free.sizes()).data_ptr());
   g.used = static_cast<const int32_t*>(dense(a[4], "used", dev, at::kInt, one).data_ptr());
+  // Every CTA reads the lengths and the free pages for itself, while others write the table.
+  lie_apart(table, "table", a[0], "old");
+  lie_apart(table, "table", a[1], "new");
+  lie_apart(table, "table", a[3], "free");
+  lie_apart(table, "table", a[4], "used");
   NEED(total >= 0, "total is negative");
   g.n = int32_of(n, "n");
   g.width = int32_of(table.size(1), "width");

@@ -66,7 +66,7 @@ def plan_pages(old, new, table, free, used, *, page, total):
     """Pages and slots for sentences that grow from ``old`` to ``new`` positions ([n] int32; ``old`` None: from nothing).
 
     Every page column p of sentence i with ceil(old / page) <= p < ceil(new / page) of ``table`` [n, width] int32 gets the next entry of ``free`` [n_free] int32, of
-    which ``used`` [1] int32 are taken already; ``table`` is written in place.  Returns ``slots`` [total] int64 (table[i, pos // page] * page + pos % page of each
+    which ``used`` [1] int32 are taken already; ``table`` is written in place, and overlaps none of the others.  Returns ``slots`` [total] int64 (table[i, pos // page] * page + pos % page of each
     new position, sentence by sentence, -1 behind the last), ``starts`` [n + 1] int32 (each sentence's first in ``slots``) and the new ``used`` [1].
     Where the free list has run out a column and its slots are -1 and ``used`` comes back larger than n_free.  Lengths are taken as 0 .. width * page, a
     shorter ``new`` as ``old``."""

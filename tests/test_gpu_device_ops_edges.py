@@ -168,3 +168,38 @@ def test_attend_caps_of_all_sizes(ops, cap, dtype):
     assert np.isfinite(g).all() and np.isfinite(l).all()
     assert (np.abs(l - wlse) <= score + 2.0 ** -15 + 2.0 ** -23 * np.abs(wlse)).all(), float(np.abs(l - wlse).max())
     assert (np.abs(g - want) <= tol).all(), float((np.abs(g - want) / np.maximum(tol, 1e-300)).max())
+
+
+# ---- what is written over what is read
+
+
+def test_plan_refuses_a_table_over_what_it_reads(ops):
+    """All of the call's int32 arrays in one buffer: apart, or in the gaps between the table's rows, they are taken; where a table's row has an entry of them they are not."""
+    n, width, page = 4, 3, 16
+    old, new = np.array([5, 0, 16, 33], np.int32), np.array([20, 3, 40, 34], np.int32)
+    free = np.array([7, 3, 9, 1, 12], np.int32)
+    total = int((new - old).sum())
+    rows = np.full((n, width), -1, np.int32)
+    rows[0, 0], rows[2, 0], rows[3] = 20, 21, [22, 23, 24]
+    want = plan_ref(old, new, rows, free, 0, page, total)
+
+    def call(table_at, stride, at):
+        buf = torch.full((160,), -7, dtype=torch.int32, device="cuda")
+        place = lambda x, a: buf[a:a + len(x)].copy_(_cuda(x))
+        o, w, f, u = place(old, at[0]), place(new, at[1]), place(free, at[2]), place(np.zeros(1, np.int32), at[3])
+        table = buf[table_at:table_at + (n - 1) * stride + width].as_strided((n, width), (stride, 1))
+        keep = [x.clone() for x in (o, w, f, u)]
+        table.copy_(_cuda(rows))
+        for x, y in zip((o, w, f, u), keep):
+            x.copy_(y)
+        slots, starts, used = ops.plan_pages(o, w, table, f, u, page=page, total=total)
+        assert (slots.cpu().numpy() == want[0]).all() and (starts.cpu().numpy() == want[1]).all() and (table.cpu().numpy() == want[2]).all() and int(used) == want[3]
+        assert all(torch.equal(x, y) for x, y in zip((o, w, f, u), keep))
+
+    call(0, 3, (12, 16, 20, 25))
+    call(0, 12, (3, 7, 15, 11))                # in the gaps
+    for bad, name in (((2, 60, 70, 80), "old"), ((60, 11, 70, 80), "new"), ((60, 70, 20, 80), "free"), ((60, 70, 80, 25), "used"), ((60, 70, 33, 80), "free"), ((36, 70, 80, 90), "old")):
+        with pytest.raises(ValueError, match="table overlaps " + name):
+            call(0, 12, bad)
+    with pytest.raises(ValueError, match="overlaps free"):
+        call(0, 3, (20, 30, 11, 40))
