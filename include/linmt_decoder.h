@@ -408,7 +408,7 @@ typedef struct linmt_pages4 {
 } linmt_pages4;
 
 /* Keys and values of `t` positions into (write) or out of (read) the slots of a pool.  A slot outside 0 .. n_pages * page - 1 is not written, and reads
- * as zeros.  Slots of a write must differ: what two writes of one slot leave there is not defined. */
+ * as zeros.  Slots of a write must differ: what two writes of one slot leave there is not defined.  What is written overlaps nothing that is read. */
 typedef struct linmt_pages4_rows_args {
   uint32_t size;
   int32_t device;

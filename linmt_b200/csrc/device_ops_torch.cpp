@@ -392,6 +392,9 @@ PyObject* write_pages4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   g.dtype = dtype_of(k);
   rows_of(k, "k", g, g.k, g.k_stride_t, g.k_stride_h);
   rows_of(v, "v", g, g.v, g.v_stride_t, g.v_stride_h);
+  lie_apart(THPVariable_Unpack(a[0]), "pages", a[1], "slots");
+  lie_apart(THPVariable_Unpack(a[0]), "pages", a[2], "k");
+  lie_apart(THPVariable_Unpack(a[0]), "pages", a[3], "v");
   done_or_raise(linmt_write_pages4(&g));
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS

@@ -84,7 +84,7 @@ def new_pages4(n_pages, heads, dim, page, device="cuda"):
 def write_pages4(pages, slots, k, v):
     """Keys and values ``k``, ``v`` [t, heads, dim] (float32, bfloat16 or float16, components contiguous, rows on 16-byte boundaries) into ``slots`` [t] int64 of a
     pool, in 4 bits with a bf16 scale for 32 components (the form is in the header).  A slot outside the pool, -1 say, is not written.  No slot may be
-    named twice."""
+    named twice, and ``pages`` overlaps none of the others."""
     _front.write_pages4(pages, slots, k, v)
 
 

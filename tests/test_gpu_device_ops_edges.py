@@ -203,3 +203,31 @@ def test_plan_refuses_a_table_over_what_it_reads(ops):
             call(0, 12, bad)
     with pytest.raises(ValueError, match="overlaps free"):
         call(0, 3, (20, 30, 11, 40))
+
+
+def test_write_refuses_pages_over_what_it_reads(ops):
+    """A pool in the larger of two buffers' halves, beside what is written into it: apart it is taken, over slots, keys or values it is not."""
+    rng = _rng(48)
+    heads, dim, t = 2, 64, 20
+    size = heads * 18 * dim                    # bytes of a page of 16 positions
+    buf = torch.zeros(64 * size, dtype=torch.uint8, device="cuda")
+    pages = buf[:4 * size].view(4, heads, 1, 18 * dim)
+    at = lambda first, dtype, *shape: buf[first:first + int(np.prod(shape)) * torch.empty(0, dtype=dtype).element_size()].view(dtype).view(shape)
+    k, v = (_cuda(rng.normal(0, 1, (t, heads, dim)).astype(np.float32)) for _ in range(2))
+    slots = _cuda(rng.permutation(64)[:t].astype(np.int64))
+    ops.write_pages4(pages, slots, k, v)
+    want = ops.read_pages4(pages, slots)
+    pages.zero_()
+    far_k, far_v, far_s = at(4 * size, F32, t, heads, dim), at(16 * size, F32, t, heads, dim), at(40 * size, torch.int64, t)
+    far_k.copy_(k), far_v.copy_(v), far_s.copy_(slots)
+    ops.write_pages4(pages, far_s, far_k, far_v)
+    assert all(torch.equal(a, b) for a, b in zip(ops.read_pages4(pages, far_s), want))
+    over = at(4 * size - 16, F32, t, heads, dim)
+    for args, name in (((at(4 * size - 64, torch.int64, t), k, v), "slots"), ((slots, over, v), "k"), ((slots, k, over), "v")):
+        with pytest.raises(ValueError, match="pages overlaps " + name):
+            ops.write_pages4(pages, *args)
+    layers = buf[:48 * size].view(4, 12, heads, 1, 18 * dim)      # a layer's pages, every twelfth
+    pages, far_s = layers[:, 2], layers[1, 5].view(-1)[:8 * t].view(torch.int64)
+    far_s.copy_(slots)
+    ops.write_pages4(pages, far_s, k, v)       # slots in the gaps between them
+    assert all(torch.equal(a, b) for a, b in zip(ops.read_pages4(pages, far_s), want)) and torch.equal(far_s, slots)
