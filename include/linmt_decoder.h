@@ -440,7 +440,7 @@ typedef struct linmt_attend_pages4_args {
   linmt_pages4 pages;
   const void* q;             /* [n][g][heads][dim], components contiguous, rows 4-byte aligned */
   int64_t q_stride_n, q_stride_g, q_stride_h;
-  void* out;                 /* as q, strides of its own; q itself with q's strides, or apart from it */
+  void* out;                 /* as q, strides of its own; q itself with q's strides, or apart from it; apart from all else that is read */
   int64_t out_stride_n, out_stride_g, out_stride_h;
   float* lse;                /* [n][g][heads]; may be NULL */
   const int32_t* table;      /* [n][width], rows `table_stride` apart */

@@ -481,6 +481,9 @@ PyObject* attend_pages4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const Strides from = places(q), to = places(out);
     const bool same = from.p == to.p && from.l == to.l && from.n == to.n && from.k == to.k;
     NEED(q.numel() == 0 || same || disjoint(from, to, rows, flat ? 1 : heads), "out overlaps q");
+    static const char* const read[] = {nullptr, "pages", "table", "lens", nullptr, nullptr, "slope", "centre", "first", "last"};
+    for (int i = 1; i < 10; ++i)
+      if (read[i]) lie_apart(out, "out", a[i], read[i]);
   }
   g.out = out.data_ptr();
   g.out_stride_n = out.stride(0);

@@ -102,5 +102,5 @@ def attend_pages4(q, pages, table, lens, *, scale=None, cap=0.0, slope=None, cen
     first <= t < last only.  Positions in a column that names no page of the pool are not seen.  A row that sees nothing gets zeros and lse -inf,
     one whose query has a NaN or an infinity gets NaN in both.
 
-    Returns ``out`` like q (it may be q itself, or overlap nothing of it), and with ``want_lse`` also the log of the row's sum of exponentials, [n, g, heads] float32."""
+    Returns ``out`` like q (it may be q itself, and overlaps nothing else that the call reads), and with ``want_lse`` also the log of the row's sum of exponentials, [n, g, heads] float32."""
     return _front.attend_pages4(q, pages, table, lens, scale, cap, slope, centre, first, last, out, want_lse)

@@ -231,3 +231,30 @@ def test_write_refuses_pages_over_what_it_reads(ops):
     far_s.copy_(slots)
     ops.write_pages4(pages, far_s, k, v)       # slots in the gaps between them
     assert all(torch.equal(a, b) for a, b in zip(ops.read_pages4(pages, far_s), want)) and torch.equal(far_s, slots)
+
+
+def test_attend_refuses_a_result_over_what_it_reads(ops):
+    """A result over the table, the lengths, a bias, windows or the pool; beside them in one buffer it is taken."""
+    rng = _rng(49)
+    lens, heads, dim, g = [40, 21], 2, 64, 3
+    pages, table, kk, vv = _memory(ops, rng, lens, heads, dim, 16)
+    q = _q(rng, 2, g, heads, dim, F32)
+    args = dict(table=_cuda(table), lens=_cuda(np.array(lens, np.int32)), slope=torch.rand(heads, device="cuda"), centre=torch.rand(2, g, device="cuda"),
+                first=torch.zeros(2, g, dtype=torch.int32, device="cuda"), last=torch.full((2, g), 30, dtype=torch.int32, device="cuda"), pages=pages)
+    size = 2 * g * heads * dim
+    buf = torch.zeros(size + 64 + pages.numel() // 4, device="cuda")
+    out = buf[:size].view(2, g, heads, dim)
+    call = lambda out, a: ops.attend_pages4(q, a["pages"], a["table"], a["lens"], slope=a["slope"], centre=a["centre"], first=a["first"], last=a["last"], out=out)
+    want = call(None, args)
+    for name, x in args.items():
+        def moved(first):                      # the argument's copy in the buffer, behind `first` of its places
+            y = buf[first:first + x.numel() * x.element_size() // 4].view(x.dtype).view(x.shape)
+            y.copy_(x)
+            return dict(args, **{name: y})
+        assert torch.equal(call(out, moved(size)), want)
+        for first in (size - 4, 4):            # (a pool lies on 16 bytes)
+            with pytest.raises(ValueError, match="out overlaps " + name):
+                call(out, moved(first))
+    wide = torch.zeros(2, g, heads, dim + 8, device="cuda")
+    lens_in = wide.view(-1)[dim:dim + 2].view(torch.int32).copy_(args["lens"])      # in the gap behind the first row
+    assert torch.equal(call(wide[..., :dim], dict(args, lens=lens_in)), want) and lens_in.tolist() == lens
