@@ -4,6 +4,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -30,6 +31,7 @@ const Tensor& on_cuda(PyObject* o, const char* name) {
   const Tensor& t = tensor(o, name);
   NEED(t.is_cuda() && t.layout() == at::kStrided && !t.is_neg(), name, " has to be a CUDA tensor");
   NEED(!t.requires_grad() || !at::GradMode::is_enabled(), name, " requires a gradient, and there is no backward pass: call under torch.no_grad()");
+  NEED(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), name, " has a tangent, and there is no derivative: call with the primal (forward_ad.unpack_dual)");
   return t;
 }
 const Tensor& on_device(PyObject* o, const char* name, int dev) {

@@ -11,7 +11,8 @@ their own model.
 Tensors are torch CUDA tensors, all of one call on one device.  Work is issued on that device's current torch stream and nothing waits; results that
 are not given as ``out`` are allocated by torch on that stream, so calls follow each other, may run at once on several
 streams and may be captured into a CUDA graph like torch's own.  ``ValueError``: an argument is not allowed; ``LinmtError``: the library refused.
-There is no backward pass (the engine decodes and scores, it does not train): tensors that require a gradient are refused outside ``torch.no_grad()``.
+There is no backward pass (the engine decodes and scores, it does not train): tensors that require a gradient are refused outside ``torch.no_grad()``, and
+tensors with a tangent (``torch.autograd.forward_ad``) everywhere.
 """
 from __future__ import annotations
 

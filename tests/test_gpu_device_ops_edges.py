@@ -258,3 +258,25 @@ def test_attend_refuses_a_result_over_what_it_reads(ops):
     wide = torch.zeros(2, g, heads, dim + 8, device="cuda")
     lens_in = wide.view(-1)[dim:dim + 2].view(torch.int32).copy_(args["lens"])      # in the gap behind the first row
     assert torch.equal(call(wide[..., :dim], dict(args, lens=lens_in)), want) and lens_in.tolist() == lens
+
+
+# ---- beside autograd
+
+
+def test_tangents_are_refused(ops):
+    """No derivative forwards either: a dual tensor's tangent would be dropped."""
+    fwd = torch.autograd.forward_ad
+    x, s = torch.zeros(1, 2, 50, device="cuda"), torch.zeros(1, 2, device="cuda")
+    parents = torch.zeros(1, 2, dtype=torch.int32, device="cuda")
+    pages, table, lens = ops.new_pages4(2, 1, 64, 16), torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    q, k = torch.zeros(1, 2, 1, 64, device="cuda"), torch.ones(1, 1, 64, device="cuda")
+    slots = torch.zeros(1, dtype=torch.int64, device="cuda")
+    calls = ((lambda d: ops.beam_select(d, s), x), (lambda d: ops.beam_select(x, d), s), (lambda d: ops.beam_reorder([d], parents), x[..., :8].clone()),
+             (lambda d: ops.attend_pages4(d, pages, table, lens), q), (lambda d: ops.write_pages4(pages, slots, k, d), k))
+    with fwd.dual_level():
+        for call, primal in calls:
+            dual = fwd.make_dual(primal, torch.ones_like(primal))
+            for guard in (torch.enable_grad(), torch.no_grad()):
+                with guard, pytest.raises(ValueError, match="tangent"):
+                    call(dual)
+            call(fwd.unpack_dual(dual).primal)
