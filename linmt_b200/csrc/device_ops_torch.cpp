@@ -89,6 +89,11 @@ bool apart(const Tensor& t) {
   return true;
 }
 
+// A caller's tensor has been written: autograd finds one that it has saved for a backward pass changed.  (Tensors of the inference mode keep no count.)
+void was_written(PyObject* o) {
+  const Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 // The bytes from a tensor's first to its last.
 struct Span { const char *p, *end; };
 Span span_of(const Tensor& t) {
@@ -197,6 +202,7 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     done_or_raise(linmt_beam_select(&g));
   }
   if (a[5] != Py_None) {
+    for (int i = 0; i < 4; ++i) was_written(PyTuple_GET_ITEM(a[5], i));
     Py_INCREF(a[5]);
     return a[5];
   }
@@ -296,6 +302,7 @@ PyObject* beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     std::copy(states.begin() + i, states.begin() + i + g.n_states, g.state);
     done_or_raise(linmt_beam_reorder(&g));
   }
+  for (Py_ssize_t i = 0; i < all; ++i) was_written(PyList_GET_ITEM(a[2], i));
   Py_INCREF(a[2]);
   return a[2];
   END_HANDLE_TH_ERRORS
@@ -346,6 +353,7 @@ PyObject* plan_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   g.out_starts = static_cast<int32_t*>(starts.data_ptr());
   g.out_used = static_cast<int32_t*>(used.data_ptr());
   done_or_raise(linmt_plan_pages(&g));
+  was_written(a[2]);
   PyObject* r = PyTuple_New(3);
   if (!r) throw python_error();
   PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(slots)));
@@ -398,6 +406,7 @@ PyObject* write_pages4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   lie_apart(THPVariable_Unpack(a[0]), "pages", a[2], "k");
   lie_apart(THPVariable_Unpack(a[0]), "pages", a[3], "v");
   done_or_raise(linmt_write_pages4(&g));
+  was_written(a[0]);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -510,7 +519,10 @@ PyObject* attend_pages4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   }
   PyObject* o = a[10];
   if (o == Py_None) o = THPVariable_Wrap(std::move(out));
-  else Py_INCREF(o);
+  else {
+    was_written(o);
+    Py_INCREF(o);
+  }
   if (!want_lse) return o;
   PyObject* r = PyTuple_New(2);
   if (!r) { Py_DECREF(o); throw python_error(); }

@@ -280,3 +280,33 @@ def test_tangents_are_refused(ops):
                 with guard, pytest.raises(ValueError, match="tangent"):
                     call(dual)
             call(fwd.unpack_dual(dual).primal)
+
+
+def test_writing_in_place_raises_versions(ops):
+    """What a call writes into a caller's tensor counts as a change of it, so that autograd refuses a backward pass through a saved tensor that was overwritten; what it only
+    reads does not.  Tensors of the inference mode have no count and are written all the same."""
+    n, k = 2, 3
+    ints = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+    x, scores, done, tokens, parents = torch.rand(n, k, 40, device="cuda"), torch.zeros(n, k, device="cuda"), torch.zeros(n, k, dtype=torch.bool, device="cuda"), ints(n, k), ints(n, k)
+    state, other = torch.rand(2, n, k, 5, device="cuda"), torch.rand(2, n, k, 5, device="cuda")
+    pages, table, lens = ops.new_pages4(4, 1, 64, 16), ints(n, 2), torch.full((n,), 20, dtype=torch.int32, device="cuda")
+    free, used = torch.arange(4, dtype=torch.int32, device="cuda"), ints(1)
+    kv, slots = torch.rand(40, 1, 64, device="cuda"), torch.arange(40, device="cuda")
+    q, out = torch.rand(n, k, 1, 64, device="cuda"), torch.zeros(n, k, 1, 64, device="cuda")
+    for call, written, read in ((lambda: ops.beam_select(x, scores, done=done, out=(tokens, parents, scores, done)), (tokens, parents, scores, done), (x,)),
+                                (lambda: ops.beam_reorder([state[:1], state[1:]], parents), (state,), (parents,)), (lambda: ops.beam_reorder([state], parents, out=[other]), (other,), (state, parents)),
+                                (lambda: ops.plan_pages(None, lens, table, free, used, page=16, total=40), (table,), (lens, free, used)),
+                                (lambda: ops.write_pages4(pages, slots, kv, kv), (pages,), (slots, kv)), (lambda: ops.read_pages4(pages, slots), (), (pages, slots)),
+                                (lambda: ops.attend_pages4(q, pages, table, lens, out=out), (out,), (q, pages, table, lens)), (lambda: ops.attend_pages4(q, pages, table, lens, out=q), (q,), (pages, table, lens))):
+        before = [t._version for t in written], [t._version for t in read]
+        call()
+        assert all(t._version > v for t, v in zip(written, before[0])) and [t._version for t in read] == before[1]
+    w = torch.ones_like(state, requires_grad=True)
+    y = (w * state).sum()
+    ops.beam_reorder([state], parents)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        kept = torch.arange(6., device="cuda").view(1, n, k)[0]
+    ops.beam_reorder([kept], torch.tensor([[1, 1, 0], [2, 0, 0]], dtype=torch.int32, device="cuda"))
+    assert kept.tolist() == [[1, 1, 0], [5, 3, 3]]
