@@ -284,6 +284,7 @@ PyObject* beam_reorder(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     Strides d = s;
     if (oy != ox) {
       NEED(y.scalar_type() == x.scalar_type() && y.sizes() == x.sizes(), "out[", i, "] has to be like states[", i, "]");
+      NEED(y.is_conj() == x.is_conj(), "out[", i, "] has to be like states[", i, "]: one of the two is a conjugate view");
       d = strides_of(y, n, k, "out", i);
     }
     if (x.numel() == 0) continue;

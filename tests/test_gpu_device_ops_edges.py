@@ -310,3 +310,22 @@ def test_writing_in_place_raises_versions(ops):
         kept = torch.arange(6., device="cuda").view(1, n, k)[0]
     ops.beam_reorder([kept], torch.tensor([[1, 1, 0], [2, 0, 0]], dtype=torch.int32, device="cuda"))
     assert kept.tolist() == [[1, 1, 0], [5, 3, 3]]
+
+
+def test_reorder_complex_states(ops):
+    """Complex rows are moved as they lie in memory: a conjugate view goes into a conjugate view, or back into itself, and nowhere else."""
+    rng = _rng(50)
+    parents = _cuda(rng.integers(0, 4, (3, 4)).astype(np.int32))
+    x = torch.complex(*(_cuda(rng.normal(0, 1, (3, 4, 5)).astype(np.float32)) for _ in range(2)))
+    out = torch.zeros_like(x)
+    for state, to in ((x, out), (x.conj(), out.conj())):
+        want = _reordered(state.resolve_conj(), parents)
+        ops.beam_reorder([state], parents, out=[to])
+        assert torch.equal(to.resolve_conj(), want)
+    for state, to in ((x.conj(), out), (x, out.conj())):
+        with pytest.raises(ValueError, match="conjugate"):
+            ops.beam_reorder([state], parents, out=[to])
+    view = x.conj()
+    want = _reordered(view.resolve_conj(), parents)
+    ops.beam_reorder([view], parents)
+    assert torch.equal(view.resolve_conj(), want)
