@@ -230,24 +230,31 @@ Strides strides_of(const Tensor& x, int64_t n, int64_t k, const char* what, Py_s
   s.end = s.p + (s.layers - 1) * s.l + (n - 1) * s.n + (k - 1) * s.k + s.row;
   return s;
 }
-// Whether two states share no byte, as far as can be told: one lies behind the other, or they are columns of the same rows.
+// Whether two states share no byte, as far as can be told: one lies behind the other, or they are columns of the same rows, whose strides nest.
 bool disjoint(const Strides& a, const Strides& b, int64_t n, int64_t k) {
   if (a.end <= b.p || b.end <= a.p) return true;
   const Strides &x = a.p <= b.p ? a : b, &y = a.p <= b.p ? b : a;
-  const int64_t d = y.p - x.p;
-  int64_t room = INT64_MAX;
+  struct Dim { int64_t stride, size; } dims[3];
+  int m = 0;
   if (x.layers > 1 || y.layers > 1) {
     if (x.layers != y.layers || x.l != y.l) return false;
-    room = std::min(room, x.l);
+    dims[m++] = {x.l, x.layers};
   }
   if (n > 1) {
     if (x.n != y.n) return false;
-    room = std::min(room, x.n);
+    dims[m++] = {x.n, n};
   }
   if (k > 1) {
     if (x.k != y.k) return false;
-    room = std::min(room, x.k);
+    dims[m++] = {x.k, k};
   }
+  std::sort(dims, dims + m, [](const Dim& p, const Dim& q) { return p.stride < q.stride; });
+  int64_t room = INT64_MAX, inner = 0;      // the least distance of two rows
+  for (int i = 0; i < m; ++i) {
+    room = std::min(room, dims[i].stride - inner);
+    inner += (dims[i].size - 1) * dims[i].stride;
+  }
+  const int64_t d = y.p - x.p;
   return d >= x.row && d + y.row <= room;
 }
 

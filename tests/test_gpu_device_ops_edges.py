@@ -329,3 +329,23 @@ def test_reorder_complex_states(ops):
     want = _reordered(view.resolve_conj(), parents)
     ops.beam_reorder([view], parents)
     assert torch.equal(view.resolve_conj(), want)
+
+
+def test_reorder_refuses_rows_whose_strides_do_not_nest(ops):
+    """Columns 0 and 1, and 4 to 7, of every tenth place in k and every 25th in n: the one's second sentence lies in the other's third beam.  Where the strides nest, in
+    any order of the dimensions and with the last row cut short, such columns are states of their own."""
+    rng = _rng(51)
+    flat = _cuda(rng.normal(0, 1, 200).astype(np.float32))
+    cut = lambda first, width, sn, sk: flat[first:].as_strided((2, 3, width), (sn, sk, 1))
+    parents = torch.tensor([[2, 0, 1], [1, 1, 0]], dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.beam_reorder([cut(0, 2, 25, 10), cut(4, 4, 25, 10)], parents)
+    for sn, sk in ((30, 10), (28, 10), (10, 20), (8, 16), (100, 9)):
+        a, b = cut(0, 2, sn, sk), cut(4, 4, sn, sk)
+        before, (wa, wb) = flat.clone(), [_reordered(x.clone(), parents) for x in (a, b)]
+        ops.beam_reorder([a, b], parents)
+        assert torch.equal(a, wa) and torch.equal(b, wb)
+        a.zero_(), b.zero_()
+        touched = flat != before
+        before[touched] = 0
+        assert torch.equal(flat, before)
