@@ -12,8 +12,10 @@
 //   code, goes off by a product of its own: the queries' sums with the keys' scales, and the weights' sums.  That is 5
 //   instructions for 8 codes where a code minus 8 in normal form takes 11, in a kernel bound by what it can issue.  Queries are scaled to
 //   fp16's upper range by a power of 2 for each row.  Weights are multiplied by their values' scales and rounded to fp16 (2^-11 each at most), with a power of 2
-//   that follows the scales, as the maximum follows the scores: the largest scale lies 2^3 above 1, and a weight 2^28 below the largest still counts.
-//   32-bit queries are two fp16 terms, and so are their weights: 2^-22 of each, or 2^-34 of the largest.  Their codes are made normal numbers less 8 (9
+//   for each row that follows its largest such product, as the maximum follows the scores: what lies far below is rounded to 2^-24 of the largest (2^-19 where that has
+//   fallen and the power has not followed yet).  A row's power follows from what it sees itself.  (One power for a warp's 16 rows that followed the largest scale and never
+//   came back was quicker with windows, 81 not 86 us for 64 paragraphs of 1 to 4001 positions, and lost rows whose values are 2^20 below those of another row, or of positions without weight.)
+//   32-bit queries are two fp16 terms, and so are their weights: 2^-22 of each, or 2^-30 (2^-25) of the largest.  Their codes are made normal numbers less 8 (9
 //   instructions for 8 codes): the matrix unit cuts addends off at a place that goes by their exponents, and subnormal operands lose up to 10 bits there, which
 //   an output rounded to 16 bits does not see but one of 32 does (2^-14 of a scale was seen).  (Three bf16 terms of each, exact to 2^-24: 18 sentences of
 //   6068 to 8725 positions with 10 beams and 28 heads of 64 in 168 us, not 155.)
@@ -36,7 +38,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 template <class T> constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;           // fp16 terms of a query and of a weight
 template <class T> constexpr float kSlack = sizeof(T) == 4 ? 2.f : 8.f;     // the reference maximum follows the true one only when it lags by 2^8 (2^2): few tiles rescale the sums
-template <class T> constexpr int kAbove = sizeof(T) == 4 ? 9 : 3;           // the largest scale, in powers of 2 above 1: with the slack and 2^4 of its own growth 2^15 at most
+template <class T> constexpr int kAbove = sizeof(T) == 4 ? 5 : -1;          // the largest weight times scale, in powers of 2 above 1
+constexpr int kRoom = 7;                                                    // and what a scale may be beside it, with a weight of up to 2^kSlack: 2^15 in all
+constexpr int kFall = 5;                                                    // and how far it falls before the power of 2 follows
+template <class T> constexpr float kFallen = sizeof(T) == 4 ? 1.f : 0.015625f;      // 2^(kAbove - kFall)
 
 struct AttendParams {
   const unsigned char* data;
@@ -528,9 +533,9 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend_kernel(co
     const bool huge = HOW == kExact && a.cap > kHugeCap;
     const float cap_by = huge ? 256.f : 1.f, cap_log2 = a.cap / cap_by * kLog2e, tanh_by = 0.5f / kLog2e * (huge ? 1.f / kHugeUp : 1.f);
 
-    // The values' sums are kept times 2^-24 where the codes are, and times the power of 2 that brings their scales into fp16's range.
-    float o[NG][4][4] = {}, extra[4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, size = 1.f;   // size: that power
-    uint32_t limit = 0;              // bits of the bf16 that no scale may reach with `size` as it is
+    // The values' sums are kept times 2^-24 where the codes are, and times a power of 2 for each row that brings its weights times scales into fp16's range.
+    float o[NG][4][4] = {}, extra[4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, size[2] = {0.f, 0.f};   // size: that power; 0: the row has none yet
+    uint32_t limit = 0xffffu;        // bits of the bf16 that no scale reaches whose weights are in range for certain, whatever they are
     int stage = 0;
     for (int i = 0; i < mine; ++i) {
       copy_wait<kPairStages - 2>();
@@ -632,20 +637,12 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend_kernel(co
         top[e] *= e ? r1 : r0;
       }
       const bool up0 = top[0] > m[0] + kSlack<T> || (m[0] == -INFINITY && top[0] > -INFINITY), up1 = top[1] > m[1] + kSlack<T> || (m[1] == -INFINITY && top[1] > -INFINITY);
+      float down[2] = {1.f, 1.f};           // what a row's sums are to be multiplied by (the first positions find sums of 0)
       if (__any_sync(~0u, up0 || up1)) {
-        const float f0 = up0 ? exp2_of(m[0] - top[0]) : 1.f, f1 = up1 ? exp2_of(m[1] - top[1]) : 1.f;
-        if (up0) m[0] = top[0];
-        if (up1) m[1] = top[1];
-        l[0] *= f0;
-        l[1] *= f1;
-        extra[0] *= f0; extra[2] *= f1;
-#pragma unroll
-        for (int gr = 0; gr < NG; ++gr)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            o[gr][e][0] *= f0; o[gr][e][1] *= f0;
-            o[gr][e][2] *= f1; o[gr][e][3] *= f1;
-          }
+        if (up0) { down[0] = m[0] == -INFINITY ? 1.f : exp2_of(m[0] - top[0]); m[0] = top[0]; }
+        if (up1) { down[1] = m[1] == -INFINITY ? 1.f : exp2_of(m[1] - top[1]); m[1] = top[1]; }
+        l[0] *= down[0];
+        l[1] *= down[1];
       }
 
       // values' scales of the lane's positions, two words for each of the four
@@ -655,35 +652,41 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend_kernel(co
         const unsigned char* const at = pair + (j >> 1) * kTileBytes + pages4::value_scales(D) + (8 * (j & 1) + 2 * c) * (2 * NG);
         if constexpr (NG == 4) *reinterpret_cast<uint4*>(vs[j]) = *reinterpret_cast<const uint4*>(at);
         else *reinterpret_cast<uint2*>(vs[j]) = *reinterpret_cast<const uint2*>(at);
-        if (edge) {            // a position that the lane's rows do not see may hold anything: 0 times its scale has to be 0
+      }
+      // A row's power of 2 takes the largest weight times scale that it sees to 2^kAbove and up to twice that.  It goes down when one would come to 2^15, which a scale of
+      // 2^kRoom times the largest may, and up with the maximum (by no more than that takes off the sums) when the largest has fallen to 2^-kFall of that: large values of
+      // positions that hardly count, or no longer, and of such as another row sees, take nothing from it.  It follows from the row's own weights and scales alone; the
+      // scales' extremes, of all that the lane's rows may see, only tell when to look.
+      bool look = false;
+      if (__any_sync(~0u, up0 || up1)) {
+        const int smaller = (int)(min(up0 ? __float_as_uint(size[0]) : ~0u, up1 ? __float_as_uint(size[1]) : ~0u) >> 23);      // (0: a row's first positions)
+        look = __any_sync(~0u, smaller == 0);
+        if (!look) {
+          __nv_bfloat162 least2 = __habs2(bf16_pair(vs[0][0]));
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i2 = 0; i2 < NG; ++i2) least2 = __hmin2(least2, __habs2(bf16_pair(vs[j][i2])));
+          const uint32_t least = min(*reinterpret_cast<const uint32_t*>(&least2) & 0xffffu, *reinterpret_cast<const uint32_t*>(&least2) >> 16);
+          look = (int)(least >> 7) <= 254 + kAbove<T> - kFall - smaller;
+        }
+      }
+      if (edge) {            // a position that the lane's rows do not see may hold anything: 0 times its scale has to be 0
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             if (x[j][e] == -INFINITY && x[j][e + 2] == -INFINITY) {
 #pragma unroll
               for (int i2 = 0; i2 < NG / 2; ++i2) vs[j][e * (NG / 2) + i2] = 0u;
             }
-        }
       }
-      // The power of 2 that takes the largest scale to 2^kAbove and up to twice that; it changes with a scale 2^4 times 2^kAbove.
       __nv_bfloat162 most2 = __habs2(bf16_pair(vs[0][0]));
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int i2 = 0; i2 < NG; ++i2) most2 = __hmax2(most2, __habs2(bf16_pair(vs[j][i2])));
       const uint32_t most = max(*reinterpret_cast<const uint32_t*>(&most2) & 0xffffu, *reinterpret_cast<const uint32_t*>(&most2) >> 16);
-      if (__any_sync(~0u, most >= limit)) {
-        const int e = min(max((int)(__reduce_max_sync(~0u, most) >> 7) - 127, -97), 103);
-        const float now = exp2_of((float)(kAbove<T> - e)), f = limit ? now / size : 1.f;
-        size = now;
-        limit = (uint32_t)min(e + 127 + 4, 255) << 7;
-        extra[0] *= f; extra[2] *= f;
-#pragma unroll
-        for (int gr = 0; gr < NG; ++gr)
-#pragma unroll
-          for (int e4 = 0; e4 < 4; ++e4)
-#pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4) o[gr][e4][i4] *= f;
-      }
       const float m0 = m[0] == -INFINITY ? 0.f : m[0], m1 = m[1] == -INFINITY ? 0.f : m[1];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -693,9 +696,57 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend_kernel(co
         x[j][3] = exp2_of(fmaf(x[j][3], r1, -m1));
         l[0] += x[j][0] + x[j][1];
         l[1] += x[j][2] + x[j][3];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[j][e] *= size;
       }
+      if (__any_sync(~0u, look || most >= limit)) {
+        limit = 0xffffu;
+        __nv_bfloat162 product2[2] = {bf16_pair(0u), bf16_pair(0u)};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t of[2];                        // largest scales of the two positions, by even and odd groups
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            __nv_bfloat162 at = __habs2(bf16_pair(vs[j][e * (NG / 2)]));
+            if constexpr (NG == 4) at = __hmax2(at, __habs2(bf16_pair(vs[j][2 * e + 1])));
+            of[e] = *reinterpret_cast<const uint32_t*>(&at);
+          }
+          const __nv_bfloat162 largest = __hmax2(bf16_pair(__byte_perm(of[0], of[1], 0x5410)), bf16_pair(__byte_perm(of[0], of[1], 0x7632)));
+#pragma unroll
+          for (int r = 0; r < 2; ++r) product2[r] = __hmax2(product2[r], __hmul2(__floats2bfloat162_rn(x[j][2 * r], x[j][2 * r + 1]), largest));
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const bool up = r ? up1 : up0;
+          float product = fmaxf(__low2float(product2[r]), __high2float(product2[r]));
+          product = fmaxf(product, __shfl_xor_sync(~0u, product, 1));      // (the row's four lanes)
+          product = fmaxf(product, __shfl_xor_sync(~0u, product, 2));
+          const float scaled = product * size[r];
+          const bool anew = size[r] == 0.f || scaled >= 32768.f;
+          const int was = (int)(__float_as_uint(size[r]) >> 23);
+          if (product > 0.f && (anew || (up && scaled < kFallen<T>))) {
+            int now = kAbove<T> + 254 - min(max((int)(__float_as_uint(product) >> 23), 127 - 97), 127 + 99);
+            if (!anew) now = max(was, min(now, was + 126 - (int)(__float_as_uint(down[r]) >> 23)));
+            if (was) down[r] *= __uint_as_float((uint32_t)max(127 + now - was, 0) << 23);
+            size[r] = __uint_as_float((uint32_t)now << 23);
+          }
+          // (a row that has seen scales of 0 only waits for another)
+          if (size[r] != 0.f) limit = min(limit, (uint32_t)min(254 + kAbove<T> + kRoom - (int)(__float_as_uint(size[r]) >> 23), 255) << 7);
+          else if (m[r] != -INFINITY) limit = 1u;
+        }
+      }
+      if (__any_sync(~0u, down[0] != 1.f || down[1] != 1.f)) {
+        extra[0] *= down[0]; extra[2] *= down[1];
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            o[gr][e][0] *= down[0]; o[gr][e][1] *= down[0];
+            o[gr][e][2] *= down[1]; o[gr][e][3] *= down[1];
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[j][e] *= size[e >> 1];
 
       // out += weights . values, a group of 32 components a time: its scales go into the weights
 #pragma unroll
@@ -739,15 +790,17 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend_kernel(co
       }
     }
 
-    // From the sums as they are kept to sums of values: times 1 / size, and with codes as they are less 8 for each and times 2^24.
-    const float by = (kOver ? 16777216.f : 1.f) / size;
+    // From the sums as they are kept to sums of values: times 1 / size, and with codes as they are less 8 for each and times 2^24.  (A row without a size has sums of 0.)
+    float by[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) by[r] = size[r] == 0.f ? 0.f : (kOver ? 16777216.f : 1.f) / size[r];
 #pragma unroll
     for (int gr = 0; gr < NG; ++gr) {
       const float e0 = kOver ? __shfl_sync(~0u, extra[0], (lane & ~3) | gr) : 0.f, e1 = kOver ? __shfl_sync(~0u, extra[2], (lane & ~3) | gr) : 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[gr][e][i] = fmaf(o[gr][e][i], kOver && (e & 1) ? 0.0625f : 1.f, -(i < 2 ? e0 : e1)) * by;
+        for (int i = 0; i < 4; ++i) o[gr][e][i] = fmaf(o[gr][e][i], kOver && (e & 1) ? 0.0625f : 1.f, -(i < 2 ? e0 : e1)) * by[i >> 1];
     }
     join_warps<T, D>(a, piece, job, smem, o, m, l);
   }

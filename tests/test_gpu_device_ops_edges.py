@@ -349,3 +349,84 @@ def test_reorder_refuses_rows_whose_strides_do_not_nest(ops):
         touched = flat != before
         before[touched] = 0
         assert torch.equal(flat, before)
+
+
+# ---- attention to values of very different sizes
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("dim,lens", [(64, [400, 90]), (128, [1500, 33])])
+def test_attend_does_not_feel_what_a_row_does_not_see(ops, dim, lens, dtype):
+    """Rows with windows of their own, among positions whose values are of any size: a row's result is the same, bit for bit, whatever the positions hold that it does not see."""
+    rng = _rng(dim, 52)
+    heads, g, page, n = 2, 6, 16, 2
+    pages, table, kk, vv = _memory(ops, rng, lens, heads, dim, page)
+    q = _q(rng, n, g, heads, dim, dtype)
+    tab, ln = _cuda(table), _cuda(np.array(lens, np.int32))
+    first, last = (torch.zeros(n, g, dtype=torch.int32, device="cuda") for _ in range(2))
+    for i, x in enumerate(lens):
+        cuts = np.linspace(0, x, g + 1).astype(np.int32)
+        first[i], last[i] = _cuda(cuts[:-1].copy()), _cuda(cuts[1:].copy())
+    call = lambda p: ops.attend_pages4(q, p, tab, ln, first=first, last=last, want_lse=True)
+    want, wl = call(pages)
+    slots = [_cuda(table[i, np.arange(x) // page].astype(np.int64) * page + np.arange(x) % page) for i, x in enumerate(lens)]
+    for row in range(g):
+        other = pages.clone()
+        for i, x in enumerate(lens):
+            at = np.ones(x, bool)
+            at[int(first[i, row]):int(last[i, row])] = False
+            size = 2.0 ** rng.integers(-40, 41, int(at.sum()))[:, None, None]
+            k, v = (_cuda((rng.normal(0, 1, (int(at.sum()), heads, dim)) * s).astype(np.float32)) for s in (1.0, size))
+            ops.write_pages4(other, slots[i][_cuda(at)], k, v)
+        got, lse = call(other)
+        assert torch.equal(got[:, row], want[:, row]) and torch.equal(lse[:, row], wl[:, row])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("where", ["first", "middle", "last", "falling", "rising"])
+def test_attend_large_values_of_positions_that_hardly_count(ops, where, dtype):
+    """Positions whose values are 2^24 (16-bit results) or 2^50 times the others' and whose weights make nothing of them, before, among and behind the others; and scores that
+    rise while values fall, so that the largest values so far no longer count."""
+    rng = _rng(len(where), 53)
+    heads, dim, page, length = 1, 64, 16, 330
+    big = 24 if dtype == F16 else 50
+    at = np.arange(length)
+    k, v = np.zeros((length, heads, dim), np.float32), rng.normal(0, 1, (length, heads, dim)).astype(np.float32)
+    score = rng.normal(0, 1, length)
+    if where in ("falling", "rising"):
+        step = at // 33                         # ten steps, at each of which values fall by 2^(big / 10) and scores rise by more, or the other way about
+        if where == "rising":
+            step = step[::-1]
+        score += step * 6.0
+        v *= (2.0 ** (12 - np.floor(step * big / 10.0))).astype(np.float32)[:, None, None]
+    else:
+        few = {"first": at < 3, "middle": (at > 150) & (at < 154), "last": at >= length - 3}[where]
+        score[few] = -60
+        v *= np.float32(2.0 ** -12)
+        v[few] *= np.float32(2.0 ** big)
+    k[:, 0, 0] = score
+    table = rng.permutation(25)[:21].reshape(1, 21).astype(np.int32)
+    slots = _cuda(table[0, at // page].astype(np.int64) * page + at % page)
+    pages = ops.new_pages4(25, heads, dim, page)
+    ops.write_pages4(pages, slots, _cuda(k), _cuda(v))
+    rk, rv = ops.read_pages4(pages, slots)
+    kk, vv = (np.zeros((25 * page, heads, dim), np.float32) for _ in range(2))
+    kk[slots.cpu().numpy()], vv[slots.cpu().numpy()] = rk.cpu().numpy(), rv.cpu().numpy()
+    q = torch.zeros(1, 2, 1, dim, device="cuda")
+    q[..., 0] = torch.tensor([[[1.0], [0.5]]], device="cuda")
+    q = q.to(dtype)
+    got = ops.attend_pages4(q, pages, _cuda(table), _cuda(np.array([length], np.int32)), scale=1.0)
+    want, wlse, wv, _, ws = attend_ref(q.double().cpu().numpy(), kk, vv, table, [length], page, 1.0, 0.0, None, None, None, None, 25)
+    # The score is one product and its change to a power of 2, a few roundings of up to 60 + 32; weights and products as in attend_check.  A weight times its scale is kept to 2^-25 in fp16 where the
+    # largest of them is 2^-5 (2^1 in 32-bit queries' second term) at least, so to 2^-20 (2^-26) of that, for each position, and goes with codes of up to 15 (8).
+    s = rk.double().cpu().numpy()[:, 0] @ q.double().cpu().numpy()[0, :, 0].T
+    w = np.exp(s - wlse[0, :, 0])
+    most = (w * np.abs(rv.cpu().numpy()[:, 0]).max(-1)[:, None] / 7).max(0)[None, :, None, None]
+    score = 8 * 2.0 ** -24 * 92
+    weight = 2.0 ** -22 if dtype == F32 else 2.0 ** -11
+    steps = length / 64 + 1
+    kept = 8 * 2.0 ** -26 * most * length if dtype == F32 else (steps * 17 + 8) * 2.0 ** -23 * 15 * ws + 15 * 2.0 ** -20 * most * length
+    tol = HALF_STEP[dtype] * np.abs(want) + (weight + 2 * score + 2.0 ** -15) * wv + kept + (2.0 ** -25 if dtype == F16 else 0)
+    g = got.double().cpu().numpy()
+    assert (np.abs(want).max((2, 3)) > 50 * tol.max((2, 3))).all()      # (the test can tell)
+    assert (np.abs(g - want) <= tol).all(), float((np.abs(g - want) / tol).max())
