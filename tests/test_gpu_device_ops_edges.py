@@ -430,3 +430,59 @@ def test_attend_large_values_of_positions_that_hardly_count(ops, where, dtype):
     g = got.double().cpu().numpy()
     assert (np.abs(want).max((2, 3)) > 50 * tol.max((2, 3))).all()      # (the test can tell)
     assert (np.abs(g - want) <= tol).all(), float((np.abs(g - want) / tol).max())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("cap", [0.0, 3.0, 500.0])
+def test_attend_negative_and_zero_scales(ops, cap, dtype):
+    """A scale of either sign is that of the queries; one of 0 makes every position alike."""
+    rng = _rng(54)
+    lens = [77, 1200]
+    pages, table, kk, vv = _memory(ops, rng, lens, 2, 64, 16)
+    q = _q(rng, 2, 3, 4, 64, dtype)
+    tab, ln = _cuda(table), _cuda(np.array(lens, np.int32))
+    for scale in (0.11, 2.0):
+        want = ops.attend_pages4(-q, pages, tab, ln, scale=scale, cap=cap, want_lse=True)
+        got = ops.attend_pages4(q, pages, tab, ln, scale=-scale, cap=cap, want_lse=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for scale in (0.0, -0.0):
+        attend_check(ops, q, pages, table, lens, kk, vv, 16, scale=scale, cap=cap)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("length", [1, 2, 16, 64, 256, 512])
+def test_attend_means_of_32_bits_are_exact(ops, length, dim):
+    """Queries of 0 make the mean of a power of two of values.  A value is an integer of four bits times a scale of eight, scales lie within 2^4 of each other: sums of 512 take 12 + 4 + 9
+    bits and a sign, so that nothing is rounded on the way in 32 bits."""
+    rng = _rng(length, dim, 55)
+    pages, table, kk, vv = _memory(ops, rng, [length, length], 2, dim, 16)
+    q = torch.zeros(2, 3, 2, dim, device="cuda")
+    got, lse = ops.attend_pages4(q, pages, _cuda(table), _cuda(np.array([length] * 2, np.int32)), want_lse=True)
+    at = np.arange(length)
+    for i in range(2):
+        mean = vv[table[i, at // 16].astype(np.int64) * 16 + at % 16].astype(np.float64).mean(0)
+        assert (got[i].double().cpu().numpy() == mean).all()
+    assert (np.abs(lse.double().cpu().numpy() - np.log(length)) <= 2.0 ** -22 * (1 + np.log(length))).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attend_few_positions_in_32_bits(ops, dim):
+    """One to three positions and queries of one component each: scores of up to 1 in a handful of roundings, so that what weights and products lose shows."""
+    rng = _rng(dim, 56)
+    lens, g, heads = [1, 2, 3, 3, 2], 16, 2
+    pages, table, kk, vv = _memory(ops, rng, lens, heads, dim, 16)
+    q = torch.zeros(5, g, heads, dim, device="cuda")
+    q.scatter_(3, _cuda(rng.integers(0, dim, (5, g, heads, 1))), _cuda(rng.uniform(-0.2, 0.2, (5, g, heads, 1)).astype(np.float32)))
+    got, lse = ops.attend_pages4(q, pages, _cuda(table), _cuda(np.array(lens, np.int32)), scale=1.0, want_lse=True)
+    want, wlse, wv, big, _ = attend_ref(q.double().cpu().numpy(), kk, vv, table, lens, 16, 1.0, 0.0, None, None, None, None, pages.shape[0])
+    assert big <= 1
+    largest = np.zeros(want.shape)
+    for i, x in enumerate(lens):
+        largest[i] = np.abs(vv[table[i, 0].astype(np.int64) * 16 + np.arange(x)]).max(0)
+    # A score: the query's two terms 2^-22, five roundings of 2^-24.  A weight: twice that (its own and the sum's), exp2 2^-22, its two terms 2^-22; two products of up to four
+    # addends, each cut off at 2^-23 of the largest; the sums' and the result's roundings, four of 2^-24.
+    score = 2.0 ** -22 + 5 * 2.0 ** -24
+    tol = (2 * score + 2 * 2.0 ** -22 + 8 * 2.0 ** -23 + 4 * 2.0 ** -24) * largest
+    err = np.abs(got.double().cpu().numpy() - want)
+    assert (err <= tol).all(), float((err / np.maximum(tol, 1e-300)).max())
+    assert (np.abs(lse.double().cpu().numpy() - wlse) <= 2 * score + 2.0 ** -21).all()
