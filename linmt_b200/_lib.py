@@ -100,7 +100,7 @@ def load():
     lib.linmt_score_batch.argtypes = [C.c_void_p] * 5 + [C.c_int32, C.c_void_p, C.c_void_p, C.c_int32]
     lib.linmt_op_error.restype = C.c_char_p
     for name in ("linmt_beam_select", "linmt_beam_reorder", "linmt_plan_pages", "linmt_write_pages4", "linmt_read_pages4", "linmt_attend_pages4"):
-        getattr(lib, name).argtypes = [C.c_char_p]     # the argument struct as packed bytes (device_ops)
+        getattr(lib, name).argtypes = [C.c_char_p]     # the argument struct as packed bytes (programs in Python fill it themselves; device_ops calls from C++)
     lib.linmt_attend_pages4_workspace.argtypes = [C.c_char_p]
     lib.linmt_attend_pages4_workspace.restype = C.c_int64
     _lib = lib

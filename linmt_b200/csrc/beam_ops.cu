@@ -1,7 +1,6 @@
 // beam_ops.cu -- beam selection and reordering on device tensors (linmt_beam_select, linmt_beam_reorder).
 #include <cooperative_groups.h>
 
-#include <atomic>
 #include <type_traits>
 
 #include "device_ops.h"

@@ -58,7 +58,6 @@ class OnDevice {
 inline bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 inline int dtype_bytes(int dtype) { return dtype == LINMT_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == LINMT_F32 || dtype == LINMT_BF16 || dtype == LINMT_F16; }
-constexpr int kOpMaxDevices = 64;
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }

@@ -21,7 +21,6 @@
 //   6068 to 8725 positions with 10 beams and 28 heads of 64 in 168 us, not 155.)
 // Every warp has a ring of tiles of its own (cp.async, no barrier among warps) and its own maximum and sums; the CTA's four are
 // joined through shared memory at the end of a piece of work, and where a sentence's positions are shared by CTAs a second kernel joins those.
-#include <atomic>
 #include <cmath>
 
 #include "device_ops.h"
@@ -873,19 +872,14 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
 }
 
 template <class T, int D>
-cudaError_t launch_attend(const AttendParams& p, int blocks, int device, cudaStream_t st) {
+cudaError_t launch_attend(const AttendParams& p, int blocks, cudaStream_t st) {
   constexpr int smem = attend_smem<T, D>();
   const Scores how = p.cap == 0.f && !p.slope && p.scale != 0.f ? kPlain : sizeof(T) == 4 || p.cap > kQuickCap ? kExact : kQuick;
   void (*kernel)(AttendParams) = how == kPlain ? attend_kernel<T, D, kPlain> : attend_kernel<T, D, kExact>;
   if constexpr (sizeof(T) == 2) {
     if (how == kQuick) kernel = attend_kernel<T, D, kQuick>;
   }
-  static std::atomic<bool> opted_in[kOpMaxDevices][3] = {};
-  if (smem + 1024 > 48 << 10 && !opted_in[device][how].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    opted_in[device][how].store(true, std::memory_order_release);
-  }
+  static_assert(smem + 2048 <= 48 << 10, "more shared memory has to be asked for");
   kernel<<<(unsigned)blocks, kWarps * 32, smem, st>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || !p.ws) return e;
@@ -954,7 +948,6 @@ int linmt_attend_pages4(const linmt_attend_pages4_args* g) {
   const int64_t need = workspace_of(g);
   if (need && (!g->workspace || g->workspace_bytes < need || !aligned(g->workspace, 16)))
     return op_fail(LINMT_EINVAL, "attend_pages4: a workspace of %lld bytes is needed, 16-byte aligned", (long long)need);
-  if (g->device < 0 || g->device >= kOpMaxDevices) return op_fail(LINMT_EINVAL, "attend_pages4: device = %d", g->device);
   OnDevice on(g->device);
   if (on.err != cudaSuccess) return op_cuda(on.err, "attend_pages4");
   AttendParams p{static_cast<const unsigned char*>(g->pages.data), g->pages.stride_page, g->pages.stride_head, g->pages.n_pages, g->pages.heads, g->pages.page,
@@ -968,9 +961,9 @@ int linmt_attend_pages4(const linmt_attend_pages4_args* g) {
   const cudaStream_t st = static_cast<cudaStream_t>(g->stream);
   cudaError_t e;
   if (g->pages.dim == 64)
-    e = g->dtype == LINMT_F32 ? launch_attend<float, 64>(p, blocks, g->device, st) : g->dtype == LINMT_BF16 ? launch_attend<__nv_bfloat16, 64>(p, blocks, g->device, st) : launch_attend<__half, 64>(p, blocks, g->device, st);
+    e = g->dtype == LINMT_F32 ? launch_attend<float, 64>(p, blocks, st) : g->dtype == LINMT_BF16 ? launch_attend<__nv_bfloat16, 64>(p, blocks, st) : launch_attend<__half, 64>(p, blocks, st);
   else
-    e = g->dtype == LINMT_F32 ? launch_attend<float, 128>(p, blocks, g->device, st) : g->dtype == LINMT_BF16 ? launch_attend<__nv_bfloat16, 128>(p, blocks, g->device, st) : launch_attend<__half, 128>(p, blocks, g->device, st);
+    e = g->dtype == LINMT_F32 ? launch_attend<float, 128>(p, blocks, st) : g->dtype == LINMT_BF16 ? launch_attend<__nv_bfloat16, 128>(p, blocks, st) : launch_attend<__half, 128>(p, blocks, st);
   return e == cudaSuccess ? LINMT_OK : op_cuda(e, "attend_pages4");
 }
 

@@ -1,7 +1,5 @@
 // pages4_ops.cu -- pages for growing sentences, keys and values in them in 4 bits (linmt_plan_pages, linmt_write_pages4,
 // linmt_read_pages4).  Attention over them: pages4_attend.cu.
-#include <atomic>
-
 #include "device_ops.h"
 #include "pages4.h"
 
@@ -278,7 +276,7 @@ __device__ __forceinline__ Rows rows_of_cta(const RowsParams& a) {
   const int tid = threadIdx.x;
   const int64_t first = (int64_t)blockIdx.x * 16, most = (int64_t)a.n_pages * a.page;
   auto place = [&](int64_t slot) {
-    const int64_t page = slot / a.page;
+    const int64_t page = pages4::slot_page(slot, a.n_pages, a.page);
     return page * a.stride_page + (int)(slot - page * a.page) / pages4::kTile * (int64_t)BYTES;
   };
   if (tid < 16 + 2 * kReach) {
