@@ -3,8 +3,8 @@
 //   out = sum_t softmax_t(f(scale q . k_t)) v_t,   k_t = sk (codes - 8), v_t = sv (codes - 8) by groups of 32 components
 //
 // A sentence's beams, and the query heads that share a head of the pool, read the same positions: up to 16 rows are the left
-// operand of mma.m16n8k16, so every code is loaded and unpacked once for all of them.  (tcgen05.mma wants both operands of at least 64
-// rows, and codes unpacked into shared memory first; with 16 rows the unpacking, not the product, is what takes the time.)
+// operand of mma.m16n8k16, so every code is loaded and unpacked once for all of them.  (tcgen05.mma could have 128 positions on the left and the
+// 16 rows as its N, but wants the codes unpacked and stored first, into shared memory or TMEM; the unpacking, not the product, is what takes the time.  Not built.)
 //   Scales stay out of the products: a key's is multiplied onto its group's sum, a value's into the weight on the left.
 //   A word's codes become matrix operands with one AND each: an integer in the low bits of an
 //   fp16 number is a subnormal one, that integer times 2^-24, and stays so up to 2047, so every second
@@ -14,7 +14,8 @@
 //   fp16's upper range by a power of 2 for each row.  Weights are multiplied by their values' scales and rounded to fp16 (2^-11 each at most), with a power of 2
 //   for each row that follows its largest such product, as the maximum follows the scores: what lies far below is rounded to 2^-24 of the largest (2^-19 where that has
 //   fallen and the power has not followed yet).  A row's power follows from what it sees itself.  (One power for a warp's 16 rows that followed the largest scale and never
-//   came back was quicker with windows, 81 not 86 us for 64 paragraphs of 1 to 4001 positions, and lost rows whose values are 2^20 below those of another row, or of positions without weight.)
+//   came back was quicker with windows, 78 not 83 us for 64 paragraphs
+//   of 1 to 4001 positions, and lost rows whose values are 2^20 below those of another row, or of positions without weight.)
 //   32-bit queries are two fp16 terms, and so are their weights: 2^-22 of each, or 2^-30 (2^-25) of the largest.  Their codes are made normal numbers less 8 (9
 //   instructions for 8 codes): the matrix unit cuts addends off at a place that goes by their exponents, and subnormal operands lose up to 10 bits there, which
 //   an output rounded to 16 bits does not see but one of 32 does (2^-14 of a scale was seen).  (Three bf16 terms of each, exact to 2^-24: 18 sentences of
@@ -147,7 +148,7 @@ __device__ __forceinline__ void write_row(const AttendParams& a, int sent, int k
 // are known on the device only, so every CTA adds them up itself.  A segment counts as kFixed units more than it has pairs, its fixed costs being as large,
 // and as kLeast at least; one of up to kLeast + kFixed units or an eighth of a part is not cut: the CTA that has its first unit takes it whole.
 constexpr int kLeast = 8;
-constexpr int kFixed = 12;      // (64 paragraphs of 1 to 4001 positions: 93, 86, 82, 78 us with 6, 8, 10, 12)
+constexpr int kFixed = 12;      // (64 paragraphs of 1 to 4001 positions: 91, 87, 83, 84, 85, 87 us with 8, 10, 12, 14, 16, 20)
 struct Share {
   int64_t begin, end;      // the CTA's units
   int64_t first;           // number of the first unit of sentence `sent`
@@ -807,7 +808,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend_kernel(co
 }
 
 // Joins the parts of the segment that ends in a CTA's share and began in one before: a CTA for each of attend's.  A thread has four components of a row, in one of kBy
-// parts in turn.  (Four CTAs with four rows each: 64 paragraphs of 1 to 4001 positions in 87 us, not 79.)
+// parts in turn.  (Four CTAs with four rows each: 64 paragraphs of 1 to 4001 positions took 8 us longer.)
 constexpr int kJoinThreads = 512;
 template <class T, int D>
 __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_constant__ AttendParams a, int blocks) {

@@ -47,6 +47,9 @@ def beam_select(logits, scores, *, done=None, allowed=None, eos=1, out=None):
     ``eos`` with its score as it is.  ``allowed`` [1 or n, ceil(vocab / 32)] int32: bit v % 32 of word v / 32 is set where word v may
     be chosen (the others do not enter the softmax and may hold anything).  A beam with a NaN or +inf at an allowed place offers nothing.
 
+    Ranks are those of 64-bit sums (to 2^-36).  The scores returned carry a normaliser that is summed in 32 bits unless a rank depended on it: good to 6e-6, and 6e-8 for
+    every 512 32-bit (1024 16-bit) words that a warp reads.  A stretch whose largest logit is 64 or more in size is read twice, its 6e-8 are 5e-7.
+
     Returns ``tokens``, ``parents`` [n, k] int32, ``scores`` [n, k] float32 and ``done`` [n, k] bool (the parent was finished, or the token is
     ``eos``).  A slot for which nothing is left has token eos, itself as the parent, -inf and True.  ``out``: a tuple of four such tensors to
     write into; they may be ``scores`` and ``done`` themselves, and overlap nothing else that the call reads."""
@@ -67,8 +70,8 @@ def plan_pages(old, new, table, free, used, *, page, total):
     """Pages and slots for sentences that grow from ``old`` to ``new`` positions ([n] int32; ``old`` None: from nothing).
 
     Every page column p of sentence i with ceil(old / page) <= p < ceil(new / page) of ``table`` [n, width] int32 gets the next entry of ``free`` [n_free] int32, of
-    which ``used`` [1] int32 are taken already; ``table`` is written in place, and overlaps none of the others.  Returns ``slots`` [total] int64 (table[i, pos // page] * page + pos % page of each
-    new position, sentence by sentence, -1 behind the last), ``starts`` [n + 1] int32 (each sentence's first in ``slots``) and the new ``used`` [1].
+    which ``used`` [1] int32 are taken already; ``table`` is written in place, and overlaps none of the others.  Returns ``slots`` [total] int64
+    (table[i, pos // page] * page + pos % page of each new position, sentence by sentence, -1 behind the last), ``starts`` [n + 1] int32 (each sentence's first in ``slots``) and the new ``used`` [1].
     Where the free list has run out a column and its slots are -1 and ``used`` comes back larger than n_free.  Lengths are taken as 0 .. width * page, a
     shorter ``new`` as ``old``."""
     return _front.plan_pages(old, new, table, free, used, page, total)
@@ -100,8 +103,8 @@ def attend_pages4(q, pages, table, lens, *, scale=None, cap=0.0, slope=None, cen
     ``q`` [n, g, heads, dim] (float32, bfloat16 or float16, components contiguous); query head h reads head h // (heads / pool heads).  ``table`` [n, width] int32
     names each sentence's pages, ``lens`` [n] int32 its positions.  ``scale``: dim ** -0.5 if None.  ``cap`` > 0: scores are cap * tanh(s / cap).  ``slope``
     [heads] with ``centre`` [n, g], float32: scores lose slope * |position - centre|.  ``first``, ``last`` [n, g] int32: a row sees positions
-    first <= t < last only.  Positions in a column that names no page of the pool are not seen.  A row that sees nothing gets zeros and lse -inf,
-    one whose query has a NaN or an infinity gets NaN in both.
+    first <= t < last only, and what others hold changes nothing of its result.  Positions in a column that names no page of the pool are not seen.  A row that
+    sees nothing gets zeros and lse -inf, one whose query has a NaN or an infinity gets NaN in both.
 
     Returns ``out`` like q (it may be q itself, and overlaps nothing else that the call reads), and with ``want_lse`` also the log of the row's sum of exponentials, [n, g, heads] float32."""
     return _front.attend_pages4(q, pages, table, lens, scale, cap, slope, centre, first, last, out, want_lse)
