@@ -430,8 +430,9 @@ int linmt_read_pages4(const linmt_pages4_rows_args* args);
  *   out = sum over seen of softmax(s) * v_t; lse = log sum over seen of exp(s).  Nothing seen: 0 and -inf.  A query with a NaN or an infinity that
  *   sees something: NaN and NaN.
  * `len` beyond width * page is taken as that.  Sums are held in 32 bits.  Weights times scales are
- * rounded to fp16, with a power of 2 for each row that follows the largest of them (2^-97 to 2^99): to 2^-11 of each, or 2^-19 of the row's largest so far; for 32-bit queries,
- * which are multiplied as two fp16 terms, they are two such terms too: 2^-22, or 2^-25.  With 16-bit queries a cap is good to 3e-7 of itself up to 64, to 2^-21 of a score above.
+ * rounded to fp16, with a power of 2 for each row that follows the largest of them (2^-97 to 2^99): to 2^-11 of each, or 2^-21 of the row's largest so far; for 32-bit queries,
+ * which are multiplied as two fp16 terms, they are two such terms too: 2^-22, or 2^-31.  With 16-bit queries the matrix unit cuts the sums off at some 2^-13 of the weighted
+ * mean of a component's scales (2^-16 of its group's largest).  With 16-bit queries a cap is good to 3e-7 of itself up to 64, to 2^-21 of a score above.
  * `workspace`: linmt_attend_pages4_workspace bytes, 16-byte aligned, the call's own until it has run; NULL where that is 0. */
 typedef struct linmt_attend_pages4_args {
   uint32_t size;

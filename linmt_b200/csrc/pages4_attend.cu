@@ -12,11 +12,11 @@
 //   code, goes off by a product of its own: the queries' sums with the keys' scales, and the weights' sums.  That is 5
 //   instructions for 8 codes where a code minus 8 in normal form takes 11, in a kernel bound by what it can issue.  Queries are scaled to
 //   fp16's upper range by a power of 2 for each row.  Weights are multiplied by their values' scales and rounded to fp16 (2^-11 each at most), with a power of 2
-//   for each row that follows its largest such product, as the maximum follows the scores: what lies far below is rounded to 2^-24 of the largest (2^-19 where that has
+//   for each row that follows its largest such product, as the maximum follows the scores: what lies far below is rounded to 2^-26 of the largest (2^-21 where that has
 //   fallen and the power has not followed yet).  A row's power follows from what it sees itself.  (One power for a warp's 16 rows that followed the largest scale and never
 //   came back was quicker with windows, 78 not 83 us for 64 paragraphs
 //   of 1 to 4001 positions, and lost rows whose values are 2^20 below those of another row, or of positions without weight.)
-//   32-bit queries are two fp16 terms, and so are their weights: 2^-22 of each, or 2^-30 (2^-25) of the largest.  Their codes are made normal numbers less 8 (9
+//   32-bit queries are two fp16 terms, and so are their weights: 2^-22 of each, or 2^-34 (2^-31) of the largest.  Their codes are made normal numbers less 8 (9
 //   instructions for 8 codes): the matrix unit cuts addends off at a place that goes by their exponents, and subnormal operands lose up to 10 bits there, which
 //   an output rounded to 16 bits does not see but one of 32 does (2^-14 of a scale was seen).  (Three bf16 terms of each, exact to 2^-24: 18 sentences of
 //   6068 to 8725 positions with 10 beams and 28 heads of 64 in 168 us, not 155.)
@@ -38,10 +38,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 template <class T> constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;           // fp16 terms of a query and of a weight
 template <class T> constexpr float kSlack = sizeof(T) == 4 ? 2.f : 8.f;     // the reference maximum follows the true one only when it lags by 2^8 (2^2): few tiles rescale the sums
-template <class T> constexpr int kAbove = sizeof(T) == 4 ? 5 : -1;          // the largest weight times scale, in powers of 2 above 1
-constexpr int kRoom = 7;                                                    // and what a scale may be beside it, with a weight of up to 2^kSlack: 2^15 in all
-constexpr int kFall = 5;                                                    // and how far it falls before the power of 2 follows
-template <class T> constexpr float kFallen = sizeof(T) == 4 ? 1.f : 0.015625f;      // 2^(kAbove - kFall)
+template <class T> constexpr int kAbove = sizeof(T) == 4 ? 9 : 1;           // the largest weight times scale, in powers of 2 above 1
+template <class T> constexpr int kRoom = sizeof(T) == 4 ? 3 : 5;            // and what a scale may be beside it, with a weight of up to 2^kSlack: 2^14 in all
+template <class T> constexpr int kFall = sizeof(T) == 4 ? 3 : 5;            // and how far it falls before the power of 2 follows
+template <class T> constexpr float kFallen = sizeof(T) == 4 ? 64.f : 0.0625f;      // 2^(kAbove - kFall)
 
 struct AttendParams {
   const unsigned char* data;
@@ -668,7 +668,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend_kernel(co
 #pragma unroll
             for (int i2 = 0; i2 < NG; ++i2) least2 = __hmin2(least2, __habs2(bf16_pair(vs[j][i2])));
           const uint32_t least = min(*reinterpret_cast<const uint32_t*>(&least2) & 0xffffu, *reinterpret_cast<const uint32_t*>(&least2) >> 16);
-          look = (int)(least >> 7) <= 254 + kAbove<T> - kFall - smaller;
+          look = (int)(least >> 7) <= 254 + kAbove<T> - kFall<T> - smaller;
         }
       }
       if (edge) {            // a position that the lane's rows do not see may hold anything: 0 times its scale has to be 0
@@ -729,7 +729,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend_kernel(co
             size[r] = __uint_as_float((uint32_t)now << 23);
           }
           // (a row that has seen scales of 0 only waits for another)
-          if (size[r] != 0.f) limit = min(limit, (uint32_t)min(254 + kAbove<T> + kRoom - (int)(__float_as_uint(size[r]) >> 23), 255) << 7);
+          if (size[r] != 0.f) limit = min(limit, (uint32_t)min(254 + kAbove<T> + kRoom<T> - (int)(__float_as_uint(size[r]) >> 23), 255) << 7);
           else if (m[r] != -INFINITY) limit = 1u;
         }
       }

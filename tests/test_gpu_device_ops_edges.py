@@ -486,3 +486,31 @@ def test_attend_few_positions_in_32_bits(ops, dim):
     err = np.abs(got.double().cpu().numpy() - want)
     assert (err <= tol).all(), float((err / np.maximum(tol, 1e-300)).max())
     assert (np.abs(lse.double().cpu().numpy() - wlse) <= 2 * score + 2.0 ** -21).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attend_small_weights_in_32_bits(ops, dim):
+    """A position that has nearly all the weight and components of 0, and others of 2^-17 of its weight, which are all that those components have: a weight times scale is kept to
+    2^-34 of the row's largest."""
+    rng = _rng(dim, 57)
+    length, page, heads = 6, 16, 2
+    k, v = np.zeros((length, heads, dim), np.float32), rng.normal(0, 1, (length, heads, dim)).astype(np.float32)
+    k[:, :, 0] = -12
+    k[3, :, 0] = 0
+    zero = rng.random((heads, dim)) < 0.5
+    zero[:, ::32] = False
+    v[3][zero] = 0
+    pages, slots = ops.new_pages4(1, heads, dim, page), torch.arange(length, device="cuda")
+    ops.write_pages4(pages, slots, _cuda(k), _cuda(v))
+    kk, vv = (np.zeros((page, heads, dim), np.float32) for _ in range(2))
+    rk, rv = ops.read_pages4(pages, slots)
+    kk[:length], vv[:length] = rk.cpu().numpy(), rv.cpu().numpy()
+    q = torch.zeros(1, 5, heads, dim, device="cuda")
+    q[..., 0] = torch.linspace(0.9, 1.1, 5, device="cuda")[None, :, None]
+    table = np.zeros((1, 1), np.int32)
+    got = ops.attend_pages4(q, pages, _cuda(table), _cuda(np.array([length], np.int32)), scale=1.0).double().cpu().numpy()
+    want, _, wv, _, _ = attend_ref(q.double().cpu().numpy(), kk, vv, table, [length], page, 1.0, 0.0, None, None, None, None, 1)
+    # Scores of up to 13.2 are good to 2^-22 and six roundings of 2^-24, weights to twice that and 2^-21, sums of 12 products to 12 cut-offs of 2^-23: 2^-16 in all.
+    scale = np.abs(v[3]).reshape(heads, -1, 32).max(-1).max(-1) / 8 * (1 + 2.0 ** -8)
+    tol = 2.0 ** -16 * wv + (length - 1) * 8 * 2.0 ** -34 * scale[None, None, :, None]
+    assert (vv[3][zero] == 0).all() and (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / np.maximum(tol, 1e-300)).max())
