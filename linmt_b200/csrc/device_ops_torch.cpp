@@ -118,7 +118,7 @@ bool meets(const char* base, const int64_t* size, const int64_t* stride, int dim
 }
 bool meets(const Tensor& t, const Span& s) {
   const Span all = span_of(t);
-  if (s.p == s.end || all.end <= s.p || s.end <= all.p) return false;
+  if (t.numel() == 0 || s.p == s.end || all.end <= s.p || s.end <= all.p) return false;
   int64_t size[8], stride[8];
   int dims = 0;
   for (int64_t i = 0; i < t.dim(); ++i) {

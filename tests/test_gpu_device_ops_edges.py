@@ -514,3 +514,11 @@ def test_attend_small_weights_in_32_bits(ops, dim):
     scale = np.abs(v[3]).reshape(heads, -1, 32).max(-1).max(-1) / 8 * (1 + 2.0 ** -8)
     tol = 2.0 ** -16 * wv + (length - 1) * 8 * 2.0 ** -34 * scale[None, None, :, None]
     assert (vv[3][zero] == 0).all() and (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / np.maximum(tol, 1e-300)).max())
+
+
+def test_plan_takes_a_table_without_columns_in_the_midst_of_what_it_reads(ops):
+    """A table of no columns has no place that could be written, wherever it points."""
+    buf = torch.tensor([0, 0, 0, 0, 11, 12, 13, 14, 15, 16, 17, 18, 0], dtype=torch.int32, device="cuda")
+    table = buf[6:].as_strided((4, 0), (1, 1))
+    slots, starts, used = ops.plan_pages(None, torch.full((4,), 5, dtype=torch.int32, device="cuda"), table, buf[4:12], buf[12:], page=16, total=2)
+    assert slots.tolist() == [-1, -1] and starts.tolist() == [0] * 5 and used.tolist() == [0]
