@@ -428,7 +428,7 @@ int linmt_read_pages4(const linmt_pages4_rows_args* args);
  *   s = scale * q . k_t;  cap > 0: s = cap * tanh(s / cap);  slope: s -= slope[h] * |t - centre[i][row]|
  *   seen: first[i][row] <= t < last[i][row] (NULL: all), 0 <= t < len[i], and the table names a page of the pool
  *   out = sum over seen of softmax(s) * v_t; lse = log sum over seen of exp(s).  Nothing seen: 0 and -inf.  A query with a NaN or an infinity that
- *   sees something: NaN and NaN.
+ *   sees something: NaN and NaN (and so may one above 1e33 in size, whose scores leave 32 bits on the way).
  * `len` beyond width * page is taken as that.  Sums are held in 32 bits.  Weights times scales are
  * rounded to fp16, with a power of 2 for each row that follows the largest of them (2^-97 to 2^99): to 2^-11 of each, or 2^-21 of the row's largest so far; for 32-bit queries,
  * which are multiplied as two fp16 terms, they are two such terms too: 2^-22, or 2^-31.  With 16-bit queries the matrix unit cuts the sums off at some 2^-13 of the weighted

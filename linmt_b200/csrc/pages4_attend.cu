@@ -485,6 +485,7 @@ __global__ void __launch_bounds__(kWarps * 32, D == 64 ? 4 : 3) attend_kernel(co
         const int up = most > 0.f && most < INFINITY ? 9 - max(-100, ilogbf(most)) : 0;      // -118 .. 109
         const float by = ldexpf(a.scale < 0.f ? -1.f : 1.f, up);
         mul[r] = ldexpf(a.mul, a.mul_up + (kOver ? 24 : 0) - up);
+        if (HOW == kPlain) mul[r] = fmaxf(mul[r], 1.4e-45f);      // (not 0: what is not seen is -inf times this)
         if (warp < NG) {
           float sum = 0.f;
 #pragma unroll

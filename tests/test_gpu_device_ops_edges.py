@@ -522,3 +522,14 @@ def test_plan_takes_a_table_without_columns_in_the_midst_of_what_it_reads(ops):
     table = buf[6:].as_strided((4, 0), (1, 1))
     slots, starts, used = ops.plan_pages(None, torch.full((4,), 5, dtype=torch.int32, device="cuda"), table, buf[4:12], buf[12:], page=16, total=2)
     assert slots.tolist() == [-1, -1] and starts.tolist() == [0] * 5 and used.tolist() == [0]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("scale", [1e-13, 1e-30, 1e-44])
+def test_attend_scores_below_the_smallest_number(ops, scale, dtype):
+    """Queries and a scale so small that their product is no number of 32 bits any more: the scores are 0, and positions behind the text stay unseen."""
+    rng = _rng(58)
+    lens = [23, 700]
+    pages, table, kk, vv = _memory(ops, rng, lens, 2, 64, 16)
+    q = _q(rng, 2, 3, 2, 64, F32).mul_(1e-30).to(dtype)
+    attend_check(ops, q, pages, table, lens, kk, vv, 16, scale=scale)
