@@ -14,8 +14,8 @@
 //   fp16's upper range by a power of 2 for each row.  Weights are multiplied by their values' scales and rounded to fp16 (2^-11 each at most), with a power of 2
 //   for each row that follows its largest such product, as the maximum follows the scores: what lies far below is rounded to 2^-26 of the largest (2^-21 where that has
 //   fallen and the power has not followed yet).  A row's power follows from what it sees itself.  (One power for a warp's 16 rows that followed the largest scale and never
-//   came back was quicker with windows, 78 not 83 us for 64 paragraphs
-//   of 1 to 4001 positions, and lost rows whose values are 2^20 below those of another row, or of positions without weight.)
+//   came back was quicker with windows, 78 not 83 us for 64 paragraphs of 1 to 4001 positions, and lost rows whose values are 2^20 below those of another row, or of
+//   positions without weight.)
 //   32-bit queries are two fp16 terms, and so are their weights: 2^-22 of each, or 2^-34 (2^-31) of the largest.  Their codes are made normal numbers less 8 (9
 //   instructions for 8 codes): the matrix unit cuts addends off at a place that goes by their exponents, and subnormal operands lose up to 10 bits there, which
 //   an output rounded to 16 bits does not see but one of 32 does (2^-14 of a scale was seen).  (Three bf16 terms of each, exact to 2^-24: 18 sentences of
@@ -122,7 +122,8 @@ template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.
 __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// Four components of row `at` of a sentence's head of the pool, and with the first the log of its weight.  A weight of 0: nothing was seen; of NaN (a query that is not finite): so are the row and the log.
+// Four components of row `at` of a sentence's head of the pool, and with the first the log of its weight.  A weight of 0:
+// nothing was seen; of NaN (a query that is not finite): so are the row and the log.
 template <class T>
 __device__ __forceinline__ void write_row(const AttendParams& a, int sent, int kvh, int at, int d, const float4& sum, float top, float weight) {
   const int g = at / a.rep, h = kvh * a.rep + at - g * a.rep;
