@@ -305,7 +305,7 @@ int linmt_gemm_f32_noalloc(const float* d_x, const float* d_wt, float* d_y, int3
 /* ------------------------------------------------------------------------------------
  * 4. Operators on device tensors, for programs that run their own model and want a decoding step's
  *    parts: beam selection and reordering, pages for a growing memory, keys and values in them in
- *    4 bits, attention over them.  They have no counterpart in the reference, whose beam search runs on the
+ *    4 or 8 bits, attention over them, pages that follow their hypotheses, scores of given tokens.  They have no counterpart in the reference, whose beam search runs on the
  *    host (src/decoder.h:340-525) and whose attention reads dense states.
  *
  *    Every pointer inside the argument structs is a DEVICE pointer on `device`, every stride is in elements unless
@@ -458,6 +458,167 @@ typedef struct linmt_attend_pages4_args {
 } linmt_attend_pages4_args;
 int64_t linmt_attend_pages4_workspace(const linmt_attend_pages4_args* args);   /* bytes, or -1: see linmt_op_error */
 int linmt_attend_pages4(const linmt_attend_pages4_args* args);
+
+/* A pool of pages in 8 bits: [n_pages][heads][page / 16] blocks of 32 * dim + 16 bytes (dim 64 or 128, page a multiple of 16), 16-byte
+ * aligned.  A block holds 16 positions of one head:
+ *   16 dim bytes of key codes: position t, component c is byte (t / 8) * 8 dim + (c / 16) * 128 + (t % 8) * 16 + c % 16
+ *   16 dim bytes of value codes: byte 16 c + t
+ *   the keys' scale and the values' scale, float, and 8 bytes of zeros
+ * A code is a signed byte, -127 .. 127, and stands for code * scale.  A scale is 4, 5, 6 or 7 times a power of 2, 2^-126 at least, or 0. */
+typedef struct linmt_pages8 {
+  void* data;
+  int64_t stride_page, stride_head;   /* bytes, multiples of 16; the blocks of a page's head are contiguous */
+  int32_t n_pages, heads, page, dim;
+} linmt_pages8;
+
+/* Keys and values of `t` positions into (write) or out of (read) the slots of a pool.  A slot outside 0 .. n_pages * page - 1 is not written, and reads
+ * as zeros.  A write goes by runs: neighbours in `slots` that are neighbours in a block, ascending, as linmt_plan_pages gives them.
+ *   A run that begins at a block's first position makes the block new: its scale is the run's.  One that begins further on keeps the
+ *   positions before it, and the block's scale if it reaches the run's; otherwise the run's becomes the block's and earlier codes are rounded to it: c = code * old / new.
+ *   Positions of the block behind the run become zeros.
+ *   The run's scale is the smallest whose 127-fold reaches its largest component in size, of the keys and the values each; code = component /
+ *   scale, a quotient in 32 bits rounded to the nearest integer, to even between two.  NaN is taken as 0, sizes above 2^127 as 2^127.  Scale 0: code 0.
+ * What two runs of one call in the same block leave there is not defined.  What is written overlaps nothing that is read. */
+typedef struct linmt_pages8_rows_args {
+  uint32_t size;
+  int32_t device;
+  void* stream;
+  linmt_pages8 pages;
+  const int64_t* slots;      /* [t] */
+  void* k;                   /* [t][heads][dim], components contiguous; 16-byte aligned rows */
+  void* v;
+  int64_t k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  int32_t t, dtype;
+} linmt_pages8_rows_args;
+int linmt_write_pages8(const linmt_pages8_rows_args* args);
+int linmt_read_pages8(const linmt_pages8_rows_args* args);
+
+/* Attention of g query rows per sentence over the sentence's positions in a pool of 8-bit pages, as linmt_attend_pages4 with one argument more:
+ *   seen: t < sinks or first[i][row] <= t < last[i][row] (NULL: all), 0 <= t < len[i], and the table names a page of the pool
+ * A query's components are taken to 2^-23 of its row's largest, scores are exact products of those and the codes in 32 bits, weights times scales are
+ * taken to 2^-31 of a row's largest, and summed exactly.  A query with a NaN or an infinity that sees something: NaN and NaN; so may one whose scores leave 32 bits. */
+typedef struct linmt_attend_pages8_args {
+  uint32_t size;
+  int32_t device;
+  void* stream;
+  linmt_pages8 pages;
+  const void* q;             /* [n][g][heads][dim], components contiguous, aligned to their type */
+  int64_t q_stride_n, q_stride_g, q_stride_h;
+  void* out;                 /* as q, strides of its own; q itself with q's strides, or apart from it; apart from all else that is read */
+  int64_t out_stride_n, out_stride_g, out_stride_h;
+  float* lse;                /* [n][g][heads]; may be NULL */
+  const int32_t* table;      /* [n][width], rows `table_stride` apart */
+  int64_t table_stride;
+  const int32_t* len;        /* [n] */
+  const float* slope;        /* [heads]; may be NULL */
+  const float* centre;       /* [n][g]; with slope */
+  const int32_t* first;      /* [n][g]; may be NULL */
+  const int32_t* last;       /* [n][g]; with first */
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t n, g, heads, width, dtype, sinks;   /* sinks >= 0; without `first` all positions are seen anyway */
+  float scale, cap;
+} linmt_attend_pages8_args;
+int64_t linmt_attend_pages8_workspace(const linmt_attend_pages8_args* args);   /* bytes, or -1: see linmt_op_error */
+int linmt_attend_pages8(const linmt_attend_pages8_args* args);
+
+/* Pages follow their hypotheses: row r = i * k + j of the new table is row i * k + parents[i][j] of the old one (parents NULL: row r itself); a parent outside
+ * 0 .. k-1, or done[i][j], leaves it without pages.  A row names ceil(len / page) pages, lengths taken as 0 .. width * page.
+ *   shares[p]   how many rows beyond the first name page p: 0 for a page of one row, and for a free one, as linmt_plan_pages hands them out
+ *   a last page that is not full stays with its row's first child; every further child names a page of its own instead, and the page to copy from and
+ *               the new one are the next entries of out_src and out_dst, in the order of the rows (linmt_copy_pages); -1 behind the last
+ *   pages that no row names any more go back in front of the free ones, ascending: free_pages[used - freed .. used - 1]; new pages are then taken
+ *               from there on.  Where they run out a column and its out_dst are -1 and out_used comes back larger than n_free.
+ * `used` is taken as 0 .. n_free.  Columns behind a row's pages, and those that name no page of the pool, come out as -1.  The same page in two columns of a row is not
+ * allowed: what becomes of its shares is not defined, though nothing outside the arrays is touched.  out_shares, out_free and out_used may be the arrays
+ * shares, free_pages and used; nothing else that is written may overlap what is read, or another result. */
+typedef struct linmt_fork_pages_args {
+  uint32_t size;
+  int32_t device;
+  void* stream;
+  const int32_t* table;      /* [n * k][width], rows `table_stride` apart */
+  int64_t table_stride;
+  const int32_t* len;        /* [n * k] */
+  const int32_t* parents;    /* [n * k]; may be NULL */
+  const uint8_t* done;       /* [n * k]; may be NULL */
+  const int32_t* shares;     /* [n_pages] */
+  const int32_t* free_pages; /* [n_free] */
+  const int32_t* used;       /* [1] */
+  int32_t* out_table;        /* [n * k][width], rows `out_table_stride` apart */
+  int64_t out_table_stride;
+  int32_t* out_len;          /* [n * k] */
+  int32_t* out_shares;       /* [n_pages] */
+  int32_t* out_free;         /* [n_free] */
+  int32_t* out_used;         /* [1] */
+  int32_t* out_src;          /* [n * k] */
+  int32_t* out_dst;          /* [n * k] */
+  int32_t n, k, width, page, n_pages, n_free;   /* n * k <= 16384 */
+} linmt_fork_pages_args;
+int linmt_fork_pages(const linmt_fork_pages_args* args);
+
+/* The pages that rows name move to the front of their pool: with U of them, each that lies at U or behind takes the place, in order, of one before U that
+ * nothing names: out_src, out_dst (linmt_copy_pages), -1 behind the last.  out_table and out_shares go by the new numbers, out_free is 0, 1, .. n_pages - 1 and out_used U.
+ * A row names ceil(len / page) pages, lengths taken as 0 .. width * page; other columns come out as -1, and so do those that name no page of the pool.
+ * out_table may be `table` (the same pointer and stride), out_shares may be `shares`; nothing else that is written may overlap what is read, or another result. */
+typedef struct linmt_compact_pages_args {
+  uint32_t size;
+  int32_t device;
+  void* stream;
+  const int32_t* table;      /* [rows][width], rows `table_stride` apart */
+  int64_t table_stride;
+  const int32_t* len;        /* [rows] */
+  const int32_t* shares;     /* [n_pages] */
+  int32_t* out_table;        /* [rows][width], rows `out_table_stride` apart */
+  int64_t out_table_stride;
+  int32_t* out_shares;       /* [n_pages] */
+  int32_t* out_free;         /* [n_pages] */
+  int32_t* out_used;         /* [1] */
+  int32_t* out_src;          /* [n_pages / 2] */
+  int32_t* out_dst;          /* [n_pages / 2] */
+  int32_t* workspace;        /* [n_pages], the call's own until it has run */
+  int32_t rows, width, page, n_pages;
+} linmt_compact_pages_args;
+int linmt_compact_pages(const linmt_compact_pages_args* args);
+
+/* Copies of whole pages: page dst[i] of every pool becomes what its page src[i] holds, one launch for up to 16 pools.  Entries with a number outside
+ * 0 .. n_pages - 1 copy nothing.  No page may be named twice in dst, or in both: what such entries leave there is not defined. */
+typedef struct linmt_page_pool {
+  void* data;
+  int64_t stride_page;       /* bytes */
+  int64_t page_bytes;        /* contiguous */
+} linmt_page_pool;
+typedef struct linmt_copy_pages_args {
+  uint32_t size;
+  int32_t device;
+  void* stream;
+  const int32_t* src;        /* [n] */
+  const int32_t* dst;        /* [n] */
+  int32_t n, n_pages, n_pools, reserved;
+  linmt_page_pool pool[16];
+} linmt_copy_pages_args;
+int linmt_copy_pages(const linmt_copy_pages_args* args);
+
+/* Scores of given tokens: of every row of logits x over its allowed words, with p = softmax(x),
+ *   out_logprob        x_token - log sum exp(x); -inf for a word that is not allowed, 0 for a token outside 0 .. vocab - 1 (a padded place)
+ *   out_entropy        - sum p log p
+ *   out_top_tokens, out_top_logprobs   the `top` words of the largest logits, equal ones by the lowest number; -1 and -inf where no word with a logit above -inf is left
+ * A row with a NaN or +inf at an allowed place: NaN, and -1 for words.  One without a word above -inf: -inf (0 for a padded place), and entropy 0. */
+typedef struct linmt_score_tokens_args {
+  uint32_t size;
+  int32_t device;
+  void* stream;
+  const void* logits;        /* [n][t][vocab], LINMT_F32 / BF16 / F16, words contiguous, aligned to their type */
+  int64_t stride_n, stride_t;
+  const int32_t* tokens;     /* [n][t] */
+  const uint32_t* allowed;   /* as in linmt_beam_select; may be NULL */
+  int64_t allowed_stride;    /* words from one n's list to the next, 0 = one list for all */
+  float* out_logprob;        /* [n][t] */
+  float* out_entropy;        /* [n][t] */
+  int32_t* out_top_tokens;   /* [n][t][top]; with top > 0 */
+  float* out_top_logprobs;   /* [n][t][top] */
+  int32_t n, t, vocab, top, dtype, reserved;   /* top <= 32, n * t below 2^31, vocab <= 2^31 - 4096 */
+} linmt_score_tokens_args;
+int linmt_score_tokens(const linmt_score_tokens_args* args);
 
 #ifdef __cplusplus
 }

@@ -40,7 +40,8 @@ EXPORTS = ["python_decoder_init", "python_decoder_do_job", "linmt_default_option
            "linmt_translate", "linmt_k_gemm", "linmt_k_logits", "linmt_k_softmax_topk", "linmt_gemm_f32_noalloc", "linmt_decode_file", "linmt_score_batch",
            "linmt_read_model_file", "python_unk_init", "python_unk_do_job", "linmt_unk_create", "linmt_unk_process", "linmt_unk_destroy",
            "linmt_op_error", "linmt_beam_select", "linmt_beam_reorder", "linmt_plan_pages", "linmt_write_pages4", "linmt_read_pages4",
-           "linmt_attend_pages4", "linmt_attend_pages4_workspace"]
+           "linmt_attend_pages4", "linmt_attend_pages4_workspace", "linmt_write_pages8", "linmt_read_pages8", "linmt_attend_pages8", "linmt_attend_pages8_workspace",
+           "linmt_fork_pages", "linmt_compact_pages", "linmt_copy_pages", "linmt_score_tokens"]
 
 _lib = None
 
@@ -99,9 +100,11 @@ def load():
     lib.linmt_unk_destroy.argtypes = [C.c_void_p]
     lib.linmt_score_batch.argtypes = [C.c_void_p] * 5 + [C.c_int32, C.c_void_p, C.c_void_p, C.c_int32]
     lib.linmt_op_error.restype = C.c_char_p
-    for name in ("linmt_beam_select", "linmt_beam_reorder", "linmt_plan_pages", "linmt_write_pages4", "linmt_read_pages4", "linmt_attend_pages4"):
+    for name in ("linmt_beam_select", "linmt_beam_reorder", "linmt_plan_pages", "linmt_write_pages4", "linmt_read_pages4", "linmt_attend_pages4", "linmt_write_pages8", "linmt_read_pages8",
+                 "linmt_attend_pages8", "linmt_fork_pages", "linmt_compact_pages", "linmt_copy_pages", "linmt_score_tokens"):
         getattr(lib, name).argtypes = [C.c_char_p]     # the argument struct as packed bytes (programs in Python fill it themselves; device_ops calls from C++)
-    lib.linmt_attend_pages4_workspace.argtypes = [C.c_char_p]
-    lib.linmt_attend_pages4_workspace.restype = C.c_int64
+    for name in ("linmt_attend_pages4_workspace", "linmt_attend_pages8_workspace"):
+        getattr(lib, name).argtypes = [C.c_char_p]
+        getattr(lib, name).restype = C.c_int64
     _lib = lib
     return lib

@@ -13,7 +13,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liblinmt_decoder.so")
 TORCH_LIB = os.path.join(HERE, "_device_ops.so")     # the operators' front for torch tensors (device_ops)
 SOURCES = ["engine.cu", "engine_tc.cu", "frontend.cu", "kernel_entry.cu", "noalloc_entry.cu", "beam_ops.cu", "pages4_ops.cu",
-           "pages4_attend.cu", "unk_post.cpp"]
+           "pages4_attend.cu", "pages8_ops.cu", "pages8_attend.cu", "page_ops.cu", "token_ops.cu", "unk_post.cpp"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC,-fopenmp,-O3", "--use_fast_math=false"]
 

@@ -33,6 +33,7 @@ inline int op_cuda(cudaError_t e, const char* what) {
 
 // What every call on a pool checks of it (pages4_ops.cu).
 int check_pages4(const linmt_pages4& p, const char* what);
+int check_pages8(const linmt_pages8& p, const char* what);      // (pages8_ops.cu)
 
 // Makes `device` current for a call and puts the caller's back.
 class OnDevice {

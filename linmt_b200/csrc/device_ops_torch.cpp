@@ -12,6 +12,8 @@
 #include <algorithm>
 #include <cmath>
 #include <string>
+#include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "../../include/linmt_decoder.h"
@@ -89,6 +91,14 @@ bool apart(const Tensor& t) {
   return true;
 }
 
+// Tensors as the tuple that a call returns.
+PyObject* tuple_of(std::vector<Tensor> ts) {
+  PyObject* r = PyTuple_New((Py_ssize_t)ts.size());
+  if (!r) throw python_error();
+  for (size_t i = 0; i < ts.size(); ++i) PyTuple_SET_ITEM(r, (Py_ssize_t)i, THPVariable_Wrap(std::move(ts[i])));
+  return r;
+}
+
 // A caller's tensor has been written: autograd finds one that it has saved for a backward pass changed.  (Tensors of the inference mode keep no count.)
 void was_written(PyObject* o) {
   const Tensor& t = THPVariable_Unpack(o);
@@ -133,10 +143,22 @@ bool meets(const Tensor& t, const Span& s) {
   return meets(all.p, size, stride, dims, (int64_t)t.element_size(), s.p, s.end);
 }
 // A tensor that is written while `read` is still read has to lie apart from it, or in the gaps between its places.
-void lie_apart(const Tensor& written, const char* name, PyObject* read, const char* of) {
-  if (read == Py_None) return;
-  const Tensor& r = THPVariable_Unpack(read);
+void lie_apart(const Tensor& written, const char* name, const Tensor& r, const char* of) {
   NEED(!meets(written, span_of(r)) || !meets(r, span_of(written)), name, " overlaps ", of);
+}
+void lie_apart(const Tensor& written, const char* name, PyObject* read, const char* of) {
+  if (read != Py_None) lie_apart(written, name, THPVariable_Unpack(read), of);
+}
+
+// Lists of allowed words, NULL where there are none.
+const uint32_t* allowed_of(PyObject* o, int dev, int64_t n, int64_t vocab, int64_t& stride) {
+  if (o == Py_None) return nullptr;
+  const Tensor& allowed = on_device(o, "allowed", dev);
+  const int64_t words = (vocab + 31) / 32;
+  NEED(allowed.dim() == 2 && (allowed.size(0) == 1 || allowed.size(0) == n), "allowed has to be [1 or n, ceil(vocab / 32)]");
+  const int64_t want[2] = {allowed.size(0), words};
+  stride = allowed.size(0) == 1 ? 0 : words;
+  return static_cast<const uint32_t*>(dense(o, "allowed", dev, at::kInt, want).data_ptr());
 }
 
 PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
@@ -156,14 +178,7 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   g.stride_k = logits.stride(1);
   g.scores = static_cast<const float*>(dense(a[1], "scores", dev, at::kFloat, shape).data_ptr());
   if (a[2] != Py_None) g.done = flags(a[2], "done", dev, shape);
-  if (a[3] != Py_None) {
-    const Tensor& allowed = on_device(a[3], "allowed", dev);
-    const int64_t words = (v + 31) / 32;
-    NEED(allowed.dim() == 2 && (allowed.size(0) == 1 || allowed.size(0) == n), "allowed has to be [1 or n, ceil(vocab / 32)]");
-    const int64_t want[2] = {allowed.size(0), words};
-    g.allowed = static_cast<const uint32_t*>(dense(a[3], "allowed", dev, at::kInt, want).data_ptr());
-    g.allowed_stride = allowed.size(0) == 1 ? 0 : words;
-  }
+  g.allowed = allowed_of(a[3], dev, n, v, g.allowed_stride);
   g.n = int32_of(n, "n");
   g.k = int32_of(k, "k");
   g.vocab = int32_of(v, "vocab");
@@ -371,21 +386,48 @@ PyObject* plan_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-linmt_pages4 pool_of(PyObject* o, int dev) {
+// The two forms of a pool's pages and their calls.
+struct In4Bits {
+  using Pool = linmt_pages4;
+  using Rows = linmt_pages4_rows_args;
+  using Attend = linmt_attend_pages4_args;
+  static constexpr const char* kForm = "18 * dim";
+  static int64_t dim(int64_t bytes) { return bytes % 18 ? -1 : bytes / 18; }
+  static int write(const Rows* g) { return linmt_write_pages4(g); }
+  static int read(const Rows* g) { return linmt_read_pages4(g); }
+  static int attend(const Attend* g) { return linmt_attend_pages4(g); }
+  static int64_t workspace(const Attend* g) { return linmt_attend_pages4_workspace(g); }
+};
+struct In8Bits {
+  using Pool = linmt_pages8;
+  using Rows = linmt_pages8_rows_args;
+  using Attend = linmt_attend_pages8_args;
+  static constexpr const char* kForm = "32 * dim + 16";
+  static int64_t dim(int64_t bytes) { return bytes % 32 != 16 ? -1 : bytes / 32; }
+  static int write(const Rows* g) { return linmt_write_pages8(g); }
+  static int read(const Rows* g) { return linmt_read_pages8(g); }
+  static int attend(const Attend* g) { return linmt_attend_pages8(g); }
+  static int64_t workspace(const Attend* g) { return linmt_attend_pages8_workspace(g); }
+};
+
+template <class F>
+typename F::Pool pool_of(PyObject* o, int dev) {
   const Tensor& p = on_device(o, "pages", dev);
-  NEED(p.scalar_type() == at::kByte && p.dim() == 4 && p.size(3) % 18 == 0, "pages have to be uint8 [n_pages, heads, page / 16, 18 * dim]");
+  NEED(p.scalar_type() == at::kByte && p.dim() == 4 && F::dim(p.size(3)) >= 0, "pages have to be uint8 [n_pages, heads, page / 16, ", F::kForm, "]");
   NEED(p.stride(3) == 1 && (p.stride(2) == p.size(3) || p.size(2) == 1), "the tiles of a page's head have to be contiguous");
-  return {p.data_ptr(), p.stride(0), p.stride(1), int32_of(p.size(0), "n_pages"), int32_of(p.size(1), "heads"), int32_of(p.size(2) * 16, "page"), int32_of(p.size(3) / 18, "dim")};
+  return {p.data_ptr(), p.stride(0), p.stride(1), int32_of(p.size(0), "n_pages"), int32_of(p.size(1), "heads"), int32_of(p.size(2) * 16, "page"), int32_of(F::dim(p.size(3)), "dim")};
 }
 
-int64_t slots_of(PyObject* o, int dev, linmt_pages4_rows_args& g) {
+template <class Rows>
+int64_t slots_of(PyObject* o, int dev, Rows& g) {
   const Tensor& slots = on_cuda(o, "slots");
   NEED(slots.dim() == 1, "slots have to be [t]");
   g.slots = static_cast<const int64_t*>(dense(o, "slots", dev, at::kLong, slots.sizes()).data_ptr());
   g.t = int32_of(slots.size(0), "t");
   return slots.size(0);
 }
-void rows_of(const Tensor& x, const char* name, const linmt_pages4_rows_args& g, void*& p, int64_t& t, int64_t& h) {
+template <class Rows>
+void rows_of(const Tensor& x, const char* name, const Rows& g, void*& p, int64_t& t, int64_t& h) {
   const int64_t want[3] = {g.t, g.pages.heads, g.pages.dim};
   NEED(dtype_of(x) == g.dtype && g.dtype >= 0, name, " has to be float32, bfloat16 or float16, k and v alike");
   NEED(x.sizes() == at::IntArrayRef(want), name, " has to have the shape ", at::IntArrayRef(want), ", not ", x.sizes());
@@ -395,15 +437,16 @@ void rows_of(const Tensor& x, const char* name, const linmt_pages4_rows_args& g,
   h = x.stride(1);
 }
 
-PyObject* write_pages4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+template <class F>
+PyObject* write_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
   arguments(n_args, 4);
   const int dev = on_cuda(a[1], "slots").get_device();
-  linmt_pages4_rows_args g{};
+  typename F::Rows g{};
   g.size = sizeof(g);
   g.device = dev;
   g.stream = stream_of(dev);
-  g.pages = pool_of(a[0], dev);
+  g.pages = pool_of<F>(a[0], dev);
   NEED(apart(THPVariable_Unpack(a[0])), "pages have places that share memory");
   slots_of(a[1], dev, g);
   const Tensor &k = on_device(a[2], "k", dev), &v = on_device(a[3], "v", dev);
@@ -413,21 +456,22 @@ PyObject* write_pages4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   lie_apart(THPVariable_Unpack(a[0]), "pages", a[1], "slots");
   lie_apart(THPVariable_Unpack(a[0]), "pages", a[2], "k");
   lie_apart(THPVariable_Unpack(a[0]), "pages", a[3], "v");
-  done_or_raise(linmt_write_pages4(&g));
+  done_or_raise(F::write(&g));
   was_written(a[0]);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
 
-PyObject* read_pages4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+template <class F>
+PyObject* read_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
   arguments(n_args, 3);
   const int dev = on_cuda(a[1], "slots").get_device();
-  linmt_pages4_rows_args g{};
+  typename F::Rows g{};
   g.size = sizeof(g);
   g.device = dev;
   g.stream = stream_of(dev);
-  g.pages = pool_of(a[0], dev);
+  g.pages = pool_of<F>(a[0], dev);
   const int64_t shape[3] = {slots_of(a[1], dev, g), g.pages.heads, g.pages.dim};
   const int64_t type = integer(a[2], "dtype");
   NEED(type >= 0 && type <= 2, "dtype has to be float32, bfloat16 or float16");
@@ -436,25 +480,24 @@ PyObject* read_pages4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   g.dtype = (int)type;
   rows_of(k, "k", g, g.k, g.k_stride_t, g.k_stride_h);
   rows_of(v, "v", g, g.v, g.v_stride_t, g.v_stride_h);
-  done_or_raise(linmt_read_pages4(&g));
-  PyObject* r = PyTuple_New(2);
-  if (!r) throw python_error();
-  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(k)));
-  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(v)));
-  return r;
+  done_or_raise(F::read(&g));
+  return tuple_of({std::move(k), std::move(v)});
   END_HANDLE_TH_ERRORS
 }
 
-PyObject* attend_pages4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+template <class F>
+PyObject* attend_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  arguments(n_args, 12);
+  constexpr bool kSinks = std::is_same<F, In8Bits>::value;
+  arguments(n_args, kSinks ? 13 : 12);
   const Tensor& q = on_cuda(a[0], "q");
   const int dev = q.get_device();
-  linmt_attend_pages4_args g{};
+  typename F::Attend g{};
   g.size = sizeof(g);
   g.device = dev;
   g.stream = stream_of(dev);
-  g.pages = pool_of(a[1], dev);
+  g.pages = pool_of<F>(a[1], dev);
+  if constexpr (kSinks) g.sinks = int32_of(integer(a[12], "sinks"), "sinks");
   g.dtype = dtype_of(q);
   NEED(q.dim() == 4 && g.dtype >= 0 && q.size(3) == g.pages.dim, "q has to be [n, g, heads, ", g.pages.dim, "] in float32, bfloat16 or float16");
   NEED(q.stride(3) == 1 || q.numel() == 0, "the components of q have to be contiguous");
@@ -516,14 +559,14 @@ PyObject* attend_pages4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   }
   Tensor ws;
   if (q.numel()) {
-    const int64_t need = linmt_attend_pages4_workspace(&g);
+    const int64_t need = F::workspace(&g);
     NEED(need >= 0, linmt_op_error());
     if (need) {
       ws = make({need}, at::kByte, dev);     // goes back to torch's pool of this stream behind the call's kernels
       g.workspace = ws.data_ptr();
       g.workspace_bytes = need;
     }
-    done_or_raise(linmt_attend_pages4(&g));
+    done_or_raise(F::attend(&g));
   }
   PyObject* o = a[10];
   if (o == Py_None) o = THPVariable_Wrap(std::move(out));
@@ -540,16 +583,248 @@ PyObject* attend_pages4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// Tables whose rows lie evenly: [n, k, width] with lens [n, k], or [n, width] with lens [n].
+struct Rows { int64_t rows, width, stride; };
+Rows rows_of_table(const Tensor& t, const Tensor& lens) {
+  const int64_t d = lens.dim();
+  NEED(t.scalar_type() == at::kInt && t.dim() == d + 1 && t.sizes().slice(0, d) == lens.sizes(), "table has to be int32, a row of columns for each of lens");
+  NEED(t.size(d) <= 1 || t.stride(d) == 1, "the rows of table have to be contiguous");
+  NEED(d == 1 || t.size(0) <= 1 || t.size(1) <= 0 || t.stride(0) == t.size(1) * t.stride(1), "the rows of table have to lie evenly");
+  return {lens.numel(), t.size(d), lens.numel() == 0 ? t.size(d) : t.stride(d - 1)};
+}
+// Results of a call: made, or the caller's; each lies apart from all that is read and from the others, but one that may be what it follows, place for place.
+struct Out {
+  const char* name;
+  at::ScalarType type;
+  std::vector<int64_t> shape;
+  int follows;               // index among what is read, -1: none
+};
+std::vector<Tensor> results(PyObject* out, const std::vector<Out>& wanted, const std::vector<std::pair<PyObject*, const char*>>& read, int dev) {
+  std::vector<Tensor> made;
+  if (out == Py_None) {
+    for (const Out& w : wanted) made.push_back(make(w.shape, w.type, dev));
+    return made;
+  }
+  NEED(PyTuple_Check(out) && PyTuple_GET_SIZE(out) == (Py_ssize_t)wanted.size(), "out has to be a tuple of ", wanted.size(), " tensors");
+  for (size_t i = 0; i < wanted.size(); ++i) {
+    PyObject* const o = PyTuple_GET_ITEM(out, (Py_ssize_t)i);
+    const Tensor& t = dense(o, wanted[i].name, dev, wanted[i].type, wanted[i].shape);
+    for (size_t j = 0; j < i; ++j) lie_apart(t, wanted[i].name, made[j], wanted[j].name);
+    for (size_t j = 0; j < read.size(); ++j) {
+      if (read[j].first == Py_None) continue;
+      const Tensor& r = THPVariable_Unpack(read[j].first);
+      if ((int)j != wanted[i].follows || r.data_ptr() != t.data_ptr() || r.strides() != t.strides()) lie_apart(t, wanted[i].name, r, read[j].second);
+    }
+    made.push_back(t);
+  }
+  return made;
+}
+PyObject* results_of(PyObject* out, std::vector<Tensor>&& made) {
+  if (out == Py_None) return tuple_of(std::move(made));
+  for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(out); ++i) was_written(PyTuple_GET_ITEM(out, i));
+  Py_INCREF(out);
+  return out;
+}
+int32_t* ints(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
+
+// table, lens, parents, done, shares, free, used, page, out.  Without parents rows keep their own pages, and there is nothing to copy.
+template <bool FORK>
+PyObject* fork_or_free(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  arguments(n_args, 9);
+  const Tensor& lens = on_cuda(a[1], "lens");
+  const int dev = lens.get_device();
+  NEED(FORK ? lens.dim() == 2 : lens.dim() == 1 || lens.dim() == 2, "lens have to be ", FORK ? "[n, k]" : "[n] or [n, k]");
+  const auto shape = lens.sizes();
+  const int64_t one[1] = {1};
+  const Tensor& table = on_device(a[0], "table", dev);
+  const Rows rows = rows_of_table(table, lens);
+  const Tensor &shares = on_device(a[4], "shares", dev), &free = on_device(a[5], "free", dev);
+  NEED(shares.dim() == 1 && free.dim() == 1, "shares have to be [n_pages], free [n_free]");
+  linmt_fork_pages_args g{};
+  g.size = sizeof(g);
+  g.device = dev;
+  g.stream = stream_of(dev);
+  g.table = ints(table);
+  g.table_stride = rows.stride;
+  g.len = ints(dense(a[1], "lens", dev, at::kInt, shape));
+  if (a[2] != Py_None) g.parents = ints(dense(a[2], "parents", dev, at::kInt, shape));
+  if (a[3] != Py_None) g.done = flags(a[3], "done", dev, shape);
+  g.shares = ints(dense(a[4], "shares", dev, at::kInt, shares.sizes()));
+  g.free_pages = ints(dense(a[5], "free", dev, at::kInt, free.sizes()));
+  g.used = ints(dense(a[6], "used", dev, at::kInt, one));
+  g.n = int32_of(FORK ? lens.size(0) : rows.rows, "n");
+  g.k = FORK ? int32_of(lens.size(1), "k") : 1;
+  g.width = int32_of(rows.width, "width");
+  g.page = int32_of(integer(a[7], "page"), "page");
+  g.n_pages = int32_of(shares.size(0), "n_pages");
+  g.n_free = int32_of(free.size(0), "n_free");
+  std::vector<Out> wanted = {{"out[0]", at::kInt, table.sizes().vec(), -1}, {"out[1]", at::kInt, shape.vec(), -1}, {"out[2]", at::kInt, shares.sizes().vec(), 4},
+                             {"out[3]", at::kInt, free.sizes().vec(), 5},   {"out[4]", at::kInt, {1}, 6}};
+  if (FORK) {
+    wanted.push_back({"out[5]", at::kInt, {rows.rows}, -1});
+    wanted.push_back({"out[6]", at::kInt, {rows.rows}, -1});
+  }
+  std::vector<Tensor> t = results(a[8], wanted, {{a[0], "table"}, {a[1], "lens"}, {a[2], "parents"}, {a[3], "done"}, {a[4], "shares"}, {a[5], "free"}, {a[6], "used"}}, dev);
+  Tensor scratch;
+  if (!FORK) scratch = make({2 * rows.rows}, at::kInt, dev);
+  g.out_table = ints(t[0]);
+  g.out_table_stride = rows.width;
+  g.out_len = ints(t[1]);
+  g.out_shares = ints(t[2]);
+  g.out_free = ints(t[3]);
+  g.out_used = ints(t[4]);
+  g.out_src = ints(FORK ? t[5] : scratch);
+  g.out_dst = FORK ? ints(t[6]) : g.out_src + rows.rows;
+  done_or_raise(linmt_fork_pages(&g));
+  return results_of(a[8], std::move(t));
+  END_HANDLE_TH_ERRORS
+}
+
+// table, lens, shares, page, out
+PyObject* compact_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  arguments(n_args, 5);
+  const Tensor& lens = on_cuda(a[1], "lens");
+  const int dev = lens.get_device();
+  NEED(lens.dim() == 1 || lens.dim() == 2, "lens have to be [n] or [n, k]");
+  const Tensor &table = on_device(a[0], "table", dev), &shares = on_device(a[2], "shares", dev);
+  const Rows rows = rows_of_table(table, lens);
+  NEED(shares.dim() == 1, "shares have to be [n_pages]");
+  const int64_t n_pages = shares.size(0);
+  linmt_compact_pages_args g{};
+  g.size = sizeof(g);
+  g.device = dev;
+  g.stream = stream_of(dev);
+  g.table = ints(table);
+  g.table_stride = rows.stride;
+  g.len = ints(dense(a[1], "lens", dev, at::kInt, lens.sizes()));
+  g.shares = ints(dense(a[2], "shares", dev, at::kInt, shares.sizes()));
+  g.rows = int32_of(rows.rows, "rows");
+  g.width = int32_of(rows.width, "width");
+  g.page = int32_of(integer(a[3], "page"), "page");
+  g.n_pages = int32_of(n_pages, "n_pages");
+  std::vector<Tensor> t = results(a[4], {{"out[0]", at::kInt, table.sizes().vec(), 0}, {"out[1]", at::kInt, {n_pages}, 2}, {"out[2]", at::kInt, {n_pages}, -1}, {"out[3]", at::kInt, {1}, -1},
+                                         {"out[4]", at::kInt, {n_pages / 2}, -1}, {"out[5]", at::kInt, {n_pages / 2}, -1}},
+                                  {{a[0], "table"}, {a[1], "lens"}, {a[2], "shares"}}, dev);
+  Tensor ws = make({n_pages}, at::kInt, dev);      // goes back to torch's pool of this stream behind the call's kernel
+  g.out_table = ints(t[0]);
+  g.out_table_stride = rows.width;
+  g.out_shares = ints(t[1]);
+  g.out_free = ints(t[2]);
+  g.out_used = ints(t[3]);
+  g.out_src = ints(t[4]);
+  g.out_dst = ints(t[5]);
+  g.workspace = ints(ws);
+  done_or_raise(linmt_compact_pages(&g));
+  return results_of(a[4], std::move(t));
+  END_HANDLE_TH_ERRORS
+}
+
+// pools, src, dst
+PyObject* copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  arguments(n_args, 3);
+  const Tensor& src = on_cuda(a[1], "src");
+  const int dev = src.get_device();
+  NEED(src.dim() == 1, "src has to be [n]");
+  linmt_copy_pages_args g{};
+  g.size = sizeof(g);
+  g.device = dev;
+  g.stream = stream_of(dev);
+  g.src = ints(dense(a[1], "src", dev, at::kInt, src.sizes()));
+  g.dst = ints(dense(a[2], "dst", dev, at::kInt, src.sizes()));
+  g.n = int32_of(src.size(0), "n");
+  NEED(PyList_Check(a[0]), "pools have to be a list of tensors");
+  const Py_ssize_t all = PyList_GET_SIZE(a[0]);
+  std::vector<linmt_page_pool> pools;
+  for (Py_ssize_t i = 0; i < all; ++i) {
+    const Tensor& p = on_device(PyList_GET_ITEM(a[0], i), "pools", dev);
+    NEED(p.dim() >= 1 && p.size(0) == THPVariable_Unpack(PyList_GET_ITEM(a[0], 0)).size(0), "pools have to have the same number of pages");
+    int64_t each = 1;
+    for (int64_t d = p.dim() - 1; d >= 1; --d) {
+      NEED(p.size(d) == 1 || p.stride(d) == each || p.numel() == 0, "the pages of pools[", i, "] have to be contiguous");
+      each *= p.size(d);
+    }
+    NEED(p.size(0) <= 1 || p.stride(0) >= each, "the pages of pools[", i, "] share memory");
+    for (Py_ssize_t j = 0; j < i; ++j) lie_apart(p, "a pool", PyList_GET_ITEM(a[0], j), "another");
+    lie_apart(p, "a pool", a[1], "src");
+    lie_apart(p, "a pool", a[2], "dst");
+    if (p.numel()) pools.push_back({p.data_ptr(), p.stride(0) * (int64_t)p.element_size(), each * (int64_t)p.element_size()});
+    g.n_pages = int32_of(p.size(0), "n_pages");
+  }
+  for (size_t i = 0; i < pools.size(); i += 16) {
+    g.n_pools = (int)std::min<size_t>(16, pools.size() - i);
+    std::copy(pools.begin() + i, pools.begin() + i + g.n_pools, g.pool);
+    done_or_raise(linmt_copy_pages(&g));
+  }
+  for (Py_ssize_t i = 0; i < all; ++i) was_written(PyList_GET_ITEM(a[0], i));
+  Py_INCREF(a[0]);
+  return a[0];
+  END_HANDLE_TH_ERRORS
+}
+
+// logits, tokens, allowed, top
+PyObject* score_tokens(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  arguments(n_args, 4);
+  const Tensor& logits = on_cuda(a[0], "logits");
+  const int dev = logits.get_device();
+  NEED(logits.dim() == 3 && dtype_of(logits) >= 0, "logits have to be [n, t, vocab] in float32, bfloat16 or float16");
+  const int64_t n = logits.size(0), t = logits.size(1), v = logits.size(2), shape[2] = {n, t}, top = integer(a[3], "top");
+  NEED(v >= 1 && (logits.stride(2) == 1 || v == 1), "the words of a row of logits have to be contiguous");
+  NEED(top >= 0 && top <= 32, "top = ", top, " has to be 0 .. 32");
+  linmt_score_tokens_args g{};
+  g.size = sizeof(g);
+  g.device = dev;
+  g.logits = logits.data_ptr();
+  g.stride_n = logits.stride(0);
+  g.stride_t = logits.stride(1);
+  g.tokens = ints(dense(a[1], "tokens", dev, at::kInt, shape));
+  g.allowed = allowed_of(a[2], dev, n, v, g.allowed_stride);
+  g.n = int32_of(n, "n");
+  g.t = int32_of(t, "t");
+  g.vocab = int32_of(v, "vocab");
+  g.top = (int)top;
+  g.dtype = dtype_of(logits);
+  std::vector<Tensor> r = {make(shape, at::kFloat, dev), make(shape, at::kFloat, dev)};
+  g.out_logprob = static_cast<float*>(r[0].data_ptr());
+  g.out_entropy = static_cast<float*>(r[1].data_ptr());
+  if (top) {
+    const int64_t tops[3] = {n, t, top};
+    r.push_back(make(tops, at::kInt, dev));
+    r.push_back(make(tops, at::kFloat, dev));
+    g.out_top_tokens = ints(r[2]);
+    g.out_top_logprobs = static_cast<float*>(r[3].data_ptr());
+  }
+  g.stream = stream_of(dev);
+  done_or_raise(linmt_score_tokens(&g));
+  return tuple_of(std::move(r));
+  END_HANDLE_TH_ERRORS
+}
+
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyCFunction fast() { return reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(F)); }
 
 }  // namespace
 
 extern "C" __attribute__((visibility("default"))) PyObject* PyInit__device_ops() {
-  static PyMethodDef methods[] = {{"beam_select", fast<beam_select>(), METH_FASTCALL, nullptr}, {"beam_reorder", fast<beam_reorder>(), METH_FASTCALL, nullptr},
-                                  {"plan_pages", fast<plan_pages>(), METH_FASTCALL, nullptr},   {"write_pages4", fast<write_pages4>(), METH_FASTCALL, nullptr},
-                                  {"read_pages4", fast<read_pages4>(), METH_FASTCALL, nullptr}, {"attend_pages4", fast<attend_pages4>(), METH_FASTCALL, nullptr},
-                                  {nullptr, nullptr, 0, nullptr}};
+  static PyMethodDef methods[] = {
+      {"beam_select", fast<beam_select>(), METH_FASTCALL, nullptr},
+      {"beam_reorder", fast<beam_reorder>(), METH_FASTCALL, nullptr},
+      {"plan_pages", fast<plan_pages>(), METH_FASTCALL, nullptr},
+      {"write_pages4", fast<write_pages<In4Bits>>(), METH_FASTCALL, nullptr},
+      {"read_pages4", fast<read_pages<In4Bits>>(), METH_FASTCALL, nullptr},
+      {"attend_pages4", fast<attend_pages<In4Bits>>(), METH_FASTCALL, nullptr},
+      {"write_pages8", fast<write_pages<In8Bits>>(), METH_FASTCALL, nullptr},
+      {"read_pages8", fast<read_pages<In8Bits>>(), METH_FASTCALL, nullptr},
+      {"attend_pages8", fast<attend_pages<In8Bits>>(), METH_FASTCALL, nullptr},
+      {"fork_pages", fast<fork_or_free<true>>(), METH_FASTCALL, nullptr},
+      {"free_pages", fast<fork_or_free<false>>(), METH_FASTCALL, nullptr},
+      {"compact_pages", fast<compact_pages>(), METH_FASTCALL, nullptr},
+      {"copy_pages", fast<copy_pages>(), METH_FASTCALL, nullptr},
+      {"score_tokens", fast<score_tokens>(), METH_FASTCALL, nullptr},
+      {nullptr, nullptr, 0, nullptr}};
   static PyModuleDef module = {PyModuleDef_HEAD_INIT, "_device_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
   PyObject* decoder = PyImport_ImportModule("linmt_b200.decoder");
   if (!decoder) return nullptr;
