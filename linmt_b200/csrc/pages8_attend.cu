@@ -14,6 +14,8 @@
 // then, every 256 chunks and at the end are O's integers taken out of TMEM, into 32-bit sums.
 // A CTA has 128 threads that turn S into weights, a position each; one warp that copies blocks (bulk copies, two rings) and one that issues the products.  Two CTAs
 // share an SM.  The work is cut into equal shares over the CTAs that fit on the GPU at once, and a second kernel joins the parts of what several of them share.
+#include <cuda.h>
+
 #include <cmath>
 
 #include "device_ops.h"
@@ -23,20 +25,26 @@ namespace linmt {
 namespace ops {
 namespace {
 
-constexpr int kRows = 16;
 constexpr int kChunk = 128;                  // positions of a product
 constexpr int kBlocks = kChunk / pages8::kBlock;
-constexpr int kWeightWarps = 4, kCopyWarp = 4, kIssueWarp = 5;
-constexpr int kThreads = 192;
 constexpr int kQueryDigits = 3, kWeightDigits = 4;
-constexpr int kQueryCols = kRows * kQueryDigits, kWeightCols = kRows * kWeightDigits;
-constexpr int kTmemCols = 256, kTmemS = 64, kTmemO = 128;      // S twice, 64 columns apart, then O
+// R rows: 4, 8 or 16 of a head of the pool at once.
+template <int R> constexpr int kQueryCols = (R * kQueryDigits + 15) / 16 * 16;
+template <int R> constexpr int kWeightCols = R * kWeightDigits;
+template <int R> constexpr int kTmemCols = R == 16 ? 256 : R == 8 ? 128 : 64;      // S twice, then O
+template <int R> constexpr int kTmemO = 2 * kQueryCols<R>;
+template <int R> constexpr int kCtas = R == 4 ? 3 : 2;                             // of an SM
+// A thread of the weights has a position and kRows rows: with 16, two groups of four warps (the products' rows are 32 to a warp) share them.
+template <int R> constexpr int kRows = R == 16 ? 8 : R;
+template <int R> constexpr int kWeightWarps = 4 * (R / kRows<R>);
+template <int R> constexpr int kThreads = 32 * (kWeightWarps<R> + 2);              // and a warp that copies, one that issues
 constexpr int kDrain = 256;                  // chunks between two drains: 127 * 255 * 128 * 256 < 2^31
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kAbove = 40.f;               // of L above the exponents so far
 constexpr unsigned long long kWaitCycles = 2000000000ull;      // about a second
-template <int D> constexpr int kStages = D == 128 ? 3 : 5;
+template <int D, int R> constexpr int kKeyStages = (R == 8 ? 3 : 2) * 128 / D;
+template <int D, int R> constexpr int kValueStages = (R == 4 ? 2 : 3) * 128 / D;
 
 enum Scores { kPlain, kQuick, kExact };      // neither cap nor bias; caps to 3e-7 of the cap; caps by tanhf
 
@@ -59,7 +67,12 @@ struct AttendParams {
   float* ws;
   int32_t n, g, heads, rep, width, row_tiles, sinks, by_window, dtype, q_wide;
   float cap, mul;            // mul: scale, times what the form of the scores takes it by
+  int32_t row_page, row_head, rows;      // the pool as rows of blocks: from a page, a head to the next, and all (0: its strides are none of whole blocks)
+  int32_t slack;             // by how many powers of 2 a weight may exceed what it is relative to
 };
+
+// The pool's rows of blocks: codes of a block (keys, or values), and its scales.
+struct alignas(64) AttendMaps { CUtensorMap codes, scales; };
 
 // ---- PTX
 __device__ __forceinline__ uint32_t shared(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -88,6 +101,11 @@ __device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, volatile
 __device__ __forceinline__ void copy_bulk(uint32_t to, const void* from, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
 }
+// Columns from x on of four rows of a tensor, one behind the other.
+__device__ __forceinline__ void copy_rows(uint32_t to, const CUtensorMap* map, int x, int r0, int r1, int r2, int r3, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+               ::"r"(to), "l"(map), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar) : "memory");
+}
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
@@ -107,25 +125,42 @@ __device__ __forceinline__ void mma_bytes(uint32_t d, uint64_t a, uint64_t b, ui
 __device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t along, uint32_t across) {
   return (uint64_t)(at >> 4 & 0x3fff) | (uint64_t)(along >> 4) << 16 | (uint64_t)(across >> 4) << 32 | (uint64_t)1 << 46;
 }
-// 32-bit integers of signed bytes times signed (or unsigned) ones, both along the sum; 128 rows, n columns.
-__host__ __device__ constexpr uint32_t form_of(int n, bool is_signed) { return 2u << 4 | 1u << 7 | (is_signed ? 1u : 0u) << 10 | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24; }
+// 32-bit integers of signed bytes times bytes; 128 rows, n columns.  Queries: signed, 16 neighbouring bytes lie along the sum.  Weights: not signed, 16 neighbouring bytes are columns.
+constexpr uint32_t kForm = 2u << 4 | 1u << 7 | (128u >> 4) << 24;
+template <int R> constexpr uint32_t kQueryForm = kForm | 1u << 10 | (uint32_t)(kQueryCols<R> >> 3) << 17;
+template <int R> constexpr uint32_t kWeightForm = kForm | 1u << 16 | (uint32_t)(kWeightCols<R> >> 3) << 17;
 
-#define LINMT_OUT16(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7]), \
-    "=r"(v[o + 8]), "=r"(v[o + 9]), "=r"(v[o + 10]), "=r"(v[o + 11]), "=r"(v[o + 12]), "=r"(v[o + 13]), "=r"(v[o + 14]), "=r"(v[o + 15])
-// 16 columns of the lane's row of TMEM.
-__device__ __forceinline__ void tmem_load16(uint32_t at, int (&v)[16]) {
+#define LINMT_OUT4(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3])
+#define LINMT_OUT8(v, o) LINMT_OUT4(v, o), LINMT_OUT4(v, o + 4)
+// Columns of the lane's row of TMEM: three times N, `apart` from each other.
+__device__ __forceinline__ void tmem_load(uint32_t at, uint32_t apart, int (&v)[3][8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%24];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%25];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%16,%17,%18,%19,%20,%21,%22,%23}, [%26];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : LINMT_OUT8(v[0], 0), LINMT_OUT8(v[1], 0), LINMT_OUT8(v[2], 0) : "r"(at), "r"(at + apart), "r"(at + 2 * apart) : "memory");
+}
+__device__ __forceinline__ void tmem_load(uint32_t at, uint32_t apart, int (&v)[3][4]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%12];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x4.b32 {%4,%5,%6,%7}, [%13];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x4.b32 {%8,%9,%10,%11}, [%14];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : LINMT_OUT4(v[0], 0), LINMT_OUT4(v[1], 0), LINMT_OUT4(v[2], 0) : "r"(at), "r"(at + apart), "r"(at + 2 * apart) : "memory");
+}
+// N neighbouring ones.
+__device__ __forceinline__ void tmem_load(uint32_t at, int (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : LINMT_OUT8(v, 0), LINMT_OUT8(v, 8), LINMT_OUT8(v, 16), LINMT_OUT8(v, 24) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void tmem_load(uint32_t at, int (&v)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
       "tcgen05.wait::ld.sync.aligned;"
-      : LINMT_OUT16(v, 0) : "r"(at) : "memory");
-}
-__device__ __forceinline__ void tmem_load48(uint32_t at, int (&v)[48]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%48];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%49];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47}, [%50];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : LINMT_OUT16(v, 0), LINMT_OUT16(v, 16), LINMT_OUT16(v, 32) : "r"(at), "r"(at + 16), "r"(at + 32) : "memory");
+      : LINMT_OUT8(v, 0), LINMT_OUT8(v, 8) : "r"(at) : "memory");
 }
 __device__ __forceinline__ float exp2_of(float x) {
   float y;
@@ -137,7 +172,6 @@ __device__ __forceinline__ float warp_max(float x) {
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 // cap tanh(x) as cap - 2 cap / (2^y + 1), y = 2 x log2(e): good to 3e-7 of the cap, 2e-5 of a score with a cap of up to kQuickCap, which a 16-bit result does not see.
 constexpr float kQuickCap = 64.f;
 __device__ __forceinline__ float capped(float y, float cap) {
@@ -145,16 +179,18 @@ __device__ __forceinline__ float capped(float y, float cap) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(exp2_of(y) + 1.f));
   return fmaf(-2.f * cap, r, cap);
 }
-// The 128 threads of the weights: wait for each other; whether one of them says so.
-__device__ __forceinline__ void weights_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// The N threads of the weights: wait for each other; whether one of them says so.
+template <int N>
+__device__ __forceinline__ void weights_sync() { asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory"); }
+template <int N>
 __device__ __forceinline__ bool weights_any(bool x) {
   int r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.s32 p, %1, 0;\n\t"
-      "bar.red.or.pred q, 1, 128, p;\n\t"
+      "bar.red.or.pred q, 1, %2, p;\n\t"
       "selp.s32 %0, 1, 0, q;\n\t}"
-      : "=r"(r) : "r"((int)x) : "memory");
+      : "=r"(r) : "r"((int)x), "n"(N) : "memory");
   return r != 0;
 }
 __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -170,9 +206,9 @@ __device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.w
 constexpr int kFixed = 3;
 constexpr int kWhole = kFixed + 3;
 struct Share {
-  int64_t begin, end;      // the CTA's units
-  int64_t first;           // number of the first unit of sentence `sent`
-  int64_t per;             // units of a part
+  int begin, end;          // the CTA's units
+  int first;               // number of the first unit of sentence `sent`
+  int per;                 // units of a part
   int sent, whole;         // sentence of `begin`; segments of up to `whole` units are not cut
 };
 __device__ __forceinline__ int length_of(const AttendParams& a, int sent) {
@@ -215,8 +251,9 @@ __device__ __forceinline__ Seen seen_by_warp(const AttendParams& a, int sent) { 
 
 // Share of block `blockIdx.x` of `blocks`; all threads of the CTA call it.  The sentences are added up by all threads, then those of the thread that has the first
 // unit, until one is left.
+template <int kThreads>
 __device__ __forceinline__ Share share_of(const AttendParams& a, int blocks) {
-  __shared__ int64_t sums[kThreads / 32], found_first;
+  __shared__ int sums[kThreads / 32], found_first;
   __shared__ int found_lo, found_hi;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, segments = a.pool_heads * a.row_tiles;
   Share s{};
@@ -224,18 +261,19 @@ __device__ __forceinline__ Share share_of(const AttendParams& a, int blocks) {
   bool all = true;
   for (;;) {
     const int each = (hi - lo + kThreads - 1) / kThreads, i0 = min(hi, lo + tid * each), i1 = min(hi, i0 + each);
-    int64_t mine = 0;
-#pragma unroll 8
+    int mine = 0;
+#pragma unroll 4
     for (int i = i0; i < i1; ++i) mine += seen_of(a, i).units();
-    int64_t upto = mine;
+    int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(~0u, upto, o);
+      const int x = __shfl_up_sync(~0u, upto, o);
       if (lane >= o) upto += x;
     }
     if (lane == 31) sums[warp] = upto;
     __syncthreads();
-    int64_t total = 0;
+    int total = 0;
+#pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
       if (w == warp) upto += total;
       total += sums[w];
@@ -243,13 +281,13 @@ __device__ __forceinline__ Share share_of(const AttendParams& a, int blocks) {
     if (all) {
       all = false;
       total *= segments;
-      s.per = max((int64_t)kWhole, (total + blocks - 1) / blocks);
-      s.begin = min(total, blockIdx.x * s.per);
-      s.end = min(total, s.begin + s.per);
-      s.whole = (int)min((int64_t)0x7fffffff, max((int64_t)kWhole, s.per / 8));
+      s.per = max(kWhole, (int)(((unsigned)total + blocks - 1) / blocks));
+      s.begin = (int)min((int64_t)total, (int64_t)blockIdx.x * s.per);
+      s.end = (int)min((int64_t)total, (int64_t)s.begin + s.per);
+      s.whole = max(kWhole, s.per / 8);
     }
     if (s.begin >= s.end) return s;
-    const int64_t before = s.first + (upto - mine) * segments;
+    const int before = s.first + (upto - mine) * segments;
     if (s.begin >= before && s.begin < s.first + upto * segments) {
       found_first = before;
       found_lo = i0;
@@ -270,7 +308,7 @@ __device__ __forceinline__ Share share_of(const AttendParams& a, int blocks) {
 struct Piece {
   int sent, kvh, rt, len;
   int u0, u1, units;       // units u0 .. u1 - 1 of the segment's
-  int64_t start;           // number of the segment's first unit
+  int start;               // number of the segment's first unit
   int c0, c1;
   Seen seen;
   __device__ __forceinline__ bool whole() const { return u0 == 0 && u1 == units; }
@@ -281,19 +319,19 @@ __device__ __forceinline__ bool next_piece(const AttendParams& a, Share& s, Piec
   while (s.begin < s.end) {
     p.seen = seen_by_warp(a, s.sent);
     p.units = p.seen.units();
-    const int64_t in = s.begin - s.first, seg = in >> 32 ? in / p.units : (int64_t)((uint32_t)in / (uint32_t)p.units);
+    const int in = s.begin - s.first, seg = (int)((uint32_t)in / (uint32_t)p.units);
     if (seg >= segments) {
-      s.first += (int64_t)p.units * segments;
+      s.first += p.units * segments;
       ++s.sent;
       continue;
     }
     p.sent = s.sent;
     p.len = length_of(a, s.sent);
-    p.kvh = (int)seg / a.row_tiles;
-    p.rt = (int)seg - p.kvh * a.row_tiles;
+    p.kvh = a.row_tiles == 1 ? seg : seg / a.row_tiles;
+    p.rt = seg - p.kvh * a.row_tiles;
     p.start = s.first + seg * p.units;
-    p.u0 = (int)(s.begin - p.start);
-    p.u1 = (int)min((int64_t)p.units, s.end - p.start);
+    p.u0 = s.begin - p.start;
+    p.u1 = min(p.units, s.end - p.start);
     s.begin = p.start + p.u1;
     if (p.units <= s.whole) {
       s.begin = p.start + p.units;
@@ -308,203 +346,303 @@ __device__ __forceinline__ bool next_piece(const AttendParams& a, Share& s, Piec
 }
 
 // ---- shared memory
-template <int D>
+// A piece that is ready to be worked on: its queries and rows are in place.
+struct Ready {
+  int sent, kvh, rt, len;
+  int chunks;              // -1: there are no more pieces
+  int c0, n1, b0;          // chunk i is chunk_at(c0 + i) of the sentence
+  int whole, part, from;   // part: which of the CTA's two places in the workspace it has; from: first CTA of the segment that ends with it, -1: it ends with another
+  __device__ __forceinline__ int position(int i) const { return (c0 + i < n1 ? c0 + i : b0 + c0 + i - n1) * kChunk; }
+};
+constexpr int kQueryAlong = 128 + 16;        // bytes between cores of the queries along the sum: a lane's four (two) components of them meet different banks
+template <int D, int R>
 struct Shared {
-  static constexpr int S = kStages<D>, kPart = kChunk * D;
-  static constexpr int kAcross = 8 * 16 * kBlocks;                 // bytes from eight columns of the weights to the next
-  alignas(128) unsigned char keys[S][kPart];
-  alignas(128) unsigned char values[S][kPart];
-  alignas(128) unsigned char queries[kQueryCols * D];              // (behind the values: with 64 components a product's lower half reads a block further, into rows of O that nobody looks at)
-  alignas(128) unsigned char weights[kWeightCols / 8 * kAcross];
-  alignas(16) float scales[S][kBlocks][4];
-  float m[kRows], l[kRows], by[kRows], slope[kRows], centre[kRows];
-  int lo[kRows], span[kRows], bad[kRows];
-  float most[2][kWeightWarps][kRows];
-  unsigned valid[S];
+  static constexpr int KS = kKeyStages<D, R>, VS = kValueStages<D, R>;
+  alignas(128) unsigned char keys[KS][kChunk * D];
+  alignas(128) unsigned char values[VS][kChunk * D];
+  alignas(128) unsigned char queries[2][kQueryCols<R> / 8 * D / 16 * kQueryAlong];      // (behind the values: with 64 components a product's lower half reads a block further, into rows of O that nobody looks at)
+  alignas(128) uint4 weights[R / 4][kChunk];                                            // four rows' 32 bits a position
+  alignas(128) float scales[VS][2][8][4];                                               // of four blocks, and as much again that is free
+  // of the rows of two pieces
+  alignas(16) float by[2][R], slope[2][R], centre[2][R];
+  alignas(16) int lo[2][R], span[2][R];
+  long long out[2][R];
+  int bad[2][R];
+  Ready ready[2];
+  // what the rows' weights are relative to, as it is and as it was before
+  alignas(16) float m[2][R], l[2][R], down_m[R], down_l[R], most_m[4][R], most_l[4][R];
+  unsigned valid[VS];
   int add, gave_up;
   uint32_t tmem;
-  alignas(8) unsigned long long k_full[S], k_empty[S], v_full[S], v_empty[S], s_full[2], s_empty[2], p_full, o_full, q_full;
+  alignas(8) unsigned long long k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], s_empty[2], q_full[2], q_empty[2], p_full, o_full;
 };
 
-// A component's number of rows: where row `at` of a sentence's head of the pool is in q and out.
-struct Place { int g, h; };
-__device__ __forceinline__ Place place_of(const AttendParams& a, const Piece& p, int r) {
-  const int at = p.rt * kRows + r, g = at / a.rep;
-  return {g, p.kvh * a.rep + at - g * a.rep};
-}
-
-__device__ __forceinline__ float load_as_float(const void* p, int64_t i, int dtype) {
-  return dtype == LINMT_F32 ? __ldg(static_cast<const float*>(p) + i) : dtype == LINMT_BF16 ? to_float(__ldg(static_cast<const __nv_bfloat16*>(p) + i)) : to_float(__ldg(static_cast<const __half*>(p) + i));
-}
 __device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float x) {
   if (dtype == LINMT_F32) static_cast<float*>(p)[i] = x;
   else if (dtype == LINMT_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
   else static_cast<__half*>(p)[i] = __float2half_rn(x);
 }
 
-// N neighbouring components of a row, 16-byte aligned (q_wide) or not.
-template <int N>
-__device__ __forceinline__ void load_row(const AttendParams& a, int64_t at, float (&x)[N]) {
-  if (!a.q_wide) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = load_as_float(a.q, at + i, a.dtype);
-  } else if (a.dtype == LINMT_F32) {
-    const float4* const p = reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at);
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-      const float4 v = __ldg(p + i);
-      x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
+__device__ __forceinline__ float load_as_float(const void* p, int64_t i, int dtype) {
+  return dtype == LINMT_F32 ? __ldg(static_cast<const float*>(p) + i) : dtype == LINMT_BF16 ? to_float(__ldg(static_cast<const __nv_bfloat16*>(p) + i)) : to_float(__ldg(static_cast<const __half*>(p) + i));
+}
+// Four neighbouring rows' numbers.
+__device__ __forceinline__ void four(const float* p, float (&x)[4]) {
+  const float4 v = *reinterpret_cast<const float4*>(p);
+  x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+}
+__device__ __forceinline__ void four(const int* p, int (&x)[4]) {
+  const int4 v = *reinterpret_cast<const int4*>(p);
+  x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+}
+__device__ __forceinline__ float power_of_2(int e) { return __int_as_float((127 + e) << 23); }      // -126 .. 127
+
+// A piece's queries as bytes, what its rows see and where their results go; by a warp, a lane for two or four neighbouring components of each row.
+template <int D, int R>
+__device__ __forceinline__ void take_queries(const AttendParams& a, const Piece& p, Shared<D, R>& sh, int buffer) {
+  constexpr int N = D / 32, kAtOnce = R < 8 ? R : 8;
+  const int lane = threadIdx.x & 31, n_rows = min(R, a.g * a.rep - p.rt * R);
+  int64_t from;                                       // of row `lane`; rows that are not there have another's queries, and their products are multiplied by 0
+  {
+    const int at = p.rt * R + min(lane, n_rows - 1), g = at / a.rep, h = p.kvh * a.rep + at - g * a.rep;
+    const bool have = lane < n_rows;
+    const int64_t by_row = (int64_t)p.sent * a.g + g;
+    from = p.sent * a.q_n + g * a.q_g + h * a.q_h;
+    if (lane < R) {
+      const int lo = a.first && have ? max(__ldg(a.first + by_row), 0) : 0, hi = a.first && have ? min(__ldg(a.last + by_row), p.len) : p.len;
+      sh.slope[buffer][lane] = have && a.slope ? __ldg(a.slope + h) * kLog2e : 0.f;
+      sh.centre[buffer][lane] = have && a.slope ? __ldg(a.centre + by_row) : 0.f;
+      sh.lo[buffer][lane] = lo;
+      sh.span[buffer][lane] = max(hi - lo, 0);
+      sh.out[buffer][lane] = p.sent * a.o_n + g * a.o_g + h * a.o_h;
     }
-  } else {
-    const uint4* const p = reinterpret_cast<const uint4*>(static_cast<const __half*>(a.q) + at);
+  }
 #pragma unroll
-    for (int i = 0; i < N / 8; ++i) {
-      const uint4 v = __ldg(p + i);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  for (int r0 = 0; r0 < R; r0 += kAtOnce) {
+    // All rows' loads before the first is looked at.
+    float x[kAtOnce][N];
+    int64_t at[kAtOnce];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 two = a.dtype == LINMT_BF16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[j])) : __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-        x[8 * i + 2 * j] = two.x;
-        x[8 * i + 2 * j + 1] = two.y;
+    for (int j = 0; j < kAtOnce; ++j) at[j] = __shfl_sync(~0u, (long long)from, r0 + j) + lane * N;
+    if (!a.q_wide) {
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j)
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[j][i] = load_as_float(a.q, at[j] + i, a.dtype);
+    } else if (a.dtype == LINMT_F32) {
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const float* const q = static_cast<const float*>(a.q) + at[j];
+        if constexpr (N == 4) {
+          const float4 v = __ldg(reinterpret_cast<const float4*>(q));
+          x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
+        } else {
+          const float2 v = __ldg(reinterpret_cast<const float2*>(q));
+          x[j][0] = v.x; x[j][1] = v.y;
+        }
+      }
+    } else {
+      uint32_t raw[kAtOnce][N / 2];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const unsigned short* const q = static_cast<const unsigned short*>(a.q) + at[j];
+        if constexpr (N == 4) {
+          const uint2 v = __ldg(reinterpret_cast<const uint2*>(q));
+          raw[j][0] = v.x; raw[j][1] = v.y;
+        } else {
+          raw[j][0] = __ldg(reinterpret_cast<const uint32_t*>(q));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j)
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+          const float2 v = a.dtype == LINMT_BF16 ? make_float2(__uint_as_float(raw[j][i / 2] << 16), __uint_as_float(raw[j][i / 2] & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&raw[j][i / 2]));
+          x[j][i] = v.x;
+          x[j][i + 1] = v.y;
+        }
+    }
+    // The rows' largest components, each in a lane, and what it takes to bring them below 2^22: 2^e <= the largest < 2^(e + 1), components times 2^(21 - e).  (Below 2^-106 it stays
+    // at that of 2^-106.)
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(x[j][i]) & 0x7fffffff);
+      m = __reduce_max_sync(~0u, m);
+      if (lane == j) most = m;
+    }
+    const bool bad = most >= 0x7f800000;
+    const int e = bad ? 0 : max((int)(most >> 23) - 127, -106);
+    const float up = bad ? 0.f : power_of_2(21 - e);
+    if (lane < kAtOnce) {
+      sh.by[buffer][r0 + lane] = r0 + lane < n_rows ? a.mul * power_of_2((e - 21) / 2) * power_of_2(e - 21 - (e - 21) / 2) : 0.f;
+      sh.bad[buffer][r0 + lane] = bad;
+    }
+    // Digits to the base 256, -128 .. 127: with 128 added to each, the bytes of the sum.
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int r = r0 + j;
+      const float by = __shfl_sync(~0u, up, j);
+      uint32_t u[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) u[i] = (uint32_t)(__float2int_rn(x[j][i] * by) + 0x808080) ^ 0x808080;
+      auto place = [&](int k) { return sh.queries[buffer] + ((k * R + r) / 8 * (D / 16) + lane * N / 16) * kQueryAlong + (k * R + r) % 8 * 16 + lane * N % 16; };
+      if constexpr (N == 4) {
+        const uint32_t low01 = __byte_perm(u[0], u[1], 0x5140), low23 = __byte_perm(u[2], u[3], 0x5140);
+        *reinterpret_cast<uint32_t*>(place(0)) = __byte_perm(low01, low23, 0x5410);
+        *reinterpret_cast<uint32_t*>(place(1)) = __byte_perm(low01, low23, 0x7632);
+        *reinterpret_cast<uint32_t*>(place(2)) = __byte_perm(__byte_perm(u[0], u[1], 0x0062), __byte_perm(u[2], u[3], 0x0062), 0x5410);
+      } else {
+        const uint32_t low = __byte_perm(u[0], u[1], 0x5140);
+        *reinterpret_cast<uint16_t*>(place(0)) = (uint16_t)low;
+        *reinterpret_cast<uint16_t*>(place(1)) = (uint16_t)(low >> 16);
+        *reinterpret_cast<uint16_t*>(place(2)) = (uint16_t)__byte_perm(u[0], u[1], 0x0062);
       }
     }
   }
 }
 
-__device__ __forceinline__ float power_of_2(int e) { return __int_as_float((127 + e) << 23); }      // -126 .. 127
-
-// The piece's queries as bytes, and what its rows see; by the 128 threads of the weights, eight for a row.
-template <int D>
-__device__ __forceinline__ void take_queries(const AttendParams& a, const Piece& p, Shared<D>& sh) {
-  constexpr int N = D / 8;
-  const int tid = threadIdx.x, r = tid / 8, part = tid % 8, n_rows = min(kRows, a.g * a.rep - p.rt * kRows);
-  const bool have = r < n_rows;
-  const Place at = place_of(a, p, have ? r : 0);
-  float x[N], most = 0.f;
-  if (have) {
-    load_row<N>(a, p.sent * a.q_n + at.g * a.q_g + at.h * a.q_h + part * N, x);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = 0.f;
-  }
-#pragma unroll
-  for (int i = 0; i < N; ++i) most = max_nan(most, fabsf(x[i]));
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) most = max_nan(most, __shfl_xor_sync(~0u, most, o));
-  const bool bad = !(most < INFINITY);
-  const int e = most > 0.f && !bad ? ilogbf(most) : 0;              // 2^e <= most < 2^(e + 1); components times 2^(21 - e) are below 2^22
-  const float up0 = power_of_2((21 - e) / 2), up1 = power_of_2(21 - e - (21 - e) / 2);
-  uint32_t d[kQueryDigits][N / 4];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    int v = bad ? 0 : __float2int_rn(x[i] * up0 * up1);
-#pragma unroll
-    for (int k = 0; k < kQueryDigits; ++k) {
-      const int low = (int)(int8_t)v;
-      v = (v - low) >> 8;
-      if (i % 4 == 0) d[k][i / 4] = 0;
-      d[k][i / 4] |= (uint32_t)(low & 255) << (8 * (i % 4));
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < kQueryDigits; ++k) {
-    const int n = k * kRows + r, c = part * N;
-    uint32_t* const to = reinterpret_cast<uint32_t*>(sh.queries + n / 8 * 8 * D + c / 16 * 128 + n % 8 * 16 + c % 16);
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) to[i] = d[k][i];
-  }
-  if (part == 0) {
-    sh.m[r] = sh.l[r] = kLowest;
-    sh.by[r] = have ? ldexpf(a.mul, e - 21) : 0.f;
-    sh.bad[r] = bad;
-    sh.slope[r] = have && a.slope ? __ldg(a.slope + at.h) * kLog2e : 0.f;
-    sh.centre[r] = have && a.slope ? __ldg(a.centre + (int64_t)p.sent * a.g + at.g) : 0.f;
-    const int lo = a.first && have ? max(__ldg(a.first + (int64_t)p.sent * a.g + at.g), 0) : 0, hi = a.first && have ? min(__ldg(a.last + (int64_t)p.sent * a.g + at.g), p.len) : p.len;
-    sh.lo[r] = lo;
-    sh.span[r] = max(hi - lo, 0);
-  }
-}
-
-// What a row's weights are relative to behind a chunk, from the warps' largest exponents: `was` as long as none exceeds it by more than 1.
-template <int D>
-__device__ __forceinline__ float raised(const Shared<D>& sh, int which, int r, float was, float above) {
-  const float most = fmaxf(fmaxf(sh.most[which][0][r], sh.most[which][1][r]), fmaxf(sh.most[which][2][r], sh.most[which][3][r]));
-  return most - was > 1.f ? ceilf(most) + above : was;
-}
-
-template <int D, int HOW>
-__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_constant__ AttendParams a) {
+template <int D, int R, int HOW>
+__global__ void __launch_bounds__(kThreads<R>) __maxnreg__(65536 / (kThreads<R> * kCtas<R>) / 8 * 8) attend_kernel(const __grid_constant__ AttendParams a, const __grid_constant__ AttendMaps maps) {
   extern __shared__ __align__(128) unsigned char attend_smem[];
-  Shared<D>& sh = *reinterpret_cast<Shared<D>*>(attend_smem);
-  constexpr int S = kStages<D>;
+  Shared<D, R>& sh = *reinterpret_cast<Shared<D, R>*>(attend_smem);
+  constexpr int KS = kKeyStages<D, R>, VS = kValueStages<D, R>, kPart = R * (D + 2), RT = kRows<R>, kWeights = 32 * kWeightWarps<R>, kCopyWarp = kWeightWarps<R>, kIssueWarp = kCopyWarp + 1;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(~0u, tid >> 5, 0);
   if (tid == 0) {
-    for (int i = 0; i < S; ++i) {
+    for (int i = 0; i < KS; ++i) {
       bar_init(shared(&sh.k_full[i]), 1);
       bar_init(shared(&sh.k_empty[i]), 1);
+    }
+    for (int i = 0; i < VS; ++i) {
       bar_init(shared(&sh.v_full[i]), 1);
       bar_init(shared(&sh.v_empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       bar_init(shared(&sh.s_full[i]), 1);
-      bar_init(shared(&sh.s_empty[i]), kWeightWarps);
+      bar_init(shared(&sh.s_empty[i]), kWeightWarps<R>);
+      bar_init(shared(&sh.q_full[i]), 1);
+      bar_init(shared(&sh.q_empty[i]), 1 + kWeightWarps<R>);
     }
-    bar_init(shared(&sh.p_full), kWeightWarps);
+    bar_init(shared(&sh.p_full), kWeightWarps<R>);
     bar_init(shared(&sh.o_full), 1);
-    bar_init(shared(&sh.q_full), kWeightWarps);
     sh.gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == kIssueWarp) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared(&sh.tmem)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared(&sh.tmem)), "r"(kTmemCols<R>) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   launch_next();
-  Share share = share_of(a, gridDim.x);
+  Share share = share_of<kThreads<R>>(a, gridDim.x);
   tmem_before();
   __syncthreads();
   tmem_after();
   const uint32_t tmem = sh.tmem;
   volatile int* const gave_up = &sh.gave_up;
-  Piece p;
-  int4 ends = make_int4(-1, 0, 0, 0);                 // the segment that ends in this share and began before it: sentence, head, row tile, first CTA
 
   if (warp == kCopyWarp) {
-    // ---- blocks into the rings, a lane for each of a chunk's
-    int it = 0;
+    // ---- blocks into the rings, four with a copy where the pool is rows of whole blocks (eight documents of 20-32k: 110 us with a bulk copy for each
+    // block's keys, values and scales, which a warp issues every 50 to 100 cycles); behind a piece's first chunk its queries
+    const bool elected = elect_one();
+    Piece p;
+    int it = 0, pieces = 0;
+    auto announce = [&](int chunks) {
+      const int buffer = pieces & 1;
+      bar_wait(shared(&sh.q_empty[buffer]), (pieces >> 1 & 1) ^ 1, gave_up);
+      __syncwarp();
+      if (!*gave_up) {
+        if (chunks > 0) take_queries<D, R>(a, p, sh, buffer);
+        if (lane == 0) {
+          Ready& r = sh.ready[buffer];
+          r.chunks = chunks;
+          if (chunks >= 0) {
+            r.sent = p.sent; r.kvh = p.kvh; r.rt = p.rt; r.len = p.len;
+            r.c0 = p.c0; r.n1 = p.seen.n1; r.b0 = p.seen.b0;
+            r.whole = p.whole();
+            r.part = p.u0 == 0;
+            r.from = !p.whole() && p.u0 > 0 && p.u1 == p.units ? p.start / share.per : -1;
+          }
+        }
+        if (chunks == 0 && lane < R) {                 // (nothing to multiply: only where the zeros go)
+          const int at = min(p.rt * R + lane, a.g * a.rep - 1), g = at / a.rep;
+          sh.out[buffer][lane] = p.sent * a.o_n + g * a.o_g + (p.kvh * a.rep + at - g * a.rep) * a.o_h;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) bar_arrive(shared(&sh.q_full[buffer]));
+      }
+      ++pieces;
+    };
     while (next_piece(a, share, p)) {
-      const unsigned char* const head = a.data + p.kvh * a.stride_head;
       const int32_t* const table = a.table + p.sent * a.table_stride;
       const int blocks = (p.len + pages8::kBlock - 1) / pages8::kBlock, per_page = a.page / pages8::kBlock;
+      auto page_at = [&](int c, int& in) {            // page and block of it that the lane has of a chunk, -1: none
+        const int block = p.seen.chunk(c) * kBlocks + lane, column = block / per_page;
+        in = block - column * per_page;
+        const int page = c < p.c1 && lane < kBlocks && block < blocks ? __ldg(table + column) : -1;
+        return page < a.n_pages ? page : -1;
+      };
+      int next_in, next = page_at(p.c0, next_in);
       for (int c = p.c0; c < p.c1; ++c, ++it) {
-        const int stage = it % S, block = p.seen.chunk(c) * kBlocks + lane;
-        const uint32_t parity = (uint32_t)(it / S & 1) ^ 1;
-        const int64_t at = lane < kBlocks && block < blocks ? pages8::block_offset(table, block, per_page, a.n_pages, a.stride_page, D) : -1;
-        const unsigned valid = __ballot_sync(~0u, at >= 0);
-        const int count = __popc(valid);
-        bar_wait(shared(&sh.k_empty[stage]), parity, gave_up);
-        __syncwarp();
-        if (!*gave_up) {
-          if (lane == 0) bar_expect(shared(&sh.k_full[stage]), count * 16 * D);
+        const int ks = it % KS, vs = it % VS, page = next, in = next_in;
+        const unsigned valid = __ballot_sync(~0u, page >= 0);
+        next = page_at(c + 1, next_in);
+        const uint32_t k_full = shared(&sh.k_full[ks]), v_full = shared(&sh.v_full[vs]), to_k = shared(sh.keys[ks]), to_v = shared(sh.values[vs]);
+        if (a.rows) {
+          // A row that is not there reads as zeros.
+          const int row = page >= 0 ? page * a.row_page + p.kvh * a.row_head + in : a.rows;
+          int r[kBlocks];
+#pragma unroll
+          for (int i = 0; i < kBlocks; ++i) r[i] = __shfl_sync(~0u, row, i);
+          bar_wait(shared(&sh.k_empty[ks]), (it / KS & 1) ^ 1, gave_up);
           __syncwarp();
-          if (at >= 0) copy_bulk(shared(sh.keys[stage] + lane * 16 * D), head + at, 16 * D, shared(&sh.k_full[stage]));
-        }
-        bar_wait(shared(&sh.v_empty[stage]), parity, gave_up);
-        __syncwarp();
-        if (!*gave_up) {
-          if (lane == 0) {
-            sh.valid[stage] = valid;
-            bar_expect(shared(&sh.v_full[stage]), count * (16 * D + 16));
+          if (elected && !*gave_up) {
+            bar_expect(k_full, kBlocks * 16 * D);
+            copy_rows(to_k, &maps.codes, 0, r[0], r[1], r[2], r[3], k_full);
+            copy_rows(to_k + 4 * 16 * D, &maps.codes, 0, r[4], r[5], r[6], r[7], k_full);
           }
+          bar_wait(shared(&sh.v_empty[vs]), (it / VS & 1) ^ 1, gave_up);
           __syncwarp();
-          if (at >= 0) {
-            copy_bulk(shared(sh.values[stage] + lane * 16 * D), head + at + pages8::value_codes(D), 16 * D, shared(&sh.v_full[stage]));
-            copy_bulk(shared(sh.scales[stage][lane]), head + at + pages8::scales(D), 16, shared(&sh.v_full[stage]));
+          if (elected && !*gave_up) {
+            sh.valid[vs] = valid;
+            bar_expect(v_full, kBlocks * (16 * D + 16));
+            copy_rows(shared(sh.scales[vs][0]), &maps.scales, 32 * D / 8, r[0], r[1], r[2], r[3], v_full);
+            copy_rows(shared(sh.scales[vs][1]), &maps.scales, 32 * D / 8, r[4], r[5], r[6], r[7], v_full);
+            copy_rows(to_v, &maps.codes, 16 * D / 8, r[0], r[1], r[2], r[3], v_full);
+            copy_rows(to_v + 4 * 16 * D, &maps.codes, 16 * D / 8, r[4], r[5], r[6], r[7], v_full);
+          }
+        } else {
+          const unsigned char* const block = a.data + page * a.stride_page + p.kvh * a.stride_head + (int64_t)in * pages8::block_bytes(D);
+          const int count = __popc(valid);
+          bar_wait(shared(&sh.k_empty[ks]), (it / KS & 1) ^ 1, gave_up);
+          __syncwarp();
+          if (!*gave_up) {
+            if (lane == 0) bar_expect(k_full, count * 16 * D);
+            __syncwarp();
+            if (page >= 0) copy_bulk(to_k + lane * 16 * D, block, 16 * D, k_full);
+          }
+          bar_wait(shared(&sh.v_empty[vs]), (it / VS & 1) ^ 1, gave_up);
+          __syncwarp();
+          if (!*gave_up) {
+            if (lane == 0) {
+              sh.valid[vs] = valid;
+              bar_expect(v_full, count * (16 * D + 16));
+            }
+            __syncwarp();
+            if (page >= 0) {
+              copy_bulk(shared(sh.scales[vs][lane / 4][lane % 4]), block + pages8::scales(D), 16, v_full);
+              copy_bulk(to_v + lane * 16 * D, block + pages8::value_codes(D), 16 * D, v_full);
+            }
           }
         }
+        if (c == p.c0) announce(p.c1 - p.c0);
       }
+      if (p.c0 == p.c1) announce(0);
     }
+    announce(-1);
     if (*gave_up) {                                   // what is on its way still lands in this CTA's memory
       const unsigned long long t0 = clock64();
       while ((unsigned long long)clock64() - t0 < kWaitCycles / 100) {}
@@ -512,155 +650,196 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
   } else if (warp == kIssueWarp) {
     // ---- the products
     const bool elected = elect_one();
-    int it = 0, queries = 0;
+    int it = 0;
     auto weights_times_values = [&](int i) {
-      const int stage = i % S;
+      const int vs = i % VS;
       bar_wait(shared(&sh.p_full), i & 1, gave_up);
-      bar_wait(shared(&sh.v_full[stage]), i / S & 1, gave_up);
+      bar_wait(shared(&sh.v_full[vs]), i / VS & 1, gave_up);
       __syncwarp();
       tmem_after();
       if (elected && !*gave_up) {
         const uint32_t add = *(volatile int*)&sh.add;
-        const uint64_t left = operand(shared(sh.values[stage]), 16 * D, 128), right = operand(shared(sh.weights), 128, Shared<D>::kAcross);
+        const uint64_t left = operand(shared(sh.values[vs]), 16 * D, 128), right = operand(shared(sh.weights), 128, 16 * kChunk);
 #pragma unroll
         for (int k = 0; k < kChunk / 32; ++k)
-          mma_bytes(tmem + kTmemO, left + (uint64_t)(k * 2 * 16 * D >> 4), right + (uint64_t)(k * 2 * 128 >> 4), form_of(kWeightCols, false), k ? 1u : add);
-        commit(shared(&sh.v_empty[stage]));
+          mma_bytes(tmem + kTmemO<R>, left + (uint64_t)(k * 2 * 16 * D >> 4), right + (uint64_t)(k * 4 * 128 >> 4), kWeightForm<R>, k ? 1u : add);
+        commit(shared(&sh.v_empty[vs]));
         commit(shared(&sh.o_full));
       }
       __syncwarp();
     };
-    while (next_piece(a, share, p)) {
-      if (p.c0 == p.c1) continue;
-      bar_wait(shared(&sh.q_full), queries++ & 1, gave_up);
-      for (int c = p.c0; c < p.c1; ++c, ++it) {
-        const int stage = it % S, half = it & 1;
-        bar_wait(shared(&sh.k_full[stage]), it / S & 1, gave_up);
+    for (int pieces = 0;; ++pieces) {
+      const int buffer = pieces & 1;
+      bar_wait(shared(&sh.q_full[buffer]), pieces >> 1 & 1, gave_up);
+      const int chunks = *(volatile int*)&sh.ready[buffer].chunks;
+      if (chunks < 0 || *gave_up) break;
+      for (int c = 0; c < chunks; ++c, ++it) {
+        const int ks = it % KS, half = it & 1;
+        bar_wait(shared(&sh.k_full[ks]), it / KS & 1, gave_up);
         bar_wait(shared(&sh.s_empty[half]), (it >> 1 & 1) ^ 1, gave_up);
         __syncwarp();
         tmem_after();
         if (elected && !*gave_up) {
-          const uint64_t left = operand(shared(sh.keys[stage]), 128, 8 * D), right = operand(shared(sh.queries), 128, 8 * D);
+          const uint64_t left = operand(shared(sh.keys[ks]), 128, 8 * D), right = operand(shared(sh.queries[buffer]), kQueryAlong, D / 16 * kQueryAlong);
 #pragma unroll
           for (int k = 0; k < D / 32; ++k)
-            mma_bytes(tmem + half * kTmemS, left + (uint64_t)(k * 2 * 128 >> 4), right + (uint64_t)(k * 2 * 128 >> 4), form_of(kQueryCols, true), k ? 1u : 0u);
-          commit(shared(&sh.k_empty[stage]));
+            mma_bytes(tmem + half * kQueryCols<R>, left + (uint64_t)(k * 2 * 128 >> 4), right + (uint64_t)(k * 2 * kQueryAlong >> 4), kQueryForm<R>, k ? 1u : 0u);
+          commit(shared(&sh.k_empty[ks]));
           commit(shared(&sh.s_full[half]));
+          if (c + 1 == chunks) commit(shared(&sh.q_empty[buffer]));
         }
         __syncwarp();
-        if (c > p.c0) weights_times_values(it - 1);
+        if (c > 0) weights_times_values(it - 1);
       }
-      weights_times_values(it - 1);
+      if (chunks) weights_times_values(it - 1);
+      else if (lane == 0) bar_arrive(shared(&sh.q_empty[buffer]));
     }
   } else {
     // ---- scores to weights, a position for each thread; then a component for each thread
-    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-    int it = 0;
-    while (next_piece(a, share, p)) {
-      const int n_rows = min(kRows, a.g * a.rep - p.rt * kRows);
-      float sum[kRows], acc[kRows];
+    const int mine = tid & (kChunk - 1), row0 = warp / 4 * RT;      // the thread's position, or component, and its first row
+    const uint32_t lanes = tmem + ((uint32_t)(warp % 4 * 32) << 16);
+    const float slack = (float)a.slack, unit = power_of_2(a.slack - 31);
+    int it = 0, pieces = 0;
+    int4 ends = make_int4(-1, 0, 0, 0);               // the segment that ends in this share and began before it: sentence, head, row tile, first CTA
+    for (;; ++pieces) {
+      const int buffer = pieces & 1;
+      bar_wait(shared(&sh.q_full[buffer]), pieces >> 1 & 1, gave_up);
+      if (weights_any<kWeights>(*gave_up)) break;
+      const Ready p = sh.ready[buffer];
+      if (p.chunks < 0) break;
+      const int n_rows = min(R, a.g * a.rep - p.rt * R);
+      int now = 0, since = 0;                         // which of m and l; chunks in O
+      if (tid < R) sh.m[0][tid] = sh.l[0][tid] = kLowest;
+      weights_sync<kWeights>();
+      float sum[RT], acc[RT];
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) sum[r] = acc[r] = 0.f;
-      weights_sync();                                 // (the piece before is written: its rows' numbers are free)
-      if (p.c0 < p.c1) {
-        take_queries<D>(a, p, sh);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        weights_sync();
-        if (lane == 0) bar_arrive(shared(&sh.q_full));
-      }
-      int since = 0;                                  // chunks in O
-      // O's integers into sums, which are relative to 2^m then.
-      auto drain = [&](const float (&down)[kRows]) {
-        tmem_after();
-#pragma unroll
-        for (int i = 0; i < kRows / 4; ++i) {
-          int o[16];
-          tmem_load16(lanes + kTmemO + 16 * i, o);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r = 4 * i + j;
-            const float v = fmaf((float)o[4 * j + 3], 16777216.f, fmaf((float)o[4 * j + 2], 65536.f, fmaf((float)o[4 * j + 1], 256.f, (float)o[4 * j])));
-            acc[r] = fmaf(v, 9.3132257461547852e-10f, acc[r]) * down[r];       // 2^-30
-          }
-        }
-        tmem_before();
-        since = 0;
-      };
-      for (int c = p.c0; c < p.c1; ++c, ++it) {
-        const int stage = it % S, half = it & 1;
-        bar_wait(shared(&sh.v_full[stage]), it / S & 1, gave_up);
-        bar_wait(shared(&sh.s_full[half]), it >> 1 & 1, gave_up);
-        tmem_after();
-        int t[kQueryCols];
-        tmem_load48(lanes + half * kTmemS, t);
-        tmem_before();
-        __syncwarp();
-        if (lane == 0) bar_arrive(shared(&sh.s_empty[half]));
+      for (int r = 0; r < RT; ++r) sum[r] = acc[r] = 0.f;
+      for (int c = 0;; ++c, ++it) {
+        const bool last = c == p.chunks;
+        if (last && since == 0) break;
+        float s[RT], ve = 0.f, vf = 0.f;
+        bool over = last || since == kDrain;
+        if (!last) {
+          const int vs = it % VS, half = it & 1;
+          bar_wait(shared(&sh.v_full[vs]), it / VS & 1, gave_up);
+          bar_wait(shared(&sh.s_full[half]), it >> 1 & 1, gave_up);
+          tmem_after();
+          int t[kQueryDigits][RT];
+          tmem_load(lanes + half * kQueryCols<R> + row0, R, t);
+          tmem_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(shared(&sh.s_empty[half]));
 
-        const int at = tid / pages8::kBlock, pos = p.seen.chunk(c) * kChunk + tid;
-        // A block that is not there has left whatever was in its place before; what lies behind a sentence's end may be anything.
-        const bool there = pos < p.len && (sh.valid[stage] >> at & 1);
-        const float ks = there ? sh.scales[stage][at][0] : 0.f, none = there ? 0.f : -INFINITY;
-        const uint32_t vs = there ? __float_as_uint(sh.scales[stage][at][1]) : 0;
-        // the values' scale as 2^ve times 2^-30 vf
-        const float ve = vs ? (float)((int)(vs >> 23 & 255) - 127) : -1000.f, vf = vs ? __uint_as_float((vs & 0x7fffff) | (127 + 30) << 23) : 0.f;
-        float s[kRows], most = -INFINITY;
+          const int at = mine / pages8::kBlock, pos = p.position(c) + mine;
+          // A block that is not there has left whatever was in its place before; what lies behind a sentence's end may be anything.
+          const bool there = pos < p.len && (sh.valid[vs] >> at & 1);
+          const float2 scales = *reinterpret_cast<const float2*>(sh.scales[vs][at / 4][at % 4]);
+          const float ks = there ? scales.x : 0.f, none = there ? 0.f : -INFINITY;
+          const uint32_t scale = there ? __float_as_uint(scales.y) : 0;
+          // the values' scale as 2^ve times vf, and in vf 1 / unit
+          ve = scale ? (float)((int)(scale >> 23 & 255) - 127) : -1000.f;
+          vf = scale ? __uint_as_float((scale & 0x7fffff) | (uint32_t)(127 + 31 - a.slack) << 23) : 0.f;
+          float most = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-          const float whole = fmaf((float)t[2 * kRows + r], 65536.f, (float)(t[kRows + r] * 256 + t[r])), by = sh.by[r] * ks;
-          if constexpr (HOW == kPlain) {
-            s[r] = fmaf(whole, by, none);
-          } else {
-            float x = whole * by;
-            if constexpr (HOW == kQuick) {
-              if (a.cap > 0.f) x = capped(x, a.cap * kLog2e);
-            } else {
-              if (a.cap > 0.f) x = a.cap * kLog2e * tanhf(x);
+          for (int r4 = 0; r4 < RT; r4 += 4) {
+            float by[4], m[4], l[4], slope[4], centre[4];
+            int lo[4], span[4];
+            four(sh.by[buffer] + row0 + r4, by);
+            four(sh.m[now] + row0 + r4, m);
+            four(sh.l[now] + row0 + r4, l);
+            if constexpr (HOW != kPlain) {
+              four(sh.slope[buffer] + row0 + r4, slope);
+              four(sh.centre[buffer] + row0 + r4, centre);
             }
-            s[r] = x - sh.slope[r] * fabsf((float)pos - sh.centre[r]) + none;
-          }
-          if (a.first) s[r] = (unsigned)(pos - sh.lo[r]) < (unsigned)sh.span[r] || pos < a.sinks ? s[r] : -INFINITY;
-          most = fmaxf(most, fmaxf(s[r] + (ve - sh.m[r]), s[r] - sh.l[r]));
-        }
-        // Something exceeds what the rows' weights are relative to: that follows.
-        if (weights_any(most > 1.f) || since == kDrain) {
+            if (a.first) {
+              four(sh.lo[buffer] + row0 + r4, lo);
+              four(sh.span[buffer] + row0 + r4, span);
+            }
 #pragma unroll
-          for (int r = 0; r < kRows; ++r) {
-            const float both = warp_max(s[r] + ve), alone = warp_max(s[r]);
-            if (lane == 0) {
-              sh.most[0][warp][r] = both;
-              sh.most[1][warp][r] = alone;
+            for (int j = 0; j < 4; ++j) {
+              const int r = r4 + j;
+              const float whole = fmaf((float)t[2][r], 65536.f, (float)(t[1][r] * 256 + t[0][r]));
+              if constexpr (HOW == kPlain) {
+                s[r] = fmaf(whole, by[j] * ks, none);
+              } else {
+                float x = whole * (by[j] * ks);
+                if constexpr (HOW == kQuick) {
+                  if (a.cap > 0.f) x = capped(x, a.cap * kLog2e);
+                } else {
+                  if (a.cap > 0.f) x = a.cap * kLog2e * tanhf(x);
+                }
+                s[r] = x - slope[j] * fabsf((float)pos - centre[j]) + none;
+              }
+              if (a.first) s[r] = (unsigned)(pos - lo[j]) < (unsigned)span[j] || pos < a.sinks ? s[r] : -INFINITY;
+              most = fmaxf(most, fmaxf(s[r] + (ve - m[j]), s[r] - l[j]));
             }
           }
-          weights_sync();
-          float down[kRows];
+          over = weights_any<kWeights>(most > slack) || over;
+          if (c > 0) bar_wait(shared(&sh.o_full), it - 1 & 1, gave_up);
+          // Something exceeds what the rows' weights are relative to: that follows.
+          if (over) {
+            float most_m = kLowest, most_l = kLowest;      // of row row0 + lane
 #pragma unroll
-          for (int r = 0; r < kRows; ++r) {
-            down[r] = exp2_of(sh.m[r] - raised(sh, 0, r, sh.m[r], 0.f));
-            sum[r] *= exp2_of(sh.l[r] - raised(sh, 1, r, sh.l[r], kAbove));
+            for (int r = 0; r < RT; ++r) {
+              const float x = warp_max(s[r] + ve), y = warp_max(s[r]);
+              if (lane == r) { most_m = x; most_l = y; }
+            }
+            if (lane < RT) { sh.most_m[warp % 4][row0 + lane] = most_m; sh.most_l[warp % 4][row0 + lane] = most_l; }
+            weights_sync<kWeights>();
+            if (tid < R) {
+              const float was_m = sh.m[now][tid], was_l = sh.l[now][tid];
+              float m = fmaxf(fmaxf(sh.most_m[0][tid], sh.most_m[1][tid]), fmaxf(sh.most_m[2][tid], sh.most_m[3][tid]));
+              float l = fmaxf(fmaxf(sh.most_l[0][tid], sh.most_l[1][tid]), fmaxf(sh.most_l[2][tid], sh.most_l[3][tid]));
+              m = m - was_m > slack ? ceilf(m) : was_m;
+              l = l - was_l > slack ? ceilf(l) + kAbove : was_l;
+              sh.m[now ^ 1][tid] = m;
+              sh.l[now ^ 1][tid] = l;
+              sh.down_m[tid] = exp2_of(was_m - m);
+              sh.down_l[tid] = exp2_of(was_l - l);
+            }
+            weights_sync<kWeights>();
+            now ^= 1;
           }
-          weights_sync();
-          if (tid < kRows) {
-            sh.m[tid] = raised(sh, 0, tid, sh.m[tid], 0.f);
-            sh.l[tid] = raised(sh, 1, tid, sh.l[tid], kAbove);
-          }
-          if (c > p.c0) bar_wait(shared(&sh.o_full), it - 1 & 1, gave_up);
-          if (since) drain(down);
-          else {
-#pragma unroll
-            for (int r = 0; r < kRows; ++r) acc[r] *= down[r];
-          }
-          weights_sync();
-        } else if (c > p.c0) {
+        } else {
           bar_wait(shared(&sh.o_full), it - 1 & 1, gave_up);
         }
-        unsigned char* const to = sh.weights + at * 128 + tid % 16;
+        if (over) {
+          // O's integers into sums, which are relative to 2^m then.
+          tmem_after();
+          int o[kWeightDigits * RT];
+          if (since) tmem_load(lanes + kTmemO<R> + kWeightDigits * row0, o);
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-          sum[r] += exp2_of(s[r] - sh.l[r]);
-          const uint32_t w = __float2uint_rn(exp2_of(s[r] + (ve - sh.m[r])) * vf);
+          for (int r4 = 0; r4 < RT; r4 += 4) {
+            float down_m[4], down_l[4];
+            four(sh.down_m + row0 + r4, down_m);
+            four(sh.down_l + row0 + r4, down_l);
 #pragma unroll
-          for (int d = 0; d < kWeightDigits; ++d) to[(r * kWeightDigits + d) / 8 * Shared<D>::kAcross + (r * kWeightDigits + d) % 8 * 16] = (unsigned char)(w >> (8 * d));
+            for (int j = 0; j < 4; ++j) {
+              const int* const x = o + 4 * (r4 + j);
+              const float v = fmaf((float)x[3], 16777216.f, fmaf((float)x[2], 65536.f, fmaf((float)x[1], 256.f, (float)x[0])));
+              if (since) acc[r4 + j] = fmaf(v, unit, acc[r4 + j]);
+              if (!last) {
+                acc[r4 + j] *= down_m[j];
+                sum[r4 + j] *= down_l[j];
+              }
+            }
+          }
+          tmem_before();
+          since = 0;
+        }
+        if (last) break;
+#pragma unroll
+        for (int r4 = 0; r4 < RT; r4 += 4) {
+          float m[4], l[4];
+          uint32_t w[4];
+          four(sh.m[now] + row0 + r4, m);
+          four(sh.l[now] + row0 + r4, l);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            sum[r4 + j] += exp2_of(s[r4 + j] - l[j]);
+            w[j] = __float2uint_rn(exp2_of(s[r4 + j] + (ve - m[j])) * vf);
+          }
+          sh.weights[(row0 + r4) / 4][mine] = make_uint4(w[0], w[1], w[2], w[3]);
         }
         if (tid == 0) sh.add = since > 0;
         ++since;
@@ -668,59 +847,85 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
         __syncwarp();
         if (lane == 0) bar_arrive(shared(&sh.p_full));
       }
-      if (p.c0 < p.c1) bar_wait(shared(&sh.o_full), it - 1 & 1, gave_up);
-      if (since) {
-        float as_is[kRows];
-#pragma unroll
-        for (int r = 0; r < kRows; ++r) as_is[r] = 1.f;
-        drain(as_is);
-      }
       // The rows' sums of weights, and out with it.
+      if (p.chunks) {
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
+        for (int r = 0; r < RT; ++r) {
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) sum[r] += __shfl_xor_sync(~0u, sum[r], o);
-        if (lane == 0) sh.most[0][warp][r] = sum[r];
-      }
-      weights_sync();
-      const bool whole = p.whole();
-      if (tid == 0 && !whole && p.u0 > 0 && p.u1 == p.units) ends = make_int4(p.sent, p.kvh, p.rt, (int)(p.start / share.per));
-      // a part of the workspace: [row][D] values, [row] exponent, [row] weight.  A CTA's first is of the segment that it has from the CTA before, its second of the one that the next goes on with.
-      float* const ws = a.ws + ((int64_t)blockIdx.x * 2 + (p.u0 == 0)) * (kRows * (D + 2));
-      const bool empty = p.c0 == p.c1;
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        if (r >= n_rows) break;
-        float weight = empty ? 0.f : (sh.most[0][0][r] + sh.most[0][1][r] + sh.most[0][2][r] + sh.most[0][3][r]) * 1099511627776.f;      // 2^40
-        const float m = empty ? 0.f : sh.m[r], l = empty ? kLowest : sh.l[r] - kAbove;
-        float value = weight > 0.f ? acc[r] / weight * exp2_of(m - l) : 0.f;
-        if (!empty && ((sh.bad[r] && weight > 0.f) || *gave_up)) value = weight = NAN;
-        if (whole) {
-          const Place at = place_of(a, p, r);
-          if (tid < D) store_as(a.out, p.sent * a.o_n + at.g * a.o_g + at.h * a.o_h + tid, a.dtype, value);
-          if (tid == 0 && a.lse) a.lse[((int64_t)p.sent * a.g + at.g) * a.heads + at.h] = weight == 0.f ? -INFINITY : (l + log2f(weight)) * kLn2;
-        } else {
-          if (tid < D) ws[r * D + tid] = value;
-          if (tid == 0) { ws[kRows * D + r] = l; ws[kRows * D + kRows + r] = weight; }
+          for (int o = 1; o < 32; o <<= 1) sum[r] += __shfl_xor_sync(~0u, sum[r], o);
+          if (lane == r) sh.most_m[warp % 4][row0 + r] = sum[r];
         }
       }
+      weights_sync<kWeights>();
+      // a part of the workspace: [row][D] values, [row] exponent, [row] weight.  A CTA's first is of the segment that it has from the CTA before, its second of the one that the next goes on with.
+      float* const ws = a.ws + ((int64_t)blockIdx.x * 2 + p.part) * kPart;
+      if (tid < R) {
+        float weight = 0.f, l = kLowest, f = 0.f;
+        if (p.chunks) {
+          weight = (sh.most_m[0][tid] + sh.most_m[1][tid] + sh.most_m[2][tid] + sh.most_m[3][tid]) * 1099511627776.f;      // 2^40
+          l = sh.l[now][tid] - kAbove;
+          f = weight > 0.f ? exp2_of(sh.m[now][tid] - l) / weight : 0.f;
+          if ((sh.bad[buffer][tid] && weight > 0.f) || *gave_up) f = weight = NAN;
+        }
+        sh.down_m[tid] = f;
+        if (tid < n_rows) {
+          if (p.whole) {
+            const int row = p.rt * R + tid, g = row / a.rep;
+            if (a.lse) a.lse[((int64_t)p.sent * a.g + g) * a.heads + p.kvh * a.rep + row - g * a.rep] = weight == 0.f ? -INFINITY : (l + log2f(weight)) * kLn2;
+          } else {
+            ws[R * D + tid] = l;
+            ws[R * D + R + tid] = weight;
+          }
+        }
+      }
+      weights_sync<kWeights>();
+      if (mine < D) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const float value = acc[r] * sh.down_m[row0 + r];
+          if (row0 + r < n_rows) {
+            if (p.whole) store_as(a.out, sh.out[buffer][row0 + r] + mine, a.dtype, value);
+            else ws[(row0 + r) * D + mine] = value;
+          }
+        }
+      }
+      if (p.from >= 0) ends = make_int4(p.sent, p.kvh, p.rt, p.from);
+      __syncwarp();
+      if (lane == 0) bar_arrive(shared(&sh.q_empty[buffer]));
     }
-    if (a.ws && tid == 0) reinterpret_cast<int4*>(a.ws + (int64_t)gridDim.x * 2 * (kRows * (D + 2)))[blockIdx.x] = ends;
+    if (*gave_up) {                                   // what there is from here on is NaN
+      Piece p;
+      for (Share s = share; next_piece(a, s, p);) {
+        for (int r = 0; r < min(R, a.g * a.rep - p.rt * R); ++r) {
+          const int row = p.rt * R + r, g = row / a.rep, h = p.kvh * a.rep + row - g * a.rep;
+          if (p.whole()) {
+            if (tid < D) store_as(a.out, p.sent * a.o_n + g * a.o_g + h * a.o_h + tid, a.dtype, NAN);
+            if (tid == 0 && a.lse) a.lse[((int64_t)p.sent * a.g + g) * a.heads + h] = NAN;
+          } else if (tid == 0) {
+            float* const ws = a.ws + ((int64_t)blockIdx.x * 2 + (p.u0 == 0)) * kPart;
+            ws[R * D + r] = 0.f;
+            ws[R * D + R + r] = NAN;
+          }
+        }
+        if (!p.whole() && p.u0 > 0 && p.u1 == p.units) ends = make_int4(p.sent, p.kvh, p.rt, p.start / s.per);
+      }
+    }
+    if (a.ws && tid == 0) reinterpret_cast<int4*>(a.ws + (int64_t)gridDim.x * 2 * kPart)[blockIdx.x] = ends;
   }
   tmem_before();
   __syncthreads();
-  if (warp == kIssueWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  if (warp == kIssueWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols<R>) : "memory");
 }
 
 // Joins the parts of the segment that ends in a CTA's share and began in one before: a CTA for each of attend's.  A thread has four components of a row, in one of kBy
 // parts in turn.
 constexpr int kJoinThreads = 512;
-template <int D>
+template <int D, int R>
 __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_constant__ AttendParams a, int blocks) {
-  constexpr int kPart = kRows * (D + 2), kBy = kJoinThreads / (kRows * D / 4);
-  __shared__ float s_top[kBy][kRows], s_weight[kBy][kRows];
-  __shared__ float4 s_sum[kBy][kRows * D / 4];
-  const int at = threadIdx.x % (kRows * D / 4), by = threadIdx.x / (kRows * D / 4), r = at / (D / 4), d = at % (D / 4) * 4;
+  constexpr int kPart = R * (D + 2), kBy = kJoinThreads / (R * D / 4);
+  __shared__ float s_top[kBy][R], s_weight[kBy][R];
+  __shared__ float4 s_sum[kBy][R * D / 4];
+  const int at = threadIdx.x % (R * D / 4), by = threadIdx.x / (R * D / 4), r = at / (D / 4), d = at % (D / 4) * 4;
   wait_for_last();
   const int4 ends = reinterpret_cast<const int4*>(a.ws + (int64_t)blocks * 2 * kPart)[blockIdx.x];
   if (ends.x < 0) return;
@@ -737,8 +942,8 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
       m[j] = kLowest;
       if (i0 + j * kBy < n_parts) {
         const float* const w = part(i0 + j * kBy);
-        m[j] = w[kRows * D + r];
-        l[j] = w[kRows * D + kRows + r];
+        m[j] = w[R * D + r];
+        l[j] = w[R * D + R + r];
         v[j] = *reinterpret_cast<const float4*>(w + r * D + d);
       }
     }
@@ -760,7 +965,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
   s_sum[by][at] = sum;
   if (d == 0) { s_top[by][r] = top; s_weight[by][r] = weight; }
   __syncthreads();
-  if (by || r >= a.g * a.rep - ends.z * kRows) return;
+  if (by || r >= a.g * a.rep - ends.z * R) return;
 #pragma unroll
   for (int i = 1; i < kBy; ++i) top = fmaxf(top, s_top[i][r]);
   sum = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -772,7 +977,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
     sum.x += f * v.x; sum.y += f * v.y; sum.z += f * v.z; sum.w += f * v.w;
     weight += f * s_weight[i][r];
   }
-  const int row = ends.z * kRows + r, g = row / a.rep, h = ends.y * a.rep + row - g * a.rep;
+  const int row = ends.z * R + r, g = row / a.rep, h = ends.y * a.rep + row - g * a.rep;
   const float f = weight == 0.f ? 0.f : 1.f / weight;
   const int64_t to = ends.x * a.o_n + g * a.o_g + h * a.o_h + d;
   store_as(a.out, to, a.dtype, sum.x * f);
@@ -782,16 +987,16 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
   if (d == 0 && a.lse) a.lse[((int64_t)ends.x * a.g + g) * a.heads + h] = weight == 0.f ? -INFINITY : (top + log2f(weight)) * kLn2;
 }
 
-template <int D>
-cudaError_t launch_attend(AttendParams p, float scale, int blocks, cudaStream_t st) {
-  constexpr int smem = (int)sizeof(Shared<D>);
-  static_assert(smem <= 113 << 10, "two CTAs have to fit on an SM");
+template <int D, int R>
+cudaError_t launch_attend(AttendParams p, const AttendMaps& maps, float scale, int blocks, cudaStream_t st) {
+  constexpr int smem = (int)sizeof(Shared<D, R>);
+  static_assert((smem + 1280) * kCtas<R> <= 228 << 10, "so many CTAs have to fit on an SM");
   const Scores how = p.cap == 0.f && !p.slope ? kPlain : p.dtype == LINMT_F32 || p.cap > kQuickCap ? kExact : kQuick;
-  void (*const kernel)(AttendParams) = how == kPlain ? attend_kernel<D, kPlain> : how == kQuick ? attend_kernel<D, kQuick> : attend_kernel<D, kExact>;
+  void (*const kernel)(AttendParams, AttendMaps) = how == kPlain ? attend_kernel<D, R, kPlain> : how == kQuick ? attend_kernel<D, R, kQuick> : attend_kernel<D, R, kExact>;
   p.mul = (float)(p.cap == 0.f ? scale * 1.4426950408889634 : how == kQuick ? scale * 2.8853900817779268 / p.cap : (double)scale / p.cap);
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  kernel<<<(unsigned)blocks, kThreads, smem, st>>>(p);
+  kernel<<<(unsigned)blocks, kThreads<R>, smem, st>>>(p, maps);
   e = cudaGetLastError();
   if (e != cudaSuccess || !p.ws) return e;
   cudaLaunchConfig_t cfg{};
@@ -803,21 +1008,59 @@ cudaError_t launch_attend(AttendParams p, float scale, int blocks, cudaStream_t 
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, attend_join_kernel<D>, p, blocks);
+  e = cudaLaunchKernelEx(&cfg, attend_join_kernel<D, R>, p, blocks);
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
-int row_tiles_of(const linmt_attend_pages8_args* g) { return (int)(((int64_t)g->g * (g->heads / g->pages.heads) + kRows - 1) / kRows); }
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encoder() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess || r != cudaDriverEntryPointSuccess) p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+// The pool as a tensor of rows of blocks, where its strides are whole blocks; false where they are not.
+bool rows_of_blocks(const linmt_pages8& pool, AttendParams& p, AttendMaps& maps) {
+  const int64_t block = pages8::block_bytes(pool.dim);
+  const int64_t page = pool.n_pages > 1 ? pool.stride_page : 0, head = pool.heads > 1 ? pool.stride_head : 0;
+  if (page < 0 || head < 0 || page % block || head % block) return false;
+  const int64_t rows = (pool.n_pages - 1) * (page / block) + (pool.heads - 1) * (head / block) + pool.page / pages8::kBlock;
+  if (rows >= INT32_MAX || !encoder()) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)block / 8, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)block};
+  const cuuint32_t codes[2] = {(cuuint32_t)(2 * pool.dim), 1}, scales[2] = {2, 1}, step[2] = {1, 1};
+  auto encode = [&](CUtensorMap* map, const cuuint32_t* box) {
+    return encoder()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 2, pool.data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (!encode(&maps.codes, codes) || !encode(&maps.scales, scales)) return false;
+  p.row_page = (int)(page / block);
+  p.row_head = (int)(head / block);
+  p.rows = (int)rows;
+  return true;
+}
+
+// Rows of a head of the pool that go together: what there are, up to 16.
+int rows_of(const linmt_attend_pages8_args* g) { const int64_t all = (int64_t)g->g * (g->heads / g->pages.heads); return all <= 4 ? 4 : all <= 8 ? 8 : 16; }
+int row_tiles_of(const linmt_attend_pages8_args* g) { return (int)(((int64_t)g->g * (g->heads / g->pages.heads) + rows_of(g) - 1) / rows_of(g)); }
+template <int D>
+cudaError_t launch_rows(const AttendParams& p, const AttendMaps& maps, const linmt_attend_pages8_args* g, int blocks, cudaStream_t st) {
+  const int rows = rows_of(g);
+  return rows == 4 ? launch_attend<D, 4>(p, maps, g->scale, blocks, st) : rows == 8 ? launch_attend<D, 8>(p, maps, g->scale, blocks, st) : launch_attend<D, 16>(p, maps, g->scale, blocks, st);
+}
 
 int64_t chunks_at_most(const linmt_attend_pages8_args* g) { return ((int64_t)g->width * g->pages.page + kChunk - 1) / kChunk; }
 // CTAs: as many as fit on the GPU at once, or as the longest possible sentences give kWhole units each.
 int blocks_of(const linmt_attend_pages8_args* g) {
-  const int64_t segments = (int64_t)g->n * g->pages.heads * row_tiles_of(g), most = segments * ((chunks_at_most(g) + kFixed + kWhole - 1) / kWhole), fit = 148 * 2;
+  const int64_t segments = (int64_t)g->n * g->pages.heads * row_tiles_of(g), most = segments * ((chunks_at_most(g) + kFixed + kWhole - 1) / kWhole), fit = 148 * (rows_of(g) == 4 ? kCtas<4> : kCtas<16>);
   return (int)(most < fit ? most : fit);
 }
 // Two parts for each CTA, of the segments that it shares with the CTAs before and behind it, and what the join has to know.  None where no segment can be long enough to be cut.
 int64_t workspace_of(const linmt_attend_pages8_args* g) {
-  return chunks_at_most(g) + kFixed <= kWhole ? 0 : (int64_t)blocks_of(g) * (2 * (kRows * (g->pages.dim + 2)) * 4 + 16);
+  return chunks_at_most(g) + kFixed <= kWhole ? 0 : (int64_t)blocks_of(g) * (2 * (rows_of(g) * (g->pages.dim + 2)) * 4 + 16);
 }
 
 int check(const linmt_attend_pages8_args* g) {
@@ -833,8 +1076,8 @@ int check(const linmt_attend_pages8_args* g) {
   const int size = dtype_bytes(g->dtype);
   if (!aligned(g->q, size) || !aligned(g->out, size) || !aligned(g->lse, 4) || !aligned(g->table, 4) || !aligned(g->len, 4) || !aligned(g->slope, 4) || !aligned(g->centre, 4) || !aligned(g->first, 4) || !aligned(g->last, 4))
     return op_fail(LINMT_EINVAL, "attend_pages8: an array is not aligned to its type");
-  if ((int64_t)g->g * g->heads > INT32_MAX / 2 || (int64_t)g->n * g->pages.heads * row_tiles_of(g) > (1 << 24))
-    return op_fail(LINMT_ELIMIT, "attend_pages8: %d sentences of %d rows and %d heads are too many for one call", g->n, g->g, g->heads);
+  if ((int64_t)g->g * g->heads > INT32_MAX / 2 || (int64_t)g->n * g->pages.heads * row_tiles_of(g) > (1 << 24) || (int64_t)g->n * g->pages.heads * row_tiles_of(g) * (chunks_at_most(g) + kFixed) > INT32_MAX / 2)
+    return op_fail(LINMT_ELIMIT, "attend_pages8: %d sentences of %d rows, %d heads and %d columns of pages are too many for one call", g->n, g->g, g->heads, g->width);
   return LINMT_OK;
 }
 
@@ -859,13 +1102,15 @@ int linmt_attend_pages8(const linmt_attend_pages8_args* g) {
     return op_fail(LINMT_EINVAL, "attend_pages8: a workspace of %lld bytes is needed, 16-byte aligned", (long long)need);
   OnDevice on(g->device);
   if (on.err != cudaSuccess) return op_cuda(on.err, "attend_pages8");
-  const AttendParams p{static_cast<const unsigned char*>(g->pages.data), g->pages.stride_page, g->pages.stride_head, g->pages.n_pages, g->pages.heads, g->pages.page,
+  AttendParams p{static_cast<const unsigned char*>(g->pages.data), g->pages.stride_page, g->pages.stride_head, g->pages.n_pages, g->pages.heads, g->pages.page,
                        g->q, g->q_stride_n, g->q_stride_g, g->q_stride_h, g->out, g->out_stride_n, g->out_stride_g, g->out_stride_h, g->lse, g->table, g->table_stride, g->len,
                        g->slope, g->centre, g->first, g->last, need ? static_cast<float*>(g->workspace) : nullptr, g->n, g->g, g->heads, g->heads / g->pages.heads, g->width, row_tiles_of(g),
                        g->sinks, g->first && g->g <= 32 && (int64_t)g->n * g->g <= 65536, g->dtype,
-                       aligned(g->q, 16) && (g->q_stride_n | g->q_stride_g | g->q_stride_h) % (16 / dtype_bytes(g->dtype)) == 0, g->cap, 0.f};
+                       aligned(g->q, 16) && (g->q_stride_n | g->q_stride_g | g->q_stride_h) % (16 / dtype_bytes(g->dtype)) == 0, g->cap, 0.f, 0, 0, 0, g->dtype == LINMT_F32 ? 1 : 4};
+  AttendMaps maps{};
+  rows_of_blocks(g->pages, p, maps);
   const cudaStream_t st = static_cast<cudaStream_t>(g->stream);
-  const cudaError_t e = g->pages.dim == 64 ? launch_attend<64>(p, g->scale, blocks_of(g), st) : launch_attend<128>(p, g->scale, blocks_of(g), st);
+  const cudaError_t e = g->pages.dim == 64 ? launch_rows<64>(p, maps, g, blocks_of(g), st) : launch_rows<128>(p, maps, g, blocks_of(g), st);
   return e == cudaSuccess ? LINMT_OK : op_cuda(e, "attend_pages8");
 }
 
