@@ -1,16 +1,20 @@
 // pages8_ops.cu -- keys and values into and out of pages in 8 bits (linmt_write_pages8, linmt_read_pages8).  Attention over them: pages8_attend.cu.
 //
-// A scale belongs to a block of 16 positions, so positions of a block that are written together have to be looked at together: a CTA
-// takes the runs (neighbours in the list that are neighbours in a block) that begin among its positions, one after the other, head by head.  Half of its threads
-// have the keys, half the values, a thread 16 components of one position.  Keys go out as they come, 16 bytes a thread.  Values
-// lie position by position within a component and are turned round in shared memory.
-// A block is written whole: a position's value codes lie in every 32-byte sector of the block's half, so they would all be touched anyway.
+// A scale belongs to a block of 16 positions, so positions of a block that are written together have to be looked at together: a warp
+// has a run (neighbours in the list that are neighbours in a block) of one head, its keys or its values, and needs nothing from another.  Of keys a lane has
+// 16 components of a position at a time, of values two components of eight positions: two lanes exchange halves then and each has the 16 positions of
+// a component, as they lie in the block.  A block is written whole: a position's value codes lie in every 32-byte sector of the block's half, so they would all be touched anyway.
+// Bound by the bytes moved (a text), by latency (a step's positions).  (One CTA for a run with the values turned round in shared memory: 100,003 positions of 8 heads of 128 and back in 392 us.)
+#include <type_traits>
+
 #include "device_ops.h"
 #include "pages8.h"
 
 namespace linmt {
 namespace ops {
 namespace {
+
+constexpr int kWarps = 8;
 
 struct RowsParams {
   unsigned char* data;
@@ -23,56 +27,28 @@ struct RowsParams {
   int32_t t, heads_each, window;
 };
 
-struct Run {
-  int64_t at;              // the block's place in the pool (head 0); -1: slots outside it (of a read)
-  int first, len, offset;  // positions first .. first + len - 1 of the call are the block's offset ..
+// The runs that begin among a window's positions, one in each lane that `begins` names; of a read also slots outside the pool, as many of the window's as there are side by side.
+struct Runs {
+  uint32_t begins;
+  long long at;            // the block's place in the pool (head 0); -1: slots outside it
+  int offset, len;         // the run is the block's positions offset ..
 };
-
-// The runs that begin at the CTA's positions; of a read those among them alone.  All threads call it.
 template <bool WRITE, int D>
-__device__ __forceinline__ int runs_of_cta(const RowsParams& a, Run* runs) {
-  __shared__ int count;
-  if (threadIdx.x < 32) {
-    const int lane = threadIdx.x;
-    const int64_t t = (int64_t)blockIdx.x * a.window - 1 + lane;                       // lane 1 has the CTA's first position
-    const bool mine = lane >= 1 && lane <= a.window && t < a.t, there = t >= 0 && t < a.t && (WRITE || mine);
-    int64_t slot = there ? __ldg(a.slots + t) : -1;
-    if (pages8::slot_page(slot, a.n_pages, a.page) < 0) slot = -1;
-    const int64_t before = __shfl_up_sync(~0u, (long long)slot, 1);
-    const uint32_t goes_on = __ballot_sync(~0u, lane > 0 && there && pages8::follows(before, slot));
-    const bool begins = mine && (WRITE ? slot >= 0 : true) && !(goes_on >> lane & 1);
-    const uint32_t all = __ballot_sync(~0u, begins);
-    if (begins) {
-      Run r;
-      r.at = pages8::slot_block(slot, a.n_pages, a.page, a.stride_page, D);
-      r.first = (int)t;
-      r.offset = slot < 0 ? 0 : (int)(slot & (pages8::kBlock - 1));
-      r.len = lane == 31 ? 1 : __ffs(~(goes_on >> (lane + 1)));                        // (lane 31 begins a run with a window of 31 only, and there is none)
-      runs[__popc(all & ((1u << lane) - 1))] = r;
-    }
-    if (lane == 0) count = __popc(all);
-  }
-  __syncthreads();
-  return count;
-}
-
-// 16 components of a row.
-template <class T> struct Raw16 { uint4 r[sizeof(T)]; };
-template <class T>
-__device__ __forceinline__ Raw16<T> load16(const T* p) {
-  Raw16<T> x;
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T); ++i) x.r[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-  return x;
-}
-template <class T>
-__device__ __forceinline__ void store16(T* p, const float (&x)[16]) {
-  uint4 r[sizeof(T)];
-  T* e = reinterpret_cast<T*>(r);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) e[i] = from_float<T>(x[i]);
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T); ++i) reinterpret_cast<uint4*>(p)[i] = r[i];
+__device__ __forceinline__ Runs runs_of_window(const RowsParams& a, int window) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = (int64_t)window * a.window - 1 + lane;                           // lane 1 has the window's first position
+  const bool mine = lane >= 1 && lane <= a.window && t < a.t;
+  long long slot = t >= 0 && t < a.t ? __ldg(a.slots + t) : -1;
+  if (pages8::slot_page(slot, a.n_pages, a.page) < 0) slot = -1;
+  const long long before = __shfl_up_sync(~0u, slot, 1);
+  const bool outside = !WRITE && mine && slot < 0;
+  const uint32_t goes_on = __ballot_sync(~0u, lane > 0 && (pages8::follows(before, slot) || (outside && lane > 1 && before < 0)));
+  Runs r;
+  r.begins = __ballot_sync(~0u, (mine && slot >= 0 || outside) && !(goes_on >> lane & 1));
+  r.at = pages8::slot_block(slot, a.n_pages, a.page, a.stride_page, D);
+  r.offset = slot < 0 ? 0 : (int)(slot & (pages8::kBlock - 1));
+  r.len = lane == 31 ? 1 : __ffs(~(goes_on >> (lane + 1)));                          // (at most 16: a block's positions, or a window's)
+  return r;
 }
 
 constexpr float kMost = 1.7014118346046923e38f;      // 2^127
@@ -93,157 +69,252 @@ __device__ __forceinline__ float scale_of(float big) {
 
 // Codes of 16 components, as bytes.  A code is the quotient in 32 bits, rounded.  With the rounded reciprocal y of s, q = x y is one unit off at most and
 // q + (x - q s) y, each a fused multiply-add, is the correctly rounded quotient (P. Markstein, IBM J. Res. Dev. 34, 1990), as long as nothing underflows
-// on the way.
-__device__ __forceinline__ uint4 codes_of(const float (&x)[16], float s) {
-  if (s == 0.f) return make_uint4(0, 0, 0, 0);
+// on the way: not with scales from 2^-90 on, and smaller ones are brought there together with the components.
+struct Numbers { float v[16]; };
+template <bool ORDINARY = false>
+__device__ __forceinline__ uint4 codes_of(Numbers x, float s) {
+  if (!ORDINARY && s < 8.0779356694631609e-28f) {      // 2^-90
+    const float up = 1.2676506002282294e30f;           // 2^100
+    s *= up;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x.v[i] *= up;
+  }
+  const float y = ORDINARY || s > 0.f ? 1.f / s : 0.f;
   uint32_t b[16];
-  if (s > 1e-30f && s < 1e30f) {
-    const float y = 1.f / s;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float q = x[i] * y;
-      b[i] = __float_as_uint(fmaf(fmaf(-q, s, x[i]), y, q) + kMagic);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) b[i] = __float_as_uint(__fdiv_rn(x[i], s) + kMagic);
+  for (int i = 0; i < 16; ++i) {
+    const float q = x.v[i] * y;
+    b[i] = __float_as_uint(fmaf(fmaf(-q, s, x.v[i]), y, q) + kMagic);
   }
   auto four = [&](int i) { return __byte_perm(__byte_perm(b[i], b[i + 1], 0x0040), __byte_perm(b[i + 2], b[i + 3], 0x0040), 0x5410); };
   return make_uint4(four(0), four(4), four(8), four(12));
 }
-__device__ __forceinline__ float code_at(const uint4& c, int i) {
-  const uint32_t w = i < 4 ? c.x : i < 8 ? c.y : i < 12 ? c.z : c.w;
-  return (float)(int8_t)(w >> (8 * (i & 3)));
+// NaN as 0, sizes above 2^127 as 2^127.
+__device__ __forceinline__ void tame(Numbers& x) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x.v[i] = x.v[i] != x.v[i] ? 0.f : fminf(fmaxf(x.v[i], -kMost), kMost);
+}
+// What 16 codes stand for.  A byte below 2^23, its sign turned round, is a float's last bits.
+__device__ __forceinline__ Numbers values_of(const uint4& c, float s) {
+  const uint32_t w[4] = {c.x ^ 0x80808080u, c.y ^ 0x80808080u, c.z ^ 0x80808080u, c.w ^ 0x80808080u};
+  Numbers x;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x.v[i] = (__uint_as_float(__byte_perm(w[i >> 2], 0x4b000000u, 0x7440 + (i & 3))) - 8388736.f) * s;
+  return x;
 }
 // Codes for one scale as codes for another.
-__device__ __forceinline__ uint4 again(const uint4& c, float from, float to) {
-  if (from == to) return c;
-  float x[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = code_at(c, i) * from;
-  return codes_of(x, to);
-}
-// Bytes lo .. hi - 1 of 16.
-__device__ __forceinline__ uint32_t byte_mask(int lo, int hi, int word) {
-  auto below = [&](int n) { n -= 4 * word; return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1; };
-  return below(hi) & ~below(lo);
-}
-__device__ __forceinline__ uint4 bytes_between(const uint4& c, int lo, int hi) {
-  return make_uint4(c.x & byte_mask(lo, hi, 0), c.y & byte_mask(lo, hi, 1), c.z & byte_mask(lo, hi, 2), c.w & byte_mask(lo, hi, 3));
+__device__ __forceinline__ uint4 again(uint4 c, float from, float to) { return from == to ? c : codes_of(values_of(c, from), to); }
+// The first n of 16 bytes.
+__device__ __forceinline__ uint4 first_bytes(const uint4& c, int n) {
+  auto word = [&](uint32_t x, int i) { const int m = n - 4 * i; return m <= 0 ? 0u : m >= 4 ? x : x & ((1u << (8 * m)) - 1); };
+  return make_uint4(word(c.x, 0), word(c.y, 1), word(c.z, 2), word(c.w, 3));
 }
 
-// Where a component's 16 positions lie in shared memory: 16 components, and 16 bytes free, so that the eight threads of a position meet different banks.
-__device__ __forceinline__ int turned(int c) { return 16 * c + (c & ~15); }
-template <int D> constexpr int kTurned = 17 * D;
-
-template <class T, int D>
-__global__ void __launch_bounds__(2 * D) write_kernel(const RowsParams a) {
-  constexpr int U = D / 16;
-  __shared__ Run runs[32];
-  __shared__ float most[2][2 * D / 32];
-  __shared__ __align__(16) unsigned char turn[2][kTurned<D>];
-  const int tid = threadIdx.x, part = tid / D, in = tid % D, r = in / U, u = in % U, h0 = blockIdx.y * a.heads_each, h1 = min(a.heads, h0 + a.heads_each);
-  const int n_runs = runs_of_cta<true, D>(a, runs);
-  const T* const rows = static_cast<const T*>(part ? a.v : a.k);
-  const int64_t stride_t = part ? a.v_t : a.k_t, stride_h = part ? a.v_h : a.k_h;
-  int turns = 0;
-  for (int i = 0; i < n_runs; ++i) {
-    const Run run = runs[i];
-    const bool have = r >= run.offset && r < run.offset + run.len;
-    const T* from = rows + (int64_t)(run.first + (have ? r - run.offset : 0)) * stride_t + h0 * stride_h + 16 * u;
-    for (int h = h0; h < h1; ++h, from += stride_h, ++turns) {
-      unsigned char* const block = a.data + run.at + h * a.stride_head;
-      // The block as it was: the thread's key unit, or component `in`'s 16 values.
-      const uint4 was = run.offset ? *reinterpret_cast<const uint4*>(block + (part ? pages8::value_unit(in, D) : pages8::key_unit(r, u, D))) : make_uint4(0, 0, 0, 0);
-      const float old = run.offset ? *reinterpret_cast<const float*>(block + pages8::scales(D) + 4 * part) : 0.f;
-      float x[16], big = 0.f;
-      if (have) {
-        const Raw16<T> raw = load16(from);
-        const T* const e = reinterpret_cast<const T*>(raw.r);
+// N components as they are in memory, and as numbers.
+template <class T, int N> struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Raw { T v[N]; };
+template <class T, int N>
+__device__ __forceinline__ Raw<T, N> load(const T* p) {
+  Raw<T, N> x;
+  if constexpr (sizeof(x) >= 16) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          x[j] = to_float(e[j]);
-          x[j] = x[j] != x[j] ? 0.f : fminf(fmaxf(x[j], -kMost), kMost);
-          big = fmaxf(big, fabsf(x[j]));
-        }
-      } else {
+    for (int i = 0; i < (int)sizeof(x) / 16; ++i) reinterpret_cast<uint4*>(&x)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  } else if constexpr (sizeof(x) == 8) {
+    *reinterpret_cast<uint2*>(&x) = __ldg(reinterpret_cast<const uint2*>(p));
+  } else {
+    *reinterpret_cast<uint32_t*>(&x) = __ldg(reinterpret_cast<const uint32_t*>(p));
+  }
+  return x;
+}
+template <class T, int N>
+__device__ __forceinline__ void store(T* p, const float (&x)[N]) {
+  Raw<T, N> r;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = 0.f;
-      }
-      big = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(big)));           // (not negative: ordered as integers)
-      if ((tid & 31) == 0) most[turns & 1][tid / 32] = big;
-      __syncthreads();                                                                // (also: the readers of the turn before last are done with `turn`)
+  for (int i = 0; i < N; ++i) r.v[i] = from_float<T>(x[i]);
+  if constexpr (sizeof(r) >= 16) {
 #pragma unroll
-      for (int w = 0; w < D / 32; ++w) big = fmaxf(big, most[turns & 1][part * (D / 32) + w]);
-      const float s = fmaxf(scale_of(big), old);
-      const uint4 c = have ? codes_of(x, s) : make_uint4(0, 0, 0, 0);
-      if (part == 0) {
-        *reinterpret_cast<uint4*>(block + pages8::key_unit(r, u, D)) = have ? c : r < run.offset ? again(was, old, s) : make_uint4(0, 0, 0, 0);
-      } else if (have) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) turn[turns & 1][turned(16 * u + j) + r] = (unsigned char)((j < 4 ? c.x : j < 8 ? c.y : j < 12 ? c.z : c.w) >> (8 * (j & 3)));
-      }
-      __syncthreads();                                                                // (before a scale is written, too: all have read it)
-      if (part == 1) {
-        const uint4 now = bytes_between(*reinterpret_cast<const uint4*>(&turn[turns & 1][turned(in)]), run.offset, run.offset + run.len);
-        const uint4 kept = bytes_between(again(was, old, s), 0, run.offset);
-        *reinterpret_cast<uint4*>(block + pages8::value_unit(in, D)) = make_uint4(now.x | kept.x, now.y | kept.y, now.z | kept.z, now.w | kept.w);
-      }
-      if (in == 0) *reinterpret_cast<float*>(block + pages8::scales(D) + 4 * part) = s;
-      if (in == 1) *reinterpret_cast<float*>(block + pages8::scales(D) + 8 + 4 * part) = 0.f;
-    }
+    for (int i = 0; i < (int)sizeof(r) / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(&r)[i];
+  } else if constexpr (sizeof(r) == 8) {
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(&r);
+  } else {
+    *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(&r);
   }
 }
-
-template <class T, int D>
-__global__ void __launch_bounds__(2 * D) read_kernel(const RowsParams a) {
-  constexpr int U = D / 16;
-  __shared__ Run runs[32];
-  __shared__ __align__(16) unsigned char turn[2][kTurned<D>];
-  const int tid = threadIdx.x, part = tid / D, in = tid % D, r = in / U, u = in % U, h0 = blockIdx.y * a.heads_each, h1 = min(a.heads, h0 + a.heads_each);
-  const int n_runs = runs_of_cta<false, D>(a, runs);
-  T* const rows = static_cast<T*>(part ? a.v : a.k);
-  const int64_t stride_t = part ? a.v_t : a.k_t, stride_h = part ? a.v_h : a.k_h;
-  int turns = 0;
-  for (int i = 0; i < n_runs; ++i) {
-    const Run run = runs[i];
-    const bool have = r >= run.offset && r < run.offset + run.len;
-    T* to = rows + (int64_t)(run.first + (have ? r - run.offset : 0)) * stride_t + h0 * stride_h + 16 * u;
-    for (int h = h0; h < h1; ++h, to += stride_h, ++turns) {
-      const unsigned char* const block = a.data + run.at + h * a.stride_head;
-      float s = 0.f;
-      uint4 c = make_uint4(0, 0, 0, 0);
-      if (run.at >= 0) {
-        s = __ldg(reinterpret_cast<const float*>(block + pages8::scales(D)) + part);
-        c = __ldg(reinterpret_cast<const uint4*>(block + (part ? pages8::value_unit(in, D) : pages8::key_unit(r, u, D))));
-      }
-      if (part) *reinterpret_cast<uint4*>(&turn[turns & 1][turned(in)]) = c;
-      __syncthreads();                                                                // (one a turn: the readers of the turn before last have come here too)
-      if (have) {
-        float x[16];
+// The largest size of two, four, .. numbers, NaN if one is: as bits of a float, so that the larger size is the larger integer.
+template <int N>
+__device__ __forceinline__ uint32_t most_of(const Raw<float, N>& x) {
+  uint32_t m = 0;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = (part ? (float)(int8_t)turn[turns & 1][turned(16 * u + j) + r] : code_at(c, j)) * s;
-        store16(to, x);
+  for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(x.v[i]) & 0x7fffffff);
+  return m;
+}
+template <class T, class T2, int N>
+__device__ __forceinline__ uint32_t most_of_pairs(const Raw<T, N>& x) {
+  const T2* const p = reinterpret_cast<const T2*>(&x);
+  T2 m = __habs2(p[0]);
+#pragma unroll
+  for (int i = 1; i < N / 2; ++i) m = __hmax2_nan(m, __habs2(p[i]));
+  return max(__float_as_uint(to_float(T(m.x))) & 0x7fffffff, __float_as_uint(to_float(T(m.y))) & 0x7fffffff);
+}
+template <int N> __device__ __forceinline__ uint32_t most_of(const Raw<__nv_bfloat16, N>& x) { return most_of_pairs<__nv_bfloat16, __nv_bfloat162>(x); }
+template <int N> __device__ __forceinline__ uint32_t most_of(const Raw<__half, N>& x) { return most_of_pairs<__half, __half2>(x); }
+
+// Of eight positions of two components the lane's own component's 16: `mine` has the first component's codes in x, y and the other's in z, w; the neighbour has the other eight positions.
+__device__ __forceinline__ uint4 exchange(const uint4& mine, int h) {
+  const uint32_t g0 = __shfl_xor_sync(~0u, h ? mine.x : mine.z, 1), g1 = __shfl_xor_sync(~0u, h ? mine.y : mine.w, 1);
+  return h ? make_uint4(g0, g1, mine.z, mine.w) : make_uint4(mine.x, mine.y, g0, g1);
+}
+
+// One run of one head, its keys or its values, in turns of 16 codes a lane: of keys components 16 u .. of position r, of values components 2 c, 2 c + 1 of positions 8 h ..
+// FULL: the run is a whole block; where its largest component is not an ordinary one nothing is done, and false returned.
+template <class T, int D, bool VALUES, bool FULL>
+__device__ __forceinline__ bool write_run(unsigned char* block, const T* rows, int64_t stride_t, int offset, int len) {
+  constexpr int U = D / 16, kTurns = D / 32, kEach = VALUES ? 8 : 1, kPart = VALUES ? 2 : 16;
+  const int lane = threadIdx.x & 31, h = lane & 1, end = offset + len;
+  const float old = !FULL && offset ? *reinterpret_cast<const float*>(block + pages8::scales(D) + 4 * VALUES) : 0.f;
+  Raw<T, kPart> in[kTurns][kEach];
+  uint32_t most = 0;
+  // (of keys the lane's positions are 32 / U apart from turn to turn, of values its components 32)
+  const T* row = rows + (VALUES ? (8 * h - offset) * stride_t + 2 * (lane >> 1) : (lane / U - offset) * stride_t + 16 * (lane % U));
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      const int r = VALUES ? 8 * h + j : lane / U + 32 / U * i;
+      const T* const from = VALUES ? row + 32 * i : row + 32 / U * i * stride_t;
+      if constexpr (FULL) {
+        in[i][j] = load<T, kPart>(from);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kPart; ++e) in[i][j].v[e] = from_float<T>(0.f);
+        if (r >= offset && r < end) in[i][j] = load<T, kPart>(from);
       }
     }
+    if (VALUES) row += stride_t;
+  }
+#pragma unroll
+  for (int j = 0; j < kEach; ++j)
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) most = max(most, most_of(in[i][j]));
+  most = __reduce_max_sync(~0u, most);
+  auto numbers = [&](int i) {
+    Numbers x;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x.v[e] = VALUES ? to_float(in[i][e & (kEach - 1)].v[(e >> 3) & (kPart - 1)]) : to_float(in[i][0].v[e & (kPart - 1)]);
+    return x;
+  };
+  const bool wild = most > 0x7f000000u;                 // a NaN, or something above 2^127
+  if (FULL && (wild || most < 0x17000000u)) return false;       // (below 2^-81)
+  if (!FULL && wild) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      Numbers x = numbers(i);
+      tame(x);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(x.v[e]));
+    }
+    most = __reduce_max_sync(~0u, __float_as_uint(m));
+  }
+  const float s = fmaxf(scale_of(__uint_as_float(most)), old);
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) {
+    const int at = lane + 32 * i;
+    unsigned char* const to = block + (VALUES ? pages8::value_unit(at, D) : pages8::key_unit(at / U, at % U, D));
+    uint4 c = make_uint4(0, 0, 0, 0);
+    if (FULL || VALUES || (32 / U * i < end && 32 / U * (i + 1) > offset)) {
+      Numbers x = numbers(i);
+      if (!FULL && wild) tame(x);
+      c = codes_of<FULL>(x, s);
+    }
+    if constexpr (VALUES) c = exchange(c, h);
+    if (!FULL && offset) {
+      if constexpr (VALUES) {
+        const uint4 kept = first_bytes(again(*reinterpret_cast<const uint4*>(to), old, s), offset);
+        c = make_uint4(c.x | kept.x, c.y | kept.y, c.z | kept.z, c.w | kept.w);
+      } else if (at / U < offset) {
+        c = again(*reinterpret_cast<const uint4*>(to), old, s);
+      }
+    }
+    *reinterpret_cast<uint4*>(to) = c;
+  }
+  if (lane == 0) *reinterpret_cast<float*>(block + pages8::scales(D) + 4 * VALUES) = s;
+  if (lane == 1) *reinterpret_cast<float*>(block + pages8::scales(D) + 8 + 4 * VALUES) = 0.f;
+  return true;
+}
+
+template <class T, int D, bool VALUES, bool FULL>
+__device__ __forceinline__ bool read_run(const unsigned char* block, T* rows, int64_t stride_t, int offset, int len) {
+  constexpr int U = D / 16, kTurns = D / 32;
+  const int lane = threadIdx.x & 31, h = lane & 1;
+  float s = 0.f;
+  uint4 c[kTurns];
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) {
+    const int at = lane + 32 * i;
+    c[i] = FULL || block ? __ldg(reinterpret_cast<const uint4*>(block + (VALUES ? pages8::value_unit(at, D) : pages8::key_unit(at / U, at % U, D)))) : make_uint4(0, 0, 0, 0);
+  }
+  if (FULL || block) s = __ldg(reinterpret_cast<const float*>(block + pages8::scales(D)) + VALUES);
+  T* const row = rows + (VALUES ? (8 * h - offset) * stride_t + 2 * (lane >> 1) : (lane / U - offset) * stride_t + 16 * (lane % U));
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) {
+    if constexpr (VALUES) {
+      // Eight positions of the first component, then of the other.
+      const uint32_t g0 = __shfl_xor_sync(~0u, h ? c[i].x : c[i].z, 1), g1 = __shfl_xor_sync(~0u, h ? c[i].y : c[i].w, 1);
+      const Numbers x = values_of(h ? make_uint4(g0, g1, c[i].z, c[i].w) : make_uint4(c[i].x, c[i].y, g0, g1), s);
+      T* to = row + 32 * i;
+#pragma unroll
+      for (int j = 0; j < 8; ++j, to += stride_t) {
+        const int r = 8 * h + j;
+        const float two[2] = {x.v[j], x.v[8 + j]};
+        if (FULL || (r >= offset && r < offset + len)) store<T, 2>(to, two);
+      }
+    } else {
+      const int r = lane / U + 32 / U * i;
+      const Numbers x = values_of(c[i], s);
+      if (FULL || (r >= offset && r < offset + len)) store<T, 16>(row + 32 / U * i * stride_t, x.v);
+    }
+  }
+  return true;
+}
+
+template <bool WRITE, class T, int D>
+__global__ void __launch_bounds__(32 * kWarps, 3) rows_kernel(const RowsParams a) {
+  const int warp = threadIdx.x / 32, h0 = blockIdx.y * a.heads_each, units = 2 * (min(a.heads, h0 + a.heads_each) - h0);
+  const Runs runs = runs_of_window<WRITE, D>(a, blockIdx.x);
+  int unit = warp;
+  for (uint32_t left = runs.begins; left; left &= left - 1) {
+    const int l = __ffs(left) - 1;
+    const long long at = __shfl_sync(~0u, runs.at, l);
+    const int offset = __shfl_sync(~0u, runs.offset, l), len = __shfl_sync(~0u, runs.len, l);
+    const int64_t first = (int64_t)blockIdx.x * a.window + l - 1;
+    for (; unit < units; unit += kWarps) {              // (the warps go on with the next run where they end with this one)
+      const int head = h0 + unit / 2;
+      unsigned char* const block = at < 0 ? nullptr : a.data + at + head * a.stride_head;
+      T* const rows = unit & 1 ? static_cast<T*>(a.v) + first * a.v_t + head * a.v_h : static_cast<T*>(a.k) + first * a.k_t + head * a.k_h;
+      auto go = [&](auto values, auto full) {
+        const int64_t stride_t = values.value ? a.v_t : a.k_t;
+        if constexpr (WRITE) return write_run<T, D, values.value, full.value>(block, rows, stride_t, offset, len);
+        else return read_run<T, D, values.value, full.value>(block, rows, stride_t, offset, len);
+      };
+      const bool values = unit & 1;
+      if (len == pages8::kBlock && at >= 0 && (values ? go(std::true_type{}, std::true_type{}) : go(std::false_type{}, std::true_type{}))) continue;
+      if (values) go(std::true_type{}, std::false_type{});
+      else go(std::false_type{}, std::false_type{});
+    }
+    unit -= units;
   }
 }
 
 template <bool WRITE, class T>
 void launch_rows(RowsParams p, int dim, cudaStream_t st) {
-  // A step's positions each in a block of their own: a CTA for each, and each head.  Texts: 16 positions and, where that leaves some 16 CTAs for each SM all the same, several heads in
-  // turn, as looking at the slots takes as long as a head.
+  // A step's positions each in a block of their own: a window for each.  Texts: windows of 16 positions, and all heads by one CTA where that leaves some eight CTAs for each SM all
+  // the same, as looking at the slots takes as long as a run.
   p.window = (int64_t)p.t * p.heads <= 16 * 16 * 148 ? 1 : 16;
-  const int64_t windows = ((int64_t)p.t + p.window - 1) / p.window, each = windows * p.heads / (16 * 148);
-  p.heads_each = (int)(each < 1 ? 1 : each > p.heads ? p.heads : each);
+  const int64_t windows = ((int64_t)p.t + p.window - 1) / p.window, each = windows * p.heads / (8 * 148);
+  p.heads_each = (int)(each < 4 ? (p.heads < 4 ? p.heads : 4) : each > p.heads ? p.heads : each);
   const dim3 grid((unsigned)windows, (unsigned)((p.heads + p.heads_each - 1) / p.heads_each));
-  if (WRITE) {
-    if (dim == 64) write_kernel<T, 64><<<grid, 128, 0, st>>>(p);
-    else write_kernel<T, 128><<<grid, 256, 0, st>>>(p);
-  } else {
-    if (dim == 64) read_kernel<T, 64><<<grid, 128, 0, st>>>(p);
-    else read_kernel<T, 128><<<grid, 256, 0, st>>>(p);
-  }
+  if (dim == 64) rows_kernel<WRITE, T, 64><<<grid, 32 * kWarps, 0, st>>>(p);
+  else rows_kernel<WRITE, T, 128><<<grid, 32 * kWarps, 0, st>>>(p);
 }
 
 template <bool WRITE>
