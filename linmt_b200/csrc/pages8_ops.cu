@@ -242,18 +242,72 @@ __device__ __forceinline__ bool write_run(unsigned char* block, const T* rows, i
   return true;
 }
 
+// One position, as a step writes it: a lane has D / 32 of its components, neighbours of the keys and 32 apart of the values.
+template <class T, int D, bool VALUES>
+__device__ __forceinline__ void write_position(unsigned char* block, const T* row, int offset) {
+  constexpr int U = D / 16, kTurns = D / 32;
+  const int lane = threadIdx.x & 31;
+  const float old = offset ? *reinterpret_cast<const float*>(block + pages8::scales(D) + 4 * VALUES) : 0.f;
+  uint4 was[kTurns];
+  float x[kTurns];
+  uint32_t most = 0;
+  if constexpr (!VALUES) {
+    const Raw<T, kTurns> raw = load<T, kTurns>(row + kTurns * lane);
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) x[i] = to_float(raw.v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) {
+    if constexpr (VALUES) {
+      x[i] = to_float(__ldg(row + lane + 32 * i));
+      was[i] = offset ? *reinterpret_cast<const uint4*>(block + pages8::value_unit(lane + 32 * i, D)) : make_uint4(0, 0, 0, 0);
+    }
+    x[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -kMost), kMost);
+    most = max(most, __float_as_uint(fabsf(x[i])));
+  }
+  const float s = fmaxf(scale_of(__uint_as_float(__reduce_max_sync(~0u, most))), old);
+  uint32_t code[kTurns];
+#pragma unroll
+  for (int i = 0; i < kTurns; ++i) code[i] = __float_as_uint((s > 0.f ? __fdiv_rn(x[i], s) : 0.f) + kMagic) & 255;
+  if constexpr (VALUES) {
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      const uint32_t byte = code[i] << (8 * (offset & 3));
+      uint4 c = offset ? first_bytes(again(was[i], old, s), offset) : make_uint4(0, 0, 0, 0);
+      const int word = offset >> 2;
+      if (word == 0) c.x |= byte;
+      else if (word == 1) c.y |= byte;
+      else if (word == 2) c.z |= byte;
+      else c.w |= byte;
+      *reinterpret_cast<uint4*>(block + pages8::value_unit(lane + 32 * i, D)) = c;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+      const int at = lane + 32 * i, r = at / U;
+      uint4* const to = reinterpret_cast<uint4*>(block + pages8::key_unit(r, at % U, D));
+      if (r > offset) *to = make_uint4(0, 0, 0, 0);
+      else if (r < offset && old != s) *to = again(*to, old, s);
+    }
+    unsigned char* const to = block + pages8::key_unit(offset, kTurns * lane / 16, D) + kTurns * lane % 16;
+    if constexpr (kTurns == 4) *reinterpret_cast<uint32_t*>(to) = code[0] | code[1] << 8 | code[kTurns - 2] << 16 | code[kTurns - 1] << 24;
+    else *reinterpret_cast<uint16_t*>(to) = (uint16_t)(code[0] | code[1] << 8);
+  }
+  if (lane == 0) *reinterpret_cast<float*>(block + pages8::scales(D) + 4 * VALUES) = s;
+  if (lane == 1) *reinterpret_cast<float*>(block + pages8::scales(D) + 8 + 4 * VALUES) = 0.f;
+}
+
 template <class T, int D, bool VALUES, bool FULL>
 __device__ __forceinline__ bool read_run(const unsigned char* block, T* rows, int64_t stride_t, int offset, int len) {
   constexpr int U = D / 16, kTurns = D / 32;
   const int lane = threadIdx.x & 31, h = lane & 1;
-  float s = 0.f;
   uint4 c[kTurns];
 #pragma unroll
   for (int i = 0; i < kTurns; ++i) {
     const int at = lane + 32 * i;
-    c[i] = FULL || block ? __ldg(reinterpret_cast<const uint4*>(block + (VALUES ? pages8::value_unit(at, D) : pages8::key_unit(at / U, at % U, D)))) : make_uint4(0, 0, 0, 0);
+    c[i] = __ldg(reinterpret_cast<const uint4*>(block + (VALUES ? pages8::value_unit(at, D) : pages8::key_unit(at / U, at % U, D))));
   }
-  if (FULL || block) s = __ldg(reinterpret_cast<const float*>(block + pages8::scales(D)) + VALUES);
+  const float s = __ldg(reinterpret_cast<const float*>(block + pages8::scales(D)) + VALUES);
   T* const row = rows + (VALUES ? (8 * h - offset) * stride_t + 2 * (lane >> 1) : (lane / U - offset) * stride_t + 16 * (lane % U));
 #pragma unroll
   for (int i = 0; i < kTurns; ++i) {
@@ -277,6 +331,21 @@ __device__ __forceinline__ bool read_run(const unsigned char* block, T* rows, in
   return true;
 }
 
+// A few positions' values, byte by byte; and zeros for slots that are none.
+template <class T, int D>
+__device__ __forceinline__ void read_values(const unsigned char* block, T* rows, int64_t stride_t, int offset, int len) {
+  const int lane = threadIdx.x & 31;
+  const float s = __ldg(reinterpret_cast<const float*>(block + pages8::scales(D)) + 1);
+  for (int r = 0; r < len; ++r, rows += stride_t)
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) rows[lane + 32 * i] = from_float<T>((float)(signed char)__ldg(block + pages8::value_unit(lane + 32 * i, D) + offset + r) * s);
+}
+template <class T, int D>
+__device__ __forceinline__ void read_nothing(T* rows, int64_t stride_t, int len) {
+  constexpr int kUnits = D * (int)sizeof(T) / 16;
+  for (int i = threadIdx.x & 31; i < len * kUnits; i += 32) reinterpret_cast<uint4*>(rows + i / kUnits * stride_t)[i % kUnits] = make_uint4(0, 0, 0, 0);
+}
+
 template <bool WRITE, class T, int D>
 __global__ void __launch_bounds__(32 * kWarps, 3) rows_kernel(const RowsParams a) {
   const int warp = threadIdx.x / 32, h0 = blockIdx.y * a.heads_each, units = 2 * (min(a.heads, h0 + a.heads_each) - h0);
@@ -298,7 +367,14 @@ __global__ void __launch_bounds__(32 * kWarps, 3) rows_kernel(const RowsParams a
       };
       const bool values = unit & 1;
       if (len == pages8::kBlock && at >= 0 && (values ? go(std::true_type{}, std::true_type{}) : go(std::false_type{}, std::true_type{}))) continue;
-      if (values) go(std::true_type{}, std::false_type{});
+      if (WRITE && len == 1) {
+        if (values) write_position<T, D, true>(block, rows, offset);
+        else write_position<T, D, false>(block, rows, offset);
+      } else if (!WRITE && at < 0) {
+        read_nothing<T, D>(rows, values ? a.v_t : a.k_t, len);
+      } else if (!WRITE && values && len <= 4) {
+        read_values<T, D>(block, rows, a.v_t, offset, len);
+      } else if (values) go(std::true_type{}, std::false_type{});
       else go(std::false_type{}, std::false_type{});
     }
     unit -= units;
@@ -307,10 +383,10 @@ __global__ void __launch_bounds__(32 * kWarps, 3) rows_kernel(const RowsParams a
 
 template <bool WRITE, class T>
 void launch_rows(RowsParams p, int dim, cudaStream_t st) {
-  // A step's positions each in a block of their own: a window for each.  Texts: windows of 16 positions, and all heads by one CTA where that leaves some eight CTAs for each SM all
-  // the same, as looking at the slots takes as long as a run.
+  // A step's positions each in a block of their own: a window for each.  Texts: windows of 16 positions, and all heads by one CTA where that leaves 16 CTAs for each SM all
+  // the same, as looking at the slots takes as long as a run; four heads otherwise, a run of each for every warp.
   p.window = (int64_t)p.t * p.heads <= 16 * 16 * 148 ? 1 : 16;
-  const int64_t windows = ((int64_t)p.t + p.window - 1) / p.window, each = windows * p.heads / (8 * 148);
+  const int64_t windows = ((int64_t)p.t + p.window - 1) / p.window, each = windows * p.heads / (16 * 148);
   p.heads_each = (int)(each < 4 ? (p.heads < 4 ? p.heads : 4) : each > p.heads ? p.heads : each);
   const dim3 grid((unsigned)windows, (unsigned)((p.heads + p.heads_each - 1) / p.heads_each));
   if (dim == 64) rows_kernel<WRITE, T, 64><<<grid, 32 * kWarps, 0, st>>>(p);
