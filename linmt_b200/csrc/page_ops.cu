@@ -18,6 +18,7 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRows = 16384;
+constexpr int kRowBytes = 3 * (int)sizeof(int) + (int)sizeof(short);
 constexpr int kMaxCluster = 8;
 
 struct ForkParams {
@@ -65,74 +66,109 @@ __device__ __forceinline__ Stretch stretch_of(int n, int at, int of) {
   return {(int)min((int64_t)n, groups * at / of * 32), (int)min((int64_t)n, groups * (at + 1) / of * 32)};
 }
 
+// Every `all`-th place of a table from `at` on, kAtOnce at a time, so that as many loads are on their way: f(row, column, inside) for each.
+constexpr int kAtOnce = 4;
+template <class F>
+__device__ __forceinline__ void for_places(int rows, int width, int at, int all, const F& f) {
+  if (width == 0) return;
+  const int down = all / width, right = all - down * width;
+  int r = at / width, c = at - r * width;
+  while (r < rows) {
+    int rs[kAtOnce], cs[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      rs[i] = r;
+      cs[i] = c;
+      r += down;
+      c += right;
+      if (c >= width) { c -= width; ++r; }
+    }
+    f(rs, cs);
+  }
+}
+
 __global__ void __launch_bounds__(kThreads) fork_kernel(const ForkParams a) {
   const cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ int fork_smem[];
   int* const children = fork_smem;              // [rows]
   int* const first = fork_smem + a.rows;        // [rows] a row's first child
+  int* const lens = fork_smem + 2 * a.rows;     // [rows]
+  short* const parents = reinterpret_cast<short*>(fork_smem + 3 * a.rows);      // [rows], -1: none
   __shared__ int sums[kWarps], total;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks(), all = ctas * kThreads, at = rank * kThreads + tid;
-  auto parent_of = [&](int r) {
-    if (a.done && __ldg(a.done + r)) return -1;
-    if (!a.parents) return r;
-    const int p = __ldg(a.parents + r);
-    return p >= 0 && p < a.k ? r - r % a.k + p : -1;
+  auto sync = [&] {
+    if (ctas > 1) cluster.sync();
+    else __syncthreads();
   };
 
   // Who has which children: every CTA for all rows.
   for (int r = tid; r < a.rows; r += kThreads) {
     children[r] = 0;
     first[r] = 0x7fffffff;
+    lens[r] = length_of(a.len, r, a.width, a.page);
+    const int p = a.parents ? __ldg(a.parents + r) : r % a.k;
+    parents[r] = (short)(p < 0 || p >= a.k || (a.done && __ldg(a.done + r)) ? -1 : r - r % a.k + p);
   }
   if (a.out_shares != a.shares)
+#pragma unroll 4
     for (int64_t i = at; i < a.n_pages; i += all) a.out_shares[i] = __ldg(a.shares + i);
   if (a.out_free != a.free_pages)
+#pragma unroll 4
     for (int64_t i = at; i < a.n_free; i += all) a.out_free[i] = __ldg(a.free_pages + i);
   __syncthreads();
   for (int r = tid; r < a.rows; r += kThreads) {
-    const int p = parent_of(r);
+    const int p = parents[r];
     if (p < 0) continue;
     atomicAdd(children + p, 1);
     atomicMin(first + p, r);
   }
-  cluster.sync();
+  sync();
 
-  // What that does to the pages' shares, and the new rows but for pages that are copied, a warp for each row.
-  for (int r = rank * kWarps + warp; r < a.rows; r += ctas * kWarps) {
-    const int32_t* const from = a.table + r * a.table_stride;
-    const int len = length_of(a.len, r, a.width, a.page), have = pages_of(len, a.page), more = children[r] - 1, half = len % a.page ? have - 1 : -1;
-    if (more != 0)
-      for (int c = lane; c < have; c += 32) {
-        const int g = __ldg(from + c), by = c == half ? min(more, 0) : more;
-        if (g >= 0 && g < a.n_pages && by) atomicAdd(a.out_shares + g, by);
-      }
-    const int p = parent_of(r), up_len = p >= 0 ? length_of(a.len, p, a.width, a.page) : 0, up = pages_of(up_len, a.page);
-    const int32_t* const take = a.table + (p >= 0 ? p : 0) * a.table_stride;
-    for (int c = lane; c < a.width; c += 32) {
-      const int g = c < up ? __ldg(take + c) : -1;
-      a.out_table[r * a.out_table_stride + c] = g >= 0 && g < a.n_pages ? g : -1;
+  // What that does to the pages' shares, and the new rows but for pages that are copied.
+  for_places(a.rows, a.width, at, all, [&](const int (&r)[kAtOnce], const int (&c)[kAtOnce]) {
+    int by[kAtOnce], page[kAtOnce], take[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      by[i] = 0;
+      take[i] = -1;
+      if (r[i] >= a.rows) continue;
+      const int len = lens[r[i]], have = pages_of(len, a.page), more = children[r[i]] - 1, p = parents[r[i]];
+      if (c[i] < have) by[i] = len % a.page && c[i] == have - 1 ? min(more, 0) : more;
+      if (by[i]) page[i] = __ldg(a.table + r[i] * a.table_stride + c[i]);
+      if (p >= 0 && c[i] < pages_of(lens[p], a.page)) take[i] = __ldg(a.table + p * a.table_stride + c[i]);
     }
-    if (lane == 0) a.out_len[r] = p >= 0 ? up_len : 0;
-  }
-  cluster.sync();
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (by[i] && page[i] >= 0 && page[i] < a.n_pages) atomicAdd(a.out_shares + page[i], by[i]);
+      if (r[i] < a.rows) a.out_table[r[i] * a.out_table_stride + c[i]] = take[i] < a.n_pages ? max(take[i], -1) : -1;
+    }
+  });
+  for (int r = at; r < a.rows; r += all) a.out_len[r] = parents[r] >= 0 ? lens[parents[r]] : 0;
+  sync();
 
   // Pages that no row names any more, ascending: those before the warp's stretch of them, and of all.
   const Stretch mine = stretch_of(a.n_pages, rank * kWarps + warp, ctas * kWarps);
+  uint32_t seen = 0;                            // the lane's of the warp's first 32 times 32 pages
   int gone = 0;
-  for (int i = mine.begin + lane; i < mine.end; i += 32) gone += __ldcg(a.out_shares + i) < 0;
+#pragma unroll 4
+  for (int i = mine.begin + lane, j = 0; i < mine.end; i += 32, ++j) {
+    const bool is = __ldcg(a.out_shares + i) < 0;
+    gone += is;
+    if (is && j < 32) seen |= 1u << j;
+  }
   int cta;
   int before = before_warp(__reduce_add_sync(~0u, gone), sums, cta);
   if (tid == 0) total = cta;
   const int used = min(max(__ldg(a.used), 0), a.n_free);
-  cluster.sync();
+  sync();
   int freed = 0;
   for (int i = 0; i < ctas; ++i) {
     const int x = *cluster.map_shared_rank(&total, i);
     if (i < rank) before += x;
     freed += x;
   }
-  for (int i0 = mine.begin; i0 < mine.end; i0 += 32) {
-    const bool is = i0 + lane < mine.end && __ldcg(a.out_shares + i0 + lane) < 0;
+  for (int i0 = mine.begin, j = 0; i0 < mine.end; i0 += 32, ++j) {
+    const bool is = j < 32 ? seen >> j & 1 : i0 + lane < mine.end && __ldcg(a.out_shares + i0 + lane) < 0;
     const uint32_t which = __ballot_sync(~0u, is);
     if (is) {
       a.out_shares[i0 + lane] = 0;
@@ -141,7 +177,7 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const ForkParams a) {
     }
     before += __popc(which);
   }
-  cluster.sync();
+  sync();
   if (rank) return;
 
   // Children that need a page of their own for what their parent's last one holds, in order.
@@ -151,9 +187,9 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const ForkParams a) {
     const int r = r0 + tid;
     int page = -1, column = 0;
     if (r < a.rows) {
-      const int p = parent_of(r);
+      const int p = parents[r];
       if (p >= 0 && first[p] != r) {
-        const int len = length_of(a.len, p, a.width, a.page);
+        const int len = lens[p];
         if (len % a.page) {
           column = len / a.page;
           page = __ldg(a.table + p * a.table_stride + column);
@@ -196,24 +232,49 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(const CompactParams a
   const cg::cluster_group cluster = cg::this_cluster();
   __shared__ int sums[kWarps], total;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks(), all = ctas * kThreads, at = rank * kThreads + tid;
-  for (int64_t i = at; i < a.n_pages; i += all) a.to[i] = 0;
-  cluster.sync();
-  for (int r = rank * kWarps + warp; r < a.rows; r += ctas * kWarps) {
-    const int have = pages_of(length_of(a.len, r, a.width, a.page), a.page);
-    for (int c = lane; c < have; c += 32) {
-      const int g = __ldg(a.table + r * a.table_stride + c);
-      if (g >= 0 && g < a.n_pages) a.to[g] = 1;
+  auto sync = [&] {
+    if (ctas > 1) cluster.sync();
+    else __syncthreads();
+  };
+  // A row's pages, -1 where there is none: loaded side by side.
+  auto named_at = [&](const int (&r)[kAtOnce], const int (&c)[kAtOnce], int (&page)[kAtOnce]) {
+    int len[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      page[i] = -1;
+      len[i] = 0;
+      if (r[i] >= a.rows) continue;
+      page[i] = a.table[r[i] * a.table_stride + c[i]];
+      len[i] = length_of(a.len, r[i], a.width, a.page);
     }
-  }
-  cluster.sync();
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i)
+      if (c[i] >= pages_of(len[i], a.page) || page[i] >= a.n_pages) page[i] = -1;
+  };
+  for (int64_t i = at; i < a.n_pages; i += all) a.to[i] = 0;
+  sync();
+  for_places(a.rows, a.width, at, all, [&](const int (&r)[kAtOnce], const int (&c)[kAtOnce]) {
+    int page[kAtOnce];
+    named_at(r, c, page);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i)
+      if (page[i] >= 0) a.to[page[i]] = 1;
+  });
+  sync();
   // How many are named: of the CTA's stretch, before the warp's, in all, and below their number.
   const Stretch mine = stretch_of(a.n_pages, rank * kWarps + warp, ctas * kWarps);
+  uint32_t seen = 0;                            // the lane's of the warp's first 32 times 32 pages
   int named = 0;
-  for (int i = mine.begin + lane; i < mine.end; i += 32) named += __ldcg(a.to + i);
+#pragma unroll 4
+  for (int i = mine.begin + lane, j = 0; i < mine.end; i += 32, ++j) {
+    const int is = __ldcg(a.to + i);
+    named += is;
+    if (is && j < 32) seen |= 1u << j;
+  }
   int cta;
   int before = before_warp(__reduce_add_sync(~0u, named), sums, cta);
   if (tid == 0) total = cta;
-  cluster.sync();
+  sync();
   int count = 0, here = 0;
   for (int i = 0; i < ctas; ++i) {
     const int x = *cluster.map_shared_rank(&total, i);
@@ -229,14 +290,15 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(const CompactParams a
     below += *cluster.map_shared_rank(&total, owner);
   }
   int more = 0;
+#pragma unroll 4
   for (int i = first + tid; i < count; i += kThreads) more += __ldcg(a.to + i);
   int part;
   before_warp(__reduce_add_sync(~0u, more), sums, part);
   below += part;
-  cluster.sync();                               // (all have counted before numbers take the marks' place)
-  for (int i0 = mine.begin; i0 < mine.end; i0 += 32) {
+  sync();                               // (all have counted before numbers take the marks' place)
+  for (int i0 = mine.begin, j = 0; i0 < mine.end; i0 += 32, ++j) {
     const int i = i0 + lane;
-    const bool in = i < mine.end, is = in && __ldcg(a.to + i);
+    const bool in = i < mine.end, is = j < 32 ? seen >> j & 1 : in && __ldcg(a.to + i);
     const uint32_t which = __ballot_sync(~0u, is);
     const int n = before + __popc(which & ((1u << lane) - 1));      // named pages before this one
     if (in) {
@@ -254,7 +316,7 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(const CompactParams a
   const int moves = count - below;
   for (int i = moves + at; i < a.n_pages / 2; i += all) a.out_src[i] = a.out_dst[i] = -1;
   if (at == 0) *a.out_used = count;
-  cluster.sync();
+  sync();
   // The shares go along; a place that is taken is one that nothing named.
   for (int64_t i = at; i < a.n_pages; i += all) {
     const int to = __ldcg(a.to + i);
@@ -265,18 +327,18 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(const CompactParams a
       if (i >= count) a.out_shares[i] = 0;
     }
   }
-  for (int r = rank * kWarps + warp; r < a.rows; r += ctas * kWarps) {
-    const int have = pages_of(length_of(a.len, r, a.width, a.page), a.page);
-    for (int c = lane; c < a.width; c += 32) {
-      const int g = c < have ? a.table[r * a.table_stride + c] : -1;
-      int to = -1;
-      if (g >= 0 && g < a.n_pages) {
-        to = __ldcg(a.to + g);
-        if (to <= -2) to = __ldcg(a.out_dst - 2 - to);
-      }
-      a.out_table[r * a.out_table_stride + c] = to;
+  for_places(a.rows, a.width, at, all, [&](const int (&r)[kAtOnce], const int (&c)[kAtOnce]) {
+    int page[kAtOnce];
+    named_at(r, c, page);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i)
+      if (page[i] >= 0) page[i] = __ldcg(a.to + page[i]);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (page[i] <= -2) page[i] = __ldcg(a.out_dst - 2 - page[i]);
+      if (r[i] < a.rows) a.out_table[r[i] * a.out_table_stride + c[i]] = page[i];
     }
-  }
+  });
 }
 
 // ---- copies
@@ -322,10 +384,10 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constan
   }
 }
 
-// CTAs of a cluster for so many things to look at: one thing a thread as long as there are CTAs to have.
+// CTAs of a cluster for so many things to look at: up to eight a thread by one, which needs no barrier of a cluster; beyond that as many as there are to have.
 int cluster_for(int64_t things) {
   int c = 1;
-  while (c < kMaxCluster && (int64_t)c * kThreads * 2 <= things) c *= 2;
+  while (c < kMaxCluster && (int64_t)c * kThreads * 8 < things) c *= 2;
   return c;
 }
 template <class P>
@@ -369,9 +431,9 @@ int linmt_fork_pages(const linmt_fork_pages_args* g) {
   if (on.err != cudaSuccess) return op_cuda(on.err, "fork_pages");
   const ForkParams p{g->table, g->table_stride, g->len, g->parents, g->done, g->shares, g->free_pages, g->used, g->out_table, g->out_table_stride, g->out_len, g->out_shares, g->out_free,
                      g->out_used, g->out_src, g->out_dst, (int)rows, g->k, g->width, g->page, g->n_pages, g->n_free};
-  const size_t smem = (size_t)rows * 2 * sizeof(int);
+  const size_t smem = (size_t)rows * kRowBytes;
   if (smem > 40 << 10) {
-    const cudaError_t e = cudaFuncSetAttribute(fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxRows * 2 * (int)sizeof(int));
+    const cudaError_t e = cudaFuncSetAttribute(fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxRows * kRowBytes);
     if (e != cudaSuccess) return op_cuda(e, "fork_pages");
   }
   const cudaError_t e = launch_cluster(fork_kernel, p, cluster_for(std::max(rows * g->width, (int64_t)g->n_pages + g->n_free)), smem, static_cast<cudaStream_t>(g->stream));
