@@ -85,15 +85,14 @@ struct Row {
     const float y = to_float(x[v]);
     return !LISTS || (__ldg(allowed + (v >> 5)) >> (v & 31) & 1) ? y : -INFINITY;
   }
-  // Words first .. first + kVec - 1 of a vector, -inf where they are not allowed.
-  __device__ __forceinline__ void open(const uint4& raw, int first, float (&y)[kVec]) const {
+  // Which of words first .. first + kVec - 1 are allowed, and a vector of them as numbers, -inf where they are not.
+  __device__ __forceinline__ uint32_t list(int first) const {
+    if (!LISTS) return ~0u;
+    const int w = first >> 5, s = first & 31;
+    return __funnelshift_r(__ldg(allowed + w), s + kVec > 32 ? __ldg(allowed + w + 1) : 0, s);
+  }
+  __device__ __forceinline__ void open(const uint4& raw, uint32_t bits, float (&y)[kVec]) const {
     const T* const e = reinterpret_cast<const T*>(&raw);
-    uint32_t bits = ~0u;
-    if (LISTS) {
-      const int w = first >> 5, s = first & 31;
-      bits = __ldg(allowed + w) >> s;
-      if (s + kVec > 32) bits |= __ldg(allowed + w + 1) << (32 - s);
-    }
 #pragma unroll
     for (int i = 0; i < kVec; ++i) y[i] = !LISTS || (bits >> i & 1) ? to_float(e[i]) : -INFINITY;
   }
@@ -141,7 +140,7 @@ struct Running {
 };
 
 template <class T, bool LISTS, int kThreads>
-__global__ void __launch_bounds__(kThreads) score_kernel(const ScoreParams a) {
+__global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && !LISTS ? 1536 : 1280) / kThreads) score_kernel(const ScoreParams a) {
   const cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row_at = blockIdx.x / ctas, i_n = row_at / a.t, i_t = row_at - i_n * a.t;
@@ -163,14 +162,18 @@ __global__ void __launch_bounds__(kThreads) score_kernel(const ScoreParams a) {
   auto each = [&](auto f) {
     for (int i0 = at; i0 < row.vectors; i0 += kAhead * all) {
       uint4 raw[kAhead];
+      uint32_t bits[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j)
-        if (i0 + j * all < row.vectors) raw[j] = __ldg(row.vector(i0 + j * all));
+        if (i0 + j * all < row.vectors) {
+          raw[j] = __ldg(row.vector(i0 + j * all));
+          bits[j] = row.list(row.lead + (i0 + j * all) * kVec);
+        }
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         if (i0 + j * all >= row.vectors) break;
         float y[kVec];
-        row.open(raw[j], row.lead + (i0 + j * all) * kVec, y);
+        row.open(raw[j], bits[j], y);
         f(y);
       }
     }
@@ -250,7 +253,7 @@ __global__ void __launch_bounds__(kThreads) score_kernel(const ScoreParams a) {
         const int from = at - lane + __ffs(left) - 1;
         for (int i = from + lane * all; i < row.vectors; i += 32 * all) {
           float y[kVec];
-          row.open(__ldg(row.vector(i)), row.lead + i * kVec, y);
+          row.open(__ldg(row.vector(i)), row.list(row.lead + i * kVec), y);
 #pragma unroll
           for (int j = 0; j < kVec; ++j) put(y[j], row.lead + i * kVec + j);
         }
@@ -278,7 +281,7 @@ __global__ void __launch_bounds__(kThreads) score_kernel(const ScoreParams a) {
         };
         for (int i = at; i < row.vectors; i += all) {
           float y[kVec];
-          row.open(__ldg(row.vector(i)), row.lead + i * kVec, y);
+          row.open(__ldg(row.vector(i)), row.list(row.lead + i * kVec), y);
 #pragma unroll
           for (int j = 0; j < kVec; ++j) look(y[j], row.lead + i * kVec + j);
         }
