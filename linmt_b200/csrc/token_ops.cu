@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && !LISTS ? 1536 : 1
     for (int i = 1; i < ctas; ++i) r = join(r, *cluster.map_shared_rank(&cta_sums, i));
     const bool nan = !(r.m == r.m) || r.m == INFINITY, none = r.m == -INFINITY;
     const float log_s = log2f(r.s);
-    auto logprob = [&](float x) { return huge(r) ? (x - r.m) - kLn2 * log_s : (fmaf(x, kLog2e, -r.k) - log_s) * kLn2; };
+    auto logprob = [&](float x) { return huge(r) ? (x - r.m) - kLn2 * log_s : fabsf(x) > kHuge ? x - (r.k + log_s) * kLn2 : (fmaf(x, kLog2e, -r.k) - log_s) * kLn2; };
     if (tid == 0) {
       const int token = __ldg(a.tokens + row_at);
       const float x = token >= 0 && token < a.vocab ? row.at(token) : 0.f;
