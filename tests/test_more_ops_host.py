@@ -118,7 +118,7 @@ def test_score_refuses(cuda_lib, code, word, kw):
 
 def test_copy_refuses(cuda_lib):
     def args(n=3, n_pages=5, n_pools=1, src=PTR, size=None, data=PTR, stride=64, page=64):
-        head = struct.pack("@IiPPPiiii", 56 + 16 * 24 if size is None else size, 0, 0, src, PTR, n, n_pages, n_pools, 0)
+        head = struct.pack("@IiPPPiiii", 48 + 16 * 24 if size is None else size, 0, 0, src, PTR, n, n_pages, n_pools, 0)
         return head + (struct.pack("@Pqq", data, stride, page) * min(max(n_pools, 0), 16)).ljust(16 * 24, b"\0")
 
     for code, word, kw in [(EINVAL, "struct", dict(size=8)), (EINVAL, "17 pools", dict(n_pools=17)), (EINVAL, "n = -1", dict(n=-1)), (EINVAL, "missing", dict(src=0)), (EINVAL, "aligned", dict(src=PTR + 2)), (EINVAL, "pool 0", dict(data=0)),
