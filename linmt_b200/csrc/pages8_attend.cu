@@ -374,7 +374,7 @@ struct Shared {
   unsigned valid[VS];
   int add, gave_up;
   uint32_t tmem;
-  alignas(8) unsigned long long k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], s_empty[2], q_full[2], q_empty[2], p_full, o_full;
+  alignas(8) unsigned long long k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], s_empty[2], q_full[2], q_empty[2], p_full, o_full, first;
 };
 
 __device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float x) {
@@ -397,109 +397,112 @@ __device__ __forceinline__ void four(const int* p, int (&x)[4]) {
 }
 __device__ __forceinline__ float power_of_2(int e) { return __int_as_float((127 + e) << 23); }      // -126 .. 127
 
-// A piece's queries as bytes, what its rows see and where their results go; by a warp, a lane for two or four neighbouring components of each row.
+// What a piece's rows see and where their results go; by a warp, a lane for each row.
 template <int D, int R>
-__device__ __forceinline__ void take_queries(const AttendParams& a, const Piece& p, Shared<D, R>& sh, int buffer) {
-  constexpr int N = D / 32, kAtOnce = R < 8 ? R : 8;
+__device__ __forceinline__ void take_rows(const AttendParams& a, const Piece& p, Shared<D, R>& sh, int buffer) {
+  const int lane = threadIdx.x & 31, row = p.rt * R + lane;
+  if (lane >= R) return;
+  const bool have = row < a.g * a.rep;
+  const int at = have ? row : p.rt * R, g = at / a.rep, h = p.kvh * a.rep + at - g * a.rep;
+  const int64_t by_row = (int64_t)p.sent * a.g + g;
+  const int lo = a.first && have ? max(__ldg(a.first + by_row), 0) : 0, hi = a.first && have ? min(__ldg(a.last + by_row), p.len) : p.len;
+  sh.slope[buffer][lane] = have && a.slope ? __ldg(a.slope + h) * kLog2e : 0.f;
+  sh.centre[buffer][lane] = have && a.slope ? __ldg(a.centre + by_row) : 0.f;
+  sh.lo[buffer][lane] = lo;
+  sh.span[buffer][lane] = max(hi - lo, 0);
+  sh.out[buffer][lane] = p.sent * a.o_n + g * a.o_g + h * a.o_h;
+}
+
+// A piece's queries from row r0 on as bytes; by a warp, a lane for two or four neighbouring components of each row.
+constexpr int kAtOnce = 4;
+template <int D, int R>
+__device__ __forceinline__ void take_queries(const AttendParams& a, const Piece& p, Shared<D, R>& sh, int buffer, int r0) {
+  constexpr int N = D / 32;
   const int lane = threadIdx.x & 31, n_rows = min(R, a.g * a.rep - p.rt * R);
-  int64_t from;                                       // of row `lane`; rows that are not there have another's queries, and their products are multiplied by 0
+  int64_t from;                                       // of row r0 + lane; rows that are not there have another's queries, and their products are multiplied by 0
   {
-    const int at = p.rt * R + min(lane, n_rows - 1), g = at / a.rep, h = p.kvh * a.rep + at - g * a.rep;
-    const bool have = lane < n_rows;
-    const int64_t by_row = (int64_t)p.sent * a.g + g;
+    const int at = p.rt * R + min(r0 + lane, n_rows - 1), g = at / a.rep, h = p.kvh * a.rep + at - g * a.rep;
     from = p.sent * a.q_n + g * a.q_g + h * a.q_h;
-    if (lane < R) {
-      const int lo = a.first && have ? max(__ldg(a.first + by_row), 0) : 0, hi = a.first && have ? min(__ldg(a.last + by_row), p.len) : p.len;
-      sh.slope[buffer][lane] = have && a.slope ? __ldg(a.slope + h) * kLog2e : 0.f;
-      sh.centre[buffer][lane] = have && a.slope ? __ldg(a.centre + by_row) : 0.f;
-      sh.lo[buffer][lane] = lo;
-      sh.span[buffer][lane] = max(hi - lo, 0);
-      sh.out[buffer][lane] = p.sent * a.o_n + g * a.o_g + h * a.o_h;
-    }
   }
+  float x[kAtOnce][N];
+  int64_t at[kAtOnce];
 #pragma unroll
-  for (int r0 = 0; r0 < R; r0 += kAtOnce) {
-    // All rows' loads before the first is looked at.
-    float x[kAtOnce][N];
-    int64_t at[kAtOnce];
+  for (int j = 0; j < kAtOnce; ++j) at[j] = __shfl_sync(~0u, (long long)from, j) + lane * N;
+  if (!a.q_wide) {
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) at[j] = __shfl_sync(~0u, (long long)from, r0 + j) + lane * N;
-    if (!a.q_wide) {
+    for (int j = 0; j < kAtOnce; ++j)
 #pragma unroll
-      for (int j = 0; j < kAtOnce; ++j)
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[j][i] = load_as_float(a.q, at[j] + i, a.dtype);
-    } else if (a.dtype == LINMT_F32) {
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        const float* const q = static_cast<const float*>(a.q) + at[j];
-        if constexpr (N == 4) {
-          const float4 v = __ldg(reinterpret_cast<const float4*>(q));
-          x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
-        } else {
-          const float2 v = __ldg(reinterpret_cast<const float2*>(q));
-          x[j][0] = v.x; x[j][1] = v.y;
-        }
-      }
-    } else {
-      uint32_t raw[kAtOnce][N / 2];
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j) {
-        const unsigned short* const q = static_cast<const unsigned short*>(a.q) + at[j];
-        if constexpr (N == 4) {
-          const uint2 v = __ldg(reinterpret_cast<const uint2*>(q));
-          raw[j][0] = v.x; raw[j][1] = v.y;
-        } else {
-          raw[j][0] = __ldg(reinterpret_cast<const uint32_t*>(q));
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < kAtOnce; ++j)
-#pragma unroll
-        for (int i = 0; i < N; i += 2) {
-          const float2 v = a.dtype == LINMT_BF16 ? make_float2(__uint_as_float(raw[j][i / 2] << 16), __uint_as_float(raw[j][i / 2] & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&raw[j][i / 2]));
-          x[j][i] = v.x;
-          x[j][i + 1] = v.y;
-        }
-    }
-    // The rows' largest components, each in a lane, and what it takes to bring them below 2^22: 2^e <= the largest < 2^(e + 1), components times 2^(21 - e).  (Below 2^-106 it stays
-    // at that of 2^-106.)
-    uint32_t most = 0;
+      for (int i = 0; i < N; ++i) x[j][i] = load_as_float(a.q, at[j] + i, a.dtype);
+  } else if (a.dtype == LINMT_F32) {
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(x[j][i]) & 0x7fffffff);
-      m = __reduce_max_sync(~0u, m);
-      if (lane == j) most = m;
-    }
-    const bool bad = most >= 0x7f800000;
-    const int e = bad ? 0 : max((int)(most >> 23) - 127, -106);
-    const float up = bad ? 0.f : power_of_2(21 - e);
-    if (lane < kAtOnce) {
-      sh.by[buffer][r0 + lane] = r0 + lane < n_rows ? a.mul * power_of_2((e - 21) / 2) * power_of_2(e - 21 - (e - 21) / 2) : 0.f;
-      sh.bad[buffer][r0 + lane] = bad;
-    }
-    // Digits to the base 256, -128 .. 127: with 128 added to each, the bytes of the sum.
-#pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) {
-      const int r = r0 + j;
-      const float by = __shfl_sync(~0u, up, j);
-      uint32_t u[N];
-#pragma unroll
-      for (int i = 0; i < N; ++i) u[i] = (uint32_t)(__float2int_rn(x[j][i] * by) + 0x808080) ^ 0x808080;
-      auto place = [&](int k) { return sh.queries[buffer] + ((k * R + r) / 8 * (D / 16) + lane * N / 16) * kQueryAlong + (k * R + r) % 8 * 16 + lane * N % 16; };
+      const float* const q = static_cast<const float*>(a.q) + at[j];
       if constexpr (N == 4) {
-        const uint32_t low01 = __byte_perm(u[0], u[1], 0x5140), low23 = __byte_perm(u[2], u[3], 0x5140);
-        *reinterpret_cast<uint32_t*>(place(0)) = __byte_perm(low01, low23, 0x5410);
-        *reinterpret_cast<uint32_t*>(place(1)) = __byte_perm(low01, low23, 0x7632);
-        *reinterpret_cast<uint32_t*>(place(2)) = __byte_perm(__byte_perm(u[0], u[1], 0x0062), __byte_perm(u[2], u[3], 0x0062), 0x5410);
+        const float4 v = __ldg(reinterpret_cast<const float4*>(q));
+        x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
       } else {
-        const uint32_t low = __byte_perm(u[0], u[1], 0x5140);
-        *reinterpret_cast<uint16_t*>(place(0)) = (uint16_t)low;
-        *reinterpret_cast<uint16_t*>(place(1)) = (uint16_t)(low >> 16);
-        *reinterpret_cast<uint16_t*>(place(2)) = (uint16_t)__byte_perm(u[0], u[1], 0x0062);
+        const float2 v = __ldg(reinterpret_cast<const float2*>(q));
+        x[j][0] = v.x; x[j][1] = v.y;
       }
+    }
+  } else {
+    uint32_t raw[kAtOnce][N / 2];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const unsigned short* const q = static_cast<const unsigned short*>(a.q) + at[j];
+      if constexpr (N == 4) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(q));
+        raw[j][0] = v.x; raw[j][1] = v.y;
+      } else {
+        raw[j][0] = __ldg(reinterpret_cast<const uint32_t*>(q));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j)
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const float2 v = a.dtype == LINMT_BF16 ? make_float2(__uint_as_float(raw[j][i / 2] << 16), __uint_as_float(raw[j][i / 2] & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2*>(&raw[j][i / 2]));
+        x[j][i] = v.x;
+        x[j][i + 1] = v.y;
+      }
+  }
+  // The rows' largest components, each in a lane, and what it takes to bring them below 2^22: 2^e <= the largest < 2^(e + 1), components times 2^(21 - e).  (Below 2^-106 it stays
+  // at that of 2^-106.)
+  uint32_t most = 0;
+#pragma unroll
+  for (int j = 0; j < kAtOnce; ++j) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(x[j][i]) & 0x7fffffff);
+    m = __reduce_max_sync(~0u, m);
+    if (lane == j) most = m;
+  }
+  const bool bad = most >= 0x7f800000;
+  const int e = bad ? 0 : max((int)(most >> 23) - 127, -106);
+  const float up = bad ? 0.f : power_of_2(21 - e);
+  if (lane < kAtOnce) {
+    sh.by[buffer][r0 + lane] = r0 + lane < n_rows ? a.mul * power_of_2((e - 21) / 2) * power_of_2(e - 21 - (e - 21) / 2) : 0.f;
+    sh.bad[buffer][r0 + lane] = bad;
+  }
+  // Digits to the base 256, -128 .. 127: with 128 added to each, the bytes of the sum.
+#pragma unroll
+  for (int j = 0; j < kAtOnce; ++j) {
+    const int r = r0 + j;
+    const float by = __shfl_sync(~0u, up, j);
+    uint32_t u[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) u[i] = (uint32_t)(__float2int_rn(x[j][i] * by) + 0x808080) ^ 0x808080;
+    auto place = [&](int k) { return sh.queries[buffer] + ((k * R + r) / 8 * (D / 16) + lane * N / 16) * kQueryAlong + (k * R + r) % 8 * 16 + lane * N % 16; };
+    if constexpr (N == 4) {
+      const uint32_t low01 = __byte_perm(u[0], u[1], 0x5140), low23 = __byte_perm(u[2], u[3], 0x5140);
+      *reinterpret_cast<uint32_t*>(place(0)) = __byte_perm(low01, low23, 0x5410);
+      *reinterpret_cast<uint32_t*>(place(1)) = __byte_perm(low01, low23, 0x7632);
+      *reinterpret_cast<uint32_t*>(place(2)) = __byte_perm(__byte_perm(u[0], u[1], 0x0062), __byte_perm(u[2], u[3], 0x0062), 0x5410);
+    } else {
+      const uint32_t low = __byte_perm(u[0], u[1], 0x5140);
+      *reinterpret_cast<uint16_t*>(place(0)) = (uint16_t)low;
+      *reinterpret_cast<uint16_t*>(place(1)) = (uint16_t)(low >> 16);
+      *reinterpret_cast<uint16_t*>(place(2)) = (uint16_t)__byte_perm(u[0], u[1], 0x0062);
     }
   }
 }
@@ -527,6 +530,7 @@ __global__ void __launch_bounds__(kThreads<R>) __maxnreg__(65536 / (kThreads<R> 
     }
     bar_init(shared(&sh.p_full), kWeightWarps<R>);
     bar_init(shared(&sh.o_full), 1);
+    bar_init(shared(&sh.first), kWeightWarps<R>);
     sh.gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -554,7 +558,13 @@ __global__ void __launch_bounds__(kThreads<R>) __maxnreg__(65536 / (kThreads<R> 
       bar_wait(shared(&sh.q_empty[buffer]), (pieces >> 1 & 1) ^ 1, gave_up);
       __syncwarp();
       if (!*gave_up) {
-        if (chunks > 0) take_queries<D, R>(a, p, sh, buffer);
+        if (chunks > 0) {
+          take_rows<D, R>(a, p, sh, buffer);
+          if (pieces == 0) bar_wait(shared(&sh.first), 0, gave_up);
+          else
+#pragma unroll 1
+            for (int r0 = 0; r0 < R; r0 += kAtOnce) take_queries<D, R>(a, p, sh, buffer, r0);
+        }
         if (lane == 0) {
           Ready& r = sh.ready[buffer];
           r.chunks = chunks;
@@ -700,6 +710,15 @@ __global__ void __launch_bounds__(kThreads<R>) __maxnreg__(65536 / (kThreads<R> 
     const uint32_t lanes = tmem + ((uint32_t)(warp % 4 * 32) << 16);
     const float slack = (float)a.slack, unit = power_of_2(a.slack - 31);
     int it = 0, pieces = 0;
+    // The first piece's queries are made ready by these warps, which have nothing else to do yet; later ones by the warp that copies.  (All by that one: 5400 cycles with 16 rows.)
+    {
+      Piece first;
+      Share s = share;
+      if (next_piece(a, s, first) && first.c0 < first.c1 && warp * kAtOnce < R) take_queries<D, R>(a, first, sh, 0, warp * kAtOnce);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(shared(&sh.first));
+    }
     int4 ends = make_int4(-1, 0, 0, 0);               // the segment that ends in this share and began before it: sentence, head, row tile, first CTA
     for (;; ++pieces) {
       const int buffer = pieces & 1;
@@ -742,6 +761,11 @@ __global__ void __launch_bounds__(kThreads<R>) __maxnreg__(65536 / (kThreads<R> 
           float most = -INFINITY;
 #pragma unroll
           for (int r4 = 0; r4 < RT; r4 += 4) {
+            if (r4 > 0 && row0 + r4 >= n_rows) {       // four rows that are not there
+#pragma unroll
+              for (int j = 0; j < 4; ++j) s[r4 + j] = -INFINITY;
+              break;
+            }
             float by[4], m[4], l[4], slope[4], centre[4];
             int lo[4], span[4];
             four(sh.by[buffer] + row0 + r4, by);
@@ -832,6 +856,10 @@ __global__ void __launch_bounds__(kThreads<R>) __maxnreg__(65536 / (kThreads<R> 
         for (int r4 = 0; r4 < RT; r4 += 4) {
           float m[4], l[4];
           uint32_t w[4];
+          if (r4 > 0 && row0 + r4 >= n_rows) {
+            sh.weights[(row0 + r4) / 4][mine] = make_uint4(0, 0, 0, 0);
+            break;
+          }
           four(sh.m[now] + row0 + r4, m);
           four(sh.l[now] + row0 + r4, l);
 #pragma unroll
