@@ -3,17 +3,23 @@
 //   out = sum_t softmax_t(f(scale q . k_t)) v_t,   k_t = ks code, v_t = vs code, a scale for each block of 16 positions
 //
 // Both products are tcgen05.mma of bytes into 32-bit integers, with codes as they lie in the pool as the left operand: nothing is unpacked, and no sum is rounded.
-//   S[128 positions x 48] = keys . queries: a query of a row is a whole number of 23 bits (to 2^-23 of the row's largest component), cut into three
-//   signed bytes, one column each for 16 rows.  s = (65536 S2 + 256 S1 + S0) ks times the row's power of 2.
-//   O[dim x 64] += values^T . weights: a weight times its block's scale is a whole number of 32 bits (to 2^-31 of about the row's largest), whose four bytes are a
-//   column each.  O = sum over the four of 256^i O_i.
-// 16 rows (beams, and the query heads that share a head of the pool) are the right operand, which may be narrow: with 128 positions (or components) on the left a
-// product of 32 KB of pages takes some 300 cycles, a fifth of the time that HBM needs for them.
-// Weights are relative to 2^M, M a whole number for each row not below the largest exponent of weight times scale less 1; the sum of weights alone is relative to
-// 2^L, 40 above such a number.  (One for both would lose rows whose values differ by more than 32 bits hold.)  Both follow when something exceeds them; only
-// then, every 256 chunks and at the end are O's integers taken out of TMEM, into 32-bit sums.
-// A CTA has 128 threads that turn S into weights, a position each; one warp that copies blocks (bulk copies, two rings) and one that issues the products.  Two CTAs
-// share an SM.  The work is cut into equal shares over the CTAs that fit on the GPU at once, and a second kernel joins the parts of what several of them share.
+//   S[128 positions x 3 R] = keys . queries: a query of a row is a whole number of 23 bits (to 2^-22 of the row's largest component), cut into three
+//   signed bytes, a column each for R rows.  s = (65536 S2 + 256 S1 + S0) ks times the row's power of 2.
+//   O[dim x 4 R] += values^T . weights: a weight times its block's scale is a whole number of 32 bits, whose four bytes are a column each.  O = sum over the
+//   four of 256^i O_i.
+// R rows (4, 8 or 16 of a sentence's beams and of the query heads that share a head of the pool) are the right operand, which may be narrow: with 128 positions (or components) on
+// the left a product of 32 KB of pages takes some 300 cycles, a fifth of the time that HBM needs for them.
+// Weights are relative to 2^M, M a whole number for each row: a power of 2 at most above the row's largest weight times scale so far, and at most one below it with 32-bit queries (weights
+// are good to 2^-30 of the largest then), four with 16-bit ones (2^-27, and M follows less often).  The sum of weights alone is relative to 2^L, L 40 above such a number.  (One for both
+// would lose rows whose values differ by more than 32 bits hold.)  Both follow when something exceeds them; only then, every 256 chunks and at the end are O's integers taken out of TMEM, into 32-bit sums.
+// A CTA has 128 threads (256 with 16 rows) that turn S into weights, a position and up to eight rows each; one warp that copies blocks and makes queries ready, two pieces ahead, and one that
+// issues the products.  Two CTAs share an SM, three with four rows.  The work is cut into equal shares over the CTAs that fit on the GPU at once, and a second kernel joins the parts of what
+// several of them share.
+// What bounds it: long sentences HBM (8 documents of 20-32k, 16 rows of 128: 83 us, 5.2 TB/s, of which 6 us until the first weights and 4 for the join) and, as much, the weights' latencies:
+// 2700 cycles a chunk of a CTA's, of which the conversions and exponentials take 640.  Where scores rise from chunk to chunk (a bias that falls with the distance) taking O out each time is another 1600.
+// Tried: weights stored byte by byte, positions as neighbours: 129 us where columns as neighbours took 105.  A bulk copy for each block's keys, values and scales: 110 us where four blocks a copy took
+// 83.  Single rows that see nothing of a chunk left out: 92 us, and no faster with windows, as what is saved in work is lost in order.  Two rows an instruction: no difference.
+
 #include <cuda.h>
 
 #include <cmath>

@@ -143,7 +143,8 @@ def attend_pages8(q, pages, table, lens, *, scale=None, cap=0.0, slope=None, cen
     """Attention of the g query rows (beams) of each sentence over its positions in a pool of 8-bit pages.
 
     Everything is as in attend_pages4, with one argument more: positions below ``sinks`` stay visible whatever ``first`` and ``last`` say (a window that slides
-    over a long text and the first few tokens before it).  Queries are taken to 2^-23 of a row's largest component, weights to 2^-31 of the row's largest."""
+    over a long text and the first few tokens before it).  Queries are taken to 2^-22 of a row's largest component, weights times scales to 2^-30 of the row's
+    largest (2^-27 with 16-bit queries); both products are exact sums of integers."""
     return _front.attend_pages8(q, pages, table, lens, scale, cap, slope, centre, first, last, out, want_lse, sinks)
 
 

@@ -386,3 +386,13 @@ def test_captured_and_on_two_streams(ops):
             w = b.cpu().numpy()
             w[dst] = b.cpu().numpy()[src]
             assert (pool.cpu().numpy() == w).all()
+
+
+def test_fork_as_many_rows_as_there_may_be(ops):
+    rng = _rng(52)
+    for n, k in ((1024, 16), (1, 16384)):
+        page = 16
+        lens = rng.integers(0, 40, (n, k))
+        table, shares, free, used = _state(rng, n, k, lens, page, n * k, shared=0)
+        fork_check(ops, table, lens, rng.integers(-1, k, (n, k)), shares, free, used, page)
+        fork_check(ops, table, lens, None, shares, free, used, page, done=rng.random((n, k)) < 0.5)

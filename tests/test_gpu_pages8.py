@@ -565,3 +565,43 @@ def test_captured_and_replayed(ops):
                 want, want_lse, tol, tol_lse = attend_ref(q.view(n, 1, heads, dim), kv, table.cpu().numpy(), [at + 1] * n, dim ** -0.5)
                 assert (np.abs(out[0].double().cpu().numpy() - want) <= tol[..., None] + HALF_STEP[BF16] * np.abs(want)).all()
                 assert (np.abs(out[1].double().cpu().numpy() - want_lse) <= tol_lse).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_attend_many_short_sentences(ops, dtype):
+    """More sentences than a CTA has threads, empty ones among them; every CTA has many."""
+    rng = _rng(41)
+    n, dim, page = 3000, 64, 16
+    lens = rng.integers(0, 40, n)
+    lens[rng.random(n) < 0.3] = 0
+    lens[1500] = 800
+    pool, table, kv = memory8(rng, n, lens, 1, dim, page)
+    attend_check(ops, _q(rng, n, 1, 2, dim, dtype), pool, table, lens, kv)
+
+
+def test_attend_integers_are_taken_out_before_they_overflow(ops):
+    """Eleven million positions of a few pages, named again and again: a CTA has more products than its 32-bit sums hold at the largest codes and equal weights."""
+    rng = _rng(42)
+    dim, page, pages, columns = 64, 128, 3, 88800
+    codes = np.full((2, pages, 1, page, dim), 127, np.int64)
+    codes[0] = rng.integers(-3, 4, codes.shape[1:])
+    codes[1, ..., 1::2] = -127
+    codes[1, 2, :, ::2] = 126
+    scales = np.full((2, pages, 1, page // 16), 0.0078125)
+    pool = _cuda(blocks(codes, scales))
+    names = rng.integers(0, pages, columns)
+    length = columns * page - 77
+    count = np.zeros((pages, page))
+    np.add.at(count, names, 1)
+    count[names[-1], page - 77:] -= 1
+    kv = codes * 0.0078125
+    q = _q(rng, 1, 16, 1, dim, F32, size=0.3)
+    out, lse = ops.attend_pages8(q, pool, _cuda(names.astype(np.int32)[None]), torch.tensor([length], dtype=torch.int32, device="cuda"), want_lse=True)
+    x = q[0, :, 0].double().cpu().numpy() @ kv[0, :, 0].reshape(-1, dim).T * dim ** -0.5
+    w = np.exp(x - x.max(1, keepdims=True)) * count.reshape(-1)
+    want = (w / w.sum(1, keepdims=True)) @ kv[1, :, 0].reshape(-1, dim)
+    want_lse = x.max(1) + np.log(w.sum(1))
+    # a weight is rounded to 2^-30 of the largest; a thread adds up 11e6 / 296 / 128 weights and 300 parts are joined, 2^-24 each; scores are below 2
+    tol = np.abs(kv[1]).max() * (length * 2.0 ** -30 + (length / 296 / 128 + 340) * 2.0 ** -23 + 2.0 ** -19)
+    assert (np.abs(out[0, :, 0].double().cpu().numpy() - want) <= tol).all()
+    assert (np.abs(lse[0, :, 0].double().cpu().numpy() - want_lse) <= (length / 296 / 128 + 340) * 2.0 ** -23 + 2.0 ** -18).all()
