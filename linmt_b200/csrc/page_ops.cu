@@ -19,7 +19,7 @@ constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRows = 16384;
 constexpr int kRowBytes = 3 * (int)sizeof(int) + (int)sizeof(short);
-constexpr int kMaxCluster = 8;
+constexpr int kPortableCluster = 8, kMaxCluster = 16;
 
 struct ForkParams {
   const int32_t* table;
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(const CompactParams a
 // ---- copies
 
 constexpr int kCopyThreads = 256;
-constexpr int kCopyEach = 4;           // loads of a thread on their way
+constexpr int kCopyEach = 8;           // loads of a thread on their way (with four: half of a pool of 0.8 GB made dense in 95 us, not 91)
 
 struct CopyParams {
   const int32_t* src;
@@ -384,10 +384,11 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constan
   }
 }
 
-// CTAs of a cluster for so many things to look at: up to eight a thread by one, which needs no barrier of a cluster; beyond that as many as there are to have.
+// CTAs of a cluster for so many things to look at: up to two a thread by one, which needs no barrier of a cluster; beyond that as many as there are to have.  (Eight a thread: 768 hypotheses
+// of 20 to 90 positions take 17.5 us with their copies, not 14.8; eight CTAs at most: 2048 of 100 to 1500 positions 30 us, not 25.)
 int cluster_for(int64_t things) {
   int c = 1;
-  while (c < kMaxCluster && (int64_t)c * kThreads * 8 < things) c *= 2;
+  while (c < kMaxCluster && (int64_t)c * kThreads * 2 < things) c *= 2;
   return c;
 }
 template <class P>
@@ -403,7 +404,8 @@ cudaError_t launch_cluster(void (*kernel)(P), const P& p, int ctas, size_t smem,
   cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  cudaError_t e = ctas > kPortableCluster ? cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) : cudaSuccess;
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, p);
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
 
