@@ -1,8 +1,9 @@
 // token_ops.cu -- scores of given tokens (linmt_score_tokens): log probability, entropy and the best alternatives of rows of logits.
 //
 //   d = x log2 e - k, S = sum 2^d, T = sum 2^d d:   log sum exp x = (k + log2 S) ln 2,   entropy = ln 2 (log2 S - T / S)
-// with a whole number k next to the largest x log2 e, so that d is rounded once.  T's large terms are all of one sign, so nothing cancels.  One pass over a row, each thread with a k of
-// its own, two logits an instruction where there is one for two.  Bound by HBM in 32 bits, by instructions (unpacking 1, list 2, the rest 6 an element) in 16.
+// with a whole number k, at most 8 below the largest x log2 e, so that d is rounded once.  (Of an entropy next to 0 that leaves 1e-6: T and log2 S are of k's size then, and cancel.)  One pass over a row, each thread
+// with a k of its own, two logits an instruction where there is one for two.  A row whose largest logit is beyond 65536 in size is added up once more relative to e^m, m that logit itself:
+// k and x log2 e have no place left behind the point from 2^23 on, and logits that far apart are told apart by x - m alone.  Bound by HBM in 32 bits, by instructions (unpacking 1, list 2, the rest 6 an element) in 16.
 // The k-th largest of 32 groups' maxima is reached by k words at least: only the words of threads whose own maximum reaches it are looked at again (from L2), by their whole warp, and what
 // reaches it goes on a list in shared memory, which is ranked by counting.  (Each such thread by itself, its warp waiting: 1968 rows of 80,000 words in 16 bits took 189 us.)  Equal logits
 // may overfill the list; then the best are found one by one, in a pass over the row for each.  Long rows where there are few go to a cluster of CTAs, joined through its shared memory.
@@ -46,11 +47,10 @@ __device__ __forceinline__ float2 pair_of(unsigned long long a) { float2 r; asm(
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { unsigned long long r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b)), "l"(bits_of(c))); return pair_of(r); }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { unsigned long long r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits_of(a)), "l"(bits_of(b))); return pair_of(r); }
 
-// m the largest logit (NaN once one was met), s and t the sums relative to 2^k.  Nothing so far: -inf and sums of 0.  Logits above 1e38 in size do not fit d: where such a one is the largest
-// the sums are relative to e^m, and k is not used.
-constexpr float kHuge = 1e38f, kNone = -1e30f, kSlack = 8.f;
+// m the largest logit (NaN once one was met), s and t the sums relative to 2^k.  Nothing so far: -inf and sums of 0.  Where m is beyond kFar the sums of a CTA are relative to e^m, and k is not used.
+constexpr float kFar = 65536.f, kLost = 4194304.f, kNone = -1e30f, kSlack = 8.f;
 struct Sums { float m, k, s, t; };
-__device__ __forceinline__ bool huge(const Sums& a) { return fabsf(a.m) > kHuge; }
+__device__ __forceinline__ bool far(const Sums& a) { return fabsf(a.m) > kFar; }
 // The sums relative to something 2^-d times as large.
 __device__ __forceinline__ void lower(Sums& a, float d) {
   d = fmaxf(d, -150.f);
@@ -58,15 +58,23 @@ __device__ __forceinline__ void lower(Sums& a, float d) {
   a.t = f * fmaf(a.s, d, a.t);
   a.s *= f;
 }
+// Of two threads: both relative to 2^k.  One's beyond kLost (2^22, where k is no longer exact) count nothing beside another's, or the row is added up again.
+__device__ __forceinline__ Sums join_threads(Sums a, Sums b) {
+  Sums r{max_nan(a.m, b.m), fmaxf(a.k, b.k), 0.f, 0.f};
+  if (fabsf(a.m) <= kLost) { lower(a, a.k - r.k); r.s += a.s; r.t += a.t; }
+  if (fabsf(b.m) <= kLost) { lower(b, b.k - r.k); r.s += b.s; r.t += b.t; }
+  return r;
+}
+// Of two threads or CTAs whose sums are relative to e^m, m far or not and the same for all; and of two CTAs, each by its own largest logit.
 __device__ __forceinline__ Sums join(Sums a, Sums b) {
   Sums r{max_nan(a.m, b.m), fmaxf(a.k, b.k), 0.f, 0.f};
-  if (!huge(r)) {
-    if (!huge(a)) { lower(a, a.k - r.k); r.s += a.s; r.t += a.t; }
-    if (!huge(b)) { lower(b, b.k - r.k); r.s += b.s; r.t += b.t; }
-  } else {
-    if (huge(a)) { lower(a, (a.m - r.m) * kLog2e); r.s += a.s; r.t += a.t; }
-    if (huge(b)) { lower(b, (b.m - r.m) * kLog2e); r.s += b.s; r.t += b.t; }
-  }
+  auto above = [&](const Sums& x) {              // of what x is relative to, above what r is
+    return far(r) ? far(x) ? (x.m - r.m) * kLog2e : -fmaf(r.m, kLog2e, -x.k) : far(x) ? fmaf(x.m, kLog2e, -r.k) : x.k - r.k;
+  };
+  lower(a, above(a));
+  lower(b, above(b));
+  r.s = a.s + b.s;
+  r.t = a.t + b.t;
   return r;
 }
 
@@ -107,7 +115,9 @@ struct Running {
   float m = -INFINITY, k = kNone;
   float2 s = {0.f, 0.f}, t = {0.f, 0.f};
   __device__ __forceinline__ void follow() {           // k follows a maximum that exceeds it
-    const float now = ceilf(m * kLog2e), d = fmaxf(k - now, -150.f), f = exp2_of(d);
+    float now = ceilf(m * kLog2e);
+    if (fabsf(now) > kLost) now += fabsf(now) * 4.76837158203125e-7f;      // (rounded: no term may exceed it, as sums that go into nothing still have to be numbers)
+    const float d = fmaxf(k - now, -150.f), f = exp2_of(d);
     t.x = f * fmaf(s.x, d, t.x);
     t.y = f * fmaf(s.y, d, t.y);
     s.x *= f;
@@ -182,10 +192,11 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && !LISTS ? 1536 : 1
       f(y);
     }
   };
-  auto join_lanes = [](Sums x, int lanes) {
-    for (int o = 1; o < lanes; o <<= 1) x = join(x, {__shfl_xor_sync(~0u, x.m, o), __shfl_xor_sync(~0u, x.k, o), __shfl_xor_sync(~0u, x.s, o), __shfl_xor_sync(~0u, x.t, o)});
+  auto join_lanes = [](Sums x, int lanes, auto two) {
+    for (int o = 1; o < lanes; o <<= 1) x = two(x, {__shfl_xor_sync(~0u, x.m, o), __shfl_xor_sync(~0u, x.k, o), __shfl_xor_sync(~0u, x.s, o), __shfl_xor_sync(~0u, x.t, o)});
     return x;
   };
+  auto near = [](const Sums& a, const Sums& b) { return join_threads(a, b); };
   const Sums nothing{-INFINITY, kNone, 0.f, 0.f};
   Running running;
   each([&](const auto& y) { running.add(y); });
@@ -193,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && !LISTS ? 1536 : 1
 
   // The row's sums, and a bar that `top` words reach.
   if (a.top) most[warp][lane] = own;
-  Sums sums = join_lanes(running.sums(), 32);
+  Sums sums = join_lanes(running.sums(), 32, near);
   if (lane == 0) warp_sums[warp] = sums;
   if (tid == 0) {
     listed = 0;
@@ -201,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && !LISTS ? 1536 : 1
   }
   __syncthreads();
   if (warp == 0) {
-    sums = join_lanes(lane < kThreads / 32 ? warp_sums[lane] : nothing, kThreads / 32);
+    sums = join_lanes(lane < kThreads / 32 ? warp_sums[lane] : nothing, kThreads / 32, near);
     if (lane == 0) cta_sums = sums;
   } else if (warp == 1 && a.top) {
     float m = most[0][lane];
@@ -217,7 +228,7 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && !LISTS ? 1536 : 1
     if (above == a.top - 1) bar = m;
   }
   __syncthreads();
-  if (huge(cta_sums) && fabsf(cta_sums.m) < INFINITY) {
+  if (far(cta_sums) && fabsf(cta_sums.m) < INFINITY) {
     const float m = cta_sums.m;
     Sums mine{m, kNone, 0.f, 0.f};
     each([&](const auto& y) {
@@ -227,11 +238,11 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && !LISTS ? 1536 : 1
         mine.t = fmaf(e, d, mine.t);
       }
     });
-    mine = join_lanes(mine, 32);
+    mine = join_lanes(mine, 32, join);
     if (lane == 0) warp_sums[warp] = mine;
     __syncthreads();
     if (warp == 0) {
-      mine = join_lanes(lane < kThreads / 32 ? warp_sums[lane] : nothing, kThreads / 32);
+      mine = join_lanes(lane < kThreads / 32 ? warp_sums[lane] : nothing, kThreads / 32, join);
       if (lane == 0) cta_sums = mine;
     }
   }
@@ -311,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 4 && !LISTS ? 1536 : 1
     for (int i = 1; i < ctas; ++i) r = join(r, *cluster.map_shared_rank(&cta_sums, i));
     const bool nan = !(r.m == r.m) || r.m == INFINITY, none = r.m == -INFINITY;
     const float log_s = log2f(r.s);
-    auto logprob = [&](float x) { return huge(r) ? (x - r.m) - kLn2 * log_s : fabsf(x) > kHuge ? x - (r.k + log_s) * kLn2 : (fmaf(x, kLog2e, -r.k) - log_s) * kLn2; };
+    auto logprob = [&](float x) { return far(r) ? (x - r.m) - kLn2 * log_s : fabsf(x) > 1e38f ? x - (r.k + log_s) * kLn2 : (fmaf(x, kLog2e, -r.k) - log_s) * kLn2; };
     if (tid == 0) {
       const int token = __ldg(a.tokens + row_at);
       const float x = token >= 0 && token < a.vocab ? row.at(token) : 0.f;
