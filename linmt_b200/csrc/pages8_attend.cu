@@ -9,9 +9,10 @@
 //   four of 256^i O_i.
 // R rows (4, 8 or 16 of a sentence's beams and of the query heads that share a head of the pool) are the right operand, which may be narrow: with 128 positions (or components) on
 // the left a product of 32 KB of pages takes some 300 cycles, a fifth of the time that HBM needs for them.
-// Weights are relative to 2^M, M a whole number for each row: a power of 2 at most above the row's largest weight times scale so far, and at most one below it with 32-bit queries (weights
-// are good to 2^-30 of the largest then), four with 16-bit ones (2^-27, and M follows less often).  The sum of weights alone is relative to 2^L, L 40 above such a number.  (One for both
-// would lose rows whose values differ by more than 32 bits hold.)  Both follow when something exceeds them; only then, every 256 chunks and at the end are O's integers taken out of TMEM, into 32-bit sums.
+// Scores s are taken relative to X, a whole number for each row next to the largest so far, before anything else is added to them: weights are 2^(s - X), and times their scales they are relative to 2^M, M
+// a whole number that is a power of 2 at most above the row's largest weight times scale so far, and at most one below it with 32-bit queries (weights
+// are good to 2^-30 of the largest then), four with 16-bit ones (2^-27, and M follows less often).  (M relative to 0, and X and M each rounded by itself, lost scores of 2^24 and more; one number for both
+// would lose rows whose values differ by more than 32 bits hold.)  M follows when something exceeds it, X when a score exceeds it by 40 more; only then, every 256 chunks and at the end are O's integers taken out of TMEM, into 32-bit sums.
 // A CTA has 128 threads (256 with 16 rows) that turn S into weights, a position and up to eight rows each; one warp that copies blocks and makes queries ready, two pieces ahead, and one that
 // issues the products.  Two CTAs share an SM, three with four rows.  The work is cut into equal shares over the CTAs that fit on the GPU at once, and a second kernel joins the parts of what
 // several of them share.
@@ -47,7 +48,8 @@ template <int R> constexpr int kThreads = 32 * (kWeightWarps<R> + 2);           
 constexpr int kDrain = 256;                  // chunks between two drains: 127 * 255 * 128 * 256 < 2^31
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 constexpr float kLowest = -3.402823466e38f;
-constexpr float kAbove = 40.f;               // of L above the exponents so far
+constexpr float kAbove = 40.f;               // by how much more a score may exceed X than a weight what it is relative to
+constexpr float kFar = 1048576.f;            // scores from here on have too few bits behind the point to find M from their sums with the scales' exponents
 constexpr unsigned long long kWaitCycles = 2000000000ull;      // about a second
 template <int D, int R> constexpr int kKeyStages = (R == 8 ? 3 : 2) * 128 / D;
 template <int D, int R> constexpr int kValueStages = (R == 4 ? 2 : 3) * 128 / D;
@@ -375,10 +377,10 @@ struct Shared {
   long long out[2][R];
   int bad[2][R];
   Ready ready[2];
-  // what the rows' weights are relative to, as it is and as it was before
-  alignas(16) float m[2][R], l[2][R], down_m[R], down_l[R], most_m[4][R], most_l[4][R];
+  // what the rows' scores, and their weights times scales, are relative to, as it is and as it was before
+  alignas(16) float x[2][R], m[2][R], down_x[R], down_m[R], most_x[4][R], most_m[4][R];
   unsigned valid[VS];
-  int add, gave_up;
+  int add, gave_up, far;
   uint32_t tmem;
   alignas(8) unsigned long long k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], s_empty[2], q_full[2], q_empty[2], p_full, o_full, first;
 };
@@ -733,8 +735,11 @@ __global__ void __launch_bounds__(kThreads<R>) __maxnreg__(65536 / (kThreads<R> 
       const Ready p = sh.ready[buffer];
       if (p.chunks < 0) break;
       const int n_rows = min(R, a.g * a.rep - p.rt * R);
-      int now = 0, since = 0;                         // which of m and l; chunks in O
-      if (tid < R) sh.m[0][tid] = sh.l[0][tid] = kLowest;
+      int now = 0, since = 0;                         // which of x and m; chunks in O
+      if (tid < R) {
+        sh.x[0][tid] = kLowest;
+        sh.m[0][tid] = 0.f;
+      }
       weights_sync<kWeights>();
       float sum[RT], acc[RT];
 #pragma unroll
@@ -772,11 +777,11 @@ __global__ void __launch_bounds__(kThreads<R>) __maxnreg__(65536 / (kThreads<R> 
               for (int j = 0; j < 4; ++j) s[r4 + j] = -INFINITY;
               break;
             }
-            float by[4], m[4], l[4], slope[4], centre[4];
+            float by[4], x[4], m[4], slope[4], centre[4];
             int lo[4], span[4];
             four(sh.by[buffer] + row0 + r4, by);
+            four(sh.x[now] + row0 + r4, x);
             four(sh.m[now] + row0 + r4, m);
-            four(sh.l[now] + row0 + r4, l);
             if constexpr (HOW != kPlain) {
               four(sh.slope[buffer] + row0 + r4, slope);
               four(sh.centre[buffer] + row0 + r4, centre);
@@ -792,57 +797,73 @@ __global__ void __launch_bounds__(kThreads<R>) __maxnreg__(65536 / (kThreads<R> 
               if constexpr (HOW == kPlain) {
                 s[r] = fmaf(whole, by[j] * ks, none);
               } else {
-                float x = whole * (by[j] * ks);
+                float y = whole * (by[j] * ks);
                 if constexpr (HOW == kQuick) {
-                  if (a.cap > 0.f) x = capped(x, a.cap * kLog2e);
+                  if (a.cap > 0.f) y = capped(y, a.cap * kLog2e);
                 } else {
-                  if (a.cap > 0.f) x = a.cap * kLog2e * tanhf(x);
+                  if (a.cap > 0.f) y = a.cap * kLog2e * tanhf(y);
                 }
-                s[r] = x - slope[j] * fabsf((float)pos - centre[j]) + none;
+                s[r] = y - slope[j] * fabsf((float)pos - centre[j]) + none;
               }
               if (a.first) s[r] = (unsigned)(pos - lo[j]) < (unsigned)span[j] || pos < a.sinks ? s[r] : -INFINITY;
-              most = fmaxf(most, fmaxf(s[r] + (ve - m[j]), s[r] - l[j]));
+              most = fmaxf(most, (s[r] - x[j]) + fmaxf(ve - m[j], -kAbove));
             }
           }
           over = weights_any<kWeights>(most > slack) || over;
           if (c > 0) bar_wait(shared(&sh.o_full), it - 1 & 1, gave_up);
           // Something exceeds what the rows' weights are relative to: that follows.
           if (over) {
-            float most_m = kLowest, most_l = kLowest;      // of row row0 + lane
+            float most_x = kLowest, most_m = kLowest;      // of row row0 + lane
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-              const float x = warp_max(s[r] + ve), y = warp_max(s[r]);
-              if (lane == r) { most_m = x; most_l = y; }
+              const float x = warp_max(s[r]), y = warp_max(s[r] + ve);
+              if (lane == r) { most_x = x; most_m = y; }
             }
-            if (lane < RT) { sh.most_m[warp % 4][row0 + lane] = most_m; sh.most_l[warp % 4][row0 + lane] = most_l; }
+            if (lane < RT) { sh.most_x[warp % 4][row0 + lane] = most_x; sh.most_m[warp % 4][row0 + lane] = most_m; }
             weights_sync<kWeights>();
+            auto most_of = [&](const float (&x)[4][R]) { return fmaxf(fmaxf(x[0][tid], x[1][tid]), fmaxf(x[2][tid], x[3][tid])); };
             if (tid < R) {
-              const float was_m = sh.m[now][tid], was_l = sh.l[now][tid];
-              float m = fmaxf(fmaxf(sh.most_m[0][tid], sh.most_m[1][tid]), fmaxf(sh.most_m[2][tid], sh.most_m[3][tid]));
-              float l = fmaxf(fmaxf(sh.most_l[0][tid], sh.most_l[1][tid]), fmaxf(sh.most_l[2][tid], sh.most_l[3][tid]));
-              m = m - was_m > slack ? ceilf(m) : was_m;
-              l = l - was_l > slack ? ceilf(l) + kAbove : was_l;
+              const float was_x = sh.x[now][tid], was = was_x + sh.m[now][tid];      // (was_x as it is where nothing has been seen)
+              const float top_x = most_of(sh.most_x), top = most_of(sh.most_m), x = top_x - was_x > kAbove + slack ? ceilf(top_x) : was_x, m = (top - was > slack ? ceilf(top) : was) - x;
+              sh.x[now ^ 1][tid] = x;
               sh.m[now ^ 1][tid] = m;
-              sh.l[now ^ 1][tid] = l;
-              sh.down_m[tid] = exp2_of(was_m - m);
-              sh.down_l[tid] = exp2_of(was_l - l);
+              sh.down_x[tid] = exp2_of(was_x - x);
+              sh.down_m[tid] = exp2_of(was_x - x + (sh.m[now][tid] - m));
+              const unsigned far = __ballot_sync((1u << R) - 1, fabsf(x) > kFar && x > kLowest);
+              if (tid == 0) sh.far = far != 0;
             }
             weights_sync<kWeights>();
+            if (sh.far) {                                  // M once more, from differences to X
+              float z = kLowest;
+#pragma unroll
+              for (int r = 0; r < RT; ++r) {
+                const float y = warp_max(s[r] - sh.x[now ^ 1][row0 + r] + ve);
+                if (lane == r) z = y;
+              }
+              if (lane < RT) sh.most_m[warp % 4][row0 + lane] = z;
+              weights_sync<kWeights>();
+              if (tid < R) {
+                const float was = sh.x[now][tid] - sh.x[now ^ 1][tid] + sh.m[now][tid], top = most_of(sh.most_m), m = top - was > slack ? ceilf(top) : was;
+                sh.m[now ^ 1][tid] = m;
+                sh.down_m[tid] = exp2_of(was - m);
+              }
+              weights_sync<kWeights>();
+            }
             now ^= 1;
           }
         } else {
           bar_wait(shared(&sh.o_full), it - 1 & 1, gave_up);
         }
         if (over) {
-          // O's integers into sums, which are relative to 2^m then.
+          // O's integers into sums, which are relative to 2^M then.
           tmem_after();
           int o[kWeightDigits * RT];
           if (since) tmem_load(lanes + kTmemO<R> + kWeightDigits * row0, o);
 #pragma unroll
           for (int r4 = 0; r4 < RT; r4 += 4) {
-            float down_m[4], down_l[4];
+            float down_x[4], down_m[4];
+            four(sh.down_x + row0 + r4, down_x);
             four(sh.down_m + row0 + r4, down_m);
-            four(sh.down_l + row0 + r4, down_l);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const int* const x = o + 4 * (r4 + j);
@@ -850,7 +871,7 @@ __global__ void __launch_bounds__(kThreads<R>) __maxnreg__(65536 / (kThreads<R> 
               if (since) acc[r4 + j] = fmaf(v, unit, acc[r4 + j]);
               if (!last) {
                 acc[r4 + j] *= down_m[j];
-                sum[r4 + j] *= down_l[j];
+                sum[r4 + j] *= down_x[j];
               }
             }
           }
@@ -860,18 +881,19 @@ __global__ void __launch_bounds__(kThreads<R>) __maxnreg__(65536 / (kThreads<R> 
         if (last) break;
 #pragma unroll
         for (int r4 = 0; r4 < RT; r4 += 4) {
-          float m[4], l[4];
+          float x[4], m[4];
           uint32_t w[4];
           if (r4 > 0 && row0 + r4 >= n_rows) {
             sh.weights[(row0 + r4) / 4][mine] = make_uint4(0, 0, 0, 0);
             break;
           }
+          four(sh.x[now] + row0 + r4, x);
           four(sh.m[now] + row0 + r4, m);
-          four(sh.l[now] + row0 + r4, l);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            sum[r4 + j] += exp2_of(s[r4 + j] - l[j]);
-            w[j] = __float2uint_rn(exp2_of(s[r4 + j] + (ve - m[j])) * vf);
+            const float d = s[r4 + j] - x[j];
+            sum[r4 + j] += exp2_of(d);
+            w[j] = __float2uint_rn(exp2_of(d + (ve - m[j])) * vf);
           }
           sh.weights[(row0 + r4) / 4][mine] = make_uint4(w[0], w[1], w[2], w[3]);
         }
@@ -894,20 +916,20 @@ __global__ void __launch_bounds__(kThreads<R>) __maxnreg__(65536 / (kThreads<R> 
       // a part of the workspace: [row][D] values, [row] exponent, [row] weight.  A CTA's first is of the segment that it has from the CTA before, its second of the one that the next goes on with.
       float* const ws = a.ws + ((int64_t)blockIdx.x * 2 + p.part) * kPart;
       if (tid < R) {
-        float weight = 0.f, l = kLowest, f = 0.f;
+        float weight = 0.f, x = kLowest, f = 0.f;
         if (p.chunks) {
-          weight = (sh.most_m[0][tid] + sh.most_m[1][tid] + sh.most_m[2][tid] + sh.most_m[3][tid]) * 1099511627776.f;      // 2^40
-          l = sh.l[now][tid] - kAbove;
-          f = weight > 0.f ? exp2_of(sh.m[now][tid] - l) / weight : 0.f;
+          weight = sh.most_m[0][tid] + sh.most_m[1][tid] + sh.most_m[2][tid] + sh.most_m[3][tid];
+          x = sh.x[now][tid];
+          f = weight > 0.f ? exp2_of(sh.m[now][tid]) / weight : 0.f;
           if ((sh.bad[buffer][tid] && weight > 0.f) || *gave_up) f = weight = NAN;
         }
         sh.down_m[tid] = f;
         if (tid < n_rows) {
           if (p.whole) {
             const int row = p.rt * R + tid, g = row / a.rep;
-            if (a.lse) a.lse[((int64_t)p.sent * a.g + g) * a.heads + p.kvh * a.rep + row - g * a.rep] = weight == 0.f ? -INFINITY : (l + log2f(weight)) * kLn2;
+            if (a.lse) a.lse[((int64_t)p.sent * a.g + g) * a.heads + p.kvh * a.rep + row - g * a.rep] = weight == 0.f ? -INFINITY : (x + log2f(weight)) * kLn2;
           } else {
-            ws[R * D + tid] = l;
+            ws[R * D + tid] = x;
             ws[R * D + R + tid] = weight;
           }
         }

@@ -56,3 +56,129 @@ def test_score_rows_far_from_zero(ops, n, v, dtype):
         tokens = np.full((n, 1), v // 3, np.int32)
         tokens[1::2] = v - 1
         far_check(ops, x, _cuda(tokens), 0 if at % 3 == 0 else 5)
+
+
+# ---- attention
+
+from test_gpu_pages8 import attend_ref, blocks, memory8
+
+
+def attend_far_check(ops, q, pool, table, lens, kv, scale, alike=False, slope=None, **window):
+    """As attend_ref has it, but where one position has all the weight, or all scores are `alike` to the bit, what a far score is off by does not matter: the result has to be that position's value, or the mean.
+    Returns the rows of which that was so."""
+    dev = {k: _cuda(np.asarray(v, np.int32)) for k, v in window.items()}
+    if slope is not None:
+        slope, centre = slope
+        dev.update(slope=_cuda(np.asarray(slope, np.float32)), centre=_cuda(np.asarray(centre, np.float32)))
+        window.update(slope=np.asarray(slope, np.float32).astype(np.float64), centre=np.asarray(centre, np.float32).astype(np.float64))
+    got, lse = ops.attend_pages8(q, pool, table, _cuda(np.asarray(lens, np.int32)), scale=scale, want_lse=True, **dev)
+    scale = float(np.float32(scale))
+    want, want_lse, tol, _ = attend_ref(q, kv, table.cpu().numpy(), lens, scale, **window)
+    n, g, heads, dim = q.shape
+    page, rep, clear = kv.shape[3], heads // kv.shape[2], np.zeros((n, g, heads), bool)
+    x = q.double().cpu().numpy()
+    for i in range(n):
+        pos = np.arange(lens[i])
+        for b in range(g):
+            seen = pos >= 0 if "first" not in window else (pos >= window["first"][i][b]) & (pos < window["last"][i][b])
+            if not seen.any():
+                continue
+            for h in range(heads):
+                k, v = (kv[j][table.cpu().numpy()[i][pos // page], h // rep, pos % page][seen] for j in range(2))
+                s = scale * (k @ x[i, b, h])
+                d = abs(scale) * np.abs(x[i, b, h]).max() * 2.0 ** -22 * (np.abs(k).sum(-1).max() + np.abs(k).max()) + 8 * 2.0 ** -24 * np.abs(s).max()
+                if slope is not None:
+                    s = s - window["slope"][h] * np.abs(pos[seen] - window["centre"][i, b])
+                    d += 8 * 2.0 ** -24 * np.abs(s).max()
+                first, second = np.sort(s)[::-1][[0, min(1, len(s) - 1)]]
+                clear[i, b, h] = alike or len(s) == 1 or first - second > 2 * d + 60
+                if clear[i, b, h]:
+                    want[i, b, h] = v.mean(0) if alike else v[s.argmax()]
+                    # sums of equal weights and their joins, 2^-24 each, and six roundings; the weight times its scale to 2^-27 or 2^-30 of the row's largest
+                    tol[i, b, h] = np.abs(v).max() * ((len(s) / 128 + 40) * 2.0 ** -23 + 2.0 ** -20 + len(s) * 2.0 ** (-30 if q.dtype == F32 else -27)) if alike else \
+                        np.abs(want[i, b, h]).max() * (2.0 ** -21 + 2.0 ** (-30 if q.dtype == F32 else -27))
+    out, kind = got.double().cpu().numpy(), torch.finfo(q.dtype)
+    beyond = np.abs(want) > kind.max * (1 + kind.eps / 4)      # half a step above a type's largest number it has none any more: 65520 in fp16
+    assert (out[beyond] == np.sign(want[beyond]) * INF).all()
+    off = np.where(beyond, 0, np.abs(np.where(beyond, 0, out) - want) - HALF_STEP[q.dtype] * np.abs(want))
+    assert (off <= tol[..., None]).all(), (off - tol[..., None]).max()
+    l, seen = lse.double().cpu().numpy(), np.isfinite(want_lse)
+    # a score's own roundings, and those of its components (2^-22 of the largest): all of one size here
+    assert (l[~seen] == want_lse[~seen]).all() and (np.abs(l - want_lse)[seen] <= 2.0 ** -15 * np.abs(want_lse[seen]) + 2.0 ** -12).all()
+    return clear
+
+
+EXPONENTS = [18, 20, 22, 23, 24, 25, 26, 27, 28, 30, 35, 40, 63, 100]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attend_one_position_with_a_far_score(ops, sign, dtype):
+    """A result is the value of the only position, however far its score."""
+    rng = _rng(91)
+    lens, heads, dim, page, g = [1, 600], 2, 64, 16, 3
+    pool, table, kv = memory8(rng, 2, lens, heads, dim, page, sizes=6.0)
+    q = _cuda(np.abs(rng.normal(0, 1, (2, g, heads, dim))).astype(np.float32) + 0.5, dtype)
+    first = np.array([[0] * g, [5, 300, 599]])
+    for e in EXPONENTS:
+        clear = attend_far_check(ops, q, pool, table, lens, kv, sign * 2.0 ** e / 16, first=first, last=first + 1)
+        assert clear.all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("lens", [[300, 77], [20001], [700] * 30])
+def test_attend_far_scores_that_are_alike(ops, lens, dtype):
+    """All keys and their scales alike, the values' scales differ: the mean of the values, by one CTA or by several."""
+    rng = _rng(92, len(lens))
+    n, heads, dim, page = len(lens), 1, 64, 64
+    pool, table, kv = memory8(rng, n, lens, heads, dim, page, sizes=1.0)
+    codes = np.rint(kv / np.maximum(1e-30, np.abs(kv).max((-1), keepdims=True)) * 100).astype(np.int64)
+    codes[0] = codes[0, 0, 0, 0]
+    scales = (2.0 ** rng.integers(-8, -2, (2, kv.shape[1], heads, page // 16))).astype(np.float32)
+    scales[0] = 2.0 ** -5
+    pool, kv = _cuda(blocks(codes, scales)), codes * scales.repeat(16, -1)[..., None].astype(np.float64)
+    q = _cuda(rng.normal(0, 1, (n, 2, 1, dim)).astype(np.float32), dtype)
+    size = np.abs(q.double().cpu().numpy() @ kv[0, 0, 0, 0]).max()
+    for e in EXPONENTS:
+        for sign in (1, -1):
+            attend_far_check(ops, q, pool, table, lens, kv, sign * 2.0 ** e / size, alike=True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("order", ["rising", "falling", "any"])
+def test_attend_far_scores_of_many_positions(ops, order, dtype):
+    """The position with the largest score has all the weight, first, last or anywhere; rows with ordinary scores beside them."""
+    rng = _rng(93)
+    lens, heads, dim, page, g = [4000, 900], 1, 64, 32, 9
+    pool, table, kv = memory8(rng, 2, lens, heads, dim, page, sizes=2.0)
+    codes = np.clip(np.rint(rng.normal(0, 20, kv.shape)), -60, 60).astype(np.int64)
+    scales = (2.0 ** rng.integers(-8, -3, kv.shape[1:3] + (page // 16,))).astype(np.float32)
+    scales = np.stack([np.full_like(scales, 2.0 ** -5), scales])
+    for i, length in enumerate(lens):
+        at = np.arange(length)
+        ramp = np.sort(rng.permutation(16129)[:length] - 8064)       # two digits, so that no two are alike
+        ramp = {"rising": ramp, "falling": ramp[::-1], "any": rng.permutation(ramp)}[order]
+        for c, digit in ((0, np.round(ramp / 127)), (1, ramp - 127 * np.round(ramp / 127))):
+            codes[0, table.cpu().numpy()[i][at // page], 0, at % page, c] = digit
+    codes[0, ..., 2:] = 0
+    pool, kv = _cuda(blocks(codes, scales)), codes * scales.repeat(16, -1)[..., None].astype(np.float64)
+    for e in EXPONENTS:
+        x = np.zeros((2, g, 1, dim))
+        x[..., 0], x[..., 1] = 127, 1
+        x[:, 1::3] *= -1
+        x[:, ::3] = rng.normal(0, 2.0 ** -12 if dtype == F16 else 2.0 ** -e, x[:, ::3].shape)
+        q = _cuda(x.astype(np.float32), dtype)
+        clear = attend_far_check(ops, q, pool, table, lens, kv, 2.0 ** (e - 9))
+        assert e < 22 or (clear[:, 1::3].all() and clear[:, 2::3].all())      # two scores are 2^(e - 14) apart at least, the bound of what they are off by is 2^(e - 20)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attend_far_biases(ops, dtype):
+    """A bias of up to 2^36 a position: the one next to a row's centre, or the last one before it."""
+    rng = _rng(94)
+    lens, heads, dim, page, g = [3000, 1, 200], 2, 128, 16, 4
+    pool, table, kv = memory8(rng, 3, lens, heads, dim, page, sizes=3.0)
+    q = _cuda(rng.normal(0, 1, (3, g, heads, dim)).astype(np.float32), dtype)
+    centre = np.array([[0.0, 1500.25, 1e5, -7e5], [0.0, 3e4, -3.0, 1.0], [99.75, 0.0, 1e4, 200.0]])
+    for e in (14, 20, 28, 36):
+        assert attend_far_check(ops, q, pool, table, lens, kv, dim ** -0.5, slope=([2.0 ** e, 2.0 ** (e - 2)], centre)).all()
