@@ -496,7 +496,7 @@ int linmt_read_pages8(const linmt_pages8_rows_args* args);
 /* Attention of g query rows per sentence over the sentence's positions in a pool of 8-bit pages, as linmt_attend_pages4 with one argument more:
  *   seen: t < sinks or first[i][row] <= t < last[i][row] (NULL: all), 0 <= t < len[i], and the table names a page of the pool
  * A query's components are taken to 2^-22 of its row's largest (of 2^-106 for smaller ones); their products with the codes are summed exactly, and so are those of the weights:
- * a weight times its block's scale is taken to 2^-30 of the row's largest, with 16-bit queries to 2^-27.  Scores are numbers of 32 bits, good to some 2^-21 of themselves however large they are.  With 16-bit queries a cap of up to 64 is good to 3e-7 of itself.
+ * a weight times its block's scale is taken to 2^-30 of the row's largest, with 16-bit queries to 2^-27.  Scores are held in 32 bits.  With 16-bit queries a cap of up to 64 is good to 3e-7 of itself.
  * A query with a NaN or an infinity that sees something: NaN and NaN; so may one whose scores leave 32 bits.  All waits inside the kernel are bounded: rows of a CTA that gave up are NaN. */
 typedef struct linmt_attend_pages8_args {
   uint32_t size;

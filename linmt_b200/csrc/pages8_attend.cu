@@ -404,6 +404,8 @@ __device__ __forceinline__ void four(const int* p, int (&x)[4]) {
   x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
 }
 __device__ __forceinline__ float power_of_2(int e) { return __int_as_float((127 + e) << 23); }      // -126 .. 127
+// A sum of weights, 0 or 2^-1 .. 2^76, as 2^k times something between 1 and 2; NaN goes with k = 0.
+__device__ __forceinline__ int exponent_of(float weight) { return weight > 0.f ? (__float_as_int(weight) >> 23) - 127 : 0; }
 
 // What a piece's rows see and where their results go; by a warp, a lane for each row.
 template <int D, int R>
@@ -916,13 +918,18 @@ __global__ void __launch_bounds__(kThreads<R>) __maxnreg__(65536 / (kThreads<R> 
       // a part of the workspace: [row][D] values, [row] exponent, [row] weight.  A CTA's first is of the segment that it has from the CTA before, its second of the one that the next goes on with.
       float* const ws = a.ws + ((int64_t)blockIdx.x * 2 + p.part) * kPart;
       if (tid < R) {
+        // 2^M / weight, as values of up to 2^127 ask for it, is no number of 32 bits: two factors, the first a power of 2.
         float weight = 0.f, x = kLowest, f = 0.f;
+        int e = 0;
         if (p.chunks) {
           weight = sh.most_m[0][tid] + sh.most_m[1][tid] + sh.most_m[2][tid] + sh.most_m[3][tid];
           x = sh.x[now][tid];
-          f = weight > 0.f ? exp2_of(sh.m[now][tid]) / weight : 0.f;
+          const int k = exponent_of(weight);
+          e = min(max((int)fmaxf(sh.m[now][tid], -1000.f) - k, -250), 250);
+          f = weight == 0.f ? 0.f : power_of_2(e - e / 2) / (weight * power_of_2(-k));
           if ((sh.bad[buffer][tid] && weight > 0.f) || *gave_up) f = weight = NAN;
         }
+        sh.down_x[tid] = power_of_2(e / 2);
         sh.down_m[tid] = f;
         if (tid < n_rows) {
           if (p.whole) {
@@ -938,7 +945,7 @@ __global__ void __launch_bounds__(kThreads<R>) __maxnreg__(65536 / (kThreads<R> 
       if (mine < D) {
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          const float value = acc[r] * sh.down_m[row0 + r];
+          const float value = acc[r] * sh.down_x[row0 + r] * sh.down_m[row0 + r];
           if (row0 + r < n_rows) {
             if (p.whole) store_as(a.out, sh.out[buffer][row0 + r] + mine, a.dtype, value);
             else ws[(row0 + r) * D + mine] = value;
@@ -979,7 +986,7 @@ constexpr int kJoinThreads = 512;
 template <int D, int R>
 __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_constant__ AttendParams a, int blocks) {
   constexpr int kPart = R * (D + 2), kBy = kJoinThreads / (R * D / 4);
-  __shared__ float s_top[kBy][R], s_weight[kBy][R];
+  __shared__ float s_x[kBy][R], s_k[kBy][R], s_weight[kBy][R];
   __shared__ float4 s_sum[kBy][R * D / 4];
   const int at = threadIdx.x % (R * D / 4), by = threadIdx.x / (R * D / 4), r = at / (D / 4), d = at % (D / 4) * 4;
   wait_for_last();
@@ -987,15 +994,18 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
   if (ends.x < 0) return;
   const int from = ends.w, n_parts = (int)blockIdx.x - from + 1;
   auto part = [&](int i) { return a.ws + ((int64_t)(from + i) * 2 + (i == 0)) * kPart; };
-  // The largest exponent so far goes along, so that every part is waited for once: eight of them at a time are on their way.
-  float top = kLowest, weight = 0.f;
+  // A part counts 2^(x + k) times a number between 1 and 2, k its sum's exponent.  The largest so far goes along, so that every part is waited for once: eight of them at a time are on their
+  // way.  x and k stay apart, as x may have no place for k's last bits; sums are 2^fewer smaller, so that values of up to 2^127 have room.
+  const int fewer = 33 - __clz(n_parts);
+  float x = kLowest, k = 0.f, weight = 0.f;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = by; i0 < n_parts; i0 += 8 * kBy) {
-    float m[8], l[8];
+    float m[8], l[8], n[8];
     float4 v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       m[j] = kLowest;
+      l[j] = 0.f;
       if (i0 + j * kBy < n_parts) {
         const float* const w = part(i0 + j * kBy);
         m[j] = w[R * D + r];
@@ -1003,32 +1013,37 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
         v[j] = *reinterpret_cast<const float4*>(w + r * D + d);
       }
     }
-    float now = top;
+    const float was_x = x, was_k = k;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) now = fmaxf(now, m[j]);
-    const float f0 = exp2_of(top - now);
-    top = now;
+    for (int j = 0; j < 8; ++j) {
+      const int e = exponent_of(l[j]);
+      n[j] = (float)e;
+      l[j] *= power_of_2(-e);
+      if (m[j] - x + (n[j] - k) > 0.f) { x = m[j]; k = n[j]; }
+    }
+    const float f0 = exp2_of(was_x - x + (was_k - k));
     weight *= f0;
     sum.x *= f0; sum.y *= f0; sum.z *= f0; sum.w *= f0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if (i0 + j * kBy >= n_parts) break;
-      const float f = exp2_of(m[j] - now) * l[j];
+      const float f = exp2_of(m[j] - x + (n[j] - k) - (float)fewer) * l[j];
       sum.x += f * v[j].x; sum.y += f * v[j].y; sum.z += f * v[j].z; sum.w += f * v[j].w;
       weight += f;
     }
   }
   s_sum[by][at] = sum;
-  if (d == 0) { s_top[by][r] = top; s_weight[by][r] = weight; }
+  if (d == 0) { s_x[by][r] = x; s_k[by][r] = k; s_weight[by][r] = weight; }
   __syncthreads();
   if (by || r >= a.g * a.rep - ends.z * R) return;
 #pragma unroll
-  for (int i = 1; i < kBy; ++i) top = fmaxf(top, s_top[i][r]);
+  for (int i = 1; i < kBy; ++i)
+    if (s_x[i][r] - x + (s_k[i][r] - k) > 0.f) { x = s_x[i][r]; k = s_k[i][r]; }
   sum = make_float4(0.f, 0.f, 0.f, 0.f);
   weight = 0.f;
 #pragma unroll
   for (int i = 0; i < kBy; ++i) {
-    const float f = exp2_of(s_top[i][r] - top);
+    const float f = exp2_of(s_x[i][r] - x + (s_k[i][r] - k));
     const float4 v = s_sum[i][at];
     sum.x += f * v.x; sum.y += f * v.y; sum.z += f * v.z; sum.w += f * v.w;
     weight += f * s_weight[i][r];
@@ -1040,7 +1055,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
   store_as(a.out, to + 1, a.dtype, sum.y * f);
   store_as(a.out, to + 2, a.dtype, sum.z * f);
   store_as(a.out, to + 3, a.dtype, sum.w * f);
-  if (d == 0 && a.lse) a.lse[((int64_t)ends.x * a.g + g) * a.heads + h] = weight == 0.f ? -INFINITY : (top + log2f(weight)) * kLn2;
+  if (d == 0 && a.lse) a.lse[((int64_t)ends.x * a.g + g) * a.heads + h] = weight == 0.f ? -INFINITY : (x + (k + (float)fewer + log2f(weight))) * kLn2;
 }
 
 template <int D, int R>

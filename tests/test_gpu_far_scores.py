@@ -182,3 +182,26 @@ def test_attend_far_biases(ops, dtype):
     centre = np.array([[0.0, 1500.25, 1e5, -7e5], [0.0, 3e4, -3.0, 1.0], [99.75, 0.0, 1e4, 200.0]])
     for e in (14, 20, 28, 36):
         assert attend_far_check(ops, q, pool, table, lens, kv, dim ** -0.5, slope=([2.0 ** e, 2.0 ** (e - 2)], centre)).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lens", [[700, 90], [6000], [20000]])
+@pytest.mark.parametrize("size", [-120, -60, 86, 90, 110, 119])
+def test_attend_values_of_all_sizes(ops, size, lens, dtype):
+    """Values' scales of 2^size, scores that rise by some 40 powers of 2 behind the first products: by one CTA or by several."""
+    from test_gpu_pages8 import attend_check
+    rng = _rng(95, len(lens), lens[0])
+    n, heads, dim, page, g = len(lens), 2, 64, 64, 3
+    pool, table, kv = memory8(rng, n, lens, heads, dim, page)
+    codes = rng.integers(-100, 101, kv.shape)
+    codes[1, ..., ::3] = np.abs(codes[1, ..., ::3])
+    codes[0, ..., 0] = 0
+    scales = np.stack([np.full(kv.shape[1:3] + (page // 16,), 2.0 ** -9), 2.0 ** rng.integers(size - 3, size + 1, kv.shape[1:3] + (page // 16,))]).astype(np.float32)
+    for i, length in enumerate(lens):
+        at = np.arange(length)
+        codes[0, table.cpu().numpy()[i][at // page], :, at % page, 0] = np.where(at < 300, 0, 100)[:, None]      # 300 positions: three products
+    pool, kv = _cuda(blocks(codes, scales)), codes * scales.repeat(16, -1)[..., None].astype(np.float64)
+    q = rng.normal(0, 0.05, (n, g, heads, dim))
+    for up in (0.0, 20.0, 27.0, 28.0, 29.0, 30.0, 31.0):      # 2^40 is e^27.7, 2^44 e^30.5
+        q[..., 0] = up / (100 * 2.0 ** -9)
+        attend_check(ops, _cuda(q.astype(np.float32), dtype), pool, table, lens, kv, scale=1.0)
