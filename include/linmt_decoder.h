@@ -553,7 +553,7 @@ typedef struct linmt_fork_pages_args {
   int32_t* out_used;         /* [1] */
   int32_t* out_src;          /* [n * k] */
   int32_t* out_dst;          /* [n * k] */
-  int32_t n, k, width, page, n_pages, n_free;   /* n * k <= 16384 */
+  int32_t n, k, width, page, n_pages, n_free;   /* n * k <= 16384; n * k * width, n_pages and n_free up to 2^31 - 2^17 - 1 */
 } linmt_fork_pages_args;
 int linmt_fork_pages(const linmt_fork_pages_args* args);
 
@@ -577,7 +577,7 @@ typedef struct linmt_compact_pages_args {
   int32_t* out_src;          /* [n_pages / 2] */
   int32_t* out_dst;          /* [n_pages / 2] */
   int32_t* workspace;        /* [n_pages], the call's own until it has run */
-  int32_t rows, width, page, n_pages;
+  int32_t rows, width, page, n_pages;   /* rows * width and n_pages up to 2^31 - 2^17 - 1 */
 } linmt_compact_pages_args;
 int linmt_compact_pages(const linmt_compact_pages_args* args);
 

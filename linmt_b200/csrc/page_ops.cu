@@ -18,6 +18,7 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRows = 16384;
+constexpr int kMaxPlaces = INT32_MAX - (1 << 17);    // columns of a table, pages: what is counted in 32 bits may run ahead of them by all threads' next four places
 constexpr int kRowBytes = 3 * (int)sizeof(int) + (int)sizeof(short);
 constexpr int kPortableCluster = 8, kMaxCluster = 16;
 
@@ -428,7 +429,8 @@ int linmt_fork_pages(const linmt_fork_pages_args* g) {
     return op_fail(LINMT_EINVAL, "fork_pages: an array is missing");
   if (!all_aligned4(g->table, g->len, g->parents, g->shares, g->free_pages, g->used, g->out_table, g->out_len, g->out_shares, g->out_free, g->out_used, g->out_src, g->out_dst))
     return op_fail(LINMT_EINVAL, "fork_pages: an array is not aligned to its type");
-  if (rows > kMaxRows || rows * g->width > INT32_MAX) return op_fail(LINMT_ELIMIT, "fork_pages: n * k = %lld (at most %d), rows * width = %lld (below 2^31)", (long long)rows, kMaxRows, (long long)rows * g->width);
+  if (rows > kMaxRows || rows * g->width > kMaxPlaces || g->n_pages > kMaxPlaces || g->n_free > kMaxPlaces)
+    return op_fail(LINMT_ELIMIT, "fork_pages: n * k = %lld (at most %d), rows * width = %lld, n_pages = %d, n_free = %d (at most 2^31 - 2^17 - 1)", (long long)rows, kMaxRows, (long long)rows * g->width, g->n_pages, g->n_free);
   OnDevice on(g->device);
   if (on.err != cudaSuccess) return op_cuda(on.err, "fork_pages");
   const ForkParams p{g->table, g->table_stride, g->len, g->parents, g->done, g->shares, g->free_pages, g->used, g->out_table, g->out_table_stride, g->out_len, g->out_shares, g->out_free,
@@ -451,7 +453,8 @@ int linmt_compact_pages(const linmt_compact_pages_args* g) {
     return op_fail(LINMT_EINVAL, "compact_pages: an array is missing");
   if (!all_aligned4(g->table, g->len, g->shares, g->out_table, g->out_shares, g->out_free, g->out_used, g->out_src, g->out_dst, g->workspace))
     return op_fail(LINMT_EINVAL, "compact_pages: an array is not aligned to its type");
-  if ((int64_t)g->rows * g->width > INT32_MAX) return op_fail(LINMT_ELIMIT, "compact_pages: rows * width = %lld (below 2^31)", (long long)g->rows * g->width);
+  if ((int64_t)g->rows * g->width > kMaxPlaces || g->n_pages > kMaxPlaces)
+    return op_fail(LINMT_ELIMIT, "compact_pages: rows * width = %lld, n_pages = %d (at most 2^31 - 2^17 - 1)", (long long)g->rows * g->width, g->n_pages);
   OnDevice on(g->device);
   if (on.err != cudaSuccess) return op_cuda(on.err, "compact_pages");
   const CompactParams p{g->table, g->table_stride, g->len, g->shares, g->out_table, g->out_table_stride, g->out_shares, g->out_free, g->out_used, g->out_src, g->out_dst, g->workspace,
