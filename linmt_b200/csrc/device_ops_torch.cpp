@@ -589,8 +589,8 @@ Rows rows_of_table(const Tensor& t, const Tensor& lens) {
   const int64_t d = lens.dim();
   NEED(t.scalar_type() == at::kInt && t.dim() == d + 1 && t.sizes().slice(0, d) == lens.sizes(), "table has to be int32, a row of columns for each of lens");
   NEED(t.size(d) <= 1 || t.stride(d) == 1, "the rows of table have to be contiguous");
-  NEED(d == 1 || t.size(0) <= 1 || t.size(1) <= 0 || t.stride(0) == t.size(1) * t.stride(1), "the rows of table have to lie evenly");
-  return {lens.numel(), t.size(d), lens.numel() == 0 ? t.size(d) : t.stride(d - 1)};
+  NEED(d == 1 || t.size(0) <= 1 || t.size(1) <= 1 || t.stride(0) == t.size(1) * t.stride(1), "the rows of table have to lie evenly");
+  return {lens.numel(), t.size(d), lens.numel() == 0 ? t.size(d) : t.stride(d == 2 && t.size(1) == 1 ? 0 : d - 1)};      // (a dimension of one row says nothing)
 }
 // Results of a call: made, or the caller's; each lies apart from all that is read and from the others, but one that may be what it follows, place for place.
 struct Out {
