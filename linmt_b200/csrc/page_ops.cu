@@ -6,6 +6,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "device_ops.h"
 
@@ -392,8 +393,23 @@ int cluster_for(int64_t things) {
   while (c < kMaxCluster && (int64_t)c * kThreads * 2 < things) c *= 2;
   return c;
 }
+// Whether the device has room for a cluster of 16 with as much shared memory as the kernel may ask for (a part of a GPU may not): asked once for each of the first 64 devices.
 template <class P>
-cudaError_t launch_cluster(void (*kernel)(P), const P& p, int ctas, size_t smem, cudaStream_t st) {
+bool has_room(void (*kernel)(P), int device, cudaLaunchConfig_t cfg, size_t most_smem) {
+  static std::atomic<signed char> known[64];           // 1: yes, -1: no
+  const bool keep = device >= 0 && device < 64;
+  if (const int was = keep ? known[device].load(std::memory_order_relaxed) : 0) return was > 0;
+  cfg.dynamicSmemBytes = most_smem;
+  int clusters = 0;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most_smem);
+  if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg);
+  if (e != cudaSuccess) cudaGetLastError();
+  const bool room = e == cudaSuccess && clusters > 0;
+  if (keep) known[device].store(room ? 1 : -1, std::memory_order_relaxed);
+  return room;
+}
+template <class P>
+cudaError_t launch_cluster(void (*kernel)(P), const P& p, int device, int ctas, size_t smem, size_t most_smem, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -406,6 +422,10 @@ cudaError_t launch_cluster(void (*kernel)(P), const P& p, int ctas, size_t smem,
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   cudaError_t e = ctas > kPortableCluster ? cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) : cudaSuccess;
+  if (e == cudaSuccess && ctas > kPortableCluster && !has_room(kernel, device, cfg, most_smem)) {
+    attr.val.clusterDim.x = kPortableCluster;
+    cfg.gridDim = dim3(kPortableCluster);
+  }
   if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, p);
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
@@ -440,7 +460,7 @@ int linmt_fork_pages(const linmt_fork_pages_args* g) {
     const cudaError_t e = cudaFuncSetAttribute(fork_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxRows * kRowBytes);
     if (e != cudaSuccess) return op_cuda(e, "fork_pages");
   }
-  const cudaError_t e = launch_cluster(fork_kernel, p, cluster_for(std::max(rows * g->width, (int64_t)g->n_pages + g->n_free)), smem, static_cast<cudaStream_t>(g->stream));
+  const cudaError_t e = launch_cluster(fork_kernel, p, g->device, cluster_for(std::max(rows * g->width, (int64_t)g->n_pages + g->n_free)), smem, (size_t)kMaxRows * kRowBytes, static_cast<cudaStream_t>(g->stream));
   return e == cudaSuccess ? LINMT_OK : op_cuda(e, "fork_pages");
 }
 
@@ -459,7 +479,7 @@ int linmt_compact_pages(const linmt_compact_pages_args* g) {
   if (on.err != cudaSuccess) return op_cuda(on.err, "compact_pages");
   const CompactParams p{g->table, g->table_stride, g->len, g->shares, g->out_table, g->out_table_stride, g->out_shares, g->out_free, g->out_used, g->out_src, g->out_dst, g->workspace,
                         g->rows, g->width, g->page, g->n_pages};
-  const cudaError_t e = launch_cluster(compact_kernel, p, cluster_for(std::max((int64_t)g->rows * g->width, (int64_t)g->n_pages)), 0, static_cast<cudaStream_t>(g->stream));
+  const cudaError_t e = launch_cluster(compact_kernel, p, g->device, cluster_for(std::max((int64_t)g->rows * g->width, (int64_t)g->n_pages)), 0, 0, static_cast<cudaStream_t>(g->stream));
   return e == cudaSuccess ? LINMT_OK : op_cuda(e, "compact_pages");
 }
 
