@@ -286,6 +286,9 @@ int linmt_k_logits(const float* X, const float* W, const float* bias, int32_t R,
 int linmt_k_softmax_topk(const float* logits, int32_t R, int32_t V, int32_t kk, int32_t* idx, float* logp,
                          float* eos_logp, int32_t device);
 
+/* What linmt_attend_pages8 leaves where its kernel gives up a wait: in this thread's calls from now on every `each`-th CTA does so before its first one (0: none, as at the start). */
+int linmt_k_attend8_give_up(int32_t each);
+
 /* Y[R][N] = X[R][K] . Wt[N][K]^T on the tensor-core kernel (three bf16 planes, fp32-class
  * result) WITHOUT allocating: for hosts that cannot call cudaMalloc once they are running --
  * processes that gave the whole GPU to their own memory pool at start-up, or that share the

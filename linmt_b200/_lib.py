@@ -41,7 +41,7 @@ EXPORTS = ["python_decoder_init", "python_decoder_do_job", "linmt_default_option
            "linmt_read_model_file", "python_unk_init", "python_unk_do_job", "linmt_unk_create", "linmt_unk_process", "linmt_unk_destroy",
            "linmt_op_error", "linmt_beam_select", "linmt_beam_reorder", "linmt_plan_pages", "linmt_write_pages4", "linmt_read_pages4",
            "linmt_attend_pages4", "linmt_attend_pages4_workspace", "linmt_write_pages8", "linmt_read_pages8", "linmt_attend_pages8", "linmt_attend_pages8_workspace",
-           "linmt_fork_pages", "linmt_compact_pages", "linmt_copy_pages", "linmt_score_tokens"]
+           "linmt_fork_pages", "linmt_compact_pages", "linmt_copy_pages", "linmt_score_tokens", "linmt_k_attend8_give_up"]
 
 _lib = None
 
@@ -106,5 +106,6 @@ def load():
     for name in ("linmt_attend_pages4_workspace", "linmt_attend_pages8_workspace"):
         getattr(lib, name).argtypes = [C.c_char_p]
         getattr(lib, name).restype = C.c_int64
+    lib.linmt_k_attend8_give_up.argtypes = [C.c_int32]
     _lib = lib
     return lib

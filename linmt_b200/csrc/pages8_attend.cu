@@ -77,6 +77,7 @@ struct AttendParams {
   float cap, mul;            // mul: scale, times what the form of the scores takes it by
   int32_t row_page, row_head, rows;      // the pool as rows of blocks: from a page, a head to the next, and all (0: its strides are none of whole blocks)
   int32_t slack;             // by how many powers of 2 a weight may exceed what it is relative to
+  int32_t give_up;           // every so many-th CTA gives up before its first wait; 0: none
 };
 
 // The pool's rows of blocks: codes of a block (keys, or values), and its scales.
@@ -541,7 +542,7 @@ __global__ void __launch_bounds__(kThreads<R>) __maxnreg__(65536 / (kThreads<R> 
     bar_init(shared(&sh.p_full), kWeightWarps<R>);
     bar_init(shared(&sh.o_full), 1);
     bar_init(shared(&sh.first), kWeightWarps<R>);
-    sh.gave_up = 0;
+    sh.gave_up = a.give_up && blockIdx.x % (unsigned)a.give_up == 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -1134,6 +1135,8 @@ int64_t workspace_of(const linmt_attend_pages8_args* g) {
   return chunks_at_most(g) + kFixed <= kWhole ? 0 : (int64_t)blocks_of(g) * (2 * (rows_of(g) * (g->pages.dim + 2)) * 4 + 16);
 }
 
+thread_local int give_up_each = 0;
+
 int check(const linmt_attend_pages8_args* g) {
   if (!g || g->size != sizeof(*g)) return op_fail(LINMT_EINVAL, "attend_pages8: not this library's argument struct");
   if (int rc = check_pages8(g->pages, "attend_pages8")) return rc;
@@ -1158,6 +1161,12 @@ int check(const linmt_attend_pages8_args* g) {
 
 extern "C" {
 
+int linmt_k_attend8_give_up(int32_t each) {
+  if (each < 0) return LINMT_EINVAL;
+  linmt::ops::give_up_each = each;
+  return LINMT_OK;
+}
+
 int64_t linmt_attend_pages8_workspace(const linmt_attend_pages8_args* g) {
   using namespace linmt::ops;
   if (check(g)) return -1;
@@ -1177,7 +1186,7 @@ int linmt_attend_pages8(const linmt_attend_pages8_args* g) {
                        g->q, g->q_stride_n, g->q_stride_g, g->q_stride_h, g->out, g->out_stride_n, g->out_stride_g, g->out_stride_h, g->lse, g->table, g->table_stride, g->len,
                        g->slope, g->centre, g->first, g->last, need ? static_cast<float*>(g->workspace) : nullptr, g->n, g->g, g->heads, g->heads / g->pages.heads, g->width, row_tiles_of(g),
                        g->sinks, g->first && g->g <= 32 && (int64_t)g->n * g->g <= 65536, g->dtype,
-                       aligned(g->q, 16) && (g->q_stride_n | g->q_stride_g | g->q_stride_h) % (16 / dtype_bytes(g->dtype)) == 0, g->cap, 0.f, 0, 0, 0, g->dtype == LINMT_F32 ? 1 : 4};
+                       aligned(g->q, 16) && (g->q_stride_n | g->q_stride_g | g->q_stride_h) % (16 / dtype_bytes(g->dtype)) == 0, g->cap, 0.f, 0, 0, 0, g->dtype == LINMT_F32 ? 1 : 4, give_up_each};
   AttendMaps maps{};
   rows_of_blocks(g->pages, p, maps);
   const cudaStream_t st = static_cast<cudaStream_t>(g->stream);
