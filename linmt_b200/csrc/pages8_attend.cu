@@ -49,7 +49,6 @@ constexpr int kDrain = 256;                  // chunks between two drains: 127 *
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kAbove = 40.f;               // by how much more a score may exceed X than a weight what it is relative to
-constexpr float kFar = 1048576.f;            // scores from here on have too few bits behind the point to find M from their sums with the scales' exponents
 constexpr unsigned long long kWaitCycles = 2000000000ull;      // about a second
 template <int D, int R> constexpr int kKeyStages = (R == 8 ? 3 : 2) * 128 / D;
 template <int D, int R> constexpr int kValueStages = (R == 4 ? 2 : 3) * 128 / D;
@@ -381,7 +380,7 @@ struct Shared {
   // what the rows' scores, and their weights times scales, are relative to, as it is and as it was before
   alignas(16) float x[2][R], m[2][R], down_x[R], down_m[R], most_x[4][R], most_m[4][R];
   unsigned valid[VS];
-  int add, gave_up, far;
+  int add, gave_up;
   uint32_t tmem;
   alignas(8) unsigned long long k_full[KS], k_empty[KS], v_full[VS], v_empty[VS], s_full[2], s_empty[2], q_full[2], q_empty[2], p_full, o_full, first;
 };
@@ -809,49 +808,34 @@ __global__ void __launch_bounds__(kThreads<R>) __maxnreg__(65536 / (kThreads<R> 
                 s[r] = y - slope[j] * fabsf((float)pos - centre[j]) + none;
               }
               if (a.first) s[r] = (unsigned)(pos - lo[j]) < (unsigned)span[j] || pos < a.sinks ? s[r] : -INFINITY;
-              most = fmaxf(most, (s[r] - x[j]) + fmaxf(ve - m[j], -kAbove));
+              const float d = s[r] - x[j];
+              most = fmaxf(most, fmaxf(d + (ve - m[j]), d - kAbove));
             }
           }
           over = weights_any<kWeights>(most > slack) || over;
           if (c > 0) bar_wait(shared(&sh.o_full), it - 1 & 1, gave_up);
           // Something exceeds what the rows' weights are relative to: that follows.
           if (over) {
-            float most_x = kLowest, most_m = kLowest;      // of row row0 + lane
+            float most_x = kLowest, most_m = kLowest;      // of row row0 + lane: the warp's largest score, and the largest sum of a scale's exponent and a score's distance from that, as a sum with a
+                                                           // far score itself has no bits left for it
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-              const float x = warp_max(s[r]), y = warp_max(s[r] + ve);
+              const float x = fmaxf(warp_max(s[r]), kLowest), y = warp_max(s[r] - x + ve);
               if (lane == r) { most_x = x; most_m = y; }
             }
             if (lane < RT) { sh.most_x[warp % 4][row0 + lane] = most_x; sh.most_m[warp % 4][row0 + lane] = most_m; }
             weights_sync<kWeights>();
-            auto most_of = [&](const float (&x)[4][R]) { return fmaxf(fmaxf(x[0][tid], x[1][tid]), fmaxf(x[2][tid], x[3][tid])); };
             if (tid < R) {
-              const float was_x = sh.x[now][tid], was = was_x + sh.m[now][tid];      // (was_x as it is where nothing has been seen)
-              const float top_x = most_of(sh.most_x), top = most_of(sh.most_m), x = top_x - was_x > kAbove + slack ? ceilf(top_x) : was_x, m = (top - was > slack ? ceilf(top) : was) - x;
+              const float was_x = sh.x[now][tid], x0 = sh.most_x[0][tid], x1 = sh.most_x[1][tid], x2 = sh.most_x[2][tid], x3 = sh.most_x[3][tid], top_x = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3));
+              const float x = top_x - was_x > kAbove + slack ? ceilf(top_x) : was_x, was = was_x - x + sh.m[now][tid];
+              const float top = fmaxf(fmaxf(x0 - x + sh.most_m[0][tid], x1 - x + sh.most_m[1][tid]), fmaxf(x2 - x + sh.most_m[2][tid], x3 - x + sh.most_m[3][tid]));
+              const float m = top - was > slack ? ceilf(top) : was;
               sh.x[now ^ 1][tid] = x;
               sh.m[now ^ 1][tid] = m;
               sh.down_x[tid] = exp2_of(was_x - x);
-              sh.down_m[tid] = exp2_of(was_x - x + (sh.m[now][tid] - m));
-              const unsigned far = __ballot_sync((1u << R) - 1, fabsf(x) > kFar && x > kLowest);
-              if (tid == 0) sh.far = far != 0;
+              sh.down_m[tid] = exp2_of(was - m);
             }
             weights_sync<kWeights>();
-            if (sh.far) {                                  // M once more, from differences to X
-              float z = kLowest;
-#pragma unroll
-              for (int r = 0; r < RT; ++r) {
-                const float y = warp_max(s[r] - sh.x[now ^ 1][row0 + r] + ve);
-                if (lane == r) z = y;
-              }
-              if (lane < RT) sh.most_m[warp % 4][row0 + lane] = z;
-              weights_sync<kWeights>();
-              if (tid < R) {
-                const float was = sh.x[now][tid] - sh.x[now ^ 1][tid] + sh.m[now][tid], top = most_of(sh.most_m), m = top - was > slack ? ceilf(top) : was;
-                sh.m[now ^ 1][tid] = m;
-                sh.down_m[tid] = exp2_of(was - m);
-              }
-              weights_sync<kWeights>();
-            }
             now ^= 1;
           }
         } else {
@@ -927,7 +911,9 @@ __global__ void __launch_bounds__(kThreads<R>) __maxnreg__(65536 / (kThreads<R> 
           x = sh.x[now][tid];
           const int k = exponent_of(weight);
           e = min(max((int)fmaxf(sh.m[now][tid], -1000.f) - k, -250), 250);
-          f = weight == 0.f ? 0.f : power_of_2(e - e / 2) / (weight * power_of_2(-k));
+          const float one = weight * power_of_2(-k);
+          f = weight == 0.f ? 0.f : power_of_2(e - e / 2) / one;
+          if (x + (float)k - x == (float)k) { x += (float)k; weight = one; }      // between 1 and 2 then, where x has a place for k's last bits
           if ((sh.bad[buffer][tid] && weight > 0.f) || *gave_up) f = weight = NAN;
         }
         sh.down_x[tid] = power_of_2(e / 2);
@@ -995,13 +981,13 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
   if (ends.x < 0) return;
   const int from = ends.w, n_parts = (int)blockIdx.x - from + 1;
   auto part = [&](int i) { return a.ws + ((int64_t)(from + i) * 2 + (i == 0)) * kPart; };
-  // A part counts 2^(x + k) times a number between 1 and 2, k its sum's exponent.  The largest so far goes along, so that every part is waited for once: eight of them at a time are on their
-  // way.  x and k stay apart, as x may have no place for k's last bits; sums are 2^fewer smaller, so that values of up to 2^127 have room.
-  const int fewer = 33 - __clz(n_parts);
-  float x = kLowest, k = 0.f, weight = 0.f;
+  // The largest exponent so far goes along, and the largest sum of weights, so that every part is waited for once: eight of them at a time are on their way.  A part's share is relative
+  // to 2^(x + k), k that sum's exponent, and 2^fewer times smaller, so that values of up to 2^127 have room; x may have no place for k's last bits.
+  const float fewer = (float)(33 - __clz(n_parts));
+  float x = kLowest, most = 0.f, k = 0.f, weight = 0.f;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = by; i0 < n_parts; i0 += 8 * kBy) {
-    float m[8], l[8], n[8];
+    float m[8], l[8];
     float4 v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -1017,18 +1003,17 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
     const float was_x = x, was_k = k;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int e = exponent_of(l[j]);
-      n[j] = (float)e;
-      l[j] *= power_of_2(-e);
-      if (m[j] - x + (n[j] - k) > 0.f) { x = m[j]; k = n[j]; }
+      x = fmaxf(x, m[j]);
+      most = fmaxf(most, l[j]);
     }
+    k = (float)exponent_of(most);
     const float f0 = exp2_of(was_x - x + (was_k - k));
     weight *= f0;
     sum.x *= f0; sum.y *= f0; sum.z *= f0; sum.w *= f0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if (i0 + j * kBy >= n_parts) break;
-      const float f = exp2_of(m[j] - x + (n[j] - k) - (float)fewer) * l[j];
+      const float f = exp2_of(m[j] - x - k - fewer) * l[j];
       sum.x += f * v[j].x; sum.y += f * v[j].y; sum.z += f * v[j].z; sum.w += f * v[j].w;
       weight += f;
     }
@@ -1038,8 +1023,10 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
   __syncthreads();
   if (by || r >= a.g * a.rep - ends.z * R) return;
 #pragma unroll
-  for (int i = 1; i < kBy; ++i)
-    if (s_x[i][r] - x + (s_k[i][r] - k) > 0.f) { x = s_x[i][r]; k = s_k[i][r]; }
+  for (int i = 1; i < kBy; ++i) {
+    x = fmaxf(x, s_x[i][r]);
+    k = fmaxf(k, s_k[i][r]);
+  }
   sum = make_float4(0.f, 0.f, 0.f, 0.f);
   weight = 0.f;
 #pragma unroll
@@ -1056,7 +1043,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
   store_as(a.out, to + 1, a.dtype, sum.y * f);
   store_as(a.out, to + 2, a.dtype, sum.z * f);
   store_as(a.out, to + 3, a.dtype, sum.w * f);
-  if (d == 0 && a.lse) a.lse[((int64_t)ends.x * a.g + g) * a.heads + h] = weight == 0.f ? -INFINITY : (x + (k + (float)fewer + log2f(weight))) * kLn2;
+  if (d == 0 && a.lse) a.lse[((int64_t)ends.x * a.g + g) * a.heads + h] = weight == 0.f ? -INFINITY : (x + (k + fewer + log2f(weight))) * kLn2;
 }
 
 template <int D, int R>
