@@ -16,7 +16,7 @@
 // A CTA has 128 threads (256 with 16 rows) that turn S into weights, a position and up to eight rows each; one warp that copies blocks and makes queries ready, two pieces ahead, and one that
 // issues the products.  Two CTAs share an SM, three with four rows.  The work is cut into equal shares over the CTAs that fit on the GPU at once, and a second kernel joins the parts of what
 // several of them share.
-// What bounds it: long sentences HBM (8 documents of 20-32k, 16 rows of 128: 83 us, 5.2 TB/s, of which 6 us until the first weights and 4 for the join) and, as much, the weights' latencies:
+// What bounds it: long sentences HBM (8 documents of 20-32k, 16 rows of 128: 84 us, 5.2 TB/s, of which 6 us until the first weights and 4 for the join) and, as much, the weights' latencies:
 // 2700 cycles a chunk of a CTA's, of which the conversions and exponentials take 640.  Where scores rise from chunk to chunk (a bias that falls with the distance) taking O out each time is another 1600.
 // Tried: weights stored byte by byte, positions as neighbours: 129 us where columns as neighbours took 105.  A bulk copy for each block's keys, values and scales: 110 us where four blocks a copy took
 // 83.  Single rows that see nothing of a chunk left out: 92 us, and no faster with windows, as what is saved in work is lost in order.  Two rows an instruction: no difference.

@@ -383,8 +383,9 @@ __global__ void __launch_bounds__(32 * kWarps, 3) rows_kernel(const RowsParams a
 
 template <bool WRITE, class T>
 void launch_rows(RowsParams p, int dim, cudaStream_t st) {
-  // A step's positions each in a block of their own: a window for each.  Texts: windows of 16 positions, and all heads by one CTA where that leaves 16 CTAs for each SM all
-  // the same, as looking at the slots takes as long as a run; four heads otherwise, a run of each for every warp.
+  // Few positions: a window for each, as a step's lie in a block each.  More: windows of 16 positions, and all heads by one CTA where that leaves 16 CTAs for each SM all
+  // the same, as looking at the slots takes as long as a run; four heads otherwise, a run of each for every warp.  (How many runs a window has, which is what counts, only the device
+  // knows: 16 single positions of a window are 16 runs one after the other for a warp.)
   p.window = (int64_t)p.t * p.heads <= 16 * 16 * 148 ? 1 : 16;
   const int64_t windows = ((int64_t)p.t + p.window - 1) / p.window, each = windows * p.heads / (16 * 148);
   p.heads_each = (int)(each < 4 ? (p.heads < 4 ? p.heads : 4) : each > p.heads ? p.heads : each);

@@ -1,7 +1,7 @@
 // token_ops.cu -- scores of given tokens (linmt_score_tokens): log probability, entropy and the best alternatives of rows of logits.
 //
 //   d = x log2 e - k, S = sum 2^d, T = sum 2^d d:   log sum exp x = (k + log2 S) ln 2,   entropy = ln 2 (log2 S - T / S)
-// with a whole number k, at most 8 below the largest x log2 e, so that d is rounded once.  (Of an entropy next to 0 that leaves 1e-6: T and log2 S are of k's size then, and cancel.)  One pass over a row, each thread
+// with a whole number k, at most 8 below the largest x log2 e, so that d is rounded once.  (Of an entropy next to 0 some 1e-6 are left: log2 S and T / S may both be about 8 then, and what they were rounded by is.)  One pass over a row, each thread
 // with a k of its own, two logits an instruction where there is one for two.  A row whose largest logit is beyond 65536 in size is added up once more relative to e^m, m that logit itself:
 // k and x log2 e have no place left behind the point from 2^23 on, and logits that far apart are told apart by x - m alone.  Bound by HBM in 32 bits, by instructions (unpacking 1, list 2, the rest 6 an element) in 16.
 // The k-th largest of 32 groups' maxima is reached by k words at least: only the words of threads whose own maximum reaches it are looked at again (from L2), by their whole warp, and what

@@ -164,7 +164,8 @@ def fork_pages(table, lens, parents, shares, free, used, *, page, done=None, out
 
 
 def free_pages(table, lens, done, shares, free, used, *, page, out=None):
-    """The pages of rows that are ``done`` go back to ``free`` where no other row names them.  ``table`` [n, width] with ``lens`` and ``done`` [n], or [n, k, width] with [n, k].
+    """The pages of rows that are ``done`` go back to ``free`` where no other row names them.  ``table`` [n, width] with ``lens`` and ``done`` [n], or [n, k, width] with [n, k]; up to
+    16384 rows.
     Returns ``table``, ``lens``, ``shares``, ``free`` and ``used`` as fork_pages does; ``out``: a tuple of five."""
     return _front.free_pages(table, lens, None, done, shares, free, used, page, None if out is None else tuple(out))
 
