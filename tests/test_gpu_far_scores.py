@@ -205,3 +205,64 @@ def test_attend_values_of_all_sizes(ops, size, lens, dtype):
     for up in (0.0, 20.0, 27.0, 28.0, 29.0, 30.0, 31.0):      # 2^40 is e^27.7, 2^44 e^30.5
         q[..., 0] = up / (100 * 2.0 ** -9)
         attend_check(ops, _cuda(q.astype(np.float32), dtype), pool, table, lens, kv, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,v", [(2, 700), (1, 50003), (1, 200003)])
+def test_score_one_word_far_from_the_others(ops, n, v, dtype):
+    """A single word, so that only one thread and one CTA of a row's meets it, before, among and behind the others; and beside words that are not allowed and hold anything."""
+    rng = _rng(n, v, 96)
+    ordinary = rng.normal(0, 2, v)
+    for at in (0, v // 3, v - 1):
+        rows = []
+        for c in FAR:
+            for far in (c, -c):
+                x, y = ordinary.copy(), np.full(v, far)
+                x[at], y[at] = far, far * (1 - 2.0 ** -6)
+                rows += [x, y]
+        for a, b in ((65530.0, 65545.0), (-65545.0, -65530.0), (-4.2e6, -70000.0), (-4.1e6, -60000.0)):
+            x = np.full(v, a)
+            x[at] = b
+            rows.append(x)
+        for i in range(0, len(rows) - n + 1, n):
+            x = np.stack(rows[i:i + n])[:, None].astype(np.float32)
+            far_check(ops, _cuda(x, dtype), _cuda(np.full((n, 1), at if i % 4 else v // 2, np.int32)), 4)
+            if i % 5 == 0:
+                from test_gpu_token_scores import _bits
+                allowed = rng.random((1, v)) < 0.5
+                allowed[0, at] = i % 2 == 0
+                wild = x.copy()
+                wild[:, :, ~allowed[0]] = np.nan
+                x[:, :, ~allowed[0]] = -np.inf
+                tokens = _cuda(np.full((n, 1), at, np.int32))
+                want = ops.score_tokens(_cuda(x, dtype), tokens, top=4)
+                got = ops.score_tokens(_cuda(wild, dtype), tokens, top=4, allowed=_cuda(_bits(allowed)))
+                far_check(ops, _cuda(x, dtype), tokens, 4)
+                assert all((a == b).all() for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("lens", [[300, 90], [9000]])
+@pytest.mark.parametrize("g", [4, 16])
+def test_attend_scores_that_leave_32_bits(ops, g, lens):
+    """Rows whose scores leave 32 bits may be NaN; the others of their products are as good as they are alone, and those that see nothing zeros.  (Not the same to the bit: sums are taken out for all
+    rows when one asks for it, and are rounded then.)"""
+    from test_gpu_pages8 import attend_check
+    rng = _rng(97, g)
+    n, heads, dim, page = len(lens), 2, 64, 32
+    pool, table, kv = memory8(rng, n, lens, heads, dim, page)
+    q = _cuda(rng.normal(0, 1, (n, g, heads, dim)).astype(np.float32))
+    first, last = np.zeros((n, g), np.int64), np.repeat(np.asarray(lens)[:, None], g, 1)
+    first[:, 3] = last[:, 3]                                   # sees nothing
+    attend_check(ops, q, pool, table, lens, kv, first=first, last=last)
+    want, want_lse, tol, tol_lse = attend_ref(q, kv, table.cpu().numpy(), lens, dim ** -0.5, first=first, last=last)
+    wild = q.clone()
+    wild[:, 1], wild[:, 2, 0], wild[:, 3] = 3e38, -3e38, 3e38
+    dev = dict(first=_cuda(first.astype(np.int32)), last=_cuda(last.astype(np.int32)))
+    got, lse = ops.attend_pages8(wild, pool, table, _cuda(np.asarray(lens, np.int32)), want_lse=True, **dev)
+    out, l = got.double().cpu().numpy(), lse.double().cpu().numpy()
+    ordinary = np.ones((n, g, heads), bool)
+    ordinary[:, 1] = ordinary[:, 2, 0] = ordinary[:, 3] = False
+    assert (np.abs(out - want)[ordinary] <= tol[ordinary][:, None] + HALF_STEP[F32] * np.abs(want[ordinary])).all() and (np.abs(l - want_lse)[ordinary] <= tol_lse[ordinary]).all()
+    assert (got[:, 3] == 0).all() and (lse[:, 3] == -INF).all()
+    again, _ = ops.attend_pages8(q, pool, table, _cuda(np.asarray(lens, np.int32)), want_lse=True, scale=1e38, **dev)
+    assert (again[:, 3] == 0).all() and again.shape == q.shape
